@@ -474,6 +474,48 @@ int zk_softmax_shift_decompose(void* shift, void* out_shifted, void* const* plan
 int zk_softmax_shift_decompose_i64(void* shift, void* out_shifted, void* const* planes, void* const* int_planes, const void* X64, uint32_t rows, uint32_t cols, double scale,
                                    const uint32_t* bs_host, int K, void* stream);
 
+/* ---- a decoder layer's values without their witness --------------------------------------------------------------------------- */
+/* What the forward passes of the blocks compute, for a caller who wants the answer and no proof: int32 tensors (fixed point, as the .bin files
+ * hold them) in and out, one kernel where the proof needs a field tensor a step.  Results are whole numbers and equal the class layer's.
+ * A quotient by s is floor((t + floor(s / 2)) / s), zk_rescale's.
+ * flag_dev: 4 bytes of device memory, raised (bits are added, never cleared) when a value does not fit: the caller clears it before its first call and
+ * reads it (zk_memcpy_d2h) when it is through; outputs then hold anything at the places concerned.  flag_dev null: the call waits for its kernels
+ * and returns the error.
+ * workspace: zk_i32_linear_workspace bytes of device memory that no other call uses meanwhile, or null: the library takes it from its allocator
+ * for the time of the call.  A call that is captured into a graph needs both of the caller's. */
+#define ZK_VALUES_RANGE 1u        /* a result or an intermediate value outside int32, or a sum of products of 2^62 or more */
+#define ZK_VALUES_TABLE 2u        /* an activation outside the table of function values; the output is 0 there */
+#define ZK_VALUES_POSITION 4u     /* a position outside the table of angles; the token's heads are not written */
+/* The residual stream with a block's output added, and the next block's input (rmsnorm.cu:36-39, skip-connection.cu:15-18, llama-rmsnorm.py:37-39):
+ *   h = x + q(res * q(gate * N(b; post))),   n = N(h; w),   N(v; w)_j = q(q(w_j r) v_j),   q: the quotient by sf,
+ *   r = the nearest integer to scale / sqrt(sum_j (v_j / scale)^2 / cols + eps), the sum in double precision as zk_row_sumsq_f64 takes it.
+ * x, b: rows of cols int32, ldx and ldb elements apart; b null: h = x (post and gate null then).  post null: b itself; gate: gate_rows rows of cols
+ * int32, row i for rows / gate_rows rows of x each, or null and 0; res: the residual scale, sf for 1.  h, n (rows * cols), rms_inv (rows; r of h): each may be null; h or
+ * n may be x or b themselves where the rows are cols apart.  n needs w; w is not read without n.  scale / sqrt(eps) below 2^31. */
+int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t ldx, const void* b, size_t ldb, const void* post, const void* gate, uint32_t gate_rows, int32_t res,
+                         const void* w, uint32_t rows, uint32_t cols, double eps, double scale, uint32_t sf, void* flag_dev, void* stream);
+/* Rotary positions (llama-self-attn.py:42-73, in fixed point): the first rot of a head's dim elements are rot / 2 pairs, pair i of a token at position p
+ *   (x0, x1) -> (q(c x0 - s x1), q(s x0 + c x1)),   (c, s) = table[p][i], q: the quotient by sf, the table's scale (1 .. 2^30);
+ * the rest is copied.  neighbours: pair i is (2 i, 2 i + 1), else (i, i + rot / 2).  table: table_rows * (rot / 2) pairs of int32 up to 2^30 in magnitude.  positions: one int32 a
+ * token, or null: first, first + 1, ...  Strides in elements from token to token and from head to head, heads of dim contiguous elements; out may be x with the same
+ * strides, and overlaps it in no other way.  The strides out of place are free: a stack [head][token][dim] is written as easily as [token][head][dim].
+ * zk_fr_rope: the same for field elements that stand for 32-bit integers (any other raises the flag and counts as 0). */
+int zk_i32_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
+                const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
+int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
+               const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
+/* A weight laid out for zk_i32_linear and zk_i32_gated from its int32 form (N x P, on the device; not read afterwards): two or three bytes an element.  The handles
+ * of zk_fr_matmul_rhs_prepare serve them as well; one made here has no field elements and serves no field product.  Elements up to 8355711 in magnitude, N at
+ * most 43690.  Waits for the stream; released with zk_fr_matmul_rhs_free. */
+int zk_i32_rhs_prepare(void** prepared, const void* B_i32, uint32_t N, uint32_t P, void* stream);
+size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner);
+/* A projection with its rescaling (zkfc.cu:44-58, rescaling.cu:13-19): out = q(x W), rows x P int32.  x: rows of N int32, ldx apart, each at most 0x7F7F7F7F; out
+ * overlaps nothing that is read.  At most 262144 rows. */
+int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, uint32_t rows, uint32_t sf, void* workspace, size_t workspace_bytes, void* flag_dev, void* stream);
+/* The gated half of a feed-forward block (ffn.cu:61-73): out = q_hidden(act[q_gate(x G)] * q_up(x U)), act[v] = table[v - low] of len int32.  Both weights have one shape. */
+int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared, const void* up_prepared, uint32_t rows, uint32_t sf_gate, uint32_t sf_up, const void* table_i32,
+                 int32_t low, uint32_t len, uint32_t sf_hidden, void* workspace, size_t workspace_bytes, void* flag_dev, void* stream);
+
 /* ---- measurement helpers (no counterpart in the reference) ---------------------------------------- */
 /* v_mad_u64_u32 issue peak of the device: 16 independent chains per lane, no memory traffic */
 int zk_bench_mad_peak(uint32_t blocks, uint32_t iters, double* mad_per_s_host, void* stream);

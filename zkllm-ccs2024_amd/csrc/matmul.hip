@@ -25,6 +25,7 @@
 #include <utility>
 #include <vector>
 #include "field.hpp"
+#include "planes.hpp"
 #include "rt.hpp"
 #include "../../include/zkllm_hip.h"
 
@@ -374,15 +375,7 @@ template <typename T> static int run_int_path(void* C, const void* A, const void
 }
 
 // ---- int8-plane path: digit planes and a GEMM on the matrix cores ------------------------------------------------------
-// Balanced base-256 digits of a small signed integer: x = sum_j d_j 256^j, d_j in [-128, 127].  Both operands are laid
-// out as planes of rows along the contraction index, padded with zeros to a multiple of the GEMM's K tile Kp, A[b][m][k] in rows m of the
-// planes b * pa + i and B[b][k][p], transposed on the way, in rows p of the planes b * pb + j.  A plane stands in blocks of 32 contraction
-// bytes of all its rows (plane_at): every operand fragment of the matrix instruction is 16 consecutive bytes, and the 32 rows of a step
-// that a wave brings to LDS at once are 1 KB in one piece.
-__host__ __device__ __forceinline__ size_t plane_at(size_t rows, size_t row, uint32_t k) { return ((size_t)(k >> 5) * rows + row) * 32 + (k & 31u); }
-typedef int v4i __attribute__((ext_vector_type(4)));
-typedef int v16i __attribute__((ext_vector_type(16)));
-static constexpr int GBM = 128, GBN = 128, GBK = 128;      // block tile of the pair-by-pair GEMM: 4 waves, 64 x 64 outputs each
+static constexpr int GBM = 128, GBN = 128;      // block tile (GBK along the contraction) of the pair-by-pair GEMM: 4 waves, 64 x 64 outputs each
 static constexpr int GLD = GBK + 16;                       // LDS row stride in bytes: 16-byte aligned rows whose 16-byte reads spread over all banks
 
 // src: the operand as a product of int32 forms when src.a is set (a is then not read)
@@ -453,11 +446,6 @@ __device__ __forceinline__ unsigned long long fr_magnitude(const Fr& x, bool& ne
     }
     return v > (1ull << 62) ? ~0ull : v;
 }
-// the balanced digits of a 32-bit integer, one a byte
-__device__ __forceinline__ uint32_t digit_bytes(unsigned long long mag, bool negative) {
-    const uint32_t x = negative ? 0u - (uint32_t)mag : (uint32_t)mag;
-    return (x + 0x80808080u) ^ 0x80808080u;
-}
 static constexpr int EX_ROW = 4;      // elements a lane of A has on their way at once
 __global__ void __launch_bounds__(256) k_examine_split(const ExamineArgs g) {
     __shared__ uint32_t tile[4][64][17];
@@ -483,7 +471,7 @@ __global__ void __launch_bounds__(256) k_examine_split(const ExamineArgs g) {
                 const unsigned long long v = fr_magnitude(x[i], ng);
                 mx = v > mx ? v : mx;
                 sum = sat_add(sum, v);
-                const int w = (int)digit_bytes(v, ng);
+                const int w = (int)digit_bytes(ng ? 0u - (uint32_t)v : (uint32_t)v);
                 const uint32_t w0 = (uint32_t)__builtin_amdgcn_update_dpp(0, w, 0x00, 0xF, 0xF, false), w1 = (uint32_t)__builtin_amdgcn_update_dpp(0, w, 0x55, 0xF, 0xF, false);
                 const uint32_t w2 = (uint32_t)__builtin_amdgcn_update_dpp(0, w, 0xAA, 0xF, 0xF, false), w3 = (uint32_t)__builtin_amdgcn_update_dpp(0, w, 0xFF, 0xF, 0xF, false);
                 const uint32_t lo = __builtin_amdgcn_perm(w1, w0, sel), hi = __builtin_amdgcn_perm(w3, w2, sel);
@@ -517,7 +505,7 @@ __global__ void __launch_bounds__(256) k_examine_split(const ExamineArgs g) {
             bool ng;
             const unsigned long long v = fr_magnitude(x[i], ng);
             mx = v > mx ? v : mx;
-            w[i] = digit_bytes(v, ng);
+            w[i] = digit_bytes(ng ? 0u - (uint32_t)v : (uint32_t)v);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -649,10 +637,6 @@ __global__ void __launch_bounds__(256) k_gemm_i8_planes(const PlaneGemm g) {
 // random bytes, 129 us (3.2 POP/s: what the card's power allows them), the loads alone 123 (17 TB/s out of the L2), the 268 MB of results 48,
 // which two blocks that run in step do not hide.
 static constexpr int GKT = 32, GBUF = 4;
-__device__ __forceinline__ uint32_t gemm_half(uint32_t row, uint32_t h) { return h ^ ((row >> 3) & 1u); }
-__device__ __forceinline__ void load_to_lds(const int8_t* src, int8_t* dst) {       // 16 bytes a lane, dst: the wave's first byte
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)src, (__attribute__((address_space(3))) uint32_t*)dst, 16, 0, 0);
-}
 template <int PA, int PB, int TN> __global__ void __launch_bounds__(256, 2) k_gemm_i8_planes_all(const PlaneGemm g) {
     constexpr int NS = PA + PB - 1, TM = 64, NT = TN / 64, PIECES = 2 * PA + 2 * NT * PB, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * TN) * GKT;      // NT: a wave's 32 x 32 tiles
     // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
@@ -793,16 +777,7 @@ static const int g_gemm_timer_hook = (at_shutdown([] {
     g_gemm_timer.ev.clear();
     g_gemm_timer.on = false;
 }), 0);
-static int digits_for(unsigned long long absmax) {      // planes needed for |x| <= absmax: p digits reach 127 (256^p - 1) / 255
-    int p = 1;
-    unsigned __int128 reach = 127;
-    while (reach < absmax && p < 8) { reach = reach * 256 + 127; ++p; }
-    return reach >= absmax ? p : 0;
-}
 // returns ZK status; *done = false when the path does not apply (the caller then takes a VALU kernel)
-// A right operand kept by the caller for many products (a layer's weight): its largest magnitude and, when it is a matrix of
-// small integers, its digit planes in the GEMM's layout -- neither is computed again per product.
-struct MatmulRhs { const void* B = nullptr; uint32_t N = 0, P = 0, Kp = 0; unsigned long long mb = ~0ull; int pb = 0; void* planes = nullptr; };
 static int run_int8_plane_path(void* C, const void* A, const void* B, uint32_t batch, uint32_t M, uint32_t N, uint32_t P, unsigned long long ma, unsigned long long mb,
                                hipStream_t st, bool* done, const MatmulRhs* rhs = nullptr, ProdSrc src = ProdSrc{nullptr, nullptr}, long long* C64 = nullptr,
                                bool b_transposed = false, const int8_t* pa4 = nullptr, const int8_t* pb4 = nullptr) {
@@ -1047,12 +1022,14 @@ int zk_fr_matmul_rhs_free(void* prepared) {
 int zk_fr_matmul_rhs(void* C, const void* A, const void* prepared, uint32_t M, int mode, int* path_used, void* stv) {
     const MatmulRhs* r = (const MatmulRhs*)prepared;
     ZK_ARG(r != nullptr, "zk_fr_matmul_rhs: null handle");
+    ZK_ARG(r->B != nullptr, "zk_fr_matmul_rhs: the handle was made from int32 and has no field elements");
     return matmul_dispatch(C, A, r->B, 1, M, r->N, r->P, mode, path_used, stv, r);
 }
 // the same with the left operand given by its int32 form (M * N int32 on the device): 4 bytes read per element instead of 32
 int zk_fr_matmul_rhs_ints(void* C, const void* a_ints, const void* prepared, uint32_t M, int mode, int* path_used, void* stv) {
     const MatmulRhs* r = (const MatmulRhs*)prepared;
     ZK_ARG(r != nullptr && a_ints != nullptr, "zk_fr_matmul_rhs_ints: null argument");
+    ZK_ARG(r->B != nullptr, "zk_fr_matmul_rhs_ints: the handle was made from int32 and has no field elements");
     return matmul_dispatch(C, nullptr, r->B, 1, M, r->N, r->P, mode, path_used, stv, r, ProdSrc{(const int32_t*)a_ints, nullptr});
 }
 int zk_fr_matmul(void* C, const void* A, const void* B, uint32_t M, uint32_t N, uint32_t P, int mode, int* path_used, void* stv) {
