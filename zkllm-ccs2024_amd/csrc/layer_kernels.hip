@@ -16,6 +16,7 @@
 #include <cmath>
 #include <cstring>
 #include <memory>
+#include <type_traits>
 #include "field.hpp"
 #include "planes.hpp"
 #include "rt.hpp"
@@ -24,12 +25,19 @@
 using namespace zk;
 
 // ---- quotients --------------------------------------------------------------------------------------------------------------------------
-// shift >= 0: s is 2^shift, else any.  POW2 is a template argument where a kernel divides often: the general quotient is some 60 instructions.
-struct Divisor { int64_t s, half; int shift; };
-static Divisor divisor(uint32_t s) { return Divisor{(int64_t)s, (int64_t)(s >> 1), (s & (s - 1)) == 0 ? 31 - __builtin_clz(s) : -1}; }
-__device__ __forceinline__ int64_t quotient_general(int64_t t, const Divisor& d) {      // |t| <= 2^62: the sum does not wrap
-    const int64_t n = t + d.half, q = n / d.s;
-    return q - (q * d.s > n ? 1 : 0);
+// shift >= 0: s is 2^shift, else any.  POW2 is a template argument where a kernel divides often.
+struct Divisor { int64_t s, half; double inv; int shift; };
+static Divisor divisor(uint32_t s) { return Divisor{(int64_t)s, (int64_t)(s >> 1), 1.0 / (double)s, (s & (s - 1)) == 0 ? 31 - __builtin_clz(s) : -1}; }
+// floor((t + s / 2) / s) for |t| <= 2^62, by the divisor's double-precision inverse: the first quotient is off by no more than 3 2^-53 2^62 / s + 1, what
+// it leaves is below s + 2^11 in magnitude and divided exactly up to one unit.  Some 30 instructions against some 100 of a 64-bit division.
+__device__ __forceinline__ int64_t quotient_general(int64_t t, const Divisor& d) {
+    const int64_t n = t + d.half;
+    int64_t q = (int64_t)floor((double)n * d.inv);
+    int64_t r = n - q * d.s;
+    const int64_t more = (int64_t)floor((double)r * d.inv);
+    q += more;
+    r -= more * d.s;
+    return q - (r < 0 ? 1 : 0) + (r >= d.s ? 1 : 0);
 }
 template <bool POW2> __device__ __forceinline__ int64_t quotient(int64_t t, const Divisor& d) {
     if constexpr (POW2) return (t + d.half) >> d.shift;
@@ -198,6 +206,8 @@ template <typename T, bool POW2> __global__ void __launch_bounds__(256) k_rope(c
 }
 
 // ---- products with a kept weight -----------------------------------------------------------------------------------------------------------------
+// x and W as balanced base-256 digits (planes.hpp): an integer product is an int8 product for every pair of planes, pairs of equal weight 256^(i+j)
+// in one int32 accumulator (at most three pairs of K 2^14, K below 2^17 / 3), the accumulators joined in 64 bits at the end.  Exact in any order.
 struct Epilogue {
     int32_t* out;
     Divisor sf, sf_gate, sf_hidden;      // linear: sf; gated: sf is the up projection's
@@ -212,41 +222,371 @@ __device__ __forceinline__ int32_t gated_value(int64_t g, int64_t u, const Epilo
     const int32_t up = narrow(quotient_any(u, e.sf), bad);
     return narrow(quotient_any((int64_t)e.table[at] * up, e.sf_hidden), bad);
 }
-// a weight's digit planes; a matrix of fewer planes than another reads zeros for the rest
+// a weight's digit planes
 struct Planes { const int8_t* p; uint32_t rows, Kp; int n; };
 struct ProductArgs {
     const int32_t* x;
     size_t ldx;
     uint32_t rows, inner, cols;
-    Planes w, gate;
+    int x_aligned;                       // rows of x begin at multiples of 16 bytes
+    Planes w, gate;                      // gated: w is the up projection
+    const int8_t* px;                    // x's four planes, rows_padded rows each, and how many of them 32 rows' stretch of CHUNK columns needs
+    const uint32_t* need;
+    const int8_t* zeros;                 // 1 KB
+    uint32_t rows_padded, chunks;
     Epilogue e;
 };
-// 2^62 and beyond: flagged, so that what follows works on a sum that 64 bits hold
-__device__ __forceinline__ int64_t checked_sum(__int128 v, uint32_t& bad) {
-    if (v >= ((__int128)1 << 62) || v <= -((__int128)1 << 62)) { bad |= ZK_VALUES_RANGE; return 0; }
-    return (int64_t)v;
+static constexpr uint32_t CHUNK = 256;
+// sum_s a[s] 256^s: below 2^62 in magnitude, or flagged and 0.  |a[s]| < 2^31, so the two low terms are below 2^41 together and the rest, in
+// units of 2^16, says whether the sum fits 64 bits.
+template <int NS> __device__ __forceinline__ int64_t joined(const int32_t (&a)[NS], uint32_t& bad) {
+    int64_t lo = a[0], hi = 0;
+    if constexpr (NS > 1) lo += (int64_t)a[1] << 8;
+#pragma unroll
+    for (int s = 2; s < NS; ++s) hi += (int64_t)a[s] << (8 * (s - 2));
+    const int64_t limit = (1ll << 46) + (1ll << 25), most = 1ll << 62;
+    if (hi >= limit || hi <= -limit) { bad |= ZK_VALUES_RANGE; return 0; }
+    const int64_t v = hi * 65536 + lo;
+    if (v >= most || v <= -most) { bad |= ZK_VALUES_RANGE; return 0; }
+    return v;
 }
-// A lane an output, its weight's digits straight from the planes.
-template <bool GATED> __global__ void __launch_bounds__(256) k_product_plain(const ProductArgs g) {
-    const uint32_t col = blockIdx.x * 64 + (threadIdx.x & 63u), row = blockIdx.y * 4 + (threadIdx.x >> 6);
-    if (col >= g.cols || row >= g.rows) return;
-    uint32_t bad = 0;
-    const int32_t* x = g.x + row * g.ldx;
-    auto dot = [&](const Planes& w) {
-        int64_t acc[3] = {0, 0, 0};            // |x| < 2^31, a digit below 2^8, fewer than 2^17 of them
-        for (int j = 0; j < 3; ++j) {
-            if (j >= w.n) break;
-            const int8_t* p = w.p + (size_t)j * w.rows * w.Kp;
-            for (uint32_t k = 0; k < g.inner; ++k) acc[j] += (int64_t)x[k] * p[plane_at(w.rows, col, k)];
+// the digits of 16 values, plane by plane: plane j's 16 bytes in out[j]
+__device__ __forceinline__ void digit_planes(const int32_t (&x)[16], v4i (&out)[4], uint32_t& bad) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            bad |= x[4 * w + e] > 0x7F7F7F7F ? (uint32_t)ZK_VALUES_RANGE : 0u;      // four digits reach no further
+            d[e] = digit_bytes((uint32_t)x[4 * w + e]);
         }
-        return checked_sum((__int128)acc[0] + ((__int128)acc[1] << 8) + ((__int128)acc[2] << 16), bad);
+        const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), b = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
+        const uint32_t c = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), e = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+        out[0][w] = (int)__builtin_amdgcn_perm(c, a, 0x05040100u);
+        out[1][w] = (int)__builtin_amdgcn_perm(c, a, 0x07060302u);
+        out[2][w] = (int)__builtin_amdgcn_perm(e, b, 0x05040100u);
+        out[3][w] = (int)__builtin_amdgcn_perm(e, b, 0x07060302u);
+    }
+}
+// 16 values of a row from column k on; zeros beyond the row's end and for rows that are none
+__device__ __forceinline__ void row_piece(const ProductArgs& g, uint32_t row, uint32_t k, int32_t (&x)[16]) {
+    const int32_t* p = g.x + row * g.ldx + k;
+    if (row < g.rows && g.x_aligned && k + 16 <= g.inner) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const v4i v = reinterpret_cast<const v4i*>(p)[w];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * w + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = (row < g.rows && k + e < g.inner) ? p[e] : 0;
+    }
+}
+
+// x's planes for the products of many rows.  A wave takes 32 rows and CHUNK columns, 32 columns at a time: a lane 16 values of a row, so that the wave
+// writes 1 KB of every plane in one piece.  It notes how many planes its stretch needs, in a place of its own.
+__global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __restrict__ planes, uint32_t* __restrict__ need, v4i* __restrict__ zeros) {
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) zeros[threadIdx.x] = v4i{0, 0, 0, 0};
+    const uint32_t lane = threadIdx.x & 63u, chunk = blockIdx.x * 4 + (threadIdx.x >> 6), group = blockIdx.y;
+    if (chunk >= g.chunks) return;
+    const uint32_t row = group * 32 + (lane >> 1), h = lane & 1u, Kp = g.w.Kp;
+    uint32_t bad = 0, planes_needed = 1;
+    for (uint32_t k0 = chunk * CHUNK; k0 < min((chunk + 1) * CHUNK, Kp); k0 += 32) {
+        int32_t x[16];
+        v4i d[4];
+        row_piece(g, row, k0 + 16 * h, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const uint32_t m = (uint32_t)(x[e] < 0 ? ~x[e] : x[e]);      // p digits hold -128 (256^p - 1) / 255 .. 127 (256^p - 1) / 255
+            planes_needed = max(planes_needed, m <= 127u ? 1u : m <= 32639u ? 2u : m <= 8355711u ? 3u : 4u);
+        }
+        digit_planes(x, d, bad);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<v4i*>(planes + (size_t)j * g.rows_padded * Kp + plane_at(g.rows_padded, row, k0 + 16 * h)) = d[j];
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) planes_needed = max(planes_needed, (uint32_t)__shfl_xor(planes_needed, off, 64));
+    if (lane == 0) need[(size_t)group * g.chunks + chunk] = planes_needed;
+    raise(g.e.flag, bad);
+}
+
+// Many rows.  A workgroup of four waves takes 64 MT rows by 128 columns of weights -- 64 of each where there are two: a wave's gate and up tiles lie in the same
+// lanes, and what joins them needs no exchange -- and a wave 32 MT by 64, as 32 x 32 tiles of v_mfma_i32_32x32x32_i8.
+// Steps of 32 contraction bytes go from memory to LDS without passing through registers, four buffers deep; a step's fragments are read while the step before
+// is multiplied, since one wave a SIMD (256 accumulators with MT = 2) has nobody to cover for it.
+template <bool GATED, int PA, int PB, int MT> struct Tile {
+    static constexpr int NS = PA + PB - 1, TM = 64 * MT, PIECES = PA * 2 * MT + PB * 4, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * 128) * 32;
+    v16i acc[NS][MT][2];
+    __device__ __forceinline__ void multiply(const ProductArgs& g, uint32_t m0, uint32_t n0, int8_t* const (&buf)[4]) {
+        const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) acc[s][m][q][r] = 0;
+        // The wave's pieces of a step: 32 rows of a plane each, x's first.  A weight's rows beyond the last read the last, a plane that it has not reads zeros.
+        const int8_t* src[SHARE];              // the same for all lanes, as is the step
+        uint32_t at[SHARE], dst[SHARE];
+        size_t step[SHARE];
+        const uint32_t lr = lane >> 1, lane_half = gemm_half(lr, lane & 1u) * 16;      // every piece begins at a multiple of 32 rows
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+            const uint32_t c = min(wave + 4 * i, (uint32_t)PIECES - 1);
+            if (c < PA * 2 * MT) {
+                const uint32_t plane = c / (2 * MT), r = c % (2 * MT) * 32;
+                src[i] = g.px + (size_t)plane * g.rows_padded * g.w.Kp + (size_t)(m0 + r) * 32;
+                at[i] = lr * 32 + lane_half;
+                dst[i] = (plane * TM + r) * 32;
+                step[i] = (size_t)g.rows_padded * 32;
+            } else {
+                const uint32_t cb = c - PA * 2 * MT, plane = cb >> 2, r = (cb & 3u) * 32, first = n0 + (GATED ? r & 63u : r);
+                const Planes& w = GATED && r < 64 ? g.gate : g.w;
+                const bool has = (int)plane < w.n, inside = first < w.rows;
+                src[i] = has ? w.p + (size_t)plane * w.rows * w.Kp + (size_t)(inside ? first : w.rows - 1) * 32 : g.zeros;
+                at[i] = (has && inside ? min(lr, w.rows - 1 - first) : 0u) * 32 + lane_half;
+                dst[i] = (PA * TM + plane * 128 + r) * 32;
+                step[i] = has ? (size_t)w.rows * 32 : 0;
+            }
+        }
+        const uint32_t half = lane >> 5, steps = g.w.Kp / 32;
+        const uint32_t rowA = wm * 32 * MT + (lane & 31), at_a = rowA * 32 + gemm_half(rowA, half) * 16;
+        const uint32_t rowB = wn * (GATED ? 32 : 64) + (lane & 31), next_b = GATED ? 64 : 32, at_b = (PA * TM + rowB) * 32 + gemm_half(rowB, half) * 16;      // 32 rows on: the same halves
+        auto fetch = [&](int8_t* to) {                         // the next step
+#pragma unroll
+            for (int i = 0; i < SHARE; ++i) { load_to_lds(src[i] + at[i], to + dst[i]); src[i] += step[i]; }
+        };
+        struct Fragments { v4i a[PA][MT], b[PB][2]; };
+        auto read = [&](const int8_t* from, Fragments& f) {
+#pragma unroll
+            for (int i = 0; i < PA; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; ++m) f.a[i][m] = *reinterpret_cast<const v4i*>(from + at_a + (i * TM + 32 * m) * 32);
+#pragma unroll
+            for (int j = 0; j < PB; ++j)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) f.b[j][q] = *reinterpret_cast<const v4i*>(from + at_b + (j * 128 + next_b * q) * 32);
+        };
+        auto products = [&](const Fragments& f) {
+#pragma unroll
+            for (int i = 0; i < PA; ++i)
+#pragma unroll
+                for (int j = 0; j < PB; ++j)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) acc[i + j][m][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i][m], f.b[j][q], acc[i + j][m][q], 0, 0, 0);
+        };
+        // the fragments' reads and the next loads spread over the products
+        auto spread = [&](bool fetches) {
+            constexpr int READS = PA * MT + PB * 2, PRODUCTS = PA * PB * MT * 2;
+            static_assert(PRODUCTS >= READS + SHARE, "a product for every read and load");
+#pragma unroll
+            for (int i = 0; i < READS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // an LDS read
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a matrix instruction
+            }
+            if (fetches) {
+#pragma unroll
+                for (int i = 0; i < SHARE; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // a load
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                }
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+        };
+        // Everybody's share of a step is in LDS when no more than `younger` steps' loads of a wave's own are on their way and all waves are past the barrier; with no LDS
+        // read on its way either (lgkmcnt 0), the buffer read last is free for the next fetch.
+        auto arrived = [&](auto younger) {
+            constexpr int N = decltype(younger)::value * SHARE;
+            __builtin_amdgcn_sched_barrier(0);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        const std::integral_constant<int, 0> none;
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> two;
+        const std::integral_constant<int, 3> three;
+        Fragments even, odd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) fetch(buf[i]);
+        arrived(three);
+        read(buf[0], even);
+        for (uint32_t t = 4; t < steps; t += 4) {              // Kp is a multiple of 128: four steps or more
+            arrived(two); fetch(buf[0]); read(buf[1], odd); products(even); spread(true);
+            arrived(two); fetch(buf[1]); read(buf[2], even); products(odd); spread(true);
+            arrived(two); fetch(buf[2]); read(buf[3], odd); products(even); spread(true);
+            arrived(two); fetch(buf[3]); read(buf[0], even); products(odd); spread(true);
+        }
+        arrived(two); read(buf[1], odd); products(even); spread(false);
+        arrived(one); read(buf[2], even); products(odd); spread(false);
+        arrived(none); read(buf[3], odd); products(even); spread(false);
+        products(odd);
+        __syncthreads();                                       // a next tile's loads find buffers that nobody reads any more
+    }
+    __device__ __forceinline__ void finish(const ProductArgs& g, uint32_t m0, uint32_t n0, uint32_t& bad) {
+        const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const uint32_t row = m0 + (wm * MT + m) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+                int64_t v[2];
+                uint32_t off = 0;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    int32_t a[NS];
+#pragma unroll
+                    for (int s = 0; s < NS; ++s) a[s] = acc[s][m][q][r];
+                    v[q] = joined<NS>(a, off);
+                }
+                if constexpr (GATED) {
+                    const uint32_t col = n0 + wn * 32 + (lane & 31);
+                    if (row < g.rows && col < g.cols) {
+                        g.e.out[(size_t)row * g.cols + col] = gated_value(v[0], v[1], g.e, off);
+                        bad |= off;
+                    }
+                } else {
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const uint32_t col = n0 + wn * 64 + q * 32 + (lane & 31);
+                        if (row < g.rows && col < g.cols) {
+                            uint32_t one = 0;
+                            g.e.out[(size_t)row * g.cols + col] = narrow(quotient_any(v[q], g.e.sf), one);
+                            bad |= one | off;
+                        }
+                    }
+                }
+            }
+    }
+};
+template <bool GATED, int PB, int MT> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
+    constexpr int BYTES = Tile<GATED, 3, PB, MT>::BYTES > Tile<GATED, 4, PB, 1>::BYTES ? Tile<GATED, 3, PB, MT>::BYTES : Tile<GATED, 4, PB, 1>::BYTES;
+    // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
+    __shared__ __attribute__((aligned(16))) int8_t s0[BYTES], s1[BYTES], s2[BYTES], s3[BYTES];
+    // Workgroups go to the eight dies in turn: a die takes a run of tiles in groups of eight rows of them, which share operands in its L2
+    uint32_t tm = blockIdx.y, tn = blockIdx.x;
+    {
+        const uint32_t nx = gridDim.x, ny = gridDim.y, total = nx * ny, id = blockIdx.y * nx + blockIdx.x;
+        if ((total & 7u) == 0 && total >= 64) {
+            const uint32_t lin = (id & 7u) * (total >> 3) + (id >> 3), group = lin / (8 * nx), first = group * 8, rows = ny - first < 8 ? ny - first : 8u, in = lin - group * 8 * nx;
+            tm = first + in % rows;
+            tn = in / rows;
+        }
+    }
+    const uint32_t m0 = tm * 64 * MT, n0 = tn * (GATED ? 64 : 128);
+    uint32_t need = 0, bad = 0;
+    for (uint32_t i = threadIdx.x & 63u; i < 2 * MT * g.chunks; i += 64) need = max(need, g.need[(size_t)(m0 / 32) * g.chunks + i]);
+    const bool wide = __any(need > 3);
+    int8_t* const buf[4] = {s0, s1, s2, s3};
+    if (!wide) {
+        Tile<GATED, 3, PB, MT> t;
+        t.multiply(g, m0, n0, buf);
+        t.finish(g, m0, n0, bad);
+    } else {                                   // a value of more than three digits: all four planes, 64 rows at a time
+        for (uint32_t m = m0; m < m0 + 64 * MT; m += 64) {
+            Tile<GATED, 4, PB, 1> t;
+            t.multiply(g, m, n0, buf);
+            t.finish(g, m, n0, bad);
+        }
+    }
+    raise(g.e.flag, bad);
+}
+
+// Few rows: the weights are read once and nothing else counts.  A workgroup takes 16 columns (of each weight), its waves the units of 64 contraction bytes in
+// turn, straight from memory into the fragments of v_mfma_i32_16x16x64_i8 -- a fragment of 16 columns is two pieces of 512 bytes in the planes' layout.  x is
+// split on the way, all four digits (the matrix cores idle anyway).  The waves' accumulators are added up in LDS, integers in any order.
+template <bool GATED, int PB, int RT> __global__ void __launch_bounds__(512) k_product_few(const ProductArgs g) {
+    constexpr int MATS = GATED ? 2 : 1, NS = 4 + PB - 1, WAVES = 8, DEPTH = RT == 1 ? 4 : 2;
+    __shared__ int32_t sum[NS * MATS * RT][256];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4;
+    const uint32_t units = g.w.Kp / 64, col = min(blockIdx.x * 16 + c, g.cols - 1);
+    for (uint32_t i = threadIdx.x; i < NS * MATS * RT * 256; i += 512) (&sum[0][0])[i] = 0;
+    const int8_t* src[MATS][PB];
+    const Planes* mats[2] = {GATED ? &g.gate : &g.w, &g.w};
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int j = 0; j < PB; ++j)
+            src[m][j] = mats[m]->p + (size_t)(j < mats[m]->n ? j : 0) * mats[m]->rows * g.w.Kp + ((size_t)(q >> 1) * g.cols + col) * 32 + (q & 1u) * 16;
+    v4i acc[NS][MATS][RT];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[s][m][r] = v4i{0, 0, 0, 0};
+    v4i w[DEPTH][MATS][PB];
+    int32_t x[DEPTH][RT][16];
+    uint32_t bad = 0;
+    auto load = [&](uint32_t u, int d) {
+        u = min(u, units - 1);                 // behind the last one that again: never multiplied
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int j = 0; j < PB; ++j) w[d][m][j] = *reinterpret_cast<const v4i*>(src[m][j] + (size_t)u * 2 * g.cols * 32);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) row_piece(g, r * 16 + c, u * 64 + q * 16, x[d][r]);
     };
-    for (uint32_t k = 0; k < g.inner; ++k) if (x[k] > 0x7F7F7F7F) bad |= ZK_VALUES_RANGE;
-    const int64_t v = dot(g.w);
-    int32_t y;
-    if constexpr (GATED) y = gated_value(dot(g.gate), v, g.e, bad);
-    else y = narrow(quotient_any(v, g.e.sf), bad);
-    g.e.out[(size_t)row * g.cols + col] = y;
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) load(wave + d * WAVES, d);
+    for (uint32_t u0 = wave; u0 < units; u0 += DEPTH * WAVES)
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const uint32_t u = u0 + d * WAVES;
+            if (u < units) {
+                const v4i zero = {0, 0, 0, 0};
+#pragma unroll
+                for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                    for (int j = 1; j < PB; ++j)
+                        if (j >= mats[m]->n) w[d][m][j] = zero;
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    v4i a[4];
+                    digit_planes(x[d][r], a, bad);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < PB; ++j)
+#pragma unroll
+                            for (int m = 0; m < MATS; ++m) acc[i + j][m][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], w[d][m][j], acc[i + j][m][r], 0, 0, 0);
+                }
+            }
+            load(u + DEPTH * WAVES, d);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m)
+#pragma unroll
+            for (int r = 0; r < RT; ++r)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) atomicAdd(&sum[(s * MATS + m) * RT + r][(4 * q + e) * 16 + c], acc[s][m][r][e]);      // row 4 q + e, column c
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < RT * 256; i += 512) {
+        const uint32_t r = i >> 8, row = i >> 4, out_col = blockIdx.x * 16 + (i & 15u);
+        if (row >= g.rows || out_col >= g.cols) continue;
+        int64_t v[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            int32_t a[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) a[s] = sum[(s * MATS + m) * RT + r][i & 255u];
+            v[m] = joined<NS>(a, bad);
+        }
+        int32_t y;
+        if constexpr (GATED) y = gated_value(v[0], v[1], g.e, bad);
+        else y = narrow(quotient_any(v[0], g.e.sf), bad);
+        g.e.out[(size_t)row * g.cols + out_col] = y;
+    }
     raise(g.e.flag, bad);
 }
 
@@ -329,6 +669,20 @@ static int check_weight(const MatmulRhs* w, const char* name) {
 }
 static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->planes, w->P, w->Kp, w->pb}; }
 
+static constexpr uint32_t FEW_ROWS = 32;
+static size_t padded_rows(uint32_t rows) { return ((size_t)rows + 127) / 128 * 128; }
+template <bool GATED, int PB> static void launch_few(const ProductArgs& g, hipStream_t st) {
+    if (g.rows <= 16) hipLaunchKernelGGL((k_product_few<GATED, PB, 1>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
+    else hipLaunchKernelGGL((k_product_few<GATED, PB, 2>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
+}
+template <bool GATED, int PB> static void launch_many(const ProductArgs& g, hipStream_t st) {
+    const unsigned tn = cdiv(g.cols, GATED ? 64 : 128);
+    if constexpr (PB == 2) if ((size_t)tn * cdiv(g.rows, 128) >= 256) {
+        hipLaunchKernelGGL((k_product<GATED, PB, 2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
+        return;
+    }
+    hipLaunchKernelGGL((k_product<GATED, PB, 1>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
+}
 template <bool GATED> static int product(const char* name, ProductArgs& g, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
     ZK_ARG(g.x != nullptr && g.e.out != nullptr, std::string(name) + ": null tensor");
     ZK_ARG(g.ldx >= g.inner, std::string(name) + ": rows of x overlap (ldx below the inner dimension)");
@@ -337,7 +691,31 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, void*
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
     g.e.flag = flag.dev;
-    hipLaunchKernelGGL(k_product_plain<GATED>, dim3(cdiv(g.cols, 64), cdiv(g.rows, 4)), dim3(256), 0, st, g);
+    g.x_aligned = (g.ldx & 3) == 0 && ((uintptr_t)g.x & 15) == 0;
+    const int pb = std::max(g.w.n, GATED ? g.gate.n : 0);
+    if (g.rows <= FEW_ROWS) {
+        if (pb <= 2) launch_few<GATED, 2>(g, st);
+        else launch_few<GATED, 3>(g, st);
+        ZK_LAUNCH_CHECK();
+        return flag.end(name);
+    }
+    const size_t bytes = zk_i32_linear_workspace(g.rows, g.inner);
+    std::unique_ptr<Scratch> own;
+    if (!workspace) {
+        if (const int rc = CallFlag::not_captured(st, name)) return rc;
+        own.reset(new Scratch(bytes, st));
+        if (own->rc) return own->rc;
+        workspace = own->p;
+    }
+    ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
+    g.rows_padded = padded_rows(g.rows);
+    g.chunks = cdiv(g.w.Kp, CHUNK);
+    g.px = (const int8_t*)workspace;
+    g.zeros = g.px + (size_t)4 * g.rows_padded * g.w.Kp;
+    g.need = (const uint32_t*)(g.zeros + 1024);
+    hipLaunchKernelGGL(k_split_x, dim3(cdiv(g.chunks, 4), g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
+    if (pb <= 2) launch_many<GATED, 2>(g, st);
+    else launch_many<GATED, 3>(g, st);
     ZK_LAUNCH_CHECK();
     return flag.end(name);
 }
@@ -435,7 +813,8 @@ int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, v
 }
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner) {
     const size_t Kp = ((size_t)inner + GBK - 1) / GBK * GBK;
-    return (size_t)rows * Kp * 4 + (((size_t)rows + 127) / 128 * 4 + 255) / 256 * 256;
+    if (rows <= FEW_ROWS) return 0;
+    return padded_rows(rows) * Kp * 4 + 1024 + padded_rows(rows) / 32 * ((Kp + CHUNK - 1) / CHUNK) * 4;
 }
 int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, uint32_t rows, uint32_t sf, void* workspace, size_t workspace_bytes, void* flag_dev, void* stv) {
     const MatmulRhs* w = (const MatmulRhs*)prepared;
