@@ -510,7 +510,7 @@ int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size
 int zk_i32_rhs_prepare(void** prepared, const void* B_i32, uint32_t N, uint32_t P, void* stream);
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner);
 /* A projection with its rescaling (zkfc.cu:44-58, rescaling.cu:13-19): out = q(x W), rows x P int32.  x: rows of N int32, ldx apart, each at most 0x7F7F7F7F; out
- * overlaps nothing that is read.  At most 262144 rows. */
+ * overlaps nothing that is read.  At most 262144 rows and 4194304 columns. */
 int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, uint32_t rows, uint32_t sf, void* workspace, size_t workspace_bytes, void* flag_dev, void* stream);
 /* The gated half of a feed-forward block (ffn.cu:61-73): out = q_hidden(act[q_gate(x G)] * q_up(x U)), act[v] = table[v - low] of len int32.  Both weights have one shape. */
 int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared, const void* up_prepared, uint32_t rows, uint32_t sf_gate, uint32_t sf_up, const void* table_i32,

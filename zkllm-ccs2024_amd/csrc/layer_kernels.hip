@@ -43,9 +43,8 @@ template <bool POW2> __device__ __forceinline__ int64_t quotient(int64_t t, cons
     if constexpr (POW2) return (t + d.half) >> d.shift;
     else return quotient_general(t, d);
 }
-__device__ __forceinline__ int64_t quotient_any(int64_t t, const Divisor& d) { return d.shift >= 0 ? (t + d.half) >> d.shift : quotient_general(t, d); }
 __device__ __forceinline__ int32_t narrow(int64_t v, uint32_t& bad) {
-    bad |= (v != (int64_t)(int32_t)v) ? (uint32_t)ZK_VALUES_RANGE : 0u;
+    bad |= (int32_t)(v >> 32) != ((int32_t)v >> 31) ? (uint32_t)ZK_VALUES_RANGE : 0u;
     return (int32_t)v;
 }
 __device__ __forceinline__ void raise(uint32_t* flag, uint32_t bad) { if (bad) atomicOr(flag, bad); }
@@ -91,8 +90,112 @@ template <bool POW2> __device__ __forceinline__ int32_t normed(int32_t w, int32_
     return narrow(quotient<POW2>((int64_t)g * v, sf), bad);
 }
 
-// A workgroup a row; lanes own columns threadIdx.x, threadIdx.x + blockDim.x, ...; every pass reads the row again.  A lane writes only columns that
-// it alone reads, so h and n may be x or b themselves.
+// A workgroup a row, VEC neighbouring columns NV times in each lane's registers: every tensor is read once and written once, which is what
+// bounds it.
+template <int VEC> __device__ __forceinline__ void row_load(int32_t (&v)[VEC], const int32_t* p) {
+    if constexpr (VEC == 4) {
+        const v4i q = *reinterpret_cast<const v4i*>(p);
+        v[0] = q[0]; v[1] = q[1]; v[2] = q[2]; v[3] = q[3];
+    } else v[0] = *p;
+}
+template <int VEC> __device__ __forceinline__ void row_store(int32_t* p, const int32_t (&v)[VEC]) {
+    if constexpr (VEC == 4) *reinterpret_cast<v4i*>(p) = v4i{v[0], v[1], v[2], v[3]};
+    else *p = v[0];
+}
+template <int NV, int VEC, bool POW2, int THREADS> __global__ void __launch_bounds__(THREADS) k_residual_norm(const NormArgs a) {
+    extern __shared__ double term[];           // blockDim.x * VEC
+    __shared__ unsigned long long red_s[16];
+    __shared__ uint32_t red_m[16];
+    __shared__ double total;
+    const size_t row = blockIdx.x;
+    const uint32_t stride = blockDim.x * VEC, first = threadIdx.x * VEC;
+    uint32_t bad = 0;
+    auto load = [&](int32_t (&v)[NV][VEC], const int32_t* p) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (first + i * stride < a.cols) row_load<VEC>(v[i], p + first + i * stride);
+            else
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[i][e] = 0;
+        }
+    };
+    auto store = [&](int32_t* p, const int32_t (&v)[NV][VEC]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) if (first + i * stride < a.cols) row_store<VEC>(p + first + i * stride, v[i]);
+    };
+    auto statistic = [&](const int32_t (&v)[NV][VEC]) {
+        unsigned long long s = 0;
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int32_t x = v[i][e];
+                s += (unsigned long long)((int64_t)x * x);
+                m = max(m, x < 0 ? 0u - (uint32_t)x : (uint32_t)x);
+            }
+        block_sum_max(s, m, red_s, red_m);
+        if (sum_is_exact(s, m, a)) return rms_inverse((double)s / a.scale / a.scale, a);
+        double acc = 0.0;                      // in index order, a stretch of `stride` terms at a time
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const double x = (double)v[i][e] / a.scale;
+                term[first + e] = x * x;
+            }
+            __syncthreads();
+            if (threadIdx.x == 0 && i * stride < a.cols) {
+                const uint32_t cnt = min(a.cols - i * stride, stride);
+                for (uint32_t q = 0; q < cnt; ++q) acc += term[q];
+            }
+        }
+        if (threadIdx.x == 0) total = acc;
+        __syncthreads();
+        const double t = total;
+        __syncthreads();
+        return rms_inverse(t, a);
+    };
+    int32_t v[NV][VEC], w[NV][VEC];
+    load(v, a.x + row * a.ldx);
+    if (a.b) {
+        int32_t q[NV][VEC], post[NV][VEC], gate[NV][VEC];
+        load(q, a.b + row * a.ldb);
+        if (a.post) load(post, a.post);
+        if (a.gate) load(gate, a.gate + row / a.rows_per_gate * a.cols);
+        if (a.n) load(w, a.w);
+        if (a.post) {
+            const int32_t r = statistic(q);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) q[i][e] = normed<POW2>(post[i][e], r, q[i][e], a.sf, bad);
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                int32_t y = q[i][e];
+                if (a.gate) y = narrow(quotient<POW2>((int64_t)gate[i][e] * y, a.sf), bad);
+                v[i][e] = narrow((int64_t)v[i][e] + quotient<POW2>((int64_t)a.res * y, a.sf), bad);
+            }
+    } else if (a.n) load(w, a.w);
+    if (a.h) store(a.h + row * a.cols, v);
+    if (a.n || a.rms_inv) {
+        const int32_t r = statistic(v);
+        if (a.rms_inv && threadIdx.x == 0) a.rms_inv[row] = r;
+        if (a.n) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[i][e] = normed<POW2>(w[i][e], r, v[i][e], a.sf, bad);
+            store(a.n + row * a.cols, v);
+        }
+    }
+    raise(a.flag, bad);
+}
+// Rows too long for that: every pass reads the row again.  A lane writes only columns that it alone reads, so h and n may be x or b themselves.
 template <bool POW2> __global__ void __launch_bounds__(256) k_residual_norm_long(const NormArgs a) {
     __shared__ unsigned long long red_s[4];
     __shared__ uint32_t red_m[4];
@@ -182,20 +285,39 @@ __device__ __forceinline__ int64_t rope_get(const Fr* p, uint32_t& bad) {
 }
 __device__ __forceinline__ void rope_put(int32_t* p, int64_t v, uint32_t& bad) { *p = narrow(v, bad); }
 __device__ __forceinline__ void rope_put(Fr* p, int64_t v, uint32_t&) { *p = fr_from_i64(v); }
-// a lane a pair of the rotated part or an element of the rest
-template <typename T, bool POW2> __global__ void __launch_bounds__(256) k_rope(const RopeArgs a, uint64_t base, uint64_t end) {
-    const uint64_t id = base + (uint64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= end) return;
-    const uint32_t pairs = a.rot / 2, units = pairs + (a.dim - a.rot);
-    const uint64_t th = id / units;
-    const uint32_t u = (uint32_t)(id - th * units), token = (uint32_t)(th / a.heads), head = (uint32_t)(th - (uint64_t)token * a.heads);
+// A lane VEC pairs of the rotated part or VEC elements of the rest; the heads of a token read its angles from the caches.
+template <typename T, int VEC, bool POW2> __global__ void __launch_bounds__(256) k_rope(const RopeArgs a, uint32_t token0, uint32_t total) {
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x;
+    if (id >= total) return;
+    const uint32_t pairs = a.rot / 2, groups = pairs / VEC, units = groups + (a.dim - a.rot) / VEC;
+    const uint32_t th = id / units, u = id - th * units, t = th / a.heads, head = th - t * a.heads;
+    const size_t token = (size_t)token0 + t;
     const T* x = (const T*)a.x + token * a.x_token + head * a.x_head;
     T* out = (T*)a.out + token * a.out_token + head * a.out_head;
     const uint64_t pos = a.positions ? (uint64_t)(int64_t)a.positions[token] : (uint64_t)a.first + token;
     uint32_t bad = 0;
     if (pos >= a.table_rows) bad = ZK_VALUES_POSITION;
-    else if (u >= pairs) out[a.rot + (u - pairs)] = x[a.rot + (u - pairs)];
-    else {
+    else if (u >= groups) {
+        const uint32_t i = a.rot + (u - groups) * VEC;
+        if constexpr (VEC == 4) *reinterpret_cast<v4i*>(out + i) = *reinterpret_cast<const v4i*>(x + i);
+        else out[i] = x[i];
+    } else if constexpr (VEC == 4) {
+        const int2* cs = a.table + pos * pairs + 4 * u;
+        const v4i c0 = *reinterpret_cast<const v4i*>(cs), c1 = *reinterpret_cast<const v4i*>(cs + 2);
+        const uint32_t i0 = a.neighbours ? 8 * u : 4 * u, i1 = a.neighbours ? 8 * u + 4 : 4 * u + pairs;
+        const v4i p = *reinterpret_cast<const v4i*>(x + i0), q = *reinterpret_cast<const v4i*>(x + i1);
+        const int32_t x0[4] = {p[0], a.neighbours ? p[2] : p[1], a.neighbours ? q[0] : p[2], a.neighbours ? q[2] : p[3]};
+        const int32_t x1[4] = {a.neighbours ? p[1] : q[0], a.neighbours ? p[3] : q[1], a.neighbours ? q[1] : q[2], q[3]};
+        int32_t y0[4], y1[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int2 k = angle(make_int2(e < 2 ? c0[2 * e] : c1[2 * e - 4], e < 2 ? c0[2 * e + 1] : c1[2 * e - 3]), bad);
+            y0[e] = narrow(quotient<POW2>((int64_t)k.x * x0[e] - (int64_t)k.y * x1[e], a.sf), bad);
+            y1[e] = narrow(quotient<POW2>((int64_t)k.y * x0[e] + (int64_t)k.x * x1[e], a.sf), bad);
+        }
+        *reinterpret_cast<v4i*>(out + i0) = a.neighbours ? v4i{y0[0], y1[0], y0[1], y1[1]} : v4i{y0[0], y0[1], y0[2], y0[3]};
+        *reinterpret_cast<v4i*>(out + i1) = a.neighbours ? v4i{y0[2], y1[2], y0[3], y1[3]} : v4i{y1[0], y1[1], y1[2], y1[3]};
+    } else {
         const int2 cs = angle(a.table[pos * pairs + u], bad);
         const uint32_t i0 = a.neighbours ? 2 * u : u, i1 = a.neighbours ? 2 * u + 1 : u + pairs;
         const int64_t x0 = rope_get(x + i0, bad), x1 = rope_get(x + i1, bad);
@@ -214,13 +336,16 @@ struct Epilogue {
     const int32_t* table;
     int64_t low;
     uint32_t len;
+    int pow2;                            // every divisor of the call is a power of two
     uint32_t* flag;
 };
-__device__ __forceinline__ int32_t gated_value(int64_t g, int64_t u, const Epilogue& e, uint32_t& bad) {
-    const int64_t at = quotient_any(g, e.sf_gate) - e.low;
-    if (at < 0 || at >= (int64_t)e.len) { bad |= ZK_VALUES_TABLE; return 0; }
-    const int32_t up = narrow(quotient_any(u, e.sf), bad);
-    return narrow(quotient_any((int64_t)e.table[at] * up, e.sf_hidden), bad);
+template <bool POW2> __device__ __forceinline__ uint32_t activation_at(int64_t g, const Epilogue& e, uint32_t& bad) {      // the place in the table, or the table's length
+    const uint64_t at = (uint64_t)(quotient<POW2>(g, e.sf_gate) - e.low);
+    bad |= at < e.len ? 0u : (uint32_t)ZK_VALUES_TABLE;
+    return at < e.len ? (uint32_t)at : e.len;
+}
+template <bool POW2> __device__ __forceinline__ int32_t gated_value(int32_t act, int64_t u, const Epilogue& e, uint32_t& bad) {
+    return narrow(quotient<POW2>((int64_t)act * narrow(quotient<POW2>(u, e.sf), bad), e.sf_hidden), bad);
 }
 // a weight's digit planes
 struct Planes { const int8_t* p; uint32_t rows, Kp; int n; };
@@ -237,18 +362,25 @@ struct ProductArgs {
     Epilogue e;
 };
 static constexpr uint32_t CHUNK = 256;
-// sum_s a[s] 256^s: below 2^62 in magnitude, or flagged and 0.  |a[s]| < 2^31, so the two low terms are below 2^41 together and the rest, in
-// units of 2^16, says whether the sum fits 64 bits.
+// sum_s a[s] 256^s: within -2^62 .. 2^62 - 1, or flagged and 0.  Six planes in all cannot leave that range: p digits hold 128 (256^p - 1) / 255 at most, and
+// 43690 products of three by three digits, or of four by two, stay below 2^61.5.
 template <int NS> __device__ __forceinline__ int64_t joined(const int32_t (&a)[NS], uint32_t& bad) {
-    int64_t lo = a[0], hi = 0;
-    if constexpr (NS > 1) lo += (int64_t)a[1] << 8;
+    if constexpr (NS <= 5) {
+        int64_t v = a[0];
 #pragma unroll
-    for (int s = 2; s < NS; ++s) hi += (int64_t)a[s] << (8 * (s - 2));
-    const int64_t limit = (1ll << 46) + (1ll << 25), most = 1ll << 62;
-    if (hi >= limit || hi <= -limit) { bad |= ZK_VALUES_RANGE; return 0; }
-    const int64_t v = hi * 65536 + lo;
-    if (v >= most || v <= -most) { bad |= ZK_VALUES_RANGE; return 0; }
-    return v;
+        for (int s = 1; s < NS; ++s) v += (int64_t)a[s] << (8 * s);
+        return v;
+    } else {
+        // |a[s]| < 2^31, so the two low terms are below 2^41 together, and the sum in units of 2^16, which the others' 2^56 leave room for, says whether it fits
+        const int64_t lo = a[0] + (int64_t)a[1] * 256;
+        int64_t hi = 0;
+#pragma unroll
+        for (int s = NS - 1; s >= 2; --s) hi = hi * 256 + a[s];
+        const int64_t units = hi + (lo >> 16);
+        const bool fits = (uint32_t)((int32_t)(units >> 32) + 0x4000) < 0x8000u;      // -2^46 .. 2^46 - 1
+        bad |= fits ? 0u : (uint32_t)ZK_VALUES_RANGE;
+        return fits ? (int64_t)((uint64_t)hi * 65536 + (uint64_t)lo) : 0;
+    }
 }
 // the digits of 16 values, plane by plane: plane j's 16 bytes in out[j]
 __device__ __forceinline__ void digit_planes(const int32_t (&x)[16], v4i (&out)[4], uint32_t& bad) {
@@ -270,8 +402,11 @@ __device__ __forceinline__ void digit_planes(const int32_t (&x)[16], v4i (&out)[
 }
 // 16 values of a row from column k on; zeros beyond the row's end and for rows that are none
 __device__ __forceinline__ void row_piece(const ProductArgs& g, uint32_t row, uint32_t k, int32_t (&x)[16]) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = 0;
+    if (row >= g.rows) return;
     const int32_t* p = g.x + row * g.ldx + k;
-    if (row < g.rows && g.x_aligned && k + 16 <= g.inner) {
+    if (g.x_aligned && k + 16 <= g.inner) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const v4i v = reinterpret_cast<const v4i*>(p)[w];
@@ -280,34 +415,37 @@ __device__ __forceinline__ void row_piece(const ProductArgs& g, uint32_t row, ui
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = (row < g.rows && k + e < g.inner) ? p[e] : 0;
+        for (int e = 0; e < 16; ++e) if (k + e < g.inner) x[e] = p[e];
     }
 }
 
-// x's planes for the products of many rows.  A wave takes 32 rows and CHUNK columns, 32 columns at a time: a lane 16 values of a row, so that the wave
-// writes 1 KB of every plane in one piece.  It notes how many planes its stretch needs, in a place of its own.
+// x's planes for the products of many rows.  A workgroup takes 32 rows and CHUNK columns, 32 columns of a wave's 64 at a time: a lane 16 values of a row, so that the
+// wave writes 1 KB of every plane in one piece.  How many planes the stretch needs goes to a place of its own.
 __global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __restrict__ planes, uint32_t* __restrict__ need, v4i* __restrict__ zeros) {
+    __shared__ uint32_t most[4];
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) zeros[threadIdx.x] = v4i{0, 0, 0, 0};
-    const uint32_t lane = threadIdx.x & 63u, chunk = blockIdx.x * 4 + (threadIdx.x >> 6), group = blockIdx.y;
-    if (chunk >= g.chunks) return;
-    const uint32_t row = group * 32 + (lane >> 1), h = lane & 1u, Kp = g.w.Kp;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.y * 32 + (lane >> 1), k0 = blockIdx.x * CHUNK + wave * 64 + 16 * (lane & 1u), Kp = g.w.Kp;
     uint32_t bad = 0, planes_needed = 1;
-    for (uint32_t k0 = chunk * CHUNK; k0 < min((chunk + 1) * CHUNK, Kp); k0 += 32) {
-        int32_t x[16];
+    int32_t x[2][16];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) row_piece(g, row, k0 + 32 * i, x[i]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (k0 + 32 * i >= Kp) break;          // Kp is a multiple of 128
         v4i d[4];
-        row_piece(g, row, k0 + 16 * h, x);
+        uint32_t m = 0;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const uint32_t m = (uint32_t)(x[e] < 0 ? ~x[e] : x[e]);      // p digits hold -128 (256^p - 1) / 255 .. 127 (256^p - 1) / 255
-            planes_needed = max(planes_needed, m <= 127u ? 1u : m <= 32639u ? 2u : m <= 8355711u ? 3u : 4u);
-        }
-        digit_planes(x, d, bad);
+        for (int e = 0; e < 16; ++e) m = max(m, (uint32_t)(x[i][e] < 0 ? ~x[i][e] : x[i][e]));
+        planes_needed = max(planes_needed, m <= 127u ? 1u : m <= 32639u ? 2u : m <= 8355711u ? 3u : 4u);      // p digits hold up to 127 (256^p - 1) / 255
+        digit_planes(x[i], d, bad);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<v4i*>(planes + (size_t)j * g.rows_padded * Kp + plane_at(g.rows_padded, row, k0 + 16 * h)) = d[j];
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<v4i*>(planes + (size_t)j * g.rows_padded * Kp + plane_at(g.rows_padded, row, k0 + 32 * i)) = d[j];
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) planes_needed = max(planes_needed, (uint32_t)__shfl_xor(planes_needed, off, 64));
-    if (lane == 0) need[(size_t)group * g.chunks + chunk] = planes_needed;
+    if (lane == 0) most[wave] = planes_needed;
+    __syncthreads();
+    if (threadIdx.x == 0) need[(size_t)blockIdx.y * g.chunks + blockIdx.x] = max(max(most[0], most[1]), max(most[2], most[3]));
     raise(g.e.flag, bad);
 }
 
@@ -355,9 +493,12 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
         const uint32_t half = lane >> 5, steps = g.w.Kp / 32;
         const uint32_t rowA = wm * 32 * MT + (lane & 31), at_a = rowA * 32 + gemm_half(rowA, half) * 16;
         const uint32_t rowB = wn * (GATED ? 32 : 64) + (lane & 31), next_b = GATED ? 64 : 32, at_b = (PA * TM + rowB) * 32 + gemm_half(rowB, half) * 16;      // 32 rows on: the same halves
-        auto fetch = [&](int8_t* to) {                         // the next step
+        uint32_t fetched = 1;
+        auto fetch = [&](int8_t* to) {                         // the next step; behind the last one that again, into buffers nobody reads any more
+            const size_t on = (size_t)(int64_t)__builtin_amdgcn_readfirstlane(fetched < steps ? -1 : 0);
+            ++fetched;
 #pragma unroll
-            for (int i = 0; i < SHARE; ++i) { load_to_lds(src[i] + at[i], to + dst[i]); src[i] += step[i]; }
+            for (int i = 0; i < SHARE; ++i) { load_to_lds(src[i] + at[i], to + dst[i]); src[i] += step[i] & on; }
         };
         struct Fragments { v4i a[PA][MT], b[PB][2]; };
         auto read = [&](const int8_t* from, Fragments& f) {
@@ -381,7 +522,7 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
                         for (int q = 0; q < 2; ++q) acc[i + j][m][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i][m], f.b[j][q], acc[i + j][m][q], 0, 0, 0);
         };
         // the fragments' reads and the next loads spread over the products
-        auto spread = [&](bool fetches) {
+        auto spread = [&] {
             constexpr int READS = PA * MT + PB * 2, PRODUCTS = PA * PB * MT * 2;
             static_assert(PRODUCTS >= READS + SHARE, "a product for every read and load");
 #pragma unroll
@@ -389,14 +530,12 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // an LDS read
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);      // a matrix instruction
             }
-            if (fetches) {
 #pragma unroll
-                for (int i = 0; i < SHARE; ++i) {
-                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // a load
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                }
+            for (int i = 0; i < SHARE; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);      // a load
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - READS - SHARE, 0);
         };
         // Everybody's share of a step is in LDS when no more than `younger` steps' loads of a wave's own are on their way and all waves are past the barrier; with no LDS
         // read on its way either (lgkmcnt 0), the buffer read last is free for the next fetch.
@@ -409,8 +548,6 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
             asm volatile("" ::: "memory");
             __builtin_amdgcn_sched_barrier(0);
         };
-        const std::integral_constant<int, 0> none;
-        const std::integral_constant<int, 1> one;
         const std::integral_constant<int, 2> two;
         const std::integral_constant<int, 3> three;
         Fragments even, odd;
@@ -418,55 +555,69 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
         for (int i = 0; i < 4; ++i) fetch(buf[i]);
         arrived(three);
         read(buf[0], even);
-        for (uint32_t t = 4; t < steps; t += 4) {              // Kp is a multiple of 128: four steps or more
-            arrived(two); fetch(buf[0]); read(buf[1], odd); products(even); spread(true);
-            arrived(two); fetch(buf[1]); read(buf[2], even); products(odd); spread(true);
-            arrived(two); fetch(buf[2]); read(buf[3], odd); products(even); spread(true);
-            arrived(two); fetch(buf[3]); read(buf[0], even); products(odd); spread(true);
+        for (uint32_t t = 0; t < steps; t += 4) {              // Kp is a multiple of 128
+            arrived(two); fetch(buf[0]); read(buf[1], odd); products(even); spread();
+            arrived(two); fetch(buf[1]); read(buf[2], even); products(odd); spread();
+            arrived(two); fetch(buf[2]); read(buf[3], odd); products(even); spread();
+            arrived(two); fetch(buf[3]); read(buf[0], even); products(odd); spread();
         }
-        arrived(two); read(buf[1], odd); products(even); spread(false);
-        arrived(one); read(buf[2], even); products(odd); spread(false);
-        arrived(none); read(buf[3], odd); products(even); spread(false);
-        products(odd);
+        __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);          // vmcnt 0: no load into LDS outlives the workgroup or meets a next tile's
         __syncthreads();                                       // a next tile's loads find buffers that nobody reads any more
     }
-    __device__ __forceinline__ void finish(const ProductArgs& g, uint32_t m0, uint32_t n0, uint32_t& bad) {
+    // The outputs, eight rows at a time: all their places in the table first, then the table's values, so that one wait covers them.  Stores go through a buffer
+    // that ends with the last row, and a column beyond the last has no place in it.  (Such a column repeats the last and a row beyond the last is zeros: of the flags only the
+    // table's needs to know.)
+    template <bool POW2> __device__ __forceinline__ void finish(const ProductArgs& g, uint32_t m0, uint32_t n0, uint32_t& bad) {
         const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
+        auto value = [&](int m, int q, int r) {
+            int32_t a[NS];
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const uint32_t row = m0 + (wm * MT + m) * 32 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-                int64_t v[2];
-                uint32_t off = 0;
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    int32_t a[NS];
-#pragma unroll
-                    for (int s = 0; s < NS; ++s) a[s] = acc[s][m][q][r];
-                    v[q] = joined<NS>(a, off);
-                }
-                if constexpr (GATED) {
-                    const uint32_t col = n0 + wn * 32 + (lane & 31);
-                    if (row < g.rows && col < g.cols) {
-                        g.e.out[(size_t)row * g.cols + col] = gated_value(v[0], v[1], g.e, off);
-                        bad |= off;
-                    }
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const uint32_t col = n0 + wn * 64 + q * 32 + (lane & 31);
-                        if (row < g.rows && col < g.cols) {
-                            uint32_t one = 0;
-                            g.e.out[(size_t)row * g.cols + col] = narrow(quotient_any(v[q], g.e.sf), one);
-                            bad |= one | off;
-                        }
-                    }
-                }
+            for (int s = 0; s < NS; ++s) {
+                a[s] = acc[s][m][q][r];
+                asm("" : "+v"(a[s]));          // row by row: the compiler joins 16 rows at a time otherwise and spills
             }
+            return joined<NS>(a, bad);
+        };
+        const uint32_t rows_here = m0 < g.rows ? min(g.rows - m0, (uint32_t)TM) : 0;
+        const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(g.e.out + (size_t)m0 * g.cols, 0, rows_here * g.cols * 4, 0x00027000);      // raw: plain bytes
+        auto store = [&](uint32_t row, uint32_t col, int32_t y) { __builtin_amdgcn_raw_buffer_store_b32(y, out, n0 + col < g.cols ? (row * g.cols + n0 + col) * 4 : 0xFFFFFFFFu, 0, 0); };
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const uint32_t row0 = (wm * MT + m) * 32 + 4 * (lane >> 5);
+            if constexpr (GATED) {
+                const uint32_t col = wn * 32 + (lane & 31);
+#pragma unroll
+                for (int r0 = 0; r0 < 16; r0 += 8) {
+                    uint32_t at[8];
+                    int32_t act[8];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        const uint32_t row = row0 + 8 * ((r0 + r) >> 2) + (r & 3);
+                        uint32_t off = 0;
+                        at[r] = activation_at<POW2>(value(m, 0, r0 + r), g.e, off);
+                        bad |= row < rows_here ? off : 0u;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) act[r] = g.e.table[min(at[r], g.e.len - 1)];
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        store(row0 + 8 * ((r0 + r) >> 2) + (r & 3), col, gated_value<POW2>(at[r] == g.e.len ? 0 : act[r], value(m, 1, r0 + r), g.e, bad));
+                    __builtin_amdgcn_sched_barrier(0);         // the next rows' values would only crowd the registers
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        store(row0 + 8 * (r >> 2) + (r & 3), wn * 64 + q * 32 + (lane & 31), narrow(quotient<POW2>(value(m, q, r), g.e.sf), bad));
+                        if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);      // the next rows' values would only crowd the registers
+                    }
+            }
+        }
     }
 };
-template <bool GATED, int PB, int MT> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
+// POW2: every divisor of the call is a power of two
+template <bool GATED, int PB, int MT, bool POW2> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
     constexpr int BYTES = Tile<GATED, 3, PB, MT>::BYTES > Tile<GATED, 4, PB, 1>::BYTES ? Tile<GATED, 3, PB, MT>::BYTES : Tile<GATED, 4, PB, 1>::BYTES;
     // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
     __shared__ __attribute__((aligned(16))) int8_t s0[BYTES], s1[BYTES], s2[BYTES], s3[BYTES];
@@ -488,12 +639,12 @@ template <bool GATED, int PB, int MT> __global__ void __launch_bounds__(256, MT 
     if (!wide) {
         Tile<GATED, 3, PB, MT> t;
         t.multiply(g, m0, n0, buf);
-        t.finish(g, m0, n0, bad);
+        t.template finish<POW2>(g, m0, n0, bad);
     } else {                                   // a value of more than three digits: all four planes, 64 rows at a time
         for (uint32_t m = m0; m < m0 + 64 * MT; m += 64) {
             Tile<GATED, 4, PB, 1> t;
             t.multiply(g, m, n0, buf);
-            t.finish(g, m, n0, bad);
+            t.template finish<POW2>(g, m, n0, bad);
         }
     }
     raise(g.e.flag, bad);
@@ -582,10 +733,14 @@ template <bool GATED, int PB, int RT> __global__ void __launch_bounds__(512) k_p
             for (int s = 0; s < NS; ++s) a[s] = sum[(s * MATS + m) * RT + r][i & 255u];
             v[m] = joined<NS>(a, bad);
         }
-        int32_t y;
-        if constexpr (GATED) y = gated_value(v[0], v[1], g.e, bad);
-        else y = narrow(quotient_any(v[0], g.e.sf), bad);
-        g.e.out[(size_t)row * g.cols + out_col] = y;
+        auto value = [&](auto pow2) {
+            constexpr bool POW2 = decltype(pow2)::value;
+            if constexpr (GATED) {
+                const uint32_t at = activation_at<POW2>(v[0], g.e, bad);
+                return gated_value<POW2>(at == g.e.len ? 0 : g.e.table[at], v[1], g.e, bad);
+            } else return narrow(quotient<POW2>(v[0], g.e.sf), bad);
+        };
+        g.e.out[(size_t)row * g.cols + out_col] = g.e.pow2 ? value(std::true_type()) : value(std::false_type());
     }
     raise(g.e.flag, bad);
 }
@@ -675,18 +830,19 @@ template <bool GATED, int PB> static void launch_few(const ProductArgs& g, hipSt
     if (g.rows <= 16) hipLaunchKernelGGL((k_product_few<GATED, PB, 1>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
     else hipLaunchKernelGGL((k_product_few<GATED, PB, 2>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
 }
-template <bool GATED, int PB> static void launch_many(const ProductArgs& g, hipStream_t st) {
+template <bool GATED, int PB, bool POW2> static void launch_many(const ProductArgs& g, hipStream_t st) {
     const unsigned tn = cdiv(g.cols, GATED ? 64 : 128);
     if constexpr (PB == 2) if ((size_t)tn * cdiv(g.rows, 128) >= 256) {
-        hipLaunchKernelGGL((k_product<GATED, PB, 2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((k_product<GATED, PB, 2, POW2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
         return;
     }
-    hipLaunchKernelGGL((k_product<GATED, PB, 1>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((k_product<GATED, PB, 1, POW2>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
 }
 template <bool GATED> static int product(const char* name, ProductArgs& g, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
     ZK_ARG(g.x != nullptr && g.e.out != nullptr, std::string(name) + ": null tensor");
     ZK_ARG(g.ldx >= g.inner, std::string(name) + ": rows of x overlap (ldx below the inner dimension)");
     ZK_ARG(g.rows <= (1u << 18), std::string(name) + ": more than 262144 rows in one call");
+    ZK_ARG(g.cols <= (1u << 22), std::string(name) + ": more than 4194304 columns");
     ZK_ARG(workspace == nullptr || workspace_bytes >= zk_i32_linear_workspace(g.rows, g.inner), std::string(name) + ": the workspace is smaller than zk_i32_linear_workspace says");
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
@@ -713,11 +869,27 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, void*
     g.px = (const int8_t*)workspace;
     g.zeros = g.px + (size_t)4 * g.rows_padded * g.w.Kp;
     g.need = (const uint32_t*)(g.zeros + 1024);
-    hipLaunchKernelGGL(k_split_x, dim3(cdiv(g.chunks, 4), g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
-    if (pb <= 2) launch_many<GATED, 2>(g, st);
-    else launch_many<GATED, 3>(g, st);
+    hipLaunchKernelGGL(k_split_x, dim3(g.chunks, g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
+    if (pb <= 2) { if (g.e.pow2) launch_many<GATED, 2, true>(g, st); else launch_many<GATED, 2, false>(g, st); }
+    else { if (g.e.pow2) launch_many<GATED, 3, true>(g, st); else launch_many<GATED, 3, false>(g, st); }
     ZK_LAUNCH_CHECK();
     return flag.end(name);
+}
+
+template <int NV, int VEC, bool POW2, int THREADS> static void launch_norm_n(const NormArgs& a, uint32_t rows, hipStream_t st) {
+    const unsigned threads = (unsigned)std::max<size_t>(64, ((size_t)cdiv(a.cols, NV * VEC) + 63) / 64 * 64);
+    hipLaunchKernelGGL((k_residual_norm<NV, VEC, POW2, THREADS>), dim3(rows), dim3(threads), threads * VEC * sizeof(double), st, a);
+}
+template <bool POW2> static void launch_norm(const NormArgs& a, uint32_t rows, hipStream_t st) {
+    auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
+    const bool vec = (a.cols & 3) == 0 && (a.ldx & 3) == 0 && (a.b == nullptr || (a.ldb & 3) == 0) && aligned(a.x) && aligned(a.b) && aligned(a.h) && aligned(a.n) && aligned(a.post) &&
+                     aligned(a.gate) && aligned(a.w);
+    if (vec && a.cols <= 4096 && (rows < 512 || a.cols <= 1024)) launch_norm_n<1, 4, POW2, 1024>(a, rows, st);
+    else if (vec && a.cols <= 4096) launch_norm_n<4, 4, POW2, 256>(a, rows, st);
+    else if (vec && a.cols <= 16384) launch_norm_n<4, 4, POW2, 1024>(a, rows, st);
+    else if (!vec && a.cols <= 1024) launch_norm_n<1, 1, POW2, 1024>(a, rows, st);
+    else if (!vec && a.cols <= 16384) launch_norm_n<16, 1, POW2, 1024>(a, rows, st);
+    else hipLaunchKernelGGL(k_residual_norm_long<POW2>, dim3(rows), dim3(256), 0, st, a);
 }
 
 extern "C" {
@@ -739,8 +911,8 @@ int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t 
     int e2 = 0;
     const NormArgs a{(int32_t*)h, (int32_t*)n, (int32_t*)rms_inv, (const int32_t*)x, (const int32_t*)b, (const int32_t*)post, (const int32_t*)gate, (const int32_t*)w, ldx, ldb, cols,
                      gate ? rows / gate_rows : 1, res, scale, eps, std::frexp(scale, &e2) == 0.5, divisor(sf), flag.dev};
-    if (a.sf.shift >= 0) hipLaunchKernelGGL(k_residual_norm_long<true>, dim3(rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_residual_norm_long<false>, dim3(rows), dim3(256), 0, st, a);
+    if (a.sf.shift >= 0) launch_norm<true>(a, rows, st);
+    else launch_norm<false>(a, rows, st);
     ZK_LAUNCH_CHECK();
     return flag.end("zk_i32_residual_norm");
 }
@@ -754,21 +926,28 @@ static int rope(const char* name, bool fr, void* out, size_t out_token, size_t o
     ZK_ARG(sf > 0 && sf <= (1u << 30), std::string(name) + ": the table's scale must be 1 .. 2^30");
     ZK_ARG(out != x || (out_token == x_token && out_head == x_head), std::string(name) + ": in place with other strides");
     ZK_ARG((tokens == 1 || (x_token >= dim && out_token >= dim)) && (heads == 1 || (x_head >= dim && out_head >= dim)), std::string(name) + ": heads overlap (a stride below the head's width)");
+    ZK_ARG((uint64_t)heads * dim <= (1u << 30), std::string(name) + ": more than 2^30 elements a token");
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
     const RopeArgs a{out, x, out_token, out_head, x_token, x_head, tokens, heads, dim, rot, neighbours, (const int2*)table, rot ? table_rows : 0xFFFFFFFFu, (const int32_t*)positions, first, divisor(sf), flag.dev};
-    const uint64_t total = (uint64_t)tokens * heads * (rot / 2 + (dim - rot)), step = 1ull << 30;
-    for (uint64_t base = 0; base < total; base += step) {
-        const uint64_t end = std::min(total, base + step);
-        const dim3 grid(cdiv(end - base, 256));
+    const bool vec = !fr && rot % 8 == 0 && dim % 4 == 0 && ((out_token | out_head | x_token | x_head) & 3) == 0 && (((uintptr_t)out | (uintptr_t)x | (uintptr_t)table) & 15) == 0;
+    const uint32_t units = heads * (vec ? rot / 8 + (dim - rot) / 4 : rot / 2 + (dim - rot));      // a token's
+    const uint32_t step = std::max(1u, (1u << 30) / units);
+    for (uint32_t t = 0; t < tokens; t += step) {
+        const uint32_t total = std::min(step, tokens - t) * units;
+        const dim3 grid(cdiv(total, 256)), block(256);
         if (fr) {
-            if (a.sf.shift >= 0) hipLaunchKernelGGL((k_rope<Fr, true>), grid, dim3(256), 0, st, a, base, end);
-            else hipLaunchKernelGGL((k_rope<Fr, false>), grid, dim3(256), 0, st, a, base, end);
+            if (a.sf.shift >= 0) hipLaunchKernelGGL((k_rope<Fr, 1, true>), grid, block, 0, st, a, t, total);
+            else hipLaunchKernelGGL((k_rope<Fr, 1, false>), grid, block, 0, st, a, t, total);
+        } else if (vec) {
+            if (a.sf.shift >= 0) hipLaunchKernelGGL((k_rope<int32_t, 4, true>), grid, block, 0, st, a, t, total);
+            else hipLaunchKernelGGL((k_rope<int32_t, 4, false>), grid, block, 0, st, a, t, total);
         } else {
-            if (a.sf.shift >= 0) hipLaunchKernelGGL((k_rope<int32_t, true>), grid, dim3(256), 0, st, a, base, end);
-            else hipLaunchKernelGGL((k_rope<int32_t, false>), grid, dim3(256), 0, st, a, base, end);
+            if (a.sf.shift >= 0) hipLaunchKernelGGL((k_rope<int32_t, 1, true>), grid, block, 0, st, a, t, total);
+            else hipLaunchKernelGGL((k_rope<int32_t, 1, false>), grid, block, 0, st, a, t, total);
         }
+        if (tokens - t <= step) break;
     }
     ZK_LAUNCH_CHECK();
     return flag.end(name);
@@ -823,7 +1002,7 @@ int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, ui
     if (rows == 0) return 0;
     ProductArgs g{};
     g.x = (const int32_t*)x; g.ldx = ldx; g.rows = rows; g.inner = w->N; g.cols = w->P; g.w = planes_of(w);
-    g.e.out = (int32_t*)out; g.e.sf = divisor(sf);
+    g.e.out = (int32_t*)out; g.e.sf = divisor(sf); g.e.pow2 = g.e.sf.shift >= 0;
     return product<false>("zk_i32_linear", g, flag_dev, workspace, workspace_bytes, (hipStream_t)stv);
 }
 int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared, const void* up_prepared, uint32_t rows, uint32_t sf_gate, uint32_t sf_up, const void* table, int32_t low,
@@ -838,6 +1017,7 @@ int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared
     ProductArgs g{};
     g.x = (const int32_t*)x; g.ldx = ldx; g.rows = rows; g.inner = w->N; g.cols = w->P; g.w = planes_of(w); g.gate = planes_of(gate);
     g.e.out = (int32_t*)out; g.e.sf = divisor(sf_up); g.e.sf_gate = divisor(sf_gate); g.e.sf_hidden = divisor(sf_hidden);
+    g.e.pow2 = g.e.sf.shift >= 0 && g.e.sf_gate.shift >= 0 && g.e.sf_hidden.shift >= 0;
     g.e.table = (const int32_t*)table; g.e.low = low; g.e.len = len;
     return product<true>("zk_i32_gated", g, flag_dev, workspace, workspace_bytes, (hipStream_t)stv);
 }
