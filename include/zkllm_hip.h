@@ -504,6 +504,13 @@ int zk_i32_rope(void* out, size_t out_token, size_t out_head, const void* x, siz
                 const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
 int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
                const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
+/* The table of angles: table[p][i] = the nearest integers to sf magnitude cos(p f_i) and sf magnitude sin(p f_i), p < rows, f_i = base^(-2 i / rot) / factor.
+ * original > 0 (long contexts): only what is slow is slowed down -- f_i that turns high times or more over `original` positions is left alone, one that turns low times
+ * or less divided by the factor, those between in proportion.  Double precision, correctly rounded operations in a fixed order: the same table everywhere. */
+int zk_rope_table(void* table_i32, uint32_t rows, uint32_t rot, double base, double factor, double original, double low, double high, double magnitude, uint32_t sf, void* stream);
+/* out[token][head][k] = q_second(q_first(in[head][token][k])): field elements that stand for integers up to 2^62 (attention's products with the values) to
+ * int32 with the two quotients of self-attn.cu:96-98; with one head and factors of 1 the int32 form of a tensor. */
+int zk_i32_from_heads(void* out_i32, const void* in, uint32_t heads, uint32_t tokens, uint32_t dim, uint32_t sf_first, uint32_t sf_second, void* flag_dev, void* stream);
 /* A weight laid out for zk_i32_linear and zk_i32_gated from its int32 form (N x P, on the device; not read afterwards): two or three bytes an element.  The handles
  * of zk_fr_matmul_rhs_prepare serve them as well; one made here has no field elements and serves no field product.  Elements up to 8355711 in magnitude, N at
  * most 43690.  Waits for the stream; released with zk_fr_matmul_rhs_free. */

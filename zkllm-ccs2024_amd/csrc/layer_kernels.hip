@@ -17,6 +17,7 @@
 #include <cstring>
 #include <memory>
 #include <type_traits>
+#include "detmath.hpp"
 #include "field.hpp"
 #include "planes.hpp"
 #include "rt.hpp"
@@ -325,6 +326,45 @@ template <typename T, int VEC, bool POW2> __global__ void __launch_bounds__(256)
         rope_put(out + i1, quotient<POW2>((int64_t)cs.y * (int32_t)x0 + (int64_t)cs.x * (int32_t)x1, a.sf), bad);
     }
     raise(a.flag, bad);
+}
+
+// The table of angles, a lane an entry: table[p][i] = the nearest integers to scale cos(p f_i), scale sin(p f_i), f_i = base^(-2 i / rot) slowed down by `factor` -- or, with
+// `original` positions, a frequency that turns `high` times or more over them stays, one that turns `low` times or less is slowed down, those between in proportion.
+// Correctly rounded operations in a fixed order (detmath.hpp): every device and host has the same table.
+struct RopeTableArgs { double base, factor, original, low, high, scale; };
+__global__ void __launch_bounds__(256) k_rope_table(int2* __restrict__ table, uint32_t rows, uint32_t pairs, const RopeTableArgs a) {
+    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= (size_t)rows * pairs) return;
+    const uint32_t p = (uint32_t)(id / pairs), i = (uint32_t)(id - (size_t)p * pairs);
+    double f = zkd::exp_det(-((double)i / (double)pairs) * zkd::log_det(a.base));
+    if (a.original > 0) {
+        const double turns = a.original * f / 6.283185307179586476925;
+        double keep = (turns - a.low) / (a.high - a.low);
+        keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+        f = f * (keep + (1.0 - keep) / a.factor);
+    } else f = f / a.factor;
+    double s, c;
+    zkd::sincos_det((double)p * f, &s, &c);
+    table[id] = make_int2((int32_t)rint(c * a.scale), (int32_t)rint(s * a.scale));
+}
+
+// ---- field elements that stand for integers, rescaled twice, from [head][token][dim] to int32 [token][head][dim] ------------------------------------------------
+__global__ void __launch_bounds__(256) k_i32_from_heads(int32_t* __restrict__ out, const Fr* __restrict__ in, uint32_t heads, uint32_t tokens, uint32_t dim, const Divisor first, const Divisor second,
+                                                        uint32_t* __restrict__ flag) {
+    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= (size_t)heads * tokens * dim) return;
+    const size_t row = id / dim;
+    const uint32_t j = (uint32_t)(id - row * dim);
+    const uint32_t token = (uint32_t)(row / heads), head = (uint32_t)(row - (size_t)token * heads);
+    const Fr e = in[((size_t)head * tokens + token) * dim + j];
+    int64_t v = fr_to_i64(e);
+    uint32_t bad = 0;
+    const bool zero = !(e.v[0] | e.v[1] | e.v[2] | e.v[3] | e.v[4] | e.v[5] | e.v[6] | e.v[7]);
+    if (v > (1ll << 62) || v < -(1ll << 62) || (v == 0 && !zero)) { bad = ZK_VALUES_RANGE; v = 0; }      // fr_to_i64 gives 0 for what does not fit 64 bits
+    v = first.shift >= 0 ? quotient<true>(v, first) : quotient<false>(v, first);
+    v = second.shift >= 0 ? quotient<true>(v, second) : quotient<false>(v, second);
+    out[id] = narrow(v, bad);
+    raise(flag, bad);
 }
 
 // ---- products with a kept weight -----------------------------------------------------------------------------------------------------------------
@@ -959,6 +999,31 @@ int zk_i32_rope(void* out, size_t out_token, size_t out_head, const void* x, siz
 int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
                const void* table, uint32_t table_rows, const void* positions, uint32_t first, uint32_t sf, void* flag_dev, void* stv) {
     return rope("zk_fr_rope", true, out, out_token, out_head, x, x_token, x_head, tokens, heads, dim, rot, neighbours, table, table_rows, positions, first, sf, flag_dev, stv);
+}
+
+int zk_rope_table(void* table, uint32_t rows, uint32_t rot, double base, double factor, double original, double low, double high, double magnitude, uint32_t sf, void* stv) {
+    if (rows == 0 || rot == 0) return 0;
+    ZK_ARG(table != nullptr && rot % 2 == 0, "zk_rope_table: null table or an odd part of the head");
+    ZK_ARG(base > 1 && base <= 1e15 && factor > 0 && factor >= 1e-6 && factor <= 1e6, "zk_rope_table: the base must lie above 1 (up to 1e15), the factor within 1e-6 .. 1e6");
+    ZK_ARG(original == 0 || (original > 0 && original <= 1e15 && low >= 0 && high > low && high <= 1e15), "zk_rope_table: with original positions, 0 <= low < high");
+    ZK_ARG(sf > 0 && magnitude > 0 && magnitude * (double)sf <= 1073741824.0, "zk_rope_table: scale times magnitude must lie within 2^30");
+    hipLaunchKernelGGL(k_rope_table, dim3(cdiv((size_t)rows * (rot / 2), 256)), dim3(256), 0, (hipStream_t)stv, (int2*)table, rows, rot / 2,
+                       RopeTableArgs{base, factor, original, low, high, magnitude * (double)sf});
+    ZK_LAUNCH_CHECK();
+    return 0;
+}
+int zk_i32_from_heads(void* out, const void* in, uint32_t heads, uint32_t tokens, uint32_t dim, uint32_t sf_first, uint32_t sf_second, void* flag_dev, void* stv) {
+    const size_t n = (size_t)heads * tokens * dim;
+    if (n == 0) return 0;
+    ZK_ARG(out != nullptr && in != nullptr && out != in, "zk_i32_from_heads: null tensor or in place");
+    ZK_ARG(sf_first > 0 && sf_second > 0, "zk_i32_from_heads: a scaling factor of 0");
+    ZK_ARG((n + 255) / 256 <= 0x7FFFFFFFu, "zk_i32_from_heads: too many elements in one call");
+    hipStream_t st = (hipStream_t)stv;
+    CallFlag flag;
+    if (const int rc = flag.begin(flag_dev, st, "zk_i32_from_heads")) return rc;
+    hipLaunchKernelGGL(k_i32_from_heads, dim3(cdiv(n, 256)), dim3(256), 0, st, (int32_t*)out, (const Fr*)in, heads, tokens, dim, divisor(sf_first), divisor(sf_second), flag.dev);
+    ZK_LAUNCH_CHECK();
+    return flag.end("zk_i32_from_heads");
 }
 
 int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, void* stv) {

@@ -4,7 +4,8 @@
 //         temp_head_out.bin (int32) and leaves the output file alone.
 //         With ZKLLM_ATTN_HEADS=H in the environment (an addition) the attention is proved for H heads of width
 //         embed_dim / H instead, ZKLLM_ATTN_HEAD_GROUP=g of them at a time as one stack (0 or unset: head by head), and the
-//         concatenated, twice rescaled result goes to temp_head_out.bin and to the output file.
+//         concatenated, twice rescaled result goes to temp_head_out.bin and to the output file.  rope_base and its like in ZKLLM_LAYER_CONFIG
+//         (layer.hpp) give the heads' queries and keys their rotary positions first.
 #include <cstdlib>
 #include <string>
 #include "layer.hpp"

@@ -20,6 +20,7 @@
 #include "zkrelu.hpp"
 #include "zksoftmax.hpp"
 #include "layer.hpp"
+#include "values.hpp"
 
 typedef uint32_t u32;
 static thread_local std::string g_err;
@@ -623,6 +624,33 @@ void* zkp_layer_run(void* h, void* X, double* times_ms) {
     FrTensor out = llama_layer(s.cfg, s.w, FT(X), &t);
     if (times_ms) { times_ms[0] = t.rmsnorm1; times_ms[1] = t.qkv; times_ms[2] = t.attention; times_ms[3] = t.oproj; times_ms[4] = t.rmsnorm2; times_ms[5] = t.ffn; times_ms[6] = t.total; times_ms[7] = t.open_wait; }
     return new FrTensor(std::move(out));
+    ZKP_END_PTR
+}
+
+// rotary positions of the layer's queries and keys: base (0: none), factor, original, low, high, magnitude; the rotated part of a head, neighbours, first position, scale
+void zkp_layer_set_rope(void* h, const double* f6, const u32* u4) {
+    RopeConfig& r = reinterpret_cast<LayerState*>(h)->cfg.rope;
+    r.base = f6[0]; r.factor = f6[1]; r.original = f6[2]; r.low = f6[3]; r.high = f6[4]; r.magnitude = f6[5];
+    r.dim = u4[0]; r.neighbours = u4[1] != 0; r.first = u4[2]; r.scale = u4[3];
+}
+// the layer's output without a proof (LayerValues); repeats: how many times it is computed with what the object has laid out once, ms (may be null) receives the last one's time
+void* zkp_layer_values(void* h, void* X, int repeats, double* ms) {
+    ZKP_TRY
+    LayerState& s = *reinterpret_cast<LayerState*>(h);
+    const LayerValues values(s.cfg, s.w);
+    const IntTensor x(FT(X));
+    for (int i = 1; i < repeats; ++i) (void)values(x);
+    zk_check(zk_sync(nullptr), "zk_sync");
+    const auto t0 = std::chrono::steady_clock::now();
+    const IntTensor out = values(x);          // ends with a wait of its own
+    if (ms) *ms = std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
+    return new FrTensor(out.to_fr());
+    ZKP_END_PTR
+}
+// attention of the layer's heads with its proof (attn_heads_block), as the self-attn executable runs it
+void* zkp_layer_attention(void* h, void* Q, void* K, void* V) {
+    ZKP_TRY
+    return new FrTensor(attn_heads_block(reinterpret_cast<LayerState*>(h)->cfg, FT(Q), FT(K), FT(V)));
     ZKP_END_PTR
 }
 

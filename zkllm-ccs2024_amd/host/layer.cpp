@@ -84,6 +84,16 @@ void layer_config_from_env(LayerConfig& c) {
         else if (key == "softmax_thetas") c.softmax_thetas = list();
         else if (key == "value_scale") c.value_scale = std::stod(val);
         else if (key == "rms_eps") c.rms_eps = std::stod(val);
+        else if (key == "rope_base") c.rope.base = std::stod(val);
+        else if (key == "rope_dim") c.rope.dim = (uint)std::stoul(val);
+        else if (key == "rope_neighbours") c.rope.neighbours = std::stoul(val) != 0;
+        else if (key == "rope_factor") c.rope.factor = std::stod(val);
+        else if (key == "rope_original") c.rope.original = std::stod(val);
+        else if (key == "rope_low") c.rope.low = std::stod(val);
+        else if (key == "rope_high") c.rope.high = std::stod(val);
+        else if (key == "rope_magnitude") c.rope.magnitude = std::stod(val);
+        else if (key == "rope_first") c.rope.first = (uint)std::stoul(val);
+        else if (key == "rope_scale") c.rope.scale = (uint)std::stoul(val);
         else throw std::runtime_error("ZKLLM_LAYER_CONFIG: unknown key " + key);
     }
 }
@@ -232,8 +242,14 @@ const FrTensor& AttnStackBlock::forward() {
     const uint seq = c.seq_len, E = c.embed_dim, H = c.num_heads, d = E / H;
     // seq x embed -> embed x seq = [head][d][seq] -> [head][seq][d]
     auto to_stack = [&](const FrTensor& t) { return t.swap_leading_axes(seq, H, d); };          // = t.transpose(seq, E).transpose_stack(H, d, seq)
-    Qs.emplace(to_stack(Q_));
-    Ks.emplace(to_stack(K_));
+    if (c.rope.base > 0) {      // the positions on the way to the stack
+        rotary.emplace(c.rope, seq, d);
+        Qs.emplace((*rotary)(Q_, H, true));
+        Ks.emplace((*rotary)(K_, H, true));
+    } else {
+        Qs.emplace(to_stack(Q_));
+        Ks.emplace(to_stack(K_));
+    }
     Vs.emplace(to_stack(V_));
     sm_in.emplace(H * seq * seq);
     sm_out.emplace(H * seq * seq);
@@ -261,6 +277,7 @@ void AttnStackBlock::queue() {
     p2 = rs2.prove_begin(*out_all, *out_, ch_r2);
 }
 void AttnStackBlock::finish() {
+    if (rotary) { rotary->check(); rotary.reset(); }
     vector<Polynomial> proof;
     attn.prove_finish(pending, *Qs, *Ks, *Vs, *out, *sm_out, *sm_in, *shift, in_seg, out_seg, ch.u_matmul_out_num, ch.v_matmul_out_num, ch.u_matmul_out, ch.v_matmul_out,
                       ch.w_matmul_out, ch.v_sm, ch.v_matmul_in_num, ch.v_matmul_in, proof);
@@ -281,6 +298,14 @@ FrTensor attn_heads_block(const LayerConfig& c, const FrTensor& Q_, const FrTens
         b.begin();
         b.finish();
         return std::move(*b.out__);
+    }
+    if (c.rope.base > 0) {
+        Rotary rotary(c.rope, seq, d);
+        const FrTensor Qr = rotary(Q_, H, false), Kr = rotary(K_, H, false);
+        rotary.check();
+        LayerConfig rotated = c;
+        rotated.rope.base = 0;
+        return attn_heads_block(rotated, Qr, Kr, V_);
     }
     if (c.attn_head_group) {
         FrTensor out_all = attn_stacked_heads(c, Q_, K_, V_);
@@ -385,6 +410,7 @@ FrTensor attn_heads_block(const LayerConfig& c, const FrTensor& Q_, const FrTens
 FrTensor attn_reference_block(const LayerConfig& c, const FrTensor& Q, const FrTensor& K, const FrTensor& V, std::unique_ptr<FrTensor>* softmax_out) {
     const uint seq_len = c.seq_len;
     if (seq_len == 0 || Q.size % seq_len || K.size != Q.size || V.size != Q.size) throw std::runtime_error("attn: Q, K, V must be seq_len x d");
+    if (c.rope.base > 0) throw std::runtime_error("attn: rotary positions need heads (ZKLLM_ATTN_HEADS); as one head the reference's statement has none");
     const uint d = Q.size / seq_len;
     auto X = FrTensor::matmul(Q, K.transpose(seq_len, d), seq_len, d, seq_len);
     zkSoftmax softmax(c.softmax_bs, c.softmax_L, c.softmax_M, c.softmax_sf_in, c.softmax_thetas, seq_len, seq_len, d, 1);

@@ -13,14 +13,16 @@
 //  * an output projection (zkFC + rescaling + weight opening) follows, which the reference lacks;
 //  * challenges that the reference draws inside function-argument lists (unspecified order in C++) are
 //    drawn into named variables, first argument first;
-//  * RoPE, the causal mask and the RMS statistic are the reference's unproven float steps; RoPE and the
-//    mask are left out, the RMS statistic is computed on the host in double precision.
+//  * RoPE, the causal mask and the RMS statistic are the reference's unproven float steps; the mask is left out, the RMS
+//    statistic is computed on the host in double precision.  RoPE is left out unless LayerConfig::rope has a base: then the queries and keys
+//    of the heads are rotated in whole numbers behind their projections (rotary.hpp), a step that nothing proves, as in the reference.
 #pragma once
 #include <memory>
 #include <optional>
 #include "commitment.hpp"
 #include "fr-tensor.hpp"
 #include "rescaling.hpp"
+#include "rotary.hpp"
 #include "tlookup.hpp"
 #include "zkfc.hpp"
 #include "zksoftmax.hpp"
@@ -42,11 +44,13 @@ struct LayerConfig {
     bool open_weights = true;     // run verifyWeightClaim for every weight claim
     uint attn_head_group = 0;     // 0: every head proved on its own (the flow of self-attn.cu:78-121 per head); g > 0 (a divisor of
                                   // num_heads): heads proved g at a time as head-major stacks with zkAttnStacked (zksoftmax.cu:289-320)
+    RopeConfig rope;              // rotary positions of the queries and keys; none by default
 };
 
 // The executables use the reference's constants (the defaults above).  ZKLLM_LAYER_CONFIG in the environment replaces any
 // of them, e.g. "sf_linear=256,sf_gate=1024,sf_attn=128,softmax_bs=256:256:256,softmax_sf_in=65536,softmax_thetas=64:256":
-// a lookup table cannot be larger than the tensor it serves, so shapes far below the 7B layer need smaller tables.
+// a lookup table cannot be larger than the tensor it serves, so shapes far below the 7B layer need smaller tables.  Positions: rope_base, rope_dim,
+// rope_neighbours, rope_factor, rope_original, rope_low, rope_high, rope_magnitude, rope_first, rope_scale (RopeConfig).
 void layer_config_from_env(LayerConfig& c);
 
 struct LayerWeights {
@@ -116,6 +120,7 @@ struct AttnStackBlock {
     const LayerConfig& c; const FrTensor &Q_, &K_, &V_;
     zkAttnStacked attn;
     Rescaling rs1, rs2;
+    std::optional<Rotary> rotary;
     std::optional<FrTensor> Qs, Ks, Vs, sm_in, sm_out, shift, out, out_all, out_, out__;      // out__: the output
     vector<FrTensor> in_seg, out_seg, m_seg;
     zkAttnStacked::Challenges ch;
