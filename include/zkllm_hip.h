@@ -481,7 +481,7 @@ int zk_softmax_shift_decompose_i64(void* shift, void* out_shifted, void* const* 
  * flag_dev: 4 bytes of device memory, raised (bits are added, never cleared) when a value does not fit: the caller clears it before its first call and
  * reads it (zk_memcpy_d2h) when it is through; outputs then hold anything at the places concerned.  flag_dev null: the call waits for its kernels
  * and returns the error.
- * workspace: zk_i32_linear_workspace bytes (none for 32 rows or fewer) of device memory, 16-byte aligned, that no other call uses meanwhile, or null: the library takes it from its allocator
+ * workspace: zk_i32_linear_workspace bytes (none for four rows or fewer) of device memory, 16-byte aligned, that no other call uses meanwhile, or null: the library takes it from its allocator
  * for the time of the call.  A call that is captured into a graph needs both of the caller's. */
 #define ZK_VALUES_RANGE 1u        /* a result or an intermediate value outside int32, or a sum of products of 2^62 or more */
 #define ZK_VALUES_TABLE 2u        /* an activation outside the table of function values; the output is 0 there */

@@ -510,7 +510,7 @@ def test_handles_from_field_elements_serve_both_and_those_from_int32_no_field_pr
     with pytest.raises(RuntimeError, match="different shapes"):
         call_gated(hip, dev, x, of_i32, Weight(hip, dev, w[:, :29]), 30, 1, 1, np.zeros(4), 0, 1)
     with pytest.raises(RuntimeError, match="workspace is smaller"):
-        hip.call("zk_i32_linear", C, dev.up(x), c_size_t(40), of_i32.h, c_uint(33), c_uint(1), C, c_size_t(100), dev.flag(), None)      # 33 rows: 32 need none
+        hip.call("zk_i32_linear", C, dev.up(x), c_size_t(40), of_i32.h, c_uint(33), c_uint(1), C, c_size_t(100), dev.flag(), None)      # 33 rows need more; up to four need none
 
 
 # ---- as a program calls them: on a stream of its own, captured, one after the other -------------------------------------------------------------------------

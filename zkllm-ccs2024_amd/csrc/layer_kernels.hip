@@ -690,98 +690,126 @@ template <bool GATED, int PB, int MT, bool POW2> __global__ void __launch_bounds
     raise(g.e.flag, bad);
 }
 
-// Few rows: the weights are read once and nothing else counts.  A workgroup takes 16 columns (of each weight), its waves the units of 64 contraction bytes in
-// turn, straight from memory into the fragments of v_mfma_i32_16x16x64_i8 -- a fragment of 16 columns is two pieces of 512 bytes in the planes' layout.  x is
-// split on the way, all four digits (the matrix cores idle anyway).  The waves' accumulators are added up in LDS, integers in any order.
-template <bool GATED, int PB, int RT> __global__ void __launch_bounds__(512) k_product_few(const ProductArgs g) {
-    constexpr int MATS = GATED ? 2 : 1, NS = 4 + PB - 1, WAVES = 8, DEPTH = RT == 1 ? 4 : 2;
-    __shared__ int32_t sum[NS * MATS * RT][256];
-    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4;
-    const uint32_t units = g.w.Kp / 64, col = min(blockIdx.x * 16 + c, g.cols - 1);
-    for (uint32_t i = threadIdx.x; i < NS * MATS * RT * 256; i += 512) (&sum[0][0])[i] = 0;
-    const int8_t* src[MATS][PB];
-    const Planes* mats[2] = {GATED ? &g.gate : &g.w, &g.w};
-#pragma unroll
-    for (int m = 0; m < MATS; ++m)
-#pragma unroll
-        for (int j = 0; j < PB; ++j)
-            src[m][j] = mats[m]->p + (size_t)(j < mats[m]->n ? j : 0) * mats[m]->rows * g.w.Kp + ((size_t)(q >> 1) * g.cols + col) * 32 + (q & 1u) * 16;
-    v4i acc[NS][MATS][RT];
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
+// Few rows, or few tiles: the weights' way out of memory is what counts.  A workgroup takes 16 columns (of each weight) and 16 RT rows, its waves the units of 64 contraction
+// bytes in turn, straight from memory into the fragments of v_mfma_i32_16x16x64_i8 -- a fragment of 16 columns is two pieces of 512 bytes in the planes' layout.
+// SPLIT: x is split on the way, all four digits (one launch, and the matrix cores idle anyway); else its planes are read as the weights' are.  The waves'
+// accumulators are added up in LDS, integers in any order.
+template <bool GATED, int PB, int RT, int PA, bool SPLIT, int WAVES, int DEPTH> struct Strip {
+    static constexpr int MATS = GATED ? 2 : 1, NS = PA + PB - 1, SUMS = NS * MATS * RT;
+    static __device__ __forceinline__ void run(const ProductArgs& g, uint32_t strip, uint32_t row_block, int32_t (*sum)[256], uint32_t& bad) {
+        const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4;
+        const uint32_t units = g.w.Kp / 64, col = min(strip * 16 + c, g.cols - 1), row0 = row_block * 16 * RT;
+        for (uint32_t i = threadIdx.x; i < SUMS * 256; i += WAVES * 64) (&sum[0][0])[i] = 0;
+        const int8_t* src[MATS][PB];
+        const Planes* mats[2] = {GATED ? &g.gate : &g.w, &g.w};
 #pragma unroll
         for (int m = 0; m < MATS; ++m)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) acc[s][m][r] = v4i{0, 0, 0, 0};
-    v4i w[DEPTH][MATS][PB];
-    int32_t x[DEPTH][RT][16];
-    uint32_t bad = 0;
-    auto load = [&](uint32_t u, int d) {
-        u = min(u, units - 1);                 // behind the last one that again: never multiplied
+            for (int j = 0; j < PB; ++j)
+                src[m][j] = mats[m]->p + (size_t)(j < mats[m]->n ? j : 0) * mats[m]->rows * g.w.Kp + ((size_t)(q >> 1) * g.cols + col) * 32 + (q & 1u) * 16;
+        const int8_t* px = g.px + ((size_t)(q >> 1) * g.rows_padded + row0 + c) * 32 + (q & 1u) * 16;
+        const size_t w_step = (size_t)g.cols * 64, x_step = (size_t)g.rows_padded * 64, x_plane = (size_t)g.rows_padded * g.w.Kp;
+        v4i acc[NS][MATS][RT];
 #pragma unroll
-        for (int m = 0; m < MATS; ++m)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int j = 0; j < PB; ++j) w[d][m][j] = *reinterpret_cast<const v4i*>(src[m][j] + (size_t)u * 2 * g.cols * 32);
+            for (int m = 0; m < MATS; ++m)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) row_piece(g, r * 16 + c, u * 64 + q * 16, x[d][r]);
-    };
+                for (int r = 0; r < RT; ++r) acc[s][m][r] = v4i{0, 0, 0, 0};
+        v4i w[DEPTH][MATS][PB], a[DEPTH][SPLIT ? 1 : RT][SPLIT ? 4 : PA];
+        int32_t x[DEPTH][SPLIT ? RT : 1][16];
+        auto load = [&](uint32_t u, int d) {
+            u = min(u, units - 1);             // behind the last one that again: never multiplied
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) load(wave + d * WAVES, d);
-    for (uint32_t u0 = wave; u0 < units; u0 += DEPTH * WAVES)
+            for (int m = 0; m < MATS; ++m)
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) {
-            const uint32_t u = u0 + d * WAVES;
-            if (u < units) {
-                const v4i zero = {0, 0, 0, 0};
+                for (int j = 0; j < PB; ++j) w[d][m][j] = *reinterpret_cast<const v4i*>(src[m][j] + u * w_step);
 #pragma unroll
-                for (int m = 0; m < MATS; ++m)
+            for (int r = 0; r < RT; ++r) {
+                if constexpr (SPLIT) row_piece(g, row0 + r * 16 + c, u * 64 + q * 16, x[d][r]);
+                else
 #pragma unroll
-                    for (int j = 1; j < PB; ++j)
-                        if (j >= mats[m]->n) w[d][m][j] = zero;
-#pragma unroll
-                for (int r = 0; r < RT; ++r) {
-                    v4i a[4];
-                    digit_planes(x[d][r], a, bad);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < PB; ++j)
-#pragma unroll
-                            for (int m = 0; m < MATS; ++m) acc[i + j][m][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i], w[d][m][j], acc[i + j][m][r], 0, 0, 0);
-                }
+                    for (int i = 0; i < PA; ++i) a[d][r][i] = *reinterpret_cast<const v4i*>(px + i * x_plane + u * x_step + r * 512);
             }
-            load(u + DEPTH * WAVES, d);
-        }
-    __syncthreads();
-#pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int m = 0; m < MATS; ++m)
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) atomicAdd(&sum[(s * MATS + m) * RT + r][(4 * q + e) * 16 + c], acc[s][m][r][e]);      // row 4 q + e, column c
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < RT * 256; i += 512) {
-        const uint32_t r = i >> 8, row = i >> 4, out_col = blockIdx.x * 16 + (i & 15u);
-        if (row >= g.rows || out_col >= g.cols) continue;
-        int64_t v[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) {
-            int32_t a[NS];
-#pragma unroll
-            for (int s = 0; s < NS; ++s) a[s] = sum[(s * MATS + m) * RT + r][i & 255u];
-            v[m] = joined<NS>(a, bad);
-        }
-        auto value = [&](auto pow2) {
-            constexpr bool POW2 = decltype(pow2)::value;
-            if constexpr (GATED) {
-                const uint32_t at = activation_at<POW2>(v[0], g.e, bad);
-                return gated_value<POW2>(at == g.e.len ? 0 : g.e.table[at], v[1], g.e, bad);
-            } else return narrow(quotient<POW2>(v[0], g.e.sf), bad);
         };
-        g.e.out[(size_t)row * g.cols + out_col] = g.e.pow2 ? value(std::true_type()) : value(std::false_type());
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) load(wave + d * WAVES, d);
+        for (uint32_t u0 = wave; u0 < units; u0 += DEPTH * WAVES)
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const uint32_t u = u0 + d * WAVES;
+                if (u < units) {
+                    const v4i zero = {0, 0, 0, 0};
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                        for (int j = 1; j < PB; ++j)
+                            if (j >= mats[m]->n) w[d][m][j] = zero;
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) {
+                        if constexpr (SPLIT) digit_planes(x[d][r], a[d][0], bad);
+#pragma unroll
+                        for (int i = 0; i < PA; ++i)
+#pragma unroll
+                            for (int j = 0; j < PB; ++j)
+#pragma unroll
+                                for (int m = 0; m < MATS; ++m)
+                                    acc[i + j][m][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[d][SPLIT ? 0 : r][i], w[d][m][j], acc[i + j][m][r], 0, 0, 0);
+                    }
+                }
+                load(u + DEPTH * WAVES, d);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+#pragma unroll
+                for (int r = 0; r < RT; ++r)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) atomicAdd(&sum[(s * MATS + m) * RT + r][(4 * q + e) * 16 + c], acc[s][m][r][e]);      // row 4 q + e, column c
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < RT * 256; i += WAVES * 64) {
+            const uint32_t r = i >> 8, row = row0 + (i >> 4), out_col = strip * 16 + (i & 15u);
+            if (row >= g.rows || out_col >= g.cols) continue;
+            int64_t v[MATS];
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) {
+                int32_t t[NS];
+#pragma unroll
+                for (int s = 0; s < NS; ++s) t[s] = sum[(s * MATS + m) * RT + r][i & 255u];
+                v[m] = joined<NS>(t, bad);
+            }
+            auto value = [&](auto pow2) {
+                constexpr bool POW2 = decltype(pow2)::value;
+                if constexpr (GATED) {
+                    const uint32_t at = activation_at<POW2>(v[0], g.e, bad);
+                    return gated_value<POW2>(at == g.e.len ? 0 : g.e.table[at], v[1], g.e, bad);
+                } else return narrow(quotient<POW2>(v[0], g.e.sf), bad);
+            };
+            g.e.out[(size_t)row * g.cols + out_col] = g.e.pow2 ? value(std::true_type()) : value(std::false_type());
+        }
     }
+};
+template <bool GATED, int PB> __global__ void __launch_bounds__(512) k_product_row(const ProductArgs g) {
+    using S = Strip<GATED, PB, 1, 4, true, 8, 4>;
+    __shared__ int32_t sum[S::SUMS][256];
+    uint32_t bad = 0;
+    S::run(g, blockIdx.x, 0, sum, bad);
+    raise(g.e.flag, bad);
+}
+template <bool GATED, int PB, int RT> __global__ void __launch_bounds__(512) k_product_strip(const ProductArgs g, uint32_t row_blocks) {
+    constexpr int WAVES = 8, DEPTH = RT == 1 ? 4 : 2;
+    using Three = Strip<GATED, PB, RT, 3, false, WAVES, DEPTH>;
+    using Four = Strip<GATED, PB, RT, 4, false, WAVES, DEPTH>;
+    __shared__ int32_t sum[Four::SUMS][256];
+    // workgroups go to the eight dies in turn: a strip's row blocks follow each other on one die, whose L2 has its weights then
+    const uint32_t slot = blockIdx.x >> 3, strip = slot / row_blocks * 8 + (blockIdx.x & 7u), row_block = slot % row_blocks;
+    if (strip * 16 >= g.cols) return;
+    uint32_t need = 0, bad = 0;
+    for (uint32_t i = threadIdx.x & 63u; i < g.chunks; i += 64) need = max(need, g.need[(size_t)row_block * g.chunks + i]);
+    if (!__any(need > 3)) Three::run(g, strip, row_block, sum, bad);
+    else Four::run(g, strip, row_block, sum, bad);
     raise(g.e.flag, bad);
 }
 
@@ -864,19 +892,24 @@ static int check_weight(const MatmulRhs* w, const char* name) {
 }
 static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->planes, w->P, w->Kp, w->pb}; }
 
-static constexpr uint32_t FEW_ROWS = 32;
+static constexpr uint32_t SPLIT_ROWS = 4;
+static constexpr size_t FEW_TILES = 80;
 static size_t padded_rows(uint32_t rows) { return ((size_t)rows + 127) / 128 * 128; }
-template <bool GATED, int PB> static void launch_few(const ProductArgs& g, hipStream_t st) {
-    if (g.rows <= 16) hipLaunchKernelGGL((k_product_few<GATED, PB, 1>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
-    else hipLaunchKernelGGL((k_product_few<GATED, PB, 2>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
-}
-template <bool GATED, int PB, bool POW2> static void launch_many(const ProductArgs& g, hipStream_t st) {
+template <bool GATED, int PB, bool POW2> static void launch_tiles(const ProductArgs& g, hipStream_t st) {
     const unsigned tn = cdiv(g.cols, GATED ? 64 : 128);
     if constexpr (PB == 2) if ((size_t)tn * cdiv(g.rows, 128) >= 256) {
         hipLaunchKernelGGL((k_product<GATED, PB, 2, POW2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
         return;
     }
     hipLaunchKernelGGL((k_product<GATED, PB, 1, POW2>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
+}
+template <bool GATED, int PB> static void launch_product(const ProductArgs& g, hipStream_t st) {
+    const unsigned row_blocks = cdiv(g.rows, 32), strips = (cdiv(g.cols, 16) + 7) / 8 * 8;
+    if (g.rows <= 16) hipLaunchKernelGGL((k_product_strip<GATED, PB, 1>), dim3(strips), dim3(512), 0, st, g, 1u);
+    else if (g.rows <= 32 || (size_t)cdiv(g.cols, GATED ? 64 : 128) * cdiv(g.rows, 64) < FEW_TILES)
+        hipLaunchKernelGGL((k_product_strip<GATED, PB, 2>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
+    else if (g.e.pow2) launch_tiles<GATED, PB, true>(g, st);
+    else launch_tiles<GATED, PB, false>(g, st);
 }
 template <bool GATED> static int product(const char* name, ProductArgs& g, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
     ZK_ARG(g.x != nullptr && g.e.out != nullptr, std::string(name) + ": null tensor");
@@ -889,9 +922,9 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, void*
     g.e.flag = flag.dev;
     g.x_aligned = (g.ldx & 3) == 0 && ((uintptr_t)g.x & 15) == 0;
     const int pb = std::max(g.w.n, GATED ? g.gate.n : 0);
-    if (g.rows <= FEW_ROWS) {
-        if (pb <= 2) launch_few<GATED, 2>(g, st);
-        else launch_few<GATED, 3>(g, st);
+    if (g.rows <= SPLIT_ROWS) {
+        if (pb <= 2) hipLaunchKernelGGL((k_product_row<GATED, 2>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
+        else hipLaunchKernelGGL((k_product_row<GATED, 3>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
         ZK_LAUNCH_CHECK();
         return flag.end(name);
     }
@@ -910,8 +943,8 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, void*
     g.zeros = g.px + (size_t)4 * g.rows_padded * g.w.Kp;
     g.need = (const uint32_t*)(g.zeros + 1024);
     hipLaunchKernelGGL(k_split_x, dim3(g.chunks, g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
-    if (pb <= 2) { if (g.e.pow2) launch_many<GATED, 2, true>(g, st); else launch_many<GATED, 2, false>(g, st); }
-    else { if (g.e.pow2) launch_many<GATED, 3, true>(g, st); else launch_many<GATED, 3, false>(g, st); }
+    if (pb <= 2) launch_product<GATED, 2>(g, st);
+    else launch_product<GATED, 3>(g, st);
     ZK_LAUNCH_CHECK();
     return flag.end(name);
 }
@@ -1057,7 +1090,7 @@ int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, v
 }
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner) {
     const size_t Kp = ((size_t)inner + GBK - 1) / GBK * GBK;
-    if (rows <= FEW_ROWS) return 0;
+    if (rows <= SPLIT_ROWS) return 0;
     return padded_rows(rows) * Kp * 4 + 1024 + padded_rows(rows) / 32 * ((Kp + CHUNK - 1) / CHUNK) * 4;
 }
 int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, uint32_t rows, uint32_t sf, void* workspace, size_t workspace_bytes, void* flag_dev, void* stv) {
