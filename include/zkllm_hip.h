@@ -498,7 +498,7 @@ int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t 
  *   (x0, x1) -> (q(c x0 - s x1), q(s x0 + c x1)),   (c, s) = table[p][i], q: the quotient by sf, the table's scale (1 .. 2^30);
  * the rest is copied.  neighbours: pair i is (2 i, 2 i + 1), else (i, i + rot / 2).  table: table_rows * (rot / 2) pairs of int32 up to 2^30 in magnitude.  positions: one int32 a
  * token, or null: first, first + 1, ...  Strides in elements from token to token and from head to head, heads of dim contiguous elements; out may be x with the same
- * strides, and overlaps it in no other way.  The strides out of place are free: a stack [head][token][dim] is written as easily as [token][head][dim].
+ * strides, and overlaps it in no other way.  Out of place the output's strides are its own: a stack [head][token][dim] is written as easily as [token][head][dim].
  * zk_fr_rope: the same for field elements that stand for 32-bit integers (any other raises the flag and counts as 0). */
 int zk_i32_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
                 const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
@@ -513,7 +513,7 @@ int zk_rope_table(void* table_i32, uint32_t rows, uint32_t rot, double base, dou
 int zk_i32_from_heads(void* out_i32, const void* in, uint32_t heads, uint32_t tokens, uint32_t dim, uint32_t sf_first, uint32_t sf_second, void* flag_dev, void* stream);
 /* A weight laid out for zk_i32_linear and zk_i32_gated from its int32 form (N x P, on the device; not read afterwards): two or three bytes an element.  The handles
  * of zk_fr_matmul_rhs_prepare serve them as well; one made here has no field elements and serves no field product.  Elements up to 8355711 in magnitude, N at
- * most 43690.  Waits for the stream; released with zk_fr_matmul_rhs_free. */
+ * most 43690, P at most 4194304.  Waits for the stream; released with zk_fr_matmul_rhs_free once its last call is through. */
 int zk_i32_rhs_prepare(void** prepared, const void* B_i32, uint32_t N, uint32_t P, void* stream);
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner);
 /* A projection with its rescaling (zkfc.cu:44-58, rescaling.cu:13-19): out = q(x W), rows x P int32.  x: rows of N int32, ldx apart, each at most 0x7F7F7F7F; out

@@ -142,6 +142,20 @@ def test_norm_outputs_left_out(hip, dev, want, cols):
     same(got, *ref.residual_norm(x, b, w=w))
 
 
+@gpu
+def test_norm_of_more_rows_than_a_launch_takes(hip, dev):
+    rows = 2 * ((1 << 20) + 3)
+    rng = np.random.default_rng(1)
+    x, b, w, gate = normal(rng, (rows, 2)), normal(rng, (rows, 2)), normal(rng, 2), normal(rng, (rows // 2, 2))
+    got, flag = call_norm(hip, dev, x, b, None, gate, 65536, w)
+    h = x.astype(np.int64) + ref.quotient(np.repeat(gate.astype(np.int64), 2, 0) * b, 65536)
+    r = np.rint(1.0 / np.sqrt((h.astype(np.float64) / 65536) [:, 0] ** 2 / 2 + (h.astype(np.float64) / 65536)[:, 1] ** 2 / 2 + 1e-5) * 65536)      # two squares below 2^50: no sum rounds
+    assert flag == 0 and (got["h"] == h).all() and (np.abs(got["r"] - r) <= 1).all()
+    some = np.concatenate([np.arange(5), np.arange((1 << 20) - 3, (1 << 20) + 3), np.arange(rows - 5, rows)])
+    exp = ref.residual_norm(h[some], w=w)
+    assert (got["n"][some] == exp[1]).all() and (got["r"][some] == exp[2]).all()
+
+
 # strides that break the alignment of rows, and the outputs in the inputs' place
 @gpu
 @pytest.mark.parametrize("cols,ldx,ldb", [(64, 65, 64), (64, 68, 72), (1000, 1003, 1001), (4096, 4100, 4097)])
@@ -513,6 +527,35 @@ def test_handles_from_field_elements_serve_both_and_those_from_int32_no_field_pr
         hip.call("zk_i32_linear", C, dev.up(x), c_size_t(40), of_i32.h, c_uint(33), c_uint(1), C, c_size_t(100), dev.flag(), None)      # 33 rows need more; up to four need none
 
 
+@gpu
+def test_calls_on_two_streams_without_workspaces_of_the_callers(hip, dev):
+    """Handles made on one stream and used on others at once, the library's own scratch memory in every call: each result is its own"""
+    import torch
+    rng = np.random.default_rng(6)
+    w = [normal(rng, (300, 500), 3000.0) for _ in range(2)]
+    handles, streams, x, out, flags = [], [torch.cuda.Stream() for _ in range(4)], [], [], []
+    for i, s in enumerate(streams):
+        h, p = c_void_p(), dev.up(w[i % 2])
+        hip.sync()
+        hip.call("zk_i32_rhs_prepare", ctypes.byref(h), p, c_uint(300), c_uint(500), c_void_p(s.cuda_stream))
+        handles.append(h)
+        rows = [3, 20, 50, 200][i]
+        x.append(normal(rng, (rows, 300)))
+        out.append(dev.space(4 * rows * 500))
+        flags.append(dev.flag())
+    px = [dev.up(a) for a in x]
+    hip.sync()
+    for turn in range(5):
+        for i in range(4):
+            hip.call("zk_i32_linear", out[i], px[i], c_size_t(300), handles[(i + turn) % 4], c_uint(len(x[i])), c_uint(65536), None, c_size_t(0), flags[i], c_void_p(streams[(i * 3 + turn) % 4].cuda_stream))
+        torch.cuda.synchronize()
+        for i in range(4):
+            assert (dev.down(out[i], (len(x[i]), 500)) == ref.linear(x[i], w[(i + turn) % 4 % 2], 65536)).all()
+            assert dev.down(flags[i], (1,), np.uint32)[0] == 0
+    for h in handles:
+        hip.lib.zk_fr_matmul_rhs_free(h)
+
+
 # ---- as a program calls them: on a stream of its own, captured, one after the other -------------------------------------------------------------------------
 def _step(hip, torch, s, stream):
     """one block: the residual stream and its norm, positions for the queries, a projection, the gated product and the way down; every buffer is the caller's"""
@@ -623,7 +666,7 @@ W = (ctypes.c_int32 * 64)()
 @pytest.mark.parametrize("change,text", [
     ({"x": None}, "null x"), ({"cols": 0}, "empty rows"), ({"h": None, "n": None, "r": None}, "no output"), ({"w": None}, "needs a weight"), ({"ldx": 3}, "rows overlap"), ({"ldb": 3}, "rows overlap"),
     ({"b": None}, "needs the block's output"), ({"gate": None}, "gate_rows"), ({"gate_rows": 0}, "gate_rows"), ({"gate_rows": 4}, "gate_rows"), ({"sf": 0}, "scaling factor of 0"),
-    ({"eps": 0.0}, "positive"), ({"eps": float("nan")}, "positive"), ({"scale": -1.0}, "positive"), ({"scale": float("inf")}, "positive"), ({"eps": 1e-10}, "below 2^31"), ({"rows": 0x80000000, "gate_rows": 1}, "too many rows")])
+    ({"eps": 0.0}, "positive"), ({"eps": float("nan")}, "positive"), ({"scale": -1.0}, "positive"), ({"scale": float("inf")}, "positive"), ({"eps": 1e-10}, "below 2^31")])
 def test_norm_refusals(change, text):
     a = {"h": W, "n": W, "r": W, "x": W, "ldx": 4, "b": W, "ldb": 4, "post": W, "gate": W, "gate_rows": 2, "res": 1, "w": W, "rows": 6, "cols": 4, "eps": 1e-5, "scale": 65536.0, "sf": 65536}
     a.update(change)
@@ -634,7 +677,8 @@ def test_norm_refusals(change, text):
 @pytest.mark.parametrize("name", ["zk_i32_rope", "zk_fr_rope"])
 @pytest.mark.parametrize("change,text", [
     ({"out": None}, "null tensor"), ({"x": None}, "null tensor"), ({"dim": 0, "rot": 0}, "empty heads"), ({"rot": 10}, "within the head"), ({"rot": 3}, "even"), ({"table": None}, "no table"), ({"rows": 0}, "no table"),
-    ({"sf": 0}, "scale"), ({"sf": (1 << 30) + 1}, "scale"), ({"x": "out", "xh": 9}, "in place with other strides"), ({"xt": 7}, "heads overlap"), ({"oh": 7}, "heads overlap")])
+    ({"sf": 0}, "scale"), ({"sf": (1 << 30) + 1}, "scale"), ({"x": "out", "xh": 9}, "in place with other strides"), ({"xt": 7}, "heads overlap"), ({"oh": 7}, "heads overlap"),
+    ({"ot": 8, "oh": 8}, "output's heads overlap"), ({"ot": 15, "oh": 8}, "output's heads overlap"), ({"ot": 9, "oh": 16}, "output's heads overlap"), ({"heads": 1 << 28}, "2^30 elements")])
 def test_rope_refusals(name, change, text):
     other = (ctypes.c_int32 * 64)()
     a = {"out": other, "x": W, "ot": 16, "oh": 8, "xt": 16, "xh": 8, "tokens": 2, "heads": 2, "dim": 8, "rot": 8, "table": W, "rows": 4, "sf": 65536}
@@ -651,7 +695,7 @@ def test_product_refusals():
     refused("zk_i32_linear", [W, W, c_size_t(4), None, c_uint(1), c_uint(1), None, c_size_t(0), W, None], "zk_i32_linear: null weight")
     refused("zk_i32_gated", [W, W, c_size_t(4), None, None, c_uint(1), c_uint(1), c_uint(1), W, c_int(0), c_uint(4), c_uint(1), None, c_size_t(0), W, None], "zk_i32_gated: null weight")
     h = c_void_p()
-    for B, n, p, text in ((None, 2, 2, "null argument"), (W, 0, 2, "empty matrix"), (W, 2, 0, "empty matrix"), (W, 43691, 1, "above 43690")):
+    for B, n, p, text in ((None, 2, 2, "null argument"), (W, 0, 2, "empty matrix"), (W, 2, 0, "empty matrix"), (W, 43691, 1, "above 43690"), (W, 1, (1 << 22) + 1, "4194304 columns")):
         refused("zk_i32_rhs_prepare", [ctypes.byref(h), B, c_uint(n), c_uint(p), None], text)
 
 

@@ -54,7 +54,7 @@ __device__ __forceinline__ void raise(uint32_t* flag, uint32_t bad) { if (bad) a
 struct NormArgs {
     int32_t *h, *n, *rms_inv;
     const int32_t *x, *b, *post, *gate, *w;
-    size_t ldx, ldb;
+    size_t ldx, ldb, row0;    // row0: the launch's first row
     uint32_t cols, rows_per_gate;
     int32_t res;
     double scale, eps;
@@ -108,7 +108,7 @@ template <int NV, int VEC, bool POW2, int THREADS> __global__ void __launch_boun
     __shared__ unsigned long long red_s[16];
     __shared__ uint32_t red_m[16];
     __shared__ double total;
-    const size_t row = blockIdx.x;
+    const size_t row = a.row0 + blockIdx.x;
     const uint32_t stride = blockDim.x * VEC, first = threadIdx.x * VEC;
     uint32_t bad = 0;
     auto load = [&](int32_t (&v)[NV][VEC], const int32_t* p) {
@@ -201,7 +201,7 @@ template <bool POW2> __global__ void __launch_bounds__(256) k_residual_norm_long
     __shared__ unsigned long long red_s[4];
     __shared__ uint32_t red_m[4];
     __shared__ double term[256], total;
-    const size_t row = blockIdx.x;
+    const size_t row = a.row0 + blockIdx.x;
     const int32_t* x = a.x + row * a.ldx;
     const int32_t* b = a.b ? a.b + row * a.ldb : nullptr;
     const int32_t* gate = a.gate ? a.gate + row / a.rows_per_gate * a.cols : nullptr;
@@ -791,15 +791,15 @@ template <bool GATED, int PB, int RT, int PA, bool SPLIT, int WAVES, int DEPTH> 
         }
     }
 };
-template <bool GATED, int PB> __global__ void __launch_bounds__(512) k_product_row(const ProductArgs g) {
-    using S = Strip<GATED, PB, 1, 4, true, 8, 4>;
+template <bool GATED, int PB, int WAVES> __global__ void __launch_bounds__(64 * WAVES) k_product_row(const ProductArgs g) {
+    using S = Strip<GATED, PB, 1, 4, true, WAVES, 4>;
     __shared__ int32_t sum[S::SUMS][256];
     uint32_t bad = 0;
     S::run(g, blockIdx.x, 0, sum, bad);
     raise(g.e.flag, bad);
 }
-template <bool GATED, int PB, int RT> __global__ void __launch_bounds__(512) k_product_strip(const ProductArgs g, uint32_t row_blocks) {
-    constexpr int WAVES = 8, DEPTH = RT == 1 ? 4 : 2;
+template <bool GATED, int PB, int RT, int WAVES> __global__ void __launch_bounds__(64 * WAVES) k_product_strip(const ProductArgs g, uint32_t row_blocks) {
+    constexpr int DEPTH = RT == 1 ? 4 : 2;
     using Three = Strip<GATED, PB, RT, 3, false, WAVES, DEPTH>;
     using Four = Strip<GATED, PB, RT, 4, false, WAVES, DEPTH>;
     __shared__ int32_t sum[Four::SUMS][256];
@@ -886,15 +886,16 @@ struct CallFlag {
 static constexpr uint32_t MAX_INNER = (1u << 17) / 3;      // three plane pairs of 2^14 a term in an int32 accumulator
 static int check_weight(const MatmulRhs* w, const char* name) {
     ZK_ARG(w != nullptr, std::string(name) + ": null weight");
-    ZK_ARG(w->planes != nullptr && w->pb >= 1 && w->pb <= 3, std::string(name) + ": the weight has elements beyond 8355711 (three digits of eight bits)");
     ZK_ARG(w->N <= MAX_INNER, std::string(name) + ": an inner dimension above 43690");
+    ZK_ARG(w->planes != nullptr && w->pb >= 1 && w->pb <= 3, std::string(name) + ": the weight has elements beyond 8355711 (three digits of eight bits)");
     return 0;
 }
 static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->planes, w->P, w->Kp, w->pb}; }
 
+// Up to here a product is one launch that splits x itself: 16 rows of 4096 x 11008 40 us so and 28 with a launch of k_split_x before, 4 rows 24 and 28.
 static constexpr uint32_t SPLIT_ROWS = 4;
-static constexpr size_t FEW_TILES = 80;
 static size_t padded_rows(uint32_t rows) { return ((size_t)rows + 127) / 128 * 128; }
+// Tiles of 128 rows where there is one for every compute unit (2048 x 4096 x 4096: 156 us, with 64 rows 165); a third plane of weights has no registers for that.
 template <bool GATED, int PB, bool POW2> static void launch_tiles(const ProductArgs& g, hipStream_t st) {
     const unsigned tn = cdiv(g.cols, GATED ? 64 : 128);
     if constexpr (PB == 2) if ((size_t)tn * cdiv(g.rows, 128) >= 256) {
@@ -903,11 +904,25 @@ template <bool GATED, int PB, bool POW2> static void launch_tiles(const ProductA
     }
     hipLaunchKernelGGL((k_product<GATED, PB, 1, POW2>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
 }
+// Strips of one row of tiles: with one for every compute unit at most, eight waves of a workgroup share its contraction; with more, four, and two workgroups of them lie on a
+// unit, so that one's loads go on while the other adds up (one row of both 4096 x 11008 weights, 688 strips: 42 us with eight, 36 with four; of 11008 x 4096, 256
+// strips: 17 and 20).
+static constexpr unsigned STRIPS_EACH = 256;
+template <bool GATED, int PB> static void launch_row(const ProductArgs& g, hipStream_t st) {
+    const unsigned strips = cdiv(g.cols, 16);
+    if (strips > STRIPS_EACH) hipLaunchKernelGGL((k_product_row<GATED, PB, 4>), dim3(strips), dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((k_product_row<GATED, PB, 8>), dim3(strips), dim3(512), 0, st, g);
+}
+// Rows beyond SPLIT_ROWS.  Strips read every weight once for 16 or 32 rows, whatever their number; tiles make better use of what they read, but one takes a compute
+// unit a quarter of a microsecond for 32 contraction bytes, so that they need to be many.  4096 x 4096: 64 rows (32 tiles) 19 us in strips and 34 in tiles, 128 rows (64
+// tiles) 28 and 35, 256 rows (128 tiles) 49 and 35; one block of 32 rows of 4096 x 11008 (86 tiles) 32 and 41, of both such weights (172) 57 and 51.
 template <bool GATED, int PB> static void launch_product(const ProductArgs& g, hipStream_t st) {
     const unsigned row_blocks = cdiv(g.rows, 32), strips = (cdiv(g.cols, 16) + 7) / 8 * 8;
-    if (g.rows <= 16) hipLaunchKernelGGL((k_product_strip<GATED, PB, 1>), dim3(strips), dim3(512), 0, st, g, 1u);
-    else if (g.rows <= 32 || (size_t)cdiv(g.cols, GATED ? 64 : 128) * cdiv(g.rows, 64) < FEW_TILES)
-        hipLaunchKernelGGL((k_product_strip<GATED, PB, 2>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
+    const size_t tiles = (size_t)cdiv(g.cols, GATED ? 64 : 128) * cdiv(g.rows, 64);
+    if (g.rows <= 16) {
+        if (strips > STRIPS_EACH) hipLaunchKernelGGL((k_product_strip<GATED, PB, 1, 4>), dim3(strips), dim3(256), 0, st, g, 1u);
+        else hipLaunchKernelGGL((k_product_strip<GATED, PB, 1, 8>), dim3(strips), dim3(512), 0, st, g, 1u);
+    } else if (tiles < (g.rows <= 32 ? 128u : 80u)) hipLaunchKernelGGL((k_product_strip<GATED, PB, 2, 8>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
     else if (g.e.pow2) launch_tiles<GATED, PB, true>(g, st);
     else launch_tiles<GATED, PB, false>(g, st);
 }
@@ -923,8 +938,8 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, void*
     g.x_aligned = (g.ldx & 3) == 0 && ((uintptr_t)g.x & 15) == 0;
     const int pb = std::max(g.w.n, GATED ? g.gate.n : 0);
     if (g.rows <= SPLIT_ROWS) {
-        if (pb <= 2) hipLaunchKernelGGL((k_product_row<GATED, 2>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
-        else hipLaunchKernelGGL((k_product_row<GATED, 3>), dim3(cdiv(g.cols, 16)), dim3(512), 0, st, g);
+        if (pb <= 2) launch_row<GATED, 2>(g, st);
+        else launch_row<GATED, 3>(g, st);
         ZK_LAUNCH_CHECK();
         return flag.end(name);
     }
@@ -977,15 +992,17 @@ int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t 
     ZK_ARG((gate == nullptr) == (gate_rows == 0) && (gate == nullptr || rows % gate_rows == 0), "zk_i32_residual_norm: gate_rows must divide rows, and be 0 without a gate");
     ZK_ARG(sf > 0, "zk_i32_residual_norm: a scaling factor of 0");
     ZK_ARG(scale > 0 && eps > 0 && scale <= 1e18 && scale >= 1e-18 && scale / std::sqrt(eps) <= 2147483000.0, "zk_i32_residual_norm: scale and eps must be positive, scale / sqrt(eps) below 2^31");
-    ZK_ARG(rows <= 0x7FFFFFFFu, "zk_i32_residual_norm: too many rows in one call");
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, "zk_i32_residual_norm")) return rc;
     int e2 = 0;
-    const NormArgs a{(int32_t*)h, (int32_t*)n, (int32_t*)rms_inv, (const int32_t*)x, (const int32_t*)b, (const int32_t*)post, (const int32_t*)gate, (const int32_t*)w, ldx, ldb, cols,
+    NormArgs a{(int32_t*)h, (int32_t*)n, (int32_t*)rms_inv, (const int32_t*)x, (const int32_t*)b, (const int32_t*)post, (const int32_t*)gate, (const int32_t*)w, ldx, ldb, 0, cols,
                      gate ? rows / gate_rows : 1, res, scale, eps, std::frexp(scale, &e2) == 0.5, divisor(sf), flag.dev};
-    if (a.sf.shift >= 0) launch_norm<true>(a, rows, st);
-    else launch_norm<false>(a, rows, st);
+    for (; a.row0 < rows; a.row0 += 1u << 20) {          // a launch has fewer than 2^32 lanes
+        const uint32_t n_rows = std::min<uint32_t>(1u << 20, rows - (uint32_t)a.row0);
+        if (a.sf.shift >= 0) launch_norm<true>(a, n_rows, st);
+        else launch_norm<false>(a, n_rows, st);
+    }
     ZK_LAUNCH_CHECK();
     return flag.end("zk_i32_residual_norm");
 }
@@ -1000,6 +1017,10 @@ static int rope(const char* name, bool fr, void* out, size_t out_token, size_t o
     ZK_ARG(out != x || (out_token == x_token && out_head == x_head), std::string(name) + ": in place with other strides");
     ZK_ARG((tokens == 1 || (x_token >= dim && out_token >= dim)) && (heads == 1 || (x_head >= dim && out_head >= dim)), std::string(name) + ": heads overlap (a stride below the head's width)");
     ZK_ARG((uint64_t)heads * dim <= (1u << 30), std::string(name) + ": more than 2^30 elements a token");
+    {
+        const unsigned __int128 of_heads = (unsigned __int128)(heads - 1) * out_head + dim, of_tokens = (unsigned __int128)(tokens - 1) * out_token + dim;
+        ZK_ARG(tokens == 1 || heads == 1 || out_token >= of_heads || out_head >= of_tokens, std::string(name) + ": the output's heads overlap (neither a token within the stride of heads nor a head within that of tokens)");
+    }
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
@@ -1037,6 +1058,7 @@ int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size
 int zk_rope_table(void* table, uint32_t rows, uint32_t rot, double base, double factor, double original, double low, double high, double magnitude, uint32_t sf, void* stv) {
     if (rows == 0 || rot == 0) return 0;
     ZK_ARG(table != nullptr && rot % 2 == 0, "zk_rope_table: null table or an odd part of the head");
+    ZK_ARG((size_t)rows * (rot / 2) <= 0x7FFFFFFFu, "zk_rope_table: more than 2^31 entries");
     ZK_ARG(base > 1 && base <= 1e15 && factor > 0 && factor >= 1e-6 && factor <= 1e6, "zk_rope_table: the base must lie above 1 (up to 1e15), the factor within 1e-6 .. 1e6");
     ZK_ARG(original == 0 || (original > 0 && original <= 1e15 && low >= 0 && high > low && high <= 1e15), "zk_rope_table: with original positions, 0 <= low < high");
     ZK_ARG(sf > 0 && magnitude > 0 && magnitude * (double)sf <= 1073741824.0, "zk_rope_table: scale times magnitude must lie within 2^30");
@@ -1050,7 +1072,7 @@ int zk_i32_from_heads(void* out, const void* in, uint32_t heads, uint32_t tokens
     if (n == 0) return 0;
     ZK_ARG(out != nullptr && in != nullptr && out != in, "zk_i32_from_heads: null tensor or in place");
     ZK_ARG(sf_first > 0 && sf_second > 0, "zk_i32_from_heads: a scaling factor of 0");
-    ZK_ARG((n + 255) / 256 <= 0x7FFFFFFFu, "zk_i32_from_heads: too many elements in one call");
+    ZK_ARG(n <= 0xFFFFFF00u, "zk_i32_from_heads: more elements than a tensor has");
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, "zk_i32_from_heads")) return rc;
@@ -1062,7 +1084,7 @@ int zk_i32_from_heads(void* out, const void* in, uint32_t heads, uint32_t tokens
 int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, void* stv) {
     hipStream_t st = (hipStream_t)stv;
     ZK_ARG(prepared != nullptr && B != nullptr && N > 0 && P > 0, "zk_i32_rhs_prepare: null argument or empty matrix");
-    ZK_ARG(N <= MAX_INNER && P <= (1u << 30), "zk_i32_rhs_prepare: an inner dimension above 43690, or too many columns");
+    ZK_ARG(N <= MAX_INNER && P <= (1u << 22), "zk_i32_rhs_prepare: an inner dimension above 43690, or more than 4194304 columns");
     if (const int rc = CallFlag::not_captured(st, "zk_i32_rhs_prepare")) return rc;
     std::unique_ptr<MatmulRhs> r(new MatmulRhs);
     r->N = N; r->P = P; r->Kp = (N + GBK - 1) / GBK * GBK;
@@ -1085,6 +1107,8 @@ int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, v
     hipLaunchKernelGGL(k_split_cols_i32, dim3(cdiv(P, 64), r->Kp / 64), dim3(256), 0, st, (int8_t*)r->planes, (const int32_t*)B, N, P, r->Kp, r->pb);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) { (void)pool_free(r->planes, st); return hip_fail(e, "k_split_cols_i32", __FILE__, __LINE__); }
+    const hipError_t done = hipStreamSynchronize(st);         // B is the caller's again, and any stream may read the planes
+    if (done != hipSuccess) { (void)pool_free(r->planes, st); return hip_fail(done, "hipStreamSynchronize", __FILE__, __LINE__); }
     *prepared = r.release();
     return 0;
 }
