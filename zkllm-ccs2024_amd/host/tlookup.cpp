@@ -90,6 +90,10 @@ pair<FrTensor, FrTensor> tLookupRangeMapping::map_queued(const FrTensor& vals, c
     FrTensor y = gather(vals, c, unwritten);
     return {std::move(y), std::move(*c.m)};
 }
+FrTensor tLookupRangeMapping::map_inside(const FrTensor& vals, const FrTensor* unwritten) {
+    if (!map_inside_applies(vals)) throw std::runtime_error("map_inside: queries and mapped values need int32 forms");
+    return gather(vals, CountedQueries(), unwritten);
+}
 // wait: the range check is settled here (an attention head of 2 x 128 tokens takes 20 us less so than by settle() in the next line)
 void tLookupRangeMapping::count(CountedQueries& c, const FrTensor& vals, bool positions, bool wait) {
     if (positions) c.idx.reset(new DevBuf(sizeof(uint) * (size_t)vals.size));

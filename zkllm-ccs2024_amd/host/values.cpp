@@ -73,7 +73,7 @@ IntTensor LayerValues::operator()(const IntTensor& X) const {
         uint g = H;
         while (g > 1 && ((unsigned long long)g * T * T > (1ull << 28) || H % g)) --g;
         zkAttnStacked attn(g, c.softmax_sf_in, 1UL, c.softmax_bs, c.softmax_L, c.softmax_M, c.softmax_thetas, T, T, d, 1);
-        attn.lean_forward = true;
+        attn.lean_forward = attn.values_only = true;
         FrTensor heads(T * E);
         const uint per = g * T * d;
         for (uint at = 0; at < T * E; at += per) {

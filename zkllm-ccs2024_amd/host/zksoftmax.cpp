@@ -92,8 +92,12 @@ FrTensor zkSoftmax::compute_rows(uint m, const FrTensor& X, FrTensor& shift, FrT
     for (uint i = L; i < K; ++i) lean_out = lean_out && ints_only[i];
     lean_tensors_last = lean_out ? K - L : 0;
     for (uint i = 0; i < K; ++i) lean_tensors_last += ints_only[i] ? 1 : 0;
-    for (uint i = 0; i < L; ++i) m_segments.push_back(least_significant_segments[i].prep(X_segments[i]));
+    for (uint i = 0; i < L && !values_only; ++i) m_segments.push_back(least_significant_segments[i].prep(X_segments[i]));
     for (uint i = L; i < K; ++i) {
+        if (values_only && other_segments[i - L].map_inside_applies(X_segments[i])) {      // digits below the table's length
+            Y_segments.push_back(other_segments[i - L].map_inside(X_segments[i], lean_out ? unwritten.get() : nullptr));
+            continue;
+        }
         auto p = other_segments[i - L].map_queued(X_segments[i], lean_out ? unwritten.get() : nullptr);
         Y_segments.push_back(std::move(p.first));
         m_segments.push_back(std::move(p.second));

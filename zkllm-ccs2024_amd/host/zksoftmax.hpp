@@ -15,6 +15,8 @@ class zkSoftmax {
     // int32 forms (ZKLLM_SOFTMAX_PRODUCT=0 in the environment writes it).  For a caller that hands the tensors to prove() and reads
     // none of them itself.
     bool lean_forward = false;
+    // Addition, for a caller that wants compute()'s result and no proof: the multiplicities are not counted (m_segments stays empty or holds some of them).
+    bool values_only = false;
     std::shared_ptr<FrTensor> unwritten;      // the buffer those tensors are views of: it must outlive every use of them (it lives as long as this object)
     static bool scores_i64_last;        // whether the last zkAttnStacked::compute wrote its scores as 64-bit integers only
     static uint lean_tensors_last;      // how many digit planes and mapped-value tensors the last compute() left in int32 form only
