@@ -92,16 +92,21 @@ template <bool POW2> __device__ __forceinline__ int32_t normed(int32_t w, int32_
 }
 
 // A workgroup a row, VEC neighbouring columns NV times in each lane's registers: every tensor is read once and written once, which is what
-// bounds it.
+// bounds it (2048 x 4096, x and b to h and n, 134 MB: 24 us, 5.6 TB/s; a copy of a gigabyte reaches 5.15).  One row of 4096: 4.5 us, two reductions and the way to memory and back.
+// Rows whose squares round are added up by one lane out of LDS, a few microseconds a thousand columns: activations beyond 2^26, in the hundreds at scale 2^16.
 template <int VEC> __device__ __forceinline__ void row_load(int32_t (&v)[VEC], const int32_t* p) {
     if constexpr (VEC == 4) {
         const v4i q = *reinterpret_cast<const v4i*>(p);
         v[0] = q[0]; v[1] = q[1]; v[2] = q[2]; v[3] = q[3];
     } else v[0] = *p;
 }
-template <int VEC> __device__ __forceinline__ void row_store(int32_t* p, const int32_t (&v)[VEC]) {
-    if constexpr (VEC == 4) *reinterpret_cast<v4i*>(p) = v4i{v[0], v[1], v[2], v[3]};
-    else *p = v[0];
+// STREAM: stores of large tensors go past the caches (2048 x 4096: 31 us, 24 so; with the projection that reads them behind it 206 either way)
+template <int VEC, bool STREAM> __device__ __forceinline__ void row_store(int32_t* p, const int32_t (&v)[VEC]) {
+    if constexpr (VEC == 4) {
+        const v4i q = {v[0], v[1], v[2], v[3]};
+        if constexpr (STREAM) __builtin_nontemporal_store(q, reinterpret_cast<v4i*>(p));
+        else *reinterpret_cast<v4i*>(p) = q;
+    } else *p = v[0];
 }
 template <int NV, int VEC, bool POW2, int THREADS> __global__ void __launch_bounds__(THREADS) k_residual_norm(const NormArgs a) {
     extern __shared__ double term[];           // blockDim.x * VEC
@@ -122,7 +127,7 @@ template <int NV, int VEC, bool POW2, int THREADS> __global__ void __launch_boun
     };
     auto store = [&](int32_t* p, const int32_t (&v)[NV][VEC]) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) if (first + i * stride < a.cols) row_store<VEC>(p + first + i * stride, v[i]);
+        for (int i = 0; i < NV; ++i) if (first + i * stride < a.cols) row_store<VEC, THREADS == 512>(p + first + i * stride, v[i]);
     };
     auto statistic = [&](const int32_t (&v)[NV][VEC]) {
         unsigned long long s = 0;
@@ -286,7 +291,8 @@ __device__ __forceinline__ int64_t rope_get(const Fr* p, uint32_t& bad) {
 }
 __device__ __forceinline__ void rope_put(int32_t* p, int64_t v, uint32_t& bad) { *p = narrow(v, bad); }
 __device__ __forceinline__ void rope_put(Fr* p, int64_t v, uint32_t&) { *p = fr_from_i64(v); }
-// A lane VEC pairs of the rotated part or VEC elements of the rest; the heads of a token read its angles from the caches.
+// A lane VEC pairs of the rotated part or VEC elements of the rest; the heads of a token read its angles from the caches.  HBM: 16384 tokens of 32 x 128 int32 92 us,
+// 5.9 TB/s (a pair a lane 143); 2048 tokens of field elements 103 us, 5.2 TB/s; the launches of a token's 64 heads 3 us.
 template <typename T, int VEC, bool POW2> __global__ void __launch_bounds__(256) k_rope(const RopeArgs a, uint32_t token0, uint32_t total) {
     const uint32_t id = blockIdx.x * 256 + threadIdx.x;
     if (id >= total) return;
@@ -460,7 +466,7 @@ __device__ __forceinline__ void row_piece(const ProductArgs& g, uint32_t row, ui
 }
 
 // x's planes for the products of many rows.  A workgroup takes 32 rows and CHUNK columns, 32 columns of a wave's 64 at a time: a lane 16 values of a row, so that the
-// wave writes 1 KB of every plane in one piece.  How many planes the stretch needs goes to a place of its own.
+// wave writes 1 KB of every plane in one piece.  How many planes the stretch needs goes to a place of its own.  2048 x 4096: 14 us, 67 MB.
 __global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __restrict__ planes, uint32_t* __restrict__ need, v4i* __restrict__ zeros) {
     __shared__ uint32_t most[4];
     if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) zeros[threadIdx.x] = v4i{0, 0, 0, 0};
@@ -493,6 +499,10 @@ __global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __
 // lanes, and what joins them needs no exchange -- and a wave 32 MT by 64, as 32 x 32 tiles of v_mfma_i32_32x32x32_i8.
 // Steps of 32 contraction bytes go from memory to LDS without passing through registers, four buffers deep; a step's fragments are read while the step before
 // is multiplied, since one wave a SIMD (256 accumulators with MT = 2) has nobody to cover for it.
+// 2048 x 4096 x 4096, three planes by two: 156 us; both 4096 x 11008 weights at 2048 rows 860, 2.55 POP/s (the library's int8 product of 8192^3: 2.05).  The matrix units are
+// busy 65 % of the cycles, at 1.75 to 1.85 GHz: the card's power holds the clock there (the same without the loads from memory, on what lies in LDS, 2.3 GHz and 570 us), and what
+// saves stalls costs clock.  Steps of 64 bytes (61 us against 41 for 64 rows of 4096 x 11008), eight buffers (47), the next tile's first steps ahead of a tile's outputs (936
+// against 895 for the whole) and other orders of the products or tiles (within 1 %) gained nothing.
 template <bool GATED, int PA, int PB, int MT> struct Tile {
     static constexpr int NS = PA + PB - 1, TM = 64 * MT, PIECES = PA * 2 * MT + PB * 4, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * 128) * 32;
     v16i acc[NS][MT][2];
@@ -693,7 +703,8 @@ template <bool GATED, int PB, int MT, bool POW2> __global__ void __launch_bounds
 // Few rows, or few tiles: the weights' way out of memory is what counts.  A workgroup takes 16 columns (of each weight) and 16 RT rows, its waves the units of 64 contraction
 // bytes in turn, straight from memory into the fragments of v_mfma_i32_16x16x64_i8 -- a fragment of 16 columns is two pieces of 512 bytes in the planes' layout.
 // SPLIT: x is split on the way, all four digits (one launch, and the matrix cores idle anyway); else its planes are read as the weights' are.  The waves'
-// accumulators are added up in LDS, integers in any order.
+// accumulators are added up in LDS, integers in any order.  One row of 11008 x 4096: 17.5 us, of both 4096 x 11008 weights 35, 5.15 TB/s of planes; 32 rows of
+// 4096 x 11008 32 us, where x's planes, read anew by every strip, weigh as much as the weights.
 template <bool GATED, int PB, int RT, int PA, bool SPLIT, int WAVES, int DEPTH> struct Strip {
     static constexpr int MATS = GATED ? 2 : 1, NS = PA + PB - 1, SUMS = NS * MATS * RT;
     static __device__ __forceinline__ void run(const ProductArgs& g, uint32_t strip, uint32_t row_block, int32_t (*sum)[256], uint32_t& bad) {
@@ -973,7 +984,7 @@ template <bool POW2> static void launch_norm(const NormArgs& a, uint32_t rows, h
     const bool vec = (a.cols & 3) == 0 && (a.ldx & 3) == 0 && (a.b == nullptr || (a.ldb & 3) == 0) && aligned(a.x) && aligned(a.b) && aligned(a.h) && aligned(a.n) && aligned(a.post) &&
                      aligned(a.gate) && aligned(a.w);
     if (vec && a.cols <= 4096 && (rows < 512 || a.cols <= 1024)) launch_norm_n<1, 4, POW2, 1024>(a, rows, st);
-    else if (vec && a.cols <= 4096) launch_norm_n<4, 4, POW2, 256>(a, rows, st);
+    else if (vec && a.cols <= 4096) launch_norm_n<2, 4, POW2, 512>(a, rows, st);
     else if (vec && a.cols <= 16384) launch_norm_n<4, 4, POW2, 1024>(a, rows, st);
     else if (!vec && a.cols <= 1024) launch_norm_n<1, 1, POW2, 1024>(a, rows, st);
     else if (!vec && a.cols <= 16384) launch_norm_n<16, 1, POW2, 1024>(a, rows, st);
