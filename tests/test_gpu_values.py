@@ -503,6 +503,90 @@ def test_gated_activations_outside_the_table(hip, dev, rows, side):
     assert flag == 0 and (got == ref.gated(x, g, u, 1, 1, table, -4, 1)).all()
 
 
+# Products of enough tiles for the kernel of many rows (80 tiles of 64 rows by 128 columns, of 64 by 64 where there are two weights; 128 rows a tile from 256 of those on):
+# ragged in every direction, one step of the contraction and several, rows of four digits in some tiles only, in the last row, in all
+TILED = [(300, 40, 2100), (641, 128, 1030), (130, 300, 3650), (2100, 40, 2050), (2177, 140, 1921)]
+
+
+def tiled_rows(rng, rows, inner, digits):
+    x = normal(rng, (rows, inner))
+    if digits == "some":
+        for r in (3, rows // 2, rows - 1):
+            x[r] = rng.integers(-(1 << 31), 0x7F7F7F80, inner)
+            x[r, r % inner] = 0x7F7F7F7F
+    elif digits == "all":
+        x = rng.integers(-(1 << 31), 0x7F7F7F80, (rows, inner)).astype(np.int32)
+    return x
+
+
+@gpu
+@pytest.mark.parametrize("rows,inner,cols", TILED)
+@pytest.mark.parametrize("most,sf", [(127, 1 << 16), (32639, 1 << 24), (32639, 9999991), (8355711, 1 << 31)])
+@pytest.mark.parametrize("digits", ["three", "some", "all"])
+def test_linear_in_tiles(hip, dev, rows, inner, cols, most, sf, digits):
+    rng = np.random.default_rng(rows + inner + cols + most % 1000)
+    w = rng.integers(-most, most + 1, (inner, cols)).astype(np.int32)
+    w[0, 0] = most
+    x = tiled_rows(rng, rows, inner, digits)
+    got, flag = call_linear(hip, dev, x, Weight(hip, dev, w), cols, sf, own_workspace=True, ldx=inner + (3 if digits == "some" else 4))
+    exp = ref.linear(x, w, sf)
+    assert flag == (0 if (exp == exp.astype(np.int32)).all() else ref.RANGE) and (got == exp.astype(np.int32)).all()
+
+
+@gpu
+@pytest.mark.parametrize("rows,inner,cols", [(300, 40, 1100), (641, 128, 517), (2100, 40, 1050), (2177, 140, 961)])
+@pytest.mark.parametrize("weights", [(30000, 30000), (120, 8355711), (8355711, 20000)])
+@pytest.mark.parametrize("general", [False, True])
+def test_gated_in_tiles(hip, dev, rows, inner, cols, weights, general):
+    rng = np.random.default_rng(rows + inner + cols + weights[0] % 1000)
+    g, u = (np.clip(np.round(rng.normal(0, 0.3 * m, (inner, cols))), -m, m).astype(np.int32) for m in weights)
+    g[0, 0], u[0, 0] = weights
+    x = normal(rng, (rows, inner), 3000.0)
+    if general:                                                 # a tile with rows of four digits: their activations leave the table
+        x[rows - 1] = rng.integers(-(1 << 31), 0x7F7F7F80, inner)
+    sfs = (1 << 20, 1 << 16, 1 << 20) if weights[0] < 1 << 20 else (1 << 28, 1 << 16, 1 << 20)
+    if general:
+        sfs = tuple(v - 1 for v in sfs)
+    low, n = -(1 << 20), 1 << 21
+    table = swiglu(low, n, 4096.0)
+    got, flag = call_gated(hip, dev, x, Weight(hip, dev, g), Weight(hip, dev, u), cols, sfs[0], sfs[1], table, low, sfs[2], own_workspace=True)
+    at, up = ref.linear(x, g, sfs[0]) - low, ref.linear(x, u, sfs[1])
+    inside = (at >= 0) & (at < n)
+    exp = np.where(inside, ref.quotient(table.astype(np.int64)[np.clip(at, 0, n - 1)] * up.astype(np.int32), sfs[2]), 0)
+    fits = (up == up.astype(np.int32)) & (exp == exp.astype(np.int32))
+    assert flag == (0 if inside.all() else ref.TABLE) | (0 if fits.all() else ref.RANGE)
+    assert (got == exp)[fits].all() and (general or flag == 0)
+
+
+# sums around 2^62 and values around the edges of int32 and the table, in the last row and column of the last tile; x's rows and the weight's columns beyond them do not count
+@gpu
+@pytest.mark.parametrize("rows", [321, 2200])
+def test_edges_in_tiles(hip, dev, rows):
+    inner, cols = 1024, 2050
+    w = np.zeros((inner, cols), np.int32)
+    w[:, cols - 1] = 1 << 22
+    weight = Weight(hip, dev, w)
+    x = np.zeros((rows, inner), np.int32)
+    x[rows - 1] = 1 << 30
+    assert call_linear(hip, dev, x, weight, cols, 1 << 31)[1] == ref.RANGE
+    for sign in (1, -1):
+        x[rows - 1] = sign * (1 << 30)
+        x[rows - 1, 5] -= sign
+        got, flag = call_linear(hip, dev, x, weight, cols, (1 << 32) - 1)
+        exp = np.zeros((rows, cols), np.int64)
+        exp[rows - 1, cols - 1] = ref.quotient(sign * ((1 << 62) - (1 << 22)), (1 << 32) - 1)
+        assert flag == 0 and (got == exp).all()
+    g = np.zeros((40, cols), np.int32)
+    g[0, cols - 1] = 3
+    x = np.ones((rows, 40), np.int32)
+    u = np.ones((40, cols), np.int32)
+    table = np.arange(100, 108, dtype=np.int32)                  # 1 .. 8: a sum of 0 lies outside
+    for low, bad in ((-4, False), (0, False), (1, True)):
+        got, flag = call_gated(hip, dev, x, Weight(hip, dev, g), Weight(hip, dev, u), cols, 1, 1, table, low, 1)
+        assert flag == (ref.TABLE if bad else 0)
+        assert (got[:, cols - 1] == (103 - low) * 40).all() and (got[:, :cols - 1] == (0 if bad else (100 - low) * 40)).all()
+
+
 @gpu
 def test_handles_from_field_elements_serve_both_and_those_from_int32_no_field_product(hip, dev):
     rng = np.random.default_rng(8)
