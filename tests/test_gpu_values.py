@@ -503,9 +503,9 @@ def test_gated_activations_outside_the_table(hip, dev, rows, side):
     assert flag == 0 and (got == ref.gated(x, g, u, 1, 1, table, -4, 1)).all()
 
 
-# Products of enough tiles for the kernel of many rows (80 tiles of 64 rows by 128 columns, of 64 by 64 where there are two weights; 128 rows a tile from 256 of those on):
+# Products of enough tiles for the kernel of many rows (1024 strips of 16 columns by 32 rows, 640 where there are two weights; 64 columns a tile up to 128 tiles, 128 rows from 256 on):
 # ragged in every direction, one step of the contraction and several, rows of four digits in some tiles only, in the last row, in all
-TILED = [(300, 40, 2100), (641, 128, 1030), (130, 300, 3650), (2100, 40, 2050), (2177, 140, 1921)]
+TILED = [(300, 40, 2100), (641, 128, 1030), (130, 300, 3650), (2100, 40, 2050), (2177, 140, 1921), (33, 70, 16600), (600, 33, 2000), (700, 260, 2111)]
 
 
 def tiled_rows(rng, rows, inner, digits):

@@ -495,17 +495,17 @@ __global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __
     raise(g.e.flag, bad);
 }
 
-// Many rows.  A workgroup of four waves takes 64 MT rows by 128 columns of weights -- 64 of each where there are two: a wave's gate and up tiles lie in the same
-// lanes, and what joins them needs no exchange -- and a wave 32 MT by 64, as 32 x 32 tiles of v_mfma_i32_32x32x32_i8.
+// Many rows.  A workgroup of four waves takes 64 MT rows by 64 NQ columns of weights -- with NQ = 2 64 of each where there are two: a wave's gate and up tiles lie in the same
+// lanes, and what joins them needs no exchange -- and a wave 32 MT by 32 NQ, as 32 x 32 tiles of v_mfma_i32_32x32x32_i8.
 // Steps of 32 contraction bytes go from memory to LDS without passing through registers, four buffers deep; a step's fragments are read while the step before
 // is multiplied, since one wave a SIMD (256 accumulators with MT = 2) has nobody to cover for it.
 // 2048 x 4096 x 4096, three planes by two: 156 us; both 4096 x 11008 weights at 2048 rows 860, 2.55 POP/s (the library's int8 product of 8192^3: 2.05).  The matrix units are
 // busy 65 % of the cycles, at 1.75 to 1.85 GHz: the card's power holds the clock there (the same without the loads from memory, on what lies in LDS, 2.3 GHz and 570 us), and what
 // saves stalls costs clock.  Steps of 64 bytes (61 us against 41 for 64 rows of 4096 x 11008), eight buffers (47), the next tile's first steps ahead of a tile's outputs (936
 // against 895 for the whole) and other orders of the products or tiles (within 1 %) gained nothing.
-template <bool GATED, int PA, int PB, int MT> struct Tile {
-    static constexpr int NS = PA + PB - 1, TM = 64 * MT, PIECES = PA * 2 * MT + PB * 4, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * 128) * 32;
-    v16i acc[NS][MT][2];
+template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
+    static constexpr int NS = PA + PB - 1, TM = 64 * MT, TN = 64 * NQ, PIECES = PA * 2 * MT + PB * 2 * NQ, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * TN) * 32;
+    v16i acc[NS][MT][NQ];
     __device__ __forceinline__ void multiply(const ProductArgs& g, uint32_t m0, uint32_t n0, int8_t* const (&buf)[4]) {
         const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wm = wave >> 1, wn = wave & 1;
 #pragma unroll
@@ -513,7 +513,7 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                for (int q = 0; q < NQ; ++q)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) acc[s][m][q][r] = 0;
         // The wave's pieces of a step: 32 rows of a plane each, x's first.  A weight's rows beyond the last read the last, a plane that it has not reads zeros.
@@ -531,18 +531,18 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
                 dst[i] = (plane * TM + r) * 32;
                 step[i] = (size_t)g.rows_padded * 32;
             } else {
-                const uint32_t cb = c - PA * 2 * MT, plane = cb >> 2, r = (cb & 3u) * 32, first = n0 + (GATED ? r & 63u : r);
+                const uint32_t cb = c - PA * 2 * MT, plane = cb / (2 * NQ), r = cb % (2 * NQ) * 32, first = n0 + (GATED ? r & 63u : r);
                 const Planes& w = GATED && r < 64 ? g.gate : g.w;
                 const bool has = (int)plane < w.n, inside = first < w.rows;
                 src[i] = has ? w.p + (size_t)plane * w.rows * w.Kp + (size_t)(inside ? first : w.rows - 1) * 32 : g.zeros;
                 at[i] = (has && inside ? min(lr, w.rows - 1 - first) : 0u) * 32 + lane_half;
-                dst[i] = (PA * TM + plane * 128 + r) * 32;
+                dst[i] = (PA * TM + plane * TN + r) * 32;
                 step[i] = has ? (size_t)w.rows * 32 : 0;
             }
         }
         const uint32_t half = lane >> 5, steps = g.w.Kp / 32;
         const uint32_t rowA = wm * 32 * MT + (lane & 31), at_a = rowA * 32 + gemm_half(rowA, half) * 16;
-        const uint32_t rowB = wn * (GATED ? 32 : 64) + (lane & 31), next_b = GATED ? 64 : 32, at_b = (PA * TM + rowB) * 32 + gemm_half(rowB, half) * 16;      // 32 rows on: the same halves
+        const uint32_t rowB = wn * (GATED ? 32 : 32 * NQ) + (lane & 31), next_b = GATED ? 64 : 32, at_b = (PA * TM + rowB) * 32 + gemm_half(rowB, half) * 16;      // 32 rows on: the same halves
         uint32_t fetched = 1;
         auto fetch = [&](int8_t* to) {                         // the next step; behind the last one that again, into buffers nobody reads any more
             const size_t on = (size_t)(int64_t)__builtin_amdgcn_readfirstlane(fetched < steps ? -1 : 0);
@@ -550,7 +550,7 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
 #pragma unroll
             for (int i = 0; i < SHARE; ++i) { load_to_lds(src[i] + at[i], to + dst[i]); src[i] += step[i] & on; }
         };
-        struct Fragments { v4i a[PA][MT], b[PB][2]; };
+        struct Fragments { v4i a[PA][MT], b[PB][NQ]; };
         auto read = [&](const int8_t* from, Fragments& f) {
 #pragma unroll
             for (int i = 0; i < PA; ++i)
@@ -559,7 +559,7 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
 #pragma unroll
             for (int j = 0; j < PB; ++j)
 #pragma unroll
-                for (int q = 0; q < 2; ++q) f.b[j][q] = *reinterpret_cast<const v4i*>(from + at_b + (j * 128 + next_b * q) * 32);
+                for (int q = 0; q < NQ; ++q) f.b[j][q] = *reinterpret_cast<const v4i*>(from + at_b + (j * TN + next_b * q) * 32);
         };
         auto products = [&](const Fragments& f) {
 #pragma unroll
@@ -569,12 +569,11 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) acc[i + j][m][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i][m], f.b[j][q], acc[i + j][m][q], 0, 0, 0);
+                        for (int q = 0; q < NQ; ++q) acc[i + j][m][q] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.a[i][m], f.b[j][q], acc[i + j][m][q], 0, 0, 0);
         };
         // the fragments' reads and the next loads spread over the products
         auto spread = [&] {
-            constexpr int READS = PA * MT + PB * 2, PRODUCTS = PA * PB * MT * 2;
-            static_assert(PRODUCTS >= READS + SHARE, "a product for every read and load");
+            constexpr int READS = PA * MT + PB * NQ, PRODUCTS = PA * PB * MT * NQ;
 #pragma unroll
             for (int i = 0; i < READS; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);      // an LDS read
@@ -585,7 +584,7 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
                 __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);      // a load
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS - READS - SHARE, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
         };
         // Everybody's share of a step is in LDS when no more than `younger` steps' loads of a wave's own are on their way and all waves are past the barrier; with no LDS
         // read on its way either (lgkmcnt 0), the buffer read last is free for the next fetch.
@@ -656,10 +655,10 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
                 }
             } else {
 #pragma unroll
-                for (int q = 0; q < 2; ++q)
+                for (int q = 0; q < NQ; ++q)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) {
-                        store(row0 + 8 * (r >> 2) + (r & 3), wn * 64 + q * 32 + (lane & 31), narrow(quotient<POW2>(value(m, q, r), g.e.sf), bad));
+                        store(row0 + 8 * (r >> 2) + (r & 3), wn * 32 * NQ + q * 32 + (lane & 31), narrow(quotient<POW2>(value(m, q, r), g.e.sf), bad));
                         if ((r & 3) == 3) __builtin_amdgcn_sched_barrier(0);      // the next rows' values would only crowd the registers
                     }
             }
@@ -667,8 +666,8 @@ template <bool GATED, int PA, int PB, int MT> struct Tile {
     }
 };
 // POW2: every divisor of the call is a power of two
-template <bool GATED, int PB, int MT, bool POW2> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
-    constexpr int BYTES = Tile<GATED, 3, PB, MT>::BYTES > Tile<GATED, 4, PB, 1>::BYTES ? Tile<GATED, 3, PB, MT>::BYTES : Tile<GATED, 4, PB, 1>::BYTES;
+template <bool GATED, int PB, int MT, int NQ, bool POW2> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
+    constexpr int BYTES = Tile<GATED, 3, PB, MT, NQ>::BYTES > Tile<GATED, 4, PB, 1, NQ>::BYTES ? Tile<GATED, 3, PB, MT, NQ>::BYTES : Tile<GATED, 4, PB, 1, NQ>::BYTES;
     // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
     __shared__ __attribute__((aligned(16))) int8_t s0[BYTES], s1[BYTES], s2[BYTES], s3[BYTES];
     // Workgroups go to the eight dies in turn: a die takes a run of tiles in groups of eight rows of them, which share operands in its L2
@@ -681,18 +680,18 @@ template <bool GATED, int PB, int MT, bool POW2> __global__ void __launch_bounds
             tn = in / rows;
         }
     }
-    const uint32_t m0 = tm * 64 * MT, n0 = tn * (GATED ? 64 : 128);
+    const uint32_t m0 = tm * 64 * MT, n0 = tn * (GATED ? 64 : 64 * NQ);
     uint32_t need = 0, bad = 0;
     for (uint32_t i = threadIdx.x & 63u; i < 2 * MT * g.chunks; i += 64) need = max(need, g.need[(size_t)(m0 / 32) * g.chunks + i]);
     const bool wide = __any(need > 3);
     int8_t* const buf[4] = {s0, s1, s2, s3};
     if (!wide) {
-        Tile<GATED, 3, PB, MT> t;
+        Tile<GATED, 3, PB, MT, NQ> t;
         t.multiply(g, m0, n0, buf);
         t.template finish<POW2>(g, m0, n0, bad);
     } else {                                   // a value of more than three digits: all four planes, 64 rows at a time
         for (uint32_t m = m0; m < m0 + 64 * MT; m += 64) {
-            Tile<GATED, 4, PB, 1> t;
+            Tile<GATED, 4, PB, 1, NQ> t;
             t.multiply(g, m, n0, buf);
             t.template finish<POW2>(g, m, n0, bad);
         }
@@ -907,13 +906,18 @@ static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->pl
 static constexpr uint32_t SPLIT_ROWS = 4;
 static size_t padded_rows(uint32_t rows) { return ((size_t)rows + 127) / 128 * 128; }
 // Tiles of 128 rows where there is one for every compute unit (2048 x 4096 x 4096: 156 us, with 64 rows 165); a third plane of weights has no registers for that.
+// Half as wide where every tile then finds a unit of its own (64 rows of 4096 x 11008, 86 tiles: 42 us and 36; 256 rows of 4096 x 4096, 128 tiles: 35 and 32; 384 rows, 192 tiles: 41 and 46).
 template <bool GATED, int PB, bool POW2> static void launch_tiles(const ProductArgs& g, hipStream_t st) {
     const unsigned tn = cdiv(g.cols, GATED ? 64 : 128);
     if constexpr (PB == 2) if ((size_t)tn * cdiv(g.rows, 128) >= 256) {
-        hipLaunchKernelGGL((k_product<GATED, PB, 2, POW2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((k_product<GATED, PB, 2, 2, POW2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
         return;
     }
-    hipLaunchKernelGGL((k_product<GATED, PB, 1, POW2>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
+    if constexpr (!GATED) if ((size_t)tn * cdiv(g.rows, 64) <= 128) {
+        hipLaunchKernelGGL((k_product<GATED, PB, 1, 1, POW2>), dim3(cdiv(g.cols, 64), cdiv(g.rows, 64)), dim3(256), 0, st, g);
+        return;
+    }
+    hipLaunchKernelGGL((k_product<GATED, PB, 1, 2, POW2>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
 }
 // Strips of one row of tiles: with one for every compute unit at most, eight waves of a workgroup share its contraction; with more, four, and two workgroups of them lie on a
 // unit, so that one's loads go on while the other adds up (one row of both 4096 x 11008 weights, 688 strips: 42 us with eight, 36 with four; of 11008 x 4096, 256
@@ -924,16 +928,16 @@ template <bool GATED, int PB> static void launch_row(const ProductArgs& g, hipSt
     if (strips > STRIPS_EACH) hipLaunchKernelGGL((k_product_row<GATED, PB, 4>), dim3(strips), dim3(256), 0, st, g);
     else hipLaunchKernelGGL((k_product_row<GATED, PB, 8>), dim3(strips), dim3(512), 0, st, g);
 }
-// Rows beyond SPLIT_ROWS.  Strips read every weight once for 16 or 32 rows, whatever their number; tiles make better use of what they read, but one takes a compute
-// unit a quarter of a microsecond for 32 contraction bytes, so that they need to be many.  4096 x 4096: 64 rows (32 tiles) 19 us in strips and 34 in tiles, 128 rows (64
-// tiles) 28 and 35, 256 rows (128 tiles) 49 and 35; one block of 32 rows of 4096 x 11008 (86 tiles) 32 and 41, of both such weights (172) 57 and 51.
+// Rows beyond SPLIT_ROWS.  Strips read every weight once for 16 or 32 rows, whatever their number; tiles make better use of what they read, but each takes a compute unit a
+// sixth of a microsecond and more for 32 contraction bytes, however few there are, so the count of strips decides.  4096 x 4096, strips and tiles: 64 rows (512 strips) 19 us
+// and 26, 96 rows (768) 24 and 26, 128 rows (1024) 28 and 26; 32 rows of 4096 x 11008 (688) 33 and 34, 64 rows (1376) 54 and 36.  Of both such weights, whose strips cost twice
+// and whose tiles are no wider: 64 rows of 4096 x 4096 28 and 37, 96 rows 37 and 37, 32 rows of 4096 x 11008 57 and 51.
 template <bool GATED, int PB> static void launch_product(const ProductArgs& g, hipStream_t st) {
     const unsigned row_blocks = cdiv(g.rows, 32), strips = (cdiv(g.cols, 16) + 7) / 8 * 8;
-    const size_t tiles = (size_t)cdiv(g.cols, GATED ? 64 : 128) * cdiv(g.rows, 64);
     if (g.rows <= 16) {
         if (strips > STRIPS_EACH) hipLaunchKernelGGL((k_product_strip<GATED, PB, 1, 4>), dim3(strips), dim3(256), 0, st, g, 1u);
         else hipLaunchKernelGGL((k_product_strip<GATED, PB, 1, 8>), dim3(strips), dim3(512), 0, st, g, 1u);
-    } else if (tiles < (g.rows <= 32 ? 128u : 80u)) hipLaunchKernelGGL((k_product_strip<GATED, PB, 2, 8>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
+    } else if ((size_t)strips * row_blocks < (GATED ? 640u : 1024u)) hipLaunchKernelGGL((k_product_strip<GATED, PB, 2, 8>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
     else if (g.e.pow2) launch_tiles<GATED, PB, true>(g, st);
     else launch_tiles<GATED, PB, false>(g, st);
 }
