@@ -491,7 +491,7 @@ int zk_softmax_shift_decompose_i64(void* shift, void* out_shifted, void* const* 
  *   r = the nearest integer to scale / sqrt(sum_j (v_j / scale)^2 / cols + eps), the sum in double precision as zk_row_sumsq_f64 takes it.
  * x, b: rows of cols int32, ldx and ldb elements apart; b null: h = x (post and gate null then).  post null: b itself; gate: gate_rows rows of cols
  * int32, row i for rows / gate_rows rows of x each, or null and 0; res: the residual scale, sf for 1.  h, n (rows * cols), rms_inv (rows; r of h): each may be null; h or
- * n may be x or b themselves where the rows are cols apart.  n needs w; w is not read without n.  scale / sqrt(eps) below 2^31. */
+ * n may be x or b themselves where the rows are cols apart, and overlap nothing else.  n needs w; w is not read without n.  scale / sqrt(eps) below 2^31, at most 2^24 columns. */
 int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t ldx, const void* b, size_t ldb, const void* post, const void* gate, uint32_t gate_rows, int32_t res,
                          const void* w, uint32_t rows, uint32_t cols, double eps, double scale, uint32_t sf, void* flag_dev, void* stream);
 /* Rotary positions (llama-self-attn.py:42-73, in fixed point): the first rot of a head's dim elements are rot / 2 pairs, pair i of a token at position p
@@ -506,7 +506,7 @@ int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size
                const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
 /* The table of angles: table[p][i] = the nearest integers to sf magnitude cos(p f_i) and sf magnitude sin(p f_i), p < rows, f_i = base^(-2 i / rot) / factor.
  * original > 0 (long contexts): only what is slow is slowed down -- f_i that turns high times or more over `original` positions is left alone, one that turns low times
- * or less divided by the factor, those between in proportion.  Double precision, correctly rounded operations in a fixed order: the same table everywhere. */
+ * or less divided by the factor, those between in proportion.  rows up to 2^31, times the factor where that is below 1.  Double precision, correctly rounded operations in a fixed order: the same table everywhere. */
 int zk_rope_table(void* table_i32, uint32_t rows, uint32_t rot, double base, double factor, double original, double low, double high, double magnitude, uint32_t sf, void* stream);
 /* out[token][head][k] = q_second(q_first(in[head][token][k])): field elements that stand for integers up to 2^62 (attention's products with the values) to
  * int32 with the two quotients of self-attn.cu:96-98; with one head and factors of 1 the int32 form of a tensor. */

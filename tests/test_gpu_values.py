@@ -775,6 +775,27 @@ def test_rope_refusals(name, change, text):
     assert text in pkg.load_hip().zk_last_error().decode()
 
 
+# tensors that one kernel would read and write at once, and sizes that its counters do not hold
+@pytest.mark.parametrize("change,text", [
+    ({"h": "x", "ldx": 5}, "cols apart"), ({"n": "x", "ldx": 5}, "cols apart"), ({"h": "b", "ldb": 5}, "cols apart"), ({"n": "b", "ldb": 5}, "cols apart"), ({"h": "n"}, "one tensor"),
+    ({"cols": (1 << 24) + 1, "ldx": 1 << 25, "ldb": 1 << 25}, "2^24 columns"), ({"cols": 0xFFFFFFFF, "ldx": 1 << 32, "ldb": 1 << 32}, "2^24 columns")])
+def test_norm_refuses_overlaps(change, text):
+    a = {k: (ctypes.c_int32 * 64)() for k in ("h", "n", "r", "x", "b", "w")} | {"ldx": 4, "ldb": 4, "cols": 4}
+    a.update({k: a[v] if isinstance(v, str) else v for k, v in change.items()})
+    refused("zk_i32_residual_norm", [a["h"], a["n"], a["r"], a["x"], c_size_t(a["ldx"]), a["b"], c_size_t(a["ldb"]), None, None, c_uint(0), c_int(1), a["w"], c_uint(6), c_uint(a["cols"]), c_double(1e-5),
+                                     c_double(65536.0), c_uint(65536), W, None], text)
+
+
+@pytest.mark.parametrize("heads,tokens,dim", [(1 << 16, 1 << 16, 1), (0x80000000, 0x80000000, 4), (1, 1, 0xFFFFFF01), (1 << 31, 1 << 31, 1 << 31)])
+def test_from_heads_refuses_sizes(heads, tokens, dim):
+    refused("zk_i32_from_heads", [W, (ctypes.c_int32 * 64)(), c_uint(heads), c_uint(tokens), c_uint(dim), c_uint(1), c_uint(1), W, None], "more elements")
+
+
+@pytest.mark.parametrize("rows,factor", [(2148, 1e-6), ((1 << 31) + 1, 1.0), (1 << 31, 0.5)])
+def test_table_refuses_angles(rows, factor):
+    refused("zk_rope_table", [W, c_uint(rows), c_uint(2), c_double(10000.0), c_double(factor), c_double(0.0), c_double(1.0), c_double(4.0), c_double(1.0), c_uint(65536), None], "zk_rope_table: ")
+
+
 def test_product_refusals():
     refused("zk_i32_linear", [W, W, c_size_t(4), None, c_uint(1), c_uint(1), None, c_size_t(0), W, None], "zk_i32_linear: null weight")
     refused("zk_i32_gated", [W, W, c_size_t(4), None, None, c_uint(1), c_uint(1), c_uint(1), W, c_int(0), c_uint(4), c_uint(1), None, c_size_t(0), W, None], "zk_i32_gated: null weight")

@@ -161,6 +161,16 @@ def test_values_of_a_wider_layer_with_kept_weights(pv):
     pv.layer_free(layer)
 
 
+@pytest.mark.parametrize("base", [-10000.0, 0.5, float("nan")])
+def test_a_base_that_is_none_is_refused(pv, base):
+    cu, cf = layercfg.tiny(open_weights=False)
+    layer = pv.layer_create(cu, cf, layercfg.tiny_weights(1, cu), 1)
+    set_rope(pv, layer, base=base)
+    with pytest.raises(RuntimeError, match="the base must lie above 1"):
+        values(pv, layer, np.zeros((int(cu[0]), int(cu[1])), np.int32))
+    pv.layer_free(layer)
+
+
 @pytest.mark.parametrize("head_group", [0, 1, 2])
 @pytest.mark.parametrize("rope", ROPES[1:])
 def test_positions_in_the_proof_are_those_of_rotated_queries_and_keys(pv, hip, head_group, rope):

@@ -943,6 +943,7 @@ template <bool GATED, int PB> static void launch_product(const ProductArgs& g, h
 }
 template <bool GATED> static int product(const char* name, ProductArgs& g, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
     ZK_ARG(g.x != nullptr && g.e.out != nullptr, std::string(name) + ": null tensor");
+    ZK_ARG(g.x != g.e.out, std::string(name) + ": in place");
     ZK_ARG(g.ldx >= g.inner, std::string(name) + ": rows of x overlap (ldx below the inner dimension)");
     ZK_ARG(g.rows <= (1u << 18), std::string(name) + ": more than 262144 rows in one call");
     ZK_ARG(g.cols <= (1u << 22), std::string(name) + ": more than 4194304 columns");
@@ -1007,6 +1008,10 @@ int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t 
     ZK_ARG((gate == nullptr) == (gate_rows == 0) && (gate == nullptr || rows % gate_rows == 0), "zk_i32_residual_norm: gate_rows must divide rows, and be 0 without a gate");
     ZK_ARG(sf > 0, "zk_i32_residual_norm: a scaling factor of 0");
     ZK_ARG(scale > 0 && eps > 0 && scale <= 1e18 && scale >= 1e-18 && scale / std::sqrt(eps) <= 2147483000.0, "zk_i32_residual_norm: scale and eps must be positive, scale / sqrt(eps) below 2^31");
+    ZK_ARG(cols <= (1u << 24), "zk_i32_residual_norm: rows of more than 2^24 columns");
+    auto with_x = [&](const void* out) { return out == nullptr || rows == 1 || ((out != x || ldx == cols) && (out != b || ldb == cols)); };
+    ZK_ARG(with_x(h) && with_x(n), "zk_i32_residual_norm: in place, rows must be cols apart");
+    ZK_ARG(h == nullptr || h != n, "zk_i32_residual_norm: h and n are one tensor");
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, "zk_i32_residual_norm")) return rc;
@@ -1075,6 +1080,7 @@ int zk_rope_table(void* table, uint32_t rows, uint32_t rot, double base, double 
     ZK_ARG(table != nullptr && rot % 2 == 0, "zk_rope_table: null table or an odd part of the head");
     ZK_ARG((size_t)rows * (rot / 2) <= 0x7FFFFFFFu, "zk_rope_table: more than 2^31 entries");
     ZK_ARG(base > 1 && base <= 1e15 && factor > 0 && factor >= 1e-6 && factor <= 1e6, "zk_rope_table: the base must lie above 1 (up to 1e15), the factor within 1e-6 .. 1e6");
+    ZK_ARG((double)rows <= 2147483648.0 * std::min(factor, 1.0), "zk_rope_table: a last angle beyond 2^31");
     ZK_ARG(original == 0 || (original > 0 && original <= 1e15 && low >= 0 && high > low && high <= 1e15), "zk_rope_table: with original positions, 0 <= low < high");
     ZK_ARG(sf > 0 && magnitude > 0 && magnitude * (double)sf <= 1073741824.0, "zk_rope_table: scale times magnitude must lie within 2^30");
     hipLaunchKernelGGL(k_rope_table, dim3(cdiv((size_t)rows * (rot / 2), 256)), dim3(256), 0, (hipStream_t)stv, (int2*)table, rows, rot / 2,
@@ -1083,11 +1089,11 @@ int zk_rope_table(void* table, uint32_t rows, uint32_t rot, double base, double 
     return 0;
 }
 int zk_i32_from_heads(void* out, const void* in, uint32_t heads, uint32_t tokens, uint32_t dim, uint32_t sf_first, uint32_t sf_second, void* flag_dev, void* stv) {
-    const size_t n = (size_t)heads * tokens * dim;
-    if (n == 0) return 0;
+    if (heads == 0 || tokens == 0 || dim == 0) return 0;
     ZK_ARG(out != nullptr && in != nullptr && out != in, "zk_i32_from_heads: null tensor or in place");
     ZK_ARG(sf_first > 0 && sf_second > 0, "zk_i32_from_heads: a scaling factor of 0");
-    ZK_ARG(n <= 0xFFFFFF00u, "zk_i32_from_heads: more elements than a tensor has");
+    ZK_ARG((unsigned __int128)heads * tokens * dim <= 0xFFFFFF00u, "zk_i32_from_heads: more elements than a tensor has");
+    const size_t n = (size_t)heads * tokens * dim;
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, "zk_i32_from_heads")) return rc;

@@ -242,7 +242,7 @@ const FrTensor& AttnStackBlock::forward() {
     const uint seq = c.seq_len, E = c.embed_dim, H = c.num_heads, d = E / H;
     // seq x embed -> embed x seq = [head][d][seq] -> [head][seq][d]
     auto to_stack = [&](const FrTensor& t) { return t.swap_leading_axes(seq, H, d); };          // = t.transpose(seq, E).transpose_stack(H, d, seq)
-    if (c.rope.base > 0) {      // the positions on the way to the stack
+    if (c.rope.base != 0) {      // the positions on the way to the stack
         rotary.emplace(c.rope, seq, d);
         Qs.emplace((*rotary)(Q_, H, true));
         Ks.emplace((*rotary)(K_, H, true));
@@ -299,7 +299,7 @@ FrTensor attn_heads_block(const LayerConfig& c, const FrTensor& Q_, const FrTens
         b.finish();
         return std::move(*b.out__);
     }
-    if (c.rope.base > 0) {
+    if (c.rope.base != 0) {
         Rotary rotary(c.rope, seq, d);
         const FrTensor Qr = rotary(Q_, H, false), Kr = rotary(K_, H, false);
         rotary.check();
@@ -410,7 +410,7 @@ FrTensor attn_heads_block(const LayerConfig& c, const FrTensor& Q_, const FrTens
 FrTensor attn_reference_block(const LayerConfig& c, const FrTensor& Q, const FrTensor& K, const FrTensor& V, std::unique_ptr<FrTensor>* softmax_out) {
     const uint seq_len = c.seq_len;
     if (seq_len == 0 || Q.size % seq_len || K.size != Q.size || V.size != Q.size) throw std::runtime_error("attn: Q, K, V must be seq_len x d");
-    if (c.rope.base > 0) throw std::runtime_error("attn: rotary positions need heads (ZKLLM_ATTN_HEADS); as one head the reference's statement has none");
+    if (c.rope.base != 0) throw std::runtime_error("attn: rotary positions need heads (ZKLLM_ATTN_HEADS); as one head the reference's statement has none");
     const uint d = Q.size / seq_len;
     auto X = FrTensor::matmul(Q, K.transpose(seq_len, d), seq_len, d, seq_len);
     zkSoftmax softmax(c.softmax_bs, c.softmax_L, c.softmax_M, c.softmax_sf_in, c.softmax_thetas, seq_len, seq_len, d, 1);

@@ -57,7 +57,7 @@ IntTensor LayerValues::operator()(const IntTensor& X) const {
     {
         IntTensor stack(T * E);
         std::optional<Rotary> rotary;
-        if (c.rope.base > 0) rotary.emplace(c.rope, T, d);
+        if (c.rope.base != 0) rotary.emplace(c.rope, T, d);
         auto part = [&](FrTensor& out, const Rhs& weight, bool positions) {
             linear(proj.gpu_data, n1.gpu_data, E, weight);
             if (positions && rotary) rotary->rotate(stack.gpu_data, proj.gpu_data, H, true, flag.dev());
