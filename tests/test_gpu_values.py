@@ -558,6 +558,43 @@ def test_gated_in_tiles(hip, dev, rows, inner, cols, weights, general):
     assert (got == exp)[fits].all() and (general or flag == 0)
 
 
+# Long contractions with few tiles, which are split over workgroups (more than 32 rows, two digits a weight), in parts of several lengths; and their neighbours, which are not
+LONG = [(33, 8065, 70), (64, 11008, 130), (150, 8300, 650), (1000, 8200, 40), (32, 8200, 70), (33, 8064, 70)]
+
+
+@gpu
+@pytest.mark.parametrize("rows,inner,cols", LONG)
+@pytest.mark.parametrize("most,sf", [(127, 1 << 16), (32639, 1 << 29), (32639, (1 << 29) - 3)])
+@pytest.mark.parametrize("digits", ["three", "some", "all"])
+def test_linear_of_long_rows(hip, dev, rows, inner, cols, most, sf, digits):
+    test_linear_in_tiles(hip, dev, rows, inner, cols, most, sf, digits)
+
+
+@gpu
+@pytest.mark.parametrize("rows,inner,cols", LONG)
+@pytest.mark.parametrize("weights", [(30000, 30000), (120, 8355711)])
+@pytest.mark.parametrize("general", [False, True])
+def test_gated_of_long_rows(hip, dev, rows, inner, cols, weights, general):
+    test_gated_in_tiles(hip, dev, rows, inner, cols, weights, general)
+
+
+# the parts of one sum: all of it in one part or another, and the largest that there is
+@gpu
+def test_edges_of_long_rows(hip, dev):
+    inner, cols, rows = 16384, 70, 40
+    w = np.full((inner, cols), 32639, np.int32)
+    weight = Weight(hip, dev, w)
+    x = np.zeros((rows, inner), np.int32)
+    for r in range(rows):
+        x[r, r * 420:r * 420 + 3] = (1 << 30, -(1 << 30), 1 + r)
+    got, flag = call_linear(hip, dev, x, weight, cols, 1)
+    assert flag == 0 and (got == ref.linear(x, w, 1)).all()
+    x[rows - 1] = -(1 << 31)
+    sf = 0xFFFFFFFF
+    got, flag = call_linear(hip, dev, x, weight, cols, sf)           # 2^31 2^14 32639 is the largest sum that two digits of weights have at this length
+    assert flag == 0 and (got == ref.linear(x, w, sf)).all()
+
+
 # sums around 2^62 and values around the edges of int32 and the table, in the last row and column of the last tile; x's rows and the weight's columns beyond them do not count
 @gpu
 @pytest.mark.parametrize("rows", [321, 2200])

@@ -405,6 +405,7 @@ struct ProductArgs {
     const uint32_t* need;
     const int8_t* zeros;                 // 1 KB
     uint32_t rows_padded, chunks;
+    int64_t* parts;                      // a split contraction's sums, [part][weight][row][column]
     Epilogue e;
 };
 static constexpr uint32_t CHUNK = 256;
@@ -495,18 +496,21 @@ __global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __
     raise(g.e.flag, bad);
 }
 
+// What becomes of a tile's sums: outputs, by divisors that are powers of two or any, or parts of sums
+enum class End { POW2, ANY, PARTS };
 // Many rows.  A workgroup of four waves takes 64 MT rows by 64 NQ columns of weights -- with NQ = 2 64 of each where there are two: a wave's gate and up tiles lie in the same
 // lanes, and what joins them needs no exchange -- and a wave 32 MT by 32 NQ, as 32 x 32 tiles of v_mfma_i32_32x32x32_i8.
 // Steps of 32 contraction bytes go from memory to LDS without passing through registers, four buffers deep; a step's fragments are read while the step before
 // is multiplied, since one wave a SIMD (256 accumulators with MT = 2) has nobody to cover for it.
 // 2048 x 4096 x 4096, three planes by two: 156 us; both 4096 x 11008 weights at 2048 rows 860, 2.55 POP/s (the library's int8 product of 8192^3: 2.05).  The matrix units are
 // busy 65 % of the cycles, at 1.75 to 1.85 GHz: the card's power holds the clock there (the same without the loads from memory, on what lies in LDS, 2.3 GHz and 570 us), and what
-// saves stalls costs clock.  Steps of 64 bytes (61 us against 41 for 64 rows of 4096 x 11008), eight buffers (47), the next tile's first steps ahead of a tile's outputs (936
+// saves stalls costs clock.  Steps of 64 bytes (61 us against 41 for 64 rows of 4096 x 11008 in tiles of 128 columns), eight buffers (47), the next tile's first steps ahead of a tile's outputs (936
 // against 895 for the whole) and other orders of the products or tiles (within 1 %) gained nothing.
 template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
     static constexpr int NS = PA + PB - 1, TM = 64 * MT, TN = 64 * NQ, PIECES = PA * 2 * MT + PB * 2 * NQ, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * TN) * 32;
     v16i acc[NS][MT][NQ];
-    __device__ __forceinline__ void multiply(const ProductArgs& g, uint32_t m0, uint32_t n0, int8_t* const (&buf)[4]) {
+    // steps first .. first + steps - 1 of the contraction, a multiple of four
+    __device__ __forceinline__ void multiply(const ProductArgs& g, uint32_t m0, uint32_t n0, uint32_t first, uint32_t steps, int8_t* const (&buf)[4]) {
         const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), wm = wave >> 1, wn = wave & 1;
 #pragma unroll
         for (int s = 0; s < NS; ++s)
@@ -531,16 +535,17 @@ template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
                 dst[i] = (plane * TM + r) * 32;
                 step[i] = (size_t)g.rows_padded * 32;
             } else {
-                const uint32_t cb = c - PA * 2 * MT, plane = cb / (2 * NQ), r = cb % (2 * NQ) * 32, first = n0 + (GATED ? r & 63u : r);
+                const uint32_t cb = c - PA * 2 * MT, plane = cb / (2 * NQ), r = cb % (2 * NQ) * 32, row = n0 + (GATED ? r & 63u : r);
                 const Planes& w = GATED && r < 64 ? g.gate : g.w;
-                const bool has = (int)plane < w.n, inside = first < w.rows;
-                src[i] = has ? w.p + (size_t)plane * w.rows * w.Kp + (size_t)(inside ? first : w.rows - 1) * 32 : g.zeros;
-                at[i] = (has && inside ? min(lr, w.rows - 1 - first) : 0u) * 32 + lane_half;
+                const bool has = (int)plane < w.n, inside = row < w.rows;
+                src[i] = has ? w.p + (size_t)plane * w.rows * w.Kp + (size_t)(inside ? row : w.rows - 1) * 32 : g.zeros;
+                at[i] = (has && inside ? min(lr, w.rows - 1 - row) : 0u) * 32 + lane_half;
                 dst[i] = (PA * TM + plane * TN + r) * 32;
                 step[i] = has ? (size_t)w.rows * 32 : 0;
             }
+            src[i] += step[i] * first;
         }
-        const uint32_t half = lane >> 5, steps = g.w.Kp / 32;
+        const uint32_t half = lane >> 5;
         const uint32_t rowA = wm * 32 * MT + (lane & 31), at_a = rowA * 32 + gemm_half(rowA, half) * 16;
         const uint32_t rowB = wn * (GATED ? 32 : 32 * NQ) + (lane & 31), next_b = GATED ? 64 : 32, at_b = (PA * TM + rowB) * 32 + gemm_half(rowB, half) * 16;      // 32 rows on: the same halves
         uint32_t fetched = 1;
@@ -604,7 +609,7 @@ template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
         for (int i = 0; i < 4; ++i) fetch(buf[i]);
         arrived(three);
         read(buf[0], even);
-        for (uint32_t t = 0; t < steps; t += 4) {              // Kp is a multiple of 128
+        for (uint32_t t = 0; t < steps; t += 4) {
             arrived(two); fetch(buf[0]); read(buf[1], odd); products(even); spread();
             arrived(two); fetch(buf[1]); read(buf[2], even); products(odd); spread();
             arrived(two); fetch(buf[2]); read(buf[3], odd); products(even); spread();
@@ -616,7 +621,8 @@ template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
     // The outputs, eight rows at a time: all their places in the table first, then the table's values, so that one wait covers them.  Stores go through a buffer
     // that ends with the last row, and a column beyond the last has no place in it.  (Such a column repeats the last and a row beyond the last is zeros: of the flags only the
     // table's needs to know.)
-    template <bool POW2> __device__ __forceinline__ void finish(const ProductArgs& g, uint32_t m0, uint32_t n0, uint32_t& bad) {
+    template <End END> __device__ __forceinline__ void finish(const ProductArgs& g, uint32_t m0, uint32_t n0, uint32_t& bad) {
+        constexpr bool POW2 = END == End::POW2;
         const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave >> 1, wn = wave & 1;
         auto value = [&](int m, int q, int r) {
             int32_t a[NS];
@@ -628,6 +634,21 @@ template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
             return joined<NS>(a, bad);
         };
         const uint32_t rows_here = m0 < g.rows ? min(g.rows - m0, (uint32_t)TM) : 0;
+        if constexpr (END == End::PARTS) {
+            const size_t weight = (size_t)g.rows * g.cols;
+            int64_t* out = g.parts + (size_t)blockIdx.z * (GATED ? 2 : 1) * weight;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint32_t row = (wm * MT + m) * 32 + 4 * (lane >> 5) + 8 * (r >> 2) + (r & 3), col = n0 + (GATED ? wn * 32 : wn * 32 * NQ + q * 32) + (lane & 31);
+                        const int64_t v = value(m, q, r);
+                        if (row < rows_here && col < g.cols) out[(GATED ? q * weight : 0) + (size_t)(m0 + row) * g.cols + col] = v;
+                    }
+            return;
+        }
         const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(g.e.out + (size_t)m0 * g.cols, 0, rows_here * g.cols * 4, 0x00027000);      // raw: plain bytes
         auto store = [&](uint32_t row, uint32_t col, int32_t y) { __builtin_amdgcn_raw_buffer_store_b32(y, out, n0 + col < g.cols ? (row * g.cols + n0 + col) * 4 : 0xFFFFFFFFu, 0, 0); };
 #pragma unroll
@@ -665,8 +686,7 @@ template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
         }
     }
 };
-// POW2: every divisor of the call is a power of two
-template <bool GATED, int PB, int MT, int NQ, bool POW2> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
+template <bool GATED, int PB, int MT, int NQ, End END> __global__ void __launch_bounds__(256, MT == 2 || PB == 3 ? 1 : 2) k_product(const ProductArgs g) {
     constexpr int BYTES = Tile<GATED, 3, PB, MT, NQ>::BYTES > Tile<GATED, 4, PB, 1, NQ>::BYTES ? Tile<GATED, 3, PB, MT, NQ>::BYTES : Tile<GATED, 4, PB, 1, NQ>::BYTES;
     // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
     __shared__ __attribute__((aligned(16))) int8_t s0[BYTES], s1[BYTES], s2[BYTES], s3[BYTES];
@@ -684,18 +704,38 @@ template <bool GATED, int PB, int MT, int NQ, bool POW2> __global__ void __launc
     uint32_t need = 0, bad = 0;
     for (uint32_t i = threadIdx.x & 63u; i < 2 * MT * g.chunks; i += 64) need = max(need, g.need[(size_t)(m0 / 32) * g.chunks + i]);
     const bool wide = __any(need > 3);
+    const uint32_t fours = g.w.Kp / 128, first = END == End::PARTS ? fours * blockIdx.z / gridDim.z * 4 : 0, steps = END == End::PARTS ? fours * (blockIdx.z + 1) / gridDim.z * 4 - first : fours * 4;
     int8_t* const buf[4] = {s0, s1, s2, s3};
     if (!wide) {
         Tile<GATED, 3, PB, MT, NQ> t;
-        t.multiply(g, m0, n0, buf);
-        t.template finish<POW2>(g, m0, n0, bad);
+        t.multiply(g, m0, n0, first, steps, buf);
+        t.template finish<END>(g, m0, n0, bad);
     } else {                                   // a value of more than three digits: all four planes, 64 rows at a time
         for (uint32_t m = m0; m < m0 + 64 * MT; m += 64) {
             Tile<GATED, 4, PB, 1, NQ> t;
-            t.multiply(g, m, n0, buf);
-            t.template finish<POW2>(g, m, n0, bad);
+            t.multiply(g, m, n0, first, steps, buf);
+            t.template finish<END>(g, m, n0, bad);
         }
     }
+    raise(g.e.flag, bad);
+}
+
+// The parts' sums added up, an output a lane: 64 rows of 4096 columns in four parts, 8 MB out of the caches, 4 us with its launch
+template <bool GATED, bool POW2> __global__ void __launch_bounds__(256) k_product_join(const ProductArgs g, uint32_t parts) {
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, total = g.rows * g.cols;
+    if (id >= total) return;
+    constexpr int MATS = GATED ? 2 : 1;
+    int64_t v[MATS];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m) v[m] = 0;
+    for (uint32_t p = 0; p < parts; ++p)
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) v[m] += g.parts[((size_t)p * MATS + m) * total + id];
+    uint32_t bad = 0;
+    if constexpr (GATED) {
+        const uint32_t at = activation_at<POW2>(v[0], g.e, bad);
+        g.e.out[id] = gated_value<POW2>(at == g.e.len ? 0 : g.e.table[at], v[1], g.e, bad);
+    } else g.e.out[id] = narrow(quotient<POW2>(v[0], g.e.sf), bad);
     raise(g.e.flag, bad);
 }
 
@@ -905,19 +945,35 @@ static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->pl
 // Up to here a product is one launch that splits x itself: 16 rows of 4096 x 11008 40 us so and 28 with a launch of k_split_x before, 4 rows 24 and 28.
 static constexpr uint32_t SPLIT_ROWS = 4;
 static size_t padded_rows(uint32_t rows) { return ((size_t)rows + 127) / 128 * 128; }
+// A long contraction with few tiles is split, so that every compute unit has a part of one: from 8192 on and for 33 rows and more, where neither strips nor tiles fill the card.
+// 64 rows of 11008 x 4096 36 us (strips 48, whole tiles 81), 128 rows 53 (81), of both such weights 62 (75 in strips) and 80 (104); of 4096 x 4096 the second launch
+// takes what the first gains (64 rows 19 either way, 128 rows 25 and 26; of two weights 34 and 28).  Two planes of weights: a part's sum stays in 64 bits then.
+static constexpr size_t PARTS_BYTES = (size_t)16 << 20;
+static bool may_split(uint32_t rows, uint32_t inner) { return rows > 32 && inner > 8064; }
+static unsigned parts_of(const ProductArgs& g, size_t weights) {
+    if (g.parts == nullptr) return 1;
+    const size_t tiles = (size_t)cdiv(g.cols, 64) * cdiv(g.rows, 64), each = weights * g.rows * g.cols * sizeof(int64_t);
+    return (unsigned)std::min<size_t>({256 / tiles, g.w.Kp / 512, PARTS_BYTES / each});
+}
 // Tiles of 128 rows where there is one for every compute unit (2048 x 4096 x 4096: 156 us, with 64 rows 165); a third plane of weights has no registers for that.
 // Half as wide where every tile then finds a unit of its own (64 rows of 4096 x 11008, 86 tiles: 42 us and 36; 256 rows of 4096 x 4096, 128 tiles: 35 and 32; 384 rows, 192 tiles: 41 and 46).
 template <bool GATED, int PB, bool POW2> static void launch_tiles(const ProductArgs& g, hipStream_t st) {
+    constexpr End END = POW2 ? End::POW2 : End::ANY;
     const unsigned tn = cdiv(g.cols, GATED ? 64 : 128);
     if constexpr (PB == 2) if ((size_t)tn * cdiv(g.rows, 128) >= 256) {
-        hipLaunchKernelGGL((k_product<GATED, PB, 2, 2, POW2>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((k_product<GATED, PB, 2, 2, END>), dim3(tn, cdiv(g.rows, 128)), dim3(256), 0, st, g);
+        return;
+    }
+    if constexpr (PB == 2) if (const unsigned parts = parts_of(g, GATED ? 2 : 1); parts > 1) {
+        hipLaunchKernelGGL((k_product<GATED, PB, 1, GATED ? 2 : 1, End::PARTS>), dim3(cdiv(g.cols, 64), cdiv(g.rows, 64), parts), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((k_product_join<GATED, POW2>), dim3(cdiv((size_t)g.rows * g.cols, 256)), dim3(256), 0, st, g, parts);
         return;
     }
     if constexpr (!GATED) if ((size_t)tn * cdiv(g.rows, 64) <= 128) {
-        hipLaunchKernelGGL((k_product<GATED, PB, 1, 1, POW2>), dim3(cdiv(g.cols, 64), cdiv(g.rows, 64)), dim3(256), 0, st, g);
+        hipLaunchKernelGGL((k_product<GATED, PB, 1, 1, END>), dim3(cdiv(g.cols, 64), cdiv(g.rows, 64)), dim3(256), 0, st, g);
         return;
     }
-    hipLaunchKernelGGL((k_product<GATED, PB, 1, 2, POW2>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
+    hipLaunchKernelGGL((k_product<GATED, PB, 1, 2, END>), dim3(tn, cdiv(g.rows, 64)), dim3(256), 0, st, g);
 }
 // Strips of one row of tiles: with one for every compute unit at most, eight waves of a workgroup share its contraction; with more, four, and two workgroups of them lie on a
 // unit, so that one's loads go on while the other adds up (one row of both 4096 x 11008 weights, 688 strips: 42 us with eight, 36 with four; of 11008 x 4096, 256
@@ -937,7 +993,7 @@ template <bool GATED, int PB> static void launch_product(const ProductArgs& g, h
     if (g.rows <= 16) {
         if (strips > STRIPS_EACH) hipLaunchKernelGGL((k_product_strip<GATED, PB, 1, 4>), dim3(strips), dim3(256), 0, st, g, 1u);
         else hipLaunchKernelGGL((k_product_strip<GATED, PB, 1, 8>), dim3(strips), dim3(512), 0, st, g, 1u);
-    } else if ((size_t)strips * row_blocks < (GATED ? 640u : 1024u)) hipLaunchKernelGGL((k_product_strip<GATED, PB, 2, 8>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
+    } else if ((size_t)strips * row_blocks < (GATED ? 640u : 1024u) && !(PB == 2 && parts_of(g, GATED ? 2 : 1) > 1)) hipLaunchKernelGGL((k_product_strip<GATED, PB, 2, 8>), dim3(strips * row_blocks), dim3(512), 0, st, g, row_blocks);
     else if (g.e.pow2) launch_tiles<GATED, PB, true>(g, st);
     else launch_tiles<GATED, PB, false>(g, st);
 }
@@ -973,6 +1029,7 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, void*
     g.px = (const int8_t*)workspace;
     g.zeros = g.px + (size_t)4 * g.rows_padded * g.w.Kp;
     g.need = (const uint32_t*)(g.zeros + 1024);
+    g.parts = may_split(g.rows, g.inner) ? (int64_t*)((char*)workspace + bytes - PARTS_BYTES) : nullptr;
     hipLaunchKernelGGL(k_split_x, dim3(g.chunks, g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
     if (pb <= 2) launch_product<GATED, 2>(g, st);
     else launch_product<GATED, 3>(g, st);
@@ -1136,7 +1193,7 @@ int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, v
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner) {
     const size_t Kp = ((size_t)inner + GBK - 1) / GBK * GBK;
     if (rows <= SPLIT_ROWS) return 0;
-    return padded_rows(rows) * Kp * 4 + 1024 + padded_rows(rows) / 32 * ((Kp + CHUNK - 1) / CHUNK) * 4;
+    return padded_rows(rows) * Kp * 4 + 1024 + (padded_rows(rows) / 32 * ((Kp + CHUNK - 1) / CHUNK) * 4 + 15) / 16 * 16 + (may_split(rows, inner) ? PARTS_BYTES : 0);
 }
 int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, uint32_t rows, uint32_t sf, void* workspace, size_t workspace_bytes, void* flag_dev, void* stv) {
     const MatmulRhs* w = (const MatmulRhs*)prepared;
