@@ -595,6 +595,17 @@ def test_edges_of_long_rows(hip, dev):
     assert flag == 0 and (got == ref.linear(x, w, sf)).all()
 
 
+@gpu
+def test_products_in_place_are_refused(hip, dev):
+    x = np.ones((6, 8), np.int32)
+    w, p, f = Weight(hip, dev, np.eye(8, dtype=np.int32)), dev.up(x), dev.flag()
+    with pytest.raises(RuntimeError, match="zk_i32_linear: in place"):
+        hip.call("zk_i32_linear", p, p, c_size_t(8), w.h, c_uint(6), c_uint(1), None, c_size_t(0), f, None)
+    with pytest.raises(RuntimeError, match="zk_i32_gated: in place"):
+        hip.call("zk_i32_gated", p, p, c_size_t(8), w.h, w.h, c_uint(6), c_uint(1), c_uint(1), dev.up(np.ones(4, np.int32)), c_int(0), c_uint(4), c_uint(1), None, c_size_t(0), f, None)
+    assert (dev.down(p, (6, 8)) == x).all()
+
+
 # sums around 2^62 and values around the edges of int32 and the table, in the last row and column of the last tile; x's rows and the weight's columns beyond them do not count
 @gpu
 @pytest.mark.parametrize("rows", [321, 2200])
@@ -771,6 +782,47 @@ def test_a_block_on_its_own_stream_and_captured(hip, dev, T):
     torch.cuda.synchronize()
     g.replay()
     check(states[0], exp)
+
+
+@gpu
+def test_long_rows_captured(hip, dev):
+    """Products whose contraction is split, both kinds in one graph with one workspace, replayed with new inputs and eager calls in between"""
+    import torch
+    T, K, P = 70, 8200, 130
+    rng = np.random.default_rng(1)
+    g, u = normal(rng, (K, P), 300.0), normal(rng, (K, P), 3000.0)
+    wg, wu = Weight(hip, dev, g), Weight(hip, dev, u)
+    low, n = -(1 << 16), 1 << 17
+    act = swiglu(low, n, 4096.0)
+    t = lambda a: torch.as_tensor(np.ascontiguousarray(a), device="cuda")
+    new = lambda *shape: torch.empty(shape, dtype=torch.int32, device="cuda")
+    hip.lib.zk_i32_linear_workspace.restype = c_size_t
+    room = hip.lib.zk_i32_linear_workspace(c_uint(T), c_uint(K))
+    state = lambda: {"x": new(T, K), "a": new(T, P), "b": new(T, P), "flag": torch.zeros(1, dtype=torch.int32, device="cuda"), "ws": torch.empty(room, dtype=torch.uint8, device="cuda"), "act": t(act)}
+    ptr = lambda a: c_void_p(a.data_ptr())
+
+    def step(s, stream):
+        st = c_void_p(stream.cuda_stream)
+        hip.call("zk_i32_linear", ptr(s["a"]), ptr(s["x"]), c_size_t(K), wu.h, c_uint(T), c_uint(1 << 16), ptr(s["ws"]), c_size_t(room), ptr(s["flag"]), st)
+        hip.call("zk_i32_gated", ptr(s["b"]), ptr(s["x"]), c_size_t(K), wg.h, wu.h, c_uint(T), c_uint(1 << 16), c_uint(1 << 16), ptr(s["act"]), c_int(low), c_uint(n), c_uint(1 << 16), ptr(s["ws"]),
+                 c_size_t(room), ptr(s["flag"]), st)
+
+    def turn(s, run):
+        x = normal(rng, (T, K), 3000.0)
+        s["x"].copy_(t(x))
+        torch.cuda.synchronize()
+        run()
+        torch.cuda.synchronize()
+        assert int(s["flag"]) == 0
+        assert (s["a"].cpu().numpy() == ref.linear(x, u, 1 << 16)).all() and (s["b"].cpu().numpy() == ref.gated(x, g, u, 1 << 16, 1 << 16, act, low, 1 << 16)).all()
+
+    stream, s, eager = torch.cuda.Stream(), state(), state()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(s, stream)
+    for _ in range(3):
+        turn(s, graph.replay)
+        turn(eager, lambda: step(eager, torch.cuda.current_stream()))
 
 
 # ---- refusals: nothing of these reaches a GPU ----------------------------------------------------------------------------------------------------------------
