@@ -314,6 +314,59 @@ def test_rope_values_that_do_not_fit_raise_the_flag(hip, dev):
         assert call_rope(hip, dev, y, table, 4, 0, fr=True)[1] == ref.RANGE
 
 
+# integers as Python has them: what lies outside int32, the negatives beyond 64 bits among it, raises the flag and counts as 0
+OUTSIDE = [1 << 31, -(1 << 31) - 1, 1 << 62, -(1 << 62), (1 << 63) - 1, -(1 << 63), 1 << 63, -(1 << 63) - 1, 5 - (1 << 64), 1 - (1 << 64), (1 << 31) - 1 - (1 << 64), (1 << 31) - (1 << 64), (1 << 62) - (1 << 64),
+           (1 << 64) - 1, 1 << 64, -(1 << 64), -(1 << 64) - 5, 1 << 100, -(1 << 100), 7 - (1 << 200)]
+
+
+def call_fr_rope(hip, dev, x, table, rot, neighbours, sf=65536):
+    """x: [token][head][dim] of Python integers, positions 0, 1, ..."""
+    tokens, heads, dim = x.shape
+    out, f = dev.space(32 * x.size), dev.flag()
+    strides = (c_size_t(heads * dim), c_size_t(dim))
+    hip.call("zk_fr_rope", out, *strides, dev.up(ref.elements(x), np.uint32), *strides, c_uint(tokens), c_uint(heads), c_uint(dim), c_uint(rot), c_int(neighbours), dev.up(table), c_uint(len(table)), None,
+             c_uint(0), c_uint(sf), f, None)
+    hip.sync()
+    return dev.down(out, x.shape + (8,), np.uint32), int(dev.down(f, (1,), np.uint32)[0])
+
+
+@gpu
+@pytest.mark.parametrize("neighbours", [0, 1])
+@pytest.mark.parametrize("v", OUTSIDE)
+def test_rope_of_elements_that_are_no_32_bit_integers(hip, dev, v, neighbours):
+    x = normal(np.random.default_rng(1), (3, 2, 8)).astype(object)
+    table = angles(3, 8, 65536)
+    for at in ((0, 0, 1), (2, 1, 6)):
+        y, zeroed = x.copy(), x.copy()
+        y[at], zeroed[at] = v, 0
+        got, flag = call_fr_rope(hip, dev, y, table, 8, neighbours)
+        assert flag == ref.RANGE and (got == ref.elements(ref.rope(zeroed, table, np.arange(3), 8, neighbours, 65536))).all()
+    for edge in ((1 << 31) - 1, -(1 << 31)):
+        y = x.copy()
+        y[1, 1, 3] = edge
+        got, flag = call_fr_rope(hip, dev, y, table, 8, neighbours)
+        assert flag == 0 and (got == ref.elements(ref.rope(y, table, np.arange(3), 8, neighbours, 65536))).all()
+
+
+@gpu
+@pytest.mark.parametrize("v", [v for v in OUTSIDE if abs(v) > 1 << 62])
+def test_heads_of_elements_that_are_no_63_bit_integers(hip, dev, v):
+    x = normal(np.random.default_rng(2), (2, 3, 4)).astype(object)
+    out, f = dev.space(4 * x.size), dev.flag()
+
+    def call(x):
+        hip.call("zk_memset", f, c_int(0), c_size_t(4), None)
+        hip.call("zk_i32_from_heads", out, dev.up(ref.elements(x), np.uint32), c_uint(2), c_uint(3), c_uint(4), c_uint(1 << 16), c_uint(1 << 16), f, None)
+        return dev.down(out, (3, 2, 4)).astype(np.int64), int(dev.down(f, (1,), np.uint32)[0])
+
+    for edge in (1 << 62, -(1 << 62)):
+        x[1, 2, 3] = edge
+        got, flag = call(x)
+        assert flag == 0 and (got == ref.quotient(ref.quotient(x, 1 << 16), 1 << 16).swapaxes(0, 1)).all()
+    x[1, 2, 3] = v
+    assert call(x)[1] == ref.RANGE
+
+
 # ---- products with a kept weight ---------------------------------------------------------------------------------------------------------------------------
 class Weight:
     def __init__(self, hip, dev, w, from_fr=False):

@@ -282,11 +282,8 @@ __device__ __forceinline__ int2 angle(int2 cs, uint32_t& bad) {
 }
 __device__ __forceinline__ int64_t rope_get(const int32_t* p, uint32_t&) { return *p; }
 __device__ __forceinline__ int64_t rope_get(const Fr* p, uint32_t& bad) {
-    const Fr e = *p;
-    const int64_t v = fr_to_i64(e);
-    // an element that is no 32-bit integer: fr_to_i64 gives 0 for what does not fit 64 bits, and zero is told apart by its limbs
-    const bool zero = !(e.v[0] | e.v[1] | e.v[2] | e.v[3] | e.v[4] | e.v[5] | e.v[6] | e.v[7]);
-    if (v != (int64_t)(int32_t)v || (v == 0 && !zero)) { bad |= ZK_VALUES_RANGE; return 0; }
+    int64_t v;
+    if (!fr_fits_i64(*p, v) || v != (int64_t)(int32_t)v) { bad |= ZK_VALUES_RANGE; return 0; }
     return v;
 }
 __device__ __forceinline__ void rope_put(int32_t* p, int64_t v, uint32_t& bad) { *p = narrow(v, bad); }
@@ -362,11 +359,9 @@ __global__ void __launch_bounds__(256) k_i32_from_heads(int32_t* __restrict__ ou
     const size_t row = id / dim;
     const uint32_t j = (uint32_t)(id - row * dim);
     const uint32_t token = (uint32_t)(row / heads), head = (uint32_t)(row - (size_t)token * heads);
-    const Fr e = in[((size_t)head * tokens + token) * dim + j];
-    int64_t v = fr_to_i64(e);
+    int64_t v;
     uint32_t bad = 0;
-    const bool zero = !(e.v[0] | e.v[1] | e.v[2] | e.v[3] | e.v[4] | e.v[5] | e.v[6] | e.v[7]);
-    if (v > (1ll << 62) || v < -(1ll << 62) || (v == 0 && !zero)) { bad = ZK_VALUES_RANGE; v = 0; }      // fr_to_i64 gives 0 for what does not fit 64 bits
+    if (!fr_fits_i64(in[((size_t)head * tokens + token) * dim + j], v) || v > (1ll << 62) || v < -(1ll << 62)) { bad = ZK_VALUES_RANGE; v = 0; }
     v = first.shift >= 0 ? quotient<true>(v, first) : quotient<false>(v, first);
     v = second.shift >= 0 ? quotient<true>(v, second) : quotient<false>(v, second);
     out[id] = narrow(v, bad);
