@@ -348,6 +348,23 @@ def test_rope_of_elements_that_are_no_32_bit_integers(hip, dev, v, neighbours):
         assert flag == 0 and (got == ref.elements(ref.rope(y, table, np.arange(3), 8, neighbours, 65536))).all()
 
 
+# the same in the part of a head that is not rotated, and where no part is
+@gpu
+@pytest.mark.parametrize("rot", [0, 2, 4])
+@pytest.mark.parametrize("v", OUTSIDE)
+def test_rope_copies_only_elements_that_are_32_bit_integers(hip, dev, v, rot):
+    x = normal(np.random.default_rng(3), (3, 2, 7)).astype(object)
+    table = angles(3, rot, 65536)
+    for at in ((0, 0, 4), (2, 1, 6)):
+        y, zeroed = x.copy(), x.copy()
+        y[at], zeroed[at] = v, 0
+        got, flag = call_fr_rope(hip, dev, y, table, rot, 0)
+        assert flag == ref.RANGE and (got == ref.elements(ref.rope(zeroed, table, np.arange(3), rot, 0, 65536))).all()
+    x[0, 1, 5], x[1, 0, 6], x[2, 1, 4] = (1 << 31) - 1, -(1 << 31), 0
+    got, flag = call_fr_rope(hip, dev, x, table, rot, 0)
+    assert flag == 0 and (got == ref.elements(ref.rope(x, table, np.arange(3), rot, 0, 65536))).all()
+
+
 @gpu
 @pytest.mark.parametrize("v", [v for v in OUTSIDE if abs(v) > 1 << 62])
 def test_heads_of_elements_that_are_no_63_bit_integers(hip, dev, v):

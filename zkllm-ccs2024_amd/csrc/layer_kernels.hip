@@ -304,7 +304,7 @@ template <typename T, int VEC, bool POW2> __global__ void __launch_bounds__(256)
     else if (u >= groups) {
         const uint32_t i = a.rot + (u - groups) * VEC;
         if constexpr (VEC == 4) *reinterpret_cast<v4i*>(out + i) = *reinterpret_cast<const v4i*>(x + i);
-        else out[i] = x[i];
+        else rope_put(out + i, rope_get(x + i, bad), bad);
     } else if constexpr (VEC == 4) {
         const int2* cs = a.table + pos * pairs + 4 * u;
         const v4i c0 = *reinterpret_cast<const v4i*>(cs), c1 = *reinterpret_cast<const v4i*>(cs + 2);
