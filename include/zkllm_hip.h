@@ -208,7 +208,8 @@ int zk_fr_matmul_batched_i64_bt(void* C64, const void* A, const void* Bt, uint32
 /* The right operand of many products (a layer's weight in zkFC::operator(), zkfc.cu:44-58) examined once: its largest magnitude
  * for the small-integer bound and, when it holds small integers, its int8 digit planes in the GEMM's layout.  No counterpart in
  * the reference, which converts nothing.  B stays alive and unmodified while the handle is used; zk_fr_matmul_rhs is
- * zk_fr_matmul(C, A, B, M, N, P, ...) with B's part of the preparation taken from the handle (bit-identical results). */
+ * zk_fr_matmul(C, A, B, M, N, P, ...) with B's part of the preparation taken from the handle (bit-identical results).
+ * zk_fr_matmul_rhs_prepare waits for its stream: calls on any stream may use the handle once it has returned. */
 int zk_fr_matmul_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, void* stream);
 int zk_fr_matmul_rhs(void* C, const void* A, const void* prepared, uint32_t M, int mode, int* path_used, void* stream);
 /* the same for a left operand given by its int32 form (M * N int32 on the device, zk_fr_fold_prepared_ints): the bound pass and the
@@ -513,7 +514,7 @@ int zk_rope_table(void* table_i32, uint32_t rows, uint32_t rot, double base, dou
 int zk_i32_from_heads(void* out_i32, const void* in, uint32_t heads, uint32_t tokens, uint32_t dim, uint32_t sf_first, uint32_t sf_second, void* flag_dev, void* stream);
 /* A weight laid out for zk_i32_linear and zk_i32_gated from its int32 form (N x P, on the device; not read afterwards): two or three bytes an element.  The handles
  * of zk_fr_matmul_rhs_prepare serve them as well; one made here has no field elements and serves no field product.  Elements up to 8355711 in magnitude, N at
- * most 43690, P at most 4194304.  Waits for the stream; released with zk_fr_matmul_rhs_free once its last call is through. */
+ * most 43690, P at most 4194304.  Waits for the stream, as zk_fr_matmul_rhs_prepare does; released with zk_fr_matmul_rhs_free once its last call is through. */
 int zk_i32_rhs_prepare(void** prepared, const void* B_i32, uint32_t N, uint32_t P, void* stream);
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner);
 /* A projection with its rescaling (zkfc.cu:44-58, rescaling.cu:13-19): out = q(x W), rows x P int32.  x: rows of N int32, ldx apart, each at most 0x7F7F7F7F; out

@@ -758,6 +758,40 @@ def test_calls_on_two_streams_without_workspaces_of_the_callers(hip, dev):
         hip.lib.zk_fr_matmul_rhs_free(h)
 
 
+@gpu
+@pytest.mark.parametrize("rows", [2, 40])
+def test_handles_from_field_elements_serve_other_streams_at_once(hip, dev, rows):
+    """Handles made from field elements, each on a stream of its own, and used on others right behind: the planes are there, for the int32 products and the field's"""
+    n, p = 2048, 1536
+    rng = np.random.default_rng(rows)
+    w, x = normal(rng, (n, p), 3000.0), normal(rng, (rows, n))
+    fr, px = dev.space(32 * n * p), dev.up(x)
+    hip.call("zk_fr_from_i32", fr, dev.up(w), c_size_t(n * p), None)
+    exp = x.astype(np.int64) @ w
+    low = np.where(exp < 0, exp + np.int64(-0xFFFFFFFF), exp)         # the lowest 64 bits of r + v, modulo 2^64: r's are 2^64 - (2^32 - 1)
+    streams = [c_void_p() for _ in range(3)]
+    for s in streams:                        # of the runtime that the library runs on; non-blocking
+        assert hip.lib.hipStreamCreateWithFlags(ctypes.byref(s), c_uint(1)) == 0
+    outs, fields, flags = [dev.space(4 * rows * p) for _ in streams], [dev.space(32 * rows * p) for _ in streams], [dev.flag() for _ in streams]
+    handles = []
+    hip.sync()
+    for i, s in enumerate(streams):
+        h, path, other = c_void_p(), c_int(), streams[(i + 1) % 3]
+        hip.call("zk_fr_matmul_rhs_prepare", ctypes.byref(h), fr, c_uint(n), c_uint(p), s)
+        hip.call("zk_i32_linear", outs[i], px, c_size_t(n), h, c_uint(rows), c_uint(65536), None, c_size_t(0), flags[i], other)
+        hip.call("zk_fr_matmul_rhs_ints", fields[i], px, h, c_uint(rows), c_int(0), ctypes.byref(path), other)
+        handles.append(h)
+    for s in streams:
+        hip.call("zk_sync", s)
+    for i in range(3):
+        assert dev.down(flags[i], (1,), np.uint32)[0] == 0
+        assert (dev.down(outs[i], (rows, p)) == ref.quotient(exp, 65536)).all()
+        assert (dev.down(fields[i], (rows, p, 8), np.uint32)[..., :2].copy().view(np.int64)[..., 0] == low).all()
+    for h, s in zip(handles, streams):
+        hip.lib.zk_fr_matmul_rhs_free(h)
+        assert hip.lib.hipStreamDestroy(s) == 0
+
+
 # ---- as a program calls them: on a stream of its own, captured, one after the other -------------------------------------------------------------------------
 def _step(hip, torch, s, stream):
     """one block: the residual stream and its norm, positions for the queries, a projection, the gated product and the way down; every buffer is the caller's"""
