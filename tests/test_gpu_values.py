@@ -729,6 +729,15 @@ def test_handles_from_field_elements_serve_both_and_those_from_int32_no_field_pr
         hip.call("zk_i32_linear", C, dev.up(x), c_size_t(40), of_i32.h, c_uint(33), c_uint(1), C, c_size_t(100), dev.flag(), None)      # 33 rows need more; up to four need none
 
 
+def test_torch_and_the_library_have_one_runtime():
+    """What hands torch's streams to the library needs that: two runtimes in a process, and a stream is a pointer into the other one's memory"""
+    from gpuhelp import pkg
+    pkg.load_hip()
+    import torch  # noqa: F401
+    with open("/proc/self/maps") as f:
+        assert len({line.split()[-1] for line in f if "libamdhip64" in line}) == 1
+
+
 @gpu
 def test_calls_on_two_streams_without_workspaces_of_the_callers(hip, dev):
     """Handles made on one stream and used on others at once, the library's own scratch memory in every call: each result is its own"""

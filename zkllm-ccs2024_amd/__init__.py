@@ -53,7 +53,8 @@ def _want_hw_queues():
 
 
 def load_hip():
-    """ctypes handle of the C-ABI kernel library."""
+    """ctypes handle of the C-ABI kernel library.  A program that hands it torch's streams imports torch first: torch's own HIP runtime is then the
+    library's too, where it would be a second one in the process behind it, to which the streams of the other mean nothing."""
     _want_hw_queues()
     lib = _load(HIP_LIB)
     lib.zk_last_error.restype = ctypes.c_char_p
