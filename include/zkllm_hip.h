@@ -498,7 +498,7 @@ int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t 
 /* Rotary positions (llama-self-attn.py:42-73, in fixed point): the first rot of a head's dim elements are rot / 2 pairs, pair i of a token at position p
  *   (x0, x1) -> (q(c x0 - s x1), q(s x0 + c x1)),   (c, s) = table[p][i], q: the quotient by sf, the table's scale (1 .. 2^30);
  * the rest is copied.  neighbours: pair i is (2 i, 2 i + 1), else (i, i + rot / 2).  table: table_rows * (rot / 2) pairs of int32 up to 2^30 in magnitude.  positions: one int32 a
- * token, or null: first, first + 1, ...  Strides in elements from token to token and from head to head, heads of dim contiguous elements; out may be x with the same
+ * token, or null: first, first + 1, ...; with rot 0 heads are only copied, from any position and without a table.  Strides in elements from token to token and from head to head, heads of dim contiguous elements; out may be x with the same
  * strides, and overlaps it in no other way.  Out of place the output's strides are its own: a stack [head][token][dim] is written as easily as [token][head][dim].
  * zk_fr_rope: the same for field elements that stand for 32-bit integers (any other raises the flag and counts as 0). */
 int zk_i32_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,

@@ -298,6 +298,17 @@ def test_rope_positions_outside_the_table_are_not_written(hip, dev, fr, bad):
 
 
 @gpu
+@pytest.mark.parametrize("fr", [False, True])
+@pytest.mark.parametrize("dim", [7, 8])
+def test_heads_that_are_only_copied_have_no_position(hip, dev, fr, dim):
+    rng = np.random.default_rng(dim)
+    x = normal(rng, (5, 2, dim))
+    for positions, first in ((np.array([-1, 5, 1 << 30, -(1 << 31), 0], np.int32), 0), (None, 0xFFFFFFFE)):
+        got, flag = call_rope(hip, dev, x, angles(2, 0, 65536), 0, 0, positions, first, fr=fr, by_head=True)
+        assert flag == 0 and (got == (ref.elements(x) if fr else x)).all()
+
+
+@gpu
 def test_rope_values_that_do_not_fit_raise_the_flag(hip, dev):
     x = np.zeros((1, 2, 4), np.int32)
     x[0, 1] = (1 << 31) - 1

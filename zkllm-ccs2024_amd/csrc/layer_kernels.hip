@@ -1096,7 +1096,9 @@ static int rope(const char* name, bool fr, void* out, size_t out_token, size_t o
     hipStream_t st = (hipStream_t)stv;
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
-    const RopeArgs a{out, x, out_token, out_head, x_token, x_head, tokens, heads, dim, rot, neighbours, (const int2*)table, rot ? table_rows : 0xFFFFFFFFu, (const int32_t*)positions, first, divisor(sf), flag.dev};
+    // nothing rotated: no position is looked at, and every token's own number lies within 2^32 - 1
+    const RopeArgs a{out, x, out_token, out_head, x_token, x_head, tokens, heads, dim, rot, neighbours, (const int2*)table, rot ? table_rows : 0xFFFFFFFFu, rot ? (const int32_t*)positions : nullptr,
+                     rot ? first : 0, divisor(sf), flag.dev};
     const bool vec = !fr && rot % 8 == 0 && dim % 4 == 0 && ((out_token | out_head | x_token | x_head) & 3) == 0 && (((uintptr_t)out | (uintptr_t)x | (uintptr_t)table) & 15) == 0;
     const uint32_t units = heads * (vec ? rot / 8 + (dim - rot) / 4 : rot / 2 + (dim - rot));      // a token's
     const uint32_t step = std::max(1u, (1u << 30) / units);
