@@ -1,7 +1,6 @@
 #include "int-tensor.hpp"
 
 #include "../../include/zkllm_hip.h"
-#include "ioutils.hpp"
 
 #define ZKC(call) zk_check((call), #call)
 
@@ -11,19 +10,10 @@ static int32_t* int_alloc(uint size) {
     return (int32_t*)p;
 }
 IntTensor::IntTensor(uint size) : gpu_data(int_alloc(size)), size(size) {}
-IntTensor::IntTensor(uint size, const int* cpu_data) : IntTensor(size) { ZKC(zk_memcpy_h2d(gpu_data, cpu_data, sizeof(int32_t) * (size_t)size, nullptr)); }
 IntTensor::IntTensor(const FrTensor& t) : IntTensor(t.size) { ZKC(zk_i32_from_heads(gpu_data, t.gpu_data, 1, 1, t.size, 1, 1, nullptr, nullptr)); }
 IntTensor::IntTensor(IntTensor&& t) noexcept : gpu_data(t.gpu_data), size(t.size) { t.gpu_data = nullptr; }
 IntTensor::~IntTensor() { if (gpu_data) (void)zk_free(gpu_data); }
 
-IntTensor IntTensor::from_int_bin(const string& filename) {
-    const size_t n = findsize(filename) / sizeof(int32_t);
-    if (n > 0xFFFFFFFFull) throw std::runtime_error("IntTensor: " + filename + " has more elements than a tensor holds");
-    IntTensor out((uint)n);
-    loadbin(filename, out.gpu_data, sizeof(int32_t) * n);
-    return out;
-}
-void IntTensor::save_int(const string& filename) const { savebin(filename, gpu_data, sizeof(int32_t) * (size_t)size); }
 FrTensor IntTensor::to_fr() const {
     FrTensor out(size);
     ZKC(zk_fr_from_i32(out.gpu_data, gpu_data, size, nullptr));

@@ -1,5 +1,5 @@
 // IntTensor: owning device array of int32 in fixed point, the form the activation and parameter files hold (an addition; the reference keeps
-// every tensor as field elements).  What LayerValues computes with; a quarter of a field element's bytes twice over.
+// every tensor as field elements; files are read and written by FrTensor).  What LayerValues computes with; an eighth of a field element's bytes.
 #pragma once
 #include <cstdint>
 #include "fr-tensor.hpp"
@@ -10,15 +10,12 @@ class IntTensor {
     const uint size;
 
     explicit IntTensor(uint size);
-    IntTensor(uint size, const int* cpu_data);
     explicit IntTensor(const FrTensor& t);         // throws when an element is no 32-bit integer
     IntTensor(IntTensor&& t) noexcept;
     IntTensor(const IntTensor&) = delete;
     IntTensor& operator=(const IntTensor&) = delete;
     ~IntTensor();
 
-    static IntTensor from_int_bin(const string& filename);
-    void save_int(const string& filename) const;
     FrTensor to_fr() const;
 };
 
