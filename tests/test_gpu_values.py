@@ -101,6 +101,39 @@ def test_norm_sizes(hip, dev, rows, cols, options):
     same(got, *ref.residual_norm(x, b, post, gate, res, w))
 
 
+# Prompts: the kernel whose stores go past the caches (512 rows and more of 1025 to 4096 aligned columns), with every option, in the inputs' place, rows whose sums round among the others
+@gpu
+@pytest.mark.parametrize("rows,cols", [(512, 1028), (700, 2052), (513, 4096)])
+@pytest.mark.parametrize("options", ["", "b", "post gate", "post gate in place"])
+@pytest.mark.parametrize("sf", [65536, 65521])
+def test_norm_of_prompts(hip, dev, rows, cols, options, sf):
+    rng = np.random.default_rng(rows + sf)
+    x, w = normal(rng, (rows, cols)), normal(rng, cols, 6000.0) + 65536
+    b = normal(rng, (rows, cols), 30000.0) if options else None
+    post = normal(rng, cols, 6000.0) + 65536 if "post" in options else None
+    gate = normal(rng, ({512: 32, 700: 20, 513: 27}[rows], cols), 30000.0) if "gate" in options else None
+    for at in ((0, 0), (rows // 2, 7), (rows - 1, cols - 1)):
+        x[at] = 2000 * 65536
+    x[3, 1:9] = -1500 * 65536
+    if post is not None:
+        b[5, 6] = b[rows - 2, cols - 4] = 1800 * 65536
+    got, flag = call_norm(hip, dev, x, b, post, gate, 46341, w, sf=sf, into={"h": "x", "n": "b"} if "in place" in options else None)
+    assert flag == 0
+    same(got, *ref.residual_norm(x, b, post, gate, 46341, w, sf=sf))
+
+
+# as many rows through each of the other kernels: one column a lane and four, more of either, rows too long for registers
+@gpu
+@pytest.mark.parametrize("cols", [1021, 1024, 1030, 5120, 8192, 16390])
+def test_norm_of_prompts_of_other_widths(hip, dev, cols):
+    rng = np.random.default_rng(cols)
+    x, b, w, post, gate = normal(rng, (512, cols)), normal(rng, (512, cols), 30000.0), normal(rng, cols, 6000.0) + 65536, normal(rng, cols, 6000.0) + 65536, normal(rng, (16, cols), 30000.0)
+    x[100, cols // 2] = 2000 * 65536
+    got, flag = call_norm(hip, dev, x, b, post, gate, 46341, w)
+    assert flag == 0
+    same(got, *ref.residual_norm(x, b, post, gate, 46341, w))
+
+
 # rows whose squares pass 2^53: the sum is then the one in index order, rounding and all
 @gpu
 @pytest.mark.parametrize("cols", [7, 300, 4096, 5000, 17000])
@@ -253,6 +286,35 @@ def test_rope(hip, dev, tokens, heads, dim, rot, neighbours, fr, layout):
     got, flag = call_rope(hip, dev, x, table, rot, neighbours, positions, fr=fr, by_head=layout == "heads", pad={"gaps": 3, "in place": 4}.get(layout, 0), in_place=layout == "in place")
     exp = ref.rope(x, table, positions, rot, neighbours, 65536)
     assert flag == 0 and (got == (ref.elements(exp) if fr else exp)).all()
+
+
+def limbs64(v):
+    """64-bit integers as field elements, without Python's: r's lowest 64 bits are above 2^63, so r + v borrows nothing from the limbs above for v down to -2^63"""
+    v = np.asarray(v, np.int64)
+    below, out = v < 0, np.zeros(v.shape + (8,), np.uint32)
+    out[..., :2] = np.where(below, v + np.int64(-0xFFFFFFFF), v).astype(np.int64)[..., None].view(np.uint32)
+    out[..., 2:] = np.where(below[..., None], ref.elements(np.array(-1))[2:], 0)
+    return out
+
+
+# field elements at the sizes of a prompt's heads
+@gpu
+@pytest.mark.parametrize("tokens,heads,dim,rot", [(130, 32, 128, 128), (70, 40, 80, 48), (300, 8, 126, 126)])
+@pytest.mark.parametrize("neighbours", [0, 1])
+@pytest.mark.parametrize("by_head", [False, True])
+def test_rope_of_field_elements_of_a_prompt(hip, dev, tokens, heads, dim, rot, neighbours, by_head):
+    rng = np.random.default_rng(tokens)
+    x = normal(rng, (tokens, heads, dim))
+    assert (limbs64(x[0, 0]) == ref.elements(x[0, 0])).all()
+    table, positions = angles(500, rot, 65536), rng.integers(0, 500, tokens).astype(np.int32)
+    out, f = dev.space(32 * x.size), dev.flag()
+    to = (dim, tokens * dim) if by_head else (heads * dim, dim)
+    hip.call("zk_fr_rope", out, c_size_t(to[0]), c_size_t(to[1]), dev.up(limbs64(x), np.uint32), c_size_t(heads * dim), c_size_t(dim), c_uint(tokens), c_uint(heads), c_uint(dim), c_uint(rot),
+             c_int(neighbours), dev.up(table), c_uint(500), dev.up(positions), c_uint(0), c_uint(65536), f, None)
+    hip.sync()
+    exp = ref.rope(x, table, positions, rot, neighbours, 65536)
+    assert dev.down(f, (1,), np.uint32)[0] == 0
+    assert (dev.down(out, (heads, tokens, dim, 8) if by_head else (tokens, heads, dim, 8), np.uint32) == limbs64(exp.swapaxes(0, 1) if by_head else exp)).all()
 
 
 @gpu
