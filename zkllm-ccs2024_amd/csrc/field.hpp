@@ -869,13 +869,15 @@ ZK_HD int64_t fr_to_i64(const Fr& x) {
     if (n.v[7] | n.v[6] | n.v[5] | n.v[4] | n.v[3] | n.v[2]) return 0;
     return (int64_t)(0ull - ((uint64_t)n.v[0] | ((uint64_t)n.v[1] << 32)));
 }
-// whether x stands for an integer of 64 bits (-2^63 .. 2^63 - 1), and which: fr_to_i64 takes r - x modulo 2^64 for every x above r - 2^64
+// whether x stands for an integer of 64 bits (-2^63 .. 2^63 - 1), and which: fr_to_i64 takes r - x modulo 2^64 for every x above r - 2^64.
+// r's lowest 64 bits lie above 2^63, so r - m has r's six limbs above them for every m up to 2^63.
 ZK_HD bool fr_fits_i64(const Fr& x, int64_t& v) {
-    const bool positive = !(x.v[7] | x.v[6] | x.v[5] | x.v[4] | x.v[3] | x.v[2]) && !(x.v[1] >> 31);
-    const Fr n = neg(x);
-    const uint64_t low = positive ? (uint64_t)x.v[0] | ((uint64_t)x.v[1] << 32) : 0ull - ((uint64_t)n.v[0] | ((uint64_t)n.v[1] << 32));
-    v = (int64_t)low;
-    return positive || (!(n.v[7] | n.v[6] | n.v[5] | n.v[4] | n.v[3] | n.v[2]) && v < 0);      // r - x of 1 .. 2^63
+    const uint64_t low = (uint64_t)x.v[0] | ((uint64_t)x.v[1] << 32), r_low = (uint64_t)FrK::P(0) | ((uint64_t)FrK::P(1) << 32);
+    uint32_t high = 0, from_r = 0;
+#pragma unroll
+    for (int i = 2; i < 8; ++i) { high |= x.v[i]; from_r |= x.v[i] ^ FrK::P(i); }
+    v = (int64_t)(high ? low - r_low : low);
+    return high ? from_r == 0 && v < 0 : v >= 0;
 }
 // scalar_to_int (fr-tensor.cu:922-932)
 ZK_HD int32_t fr_to_i32(const Fr& x) {
