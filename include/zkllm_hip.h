@@ -500,14 +500,15 @@ int zk_i32_residual_norm(void* h, void* n, void* rms_inv, const void* x, size_t 
  * the rest is copied.  neighbours: pair i is (2 i, 2 i + 1), else (i, i + rot / 2).  table: table_rows * (rot / 2) pairs of int32 up to 2^30 in magnitude.  positions: one int32 a
  * token, or null: first, first + 1, ...; with rot 0 heads are only copied, from any position and without a table.  Strides in elements from token to token and from head to head, heads of dim contiguous elements; out may be x with the same
  * strides, and overlaps it in no other way.  Out of place the output's strides are its own: a stack [head][token][dim] is written as easily as [token][head][dim].
- * zk_fr_rope: the same for field elements that stand for 32-bit integers (any other raises the flag and counts as 0). */
+ * zk_fr_rope: the same for field elements that stand for 32-bit integers (any other, rotated or copied, raises the flag and counts as 0); its results are elements, and may lie outside int32. */
 int zk_i32_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
                 const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
 int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size_t x_token, size_t x_head, uint32_t tokens, uint32_t heads, uint32_t dim, uint32_t rot, int neighbours,
                const void* table, uint32_t table_rows, const void* positions_i32, uint32_t first, uint32_t sf, void* flag_dev, void* stream);
 /* The table of angles: table[p][i] = the nearest integers to sf magnitude cos(p f_i) and sf magnitude sin(p f_i), p < rows, f_i = base^(-2 i / rot) / factor.
  * original > 0 (long contexts): only what is slow is slowed down -- f_i that turns high times or more over `original` positions is left alone, one that turns low times
- * or less divided by the factor, those between in proportion.  rows up to 2^31, times the factor where that is below 1.  Double precision, correctly rounded operations in a fixed order: the same table everywhere. */
+ * or less divided by the factor, those between in proportion.  rows up to 2^31, times the factor where that is below 1.  Double precision, correctly rounded operations in a fixed order: the same table everywhere; an
+ * angle p f_i is off by up to p 2^-50, so far positions at large scales may have a neighbouring integer. */
 int zk_rope_table(void* table_i32, uint32_t rows, uint32_t rot, double base, double factor, double original, double low, double high, double magnitude, uint32_t sf, void* stream);
 /* out[token][head][k] = q_second(q_first(in[head][token][k])): field elements that stand for integers up to 2^62 (attention's products with the values) to
  * int32 with the two quotients of self-attn.cu:96-98; with one head and factors of 1 the int32 form of a tensor. */

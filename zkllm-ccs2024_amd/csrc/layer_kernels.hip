@@ -93,14 +93,16 @@ template <bool POW2> __device__ __forceinline__ int32_t normed(int32_t w, int32_
 
 // A workgroup a row, VEC neighbouring columns NV times in each lane's registers: every tensor is read once and written once, which is what
 // bounds it (2048 x 4096, x and b to h and n, 134 MB: 24 us, 5.6 TB/s; a copy of a gigabyte reaches 5.15).  One row of 4096: 4.5 us, two reductions and the way to memory and back.
-// Rows whose squares round are added up by one lane out of LDS, a few microseconds a thousand columns: activations beyond 2^26, in the hundreds at scale 2^16.
+// Rows whose squares add up to more than 2^53 -- one value beyond 2^26.5, 1449 at scale 2^16, is enough -- are added up by one lane out of LDS, 8 ns a term: a row of 4096 takes 32 us
+// more, 2048 x 4096 107 us where one row in 64 is such a row and 182 where all are.
 template <int VEC> __device__ __forceinline__ void row_load(int32_t (&v)[VEC], const int32_t* p) {
     if constexpr (VEC == 4) {
         const v4i q = *reinterpret_cast<const v4i*>(p);
         v[0] = q[0]; v[1] = q[1]; v[2] = q[2]; v[3] = q[3];
     } else v[0] = *p;
 }
-// STREAM: stores of large tensors go past the caches (2048 x 4096: 31 us, 24 so; with the projection that reads them behind it 206 either way)
+// STREAM: stores go past the caches, in the kernel for 512 rows and more of 1025 to 4096 columns (2048 x 4096: 31 us, 23 so, 512 x 4096 9.0 and 8.0, 8192 x 4096 104 and 102; with the projection
+// that reads them behind it 206 either way); the other kernels' do not.
 template <int VEC, bool STREAM> __device__ __forceinline__ void row_store(int32_t* p, const int32_t (&v)[VEC]) {
     if constexpr (VEC == 4) {
         const v4i q = {v[0], v[1], v[2], v[3]};
@@ -304,7 +306,7 @@ __device__ __forceinline__ void rope_copy(Fr* to, const Fr* from, uint32_t& bad)
     asm volatile("" ::: "memory");
 }
 // A lane VEC pairs of the rotated part or VEC elements of the rest; the heads of a token read its angles from the caches.  HBM: 16384 tokens of 32 x 128 int32 92 us,
-// 5.9 TB/s (a pair a lane 143); 2048 tokens of field elements 103 us, 5.2 TB/s; the launches of a token's 64 heads 3 us.
+// 5.9 TB/s (a pair a lane 143; 51 heads of 80, 20 rotated, which take that, 274); 2048 tokens of field elements 101 us, 5.3 TB/s; the launches of a token's 64 heads 3 us.
 template <typename T, int VEC, bool POW2> __global__ void __launch_bounds__(256) k_rope(const RopeArgs a, uint32_t token0, uint32_t total) {
     const uint32_t id = blockIdx.x * 256 + threadIdx.x;
     if (id >= total) return;
@@ -513,8 +515,8 @@ enum class End { POW2, ANY, PARTS };
 // Steps of 32 contraction bytes go from memory to LDS without passing through registers, four buffers deep; a step's fragments are read while the step before
 // is multiplied, since one wave a SIMD (256 accumulators with MT = 2) has nobody to cover for it.
 // 2048 x 4096 x 4096, three planes by two: 156 us; both 4096 x 11008 weights at 2048 rows 860, 2.55 POP/s (the library's int8 product of 8192^3: 2.05).  The matrix units are
-// busy 65 % of the cycles, at 1.75 to 1.85 GHz: the card's power holds the clock there (the same without the loads from memory, on what lies in LDS, 2.3 GHz and 570 us), and what
-// saves stalls costs clock.  Steps of 64 bytes (61 us against 41 for 64 rows of 4096 x 11008 in tiles of 128 columns), eight buffers (47), the next tile's first steps ahead of a tile's outputs (936
+// busy 65 % of the cycles, at 1.75 to 1.85 GHz: the card's power holds the clock there (the same without the loads from memory, on what lies in LDS, 2.3 GHz and 570 us), and part of what
+// saves stalls costs clock.  (The instructions alone, on random bytes, 129 us and 693 for these two, 3.2 POP/s.)  Steps of 64 bytes (61 us against 41 for 64 rows of 4096 x 11008 in tiles of 128 columns), eight buffers (47), the next tile's first steps ahead of a tile's outputs (936
 // against 895 for the whole) and other orders of the products or tiles (within 1 %) gained nothing.
 template <bool GATED, int PA, int PB, int MT, int NQ> struct Tile {
     static constexpr int NS = PA + PB - 1, TM = 64 * MT, TN = 64 * NQ, PIECES = PA * 2 * MT + PB * 2 * NQ, SHARE = (PIECES + 3) / 4, BYTES = (PA * TM + PB * TN) * 32;
@@ -956,7 +958,7 @@ static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->pl
 static constexpr uint32_t SPLIT_ROWS = 4;
 static size_t padded_rows(uint32_t rows) { return ((size_t)rows + 127) / 128 * 128; }
 // A long contraction with few tiles is split, so that every compute unit has a part of one: from 8192 on and for 33 rows and more, where neither strips nor tiles fill the card.
-// 64 rows of 11008 x 4096 36 us (strips 48, whole tiles 81), 128 rows 53 (81), of both such weights 62 (75 in strips) and 80 (104); of 4096 x 4096 the second launch
+// 64 rows of 11008 x 4096 36 us (strips 48, whole tiles 81), 128 rows 52 (81), of both such weights 55 (75 in strips) and 77 (104); of 4096 x 4096 the second launch
 // takes what the first gains (64 rows 19 either way, 128 rows 25 and 26; of two weights 34 and 28).  Two planes of weights: a part's sum stays in 64 bits then.
 static constexpr size_t PARTS_BYTES = (size_t)16 << 20;
 static bool may_split(uint32_t rows, uint32_t inner) { return rows > 32 && inner > 8064; }
@@ -1051,6 +1053,9 @@ template <int NV, int VEC, bool POW2, int THREADS> static void launch_norm_n(con
     const unsigned threads = (unsigned)std::max<size_t>(64, ((size_t)cdiv(a.cols, NV * VEC) + 63) / 64 * 64);
     hipLaunchKernelGGL((k_residual_norm<NV, VEC, POW2, THREADS>), dim3(rows), dim3(threads), threads * VEC * sizeof(double), st, a);
 }
+// Four aligned columns a lane, once in its registers or, for many rows, twice, with half as many waves and streamed stores: 511 rows of 4096 10.3 us and 8.0, 1024 rows 16.9 and 12.9, 2048 rows 32.6 and
+// 22.6; up to 256 rows both take no longer than the call, 8 us.  Rows of 1024 stay with the first (2048 of them 9.7 us and 8.0, 8192 28.4 and 21.5).  Four times up to 16384 columns: 1024 x 8192 35 us, where
+// the kernel for rows of any length, which reads them again in every pass, takes 56 (2048 x 5120: 51 either way).  One column a lane where something is not aligned: 1024 x 4098 24 us.
 template <bool POW2> static void launch_norm(const NormArgs& a, uint32_t rows, hipStream_t st) {
     auto aligned = [](const void* p) { return ((uintptr_t)p & 15) == 0; };
     const bool vec = (a.cols & 3) == 0 && (a.ldx & 3) == 0 && (a.b == nullptr || (a.ldb & 3) == 0) && aligned(a.x) && aligned(a.b) && aligned(a.h) && aligned(a.n) && aligned(a.post) &&

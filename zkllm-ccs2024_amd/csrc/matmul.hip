@@ -1007,7 +1007,7 @@ int zk_fr_matmul_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_
         r->pb = pb;
         hipLaunchKernelGGL(k_split_cols, dim3(cdiv(P, 64), r->Kp / 64, 1), dim3(256), 0, st, (int8_t*)r->planes, (const Fr*)B, N, P, r->Kp, pb);
         if (hipGetLastError() != hipSuccess) { (void)pool_free(r->planes, st); return hip_fail(hipErrorLaunchFailure, "k_split_cols", __FILE__, __LINE__); }
-        const hipError_t done = hipStreamSynchronize(st);      // a call on any other stream may read the planes now
+        const hipError_t done = hipStreamSynchronize(st);      // a call on any other stream may read the planes now (4096 x 4096: 257 us in all instead of 113, once a weight)
         if (done != hipSuccess) { (void)pool_free(r->planes, st); return hip_fail(done, "hipStreamSynchronize", __FILE__, __LINE__); }
     }
     *prepared = r.release();

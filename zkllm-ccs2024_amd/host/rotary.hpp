@@ -22,7 +22,7 @@ class Rotary {
     // x: [token][head][dim] -> the same, or [head][token][dim]
     FrTensor operator()(const FrTensor& x, uint heads, bool by_head) const;
     void rotate(int32_t* out, const int32_t* x, uint heads, bool by_head, void* flag_dev) const;
-    void check() const { flag.check("rotary positions"); }      // whether every element of the tensors rotated so far was a 32-bit integer
+    void check() const { flag.check("rotary positions"); }      // whether every element of the field tensors handed in so far, rotated or copied, was a 32-bit integer
 
    private:
     const RopeConfig c;
