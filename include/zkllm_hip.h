@@ -508,7 +508,7 @@ int zk_fr_rope(void* out, size_t out_token, size_t out_head, const void* x, size
 /* The table of angles: table[p][i] = the nearest integers to sf magnitude cos(p f_i) and sf magnitude sin(p f_i), p < rows, f_i = base^(-2 i / rot) / factor.
  * original > 0 (long contexts): only what is slow is slowed down -- f_i that turns high times or more over `original` positions is left alone, one that turns low times
  * or less divided by the factor, those between in proportion.  rows up to 2^31, times the factor where that is below 1.  Double precision, correctly rounded operations in a fixed order: the same table everywhere; an
- * angle p f_i is off by up to p 2^-50, so far positions at large scales may have a neighbouring integer. */
+ * angle p f_i is off by up to p 2^-50 (divided by the factor where that is below 1), so far positions at large scales may have a neighbouring integer. */
 int zk_rope_table(void* table_i32, uint32_t rows, uint32_t rot, double base, double factor, double original, double low, double high, double magnitude, uint32_t sf, void* stream);
 /* out[token][head][k] = q_second(q_first(in[head][token][k])): field elements that stand for integers up to 2^62 (attention's products with the values) to
  * int32 with the two quotients of self-attn.cu:96-98; with one head and factors of 1 the int32 form of a tensor. */
