@@ -398,7 +398,7 @@ def _framework(s):
         cache, prefix = _own_cache(s), _prefix_cache(s)
         _ok(lib.zk_i32_attention(_p(s["out"]), _n(token), _n(case["dim"]), _p(s["q"]), _n(token), _n(case["dim"]), _u(len(s["q"])), _u(case["heads"]), _u(case["kv_heads"]), _u(case["dim"]),
                                  s["softmax"].h, ctypes.byref(prefix) if case["prefix"] else None, _u(case["prefix"]), ctypes.byref(cache), _u(case["seqs"]), _p(s["starts"]), _p(s["lengths"]),
-                                 _u(case["own"]), ctypes.c_int(case["causal"]), _u(ATTN_SCALE), _u(ATTN_SCALE), _p(ws), _n(ws.numel()), _p(s["flag"]), _stream()))
+                                 _u(case["own"]), ctypes.c_int(case["causal"]), _u(ATTN_SCALE), _u(ATTN_SCALE), None, _p(ws), _n(ws.numel()), _p(s["flag"]), _stream()))
         return s["out"]
     if case["op"] == "logits":
         rows, vocab = case["rows"], case["vocab"]
