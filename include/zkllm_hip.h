@@ -524,6 +524,61 @@ int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, ui
 /* The gated half of a feed-forward block (ffn.cu:61-73): out = q_hidden(act[q_gate(x G)] * q_up(x U)), act[v] = table[v - low] of len int32.  Both weights have one shape. */
 int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared, const void* up_prepared, uint32_t rows, uint32_t sf_gate, uint32_t sf_up, const void* table_i32,
                  int32_t low, uint32_t len, uint32_t sf_hidden, void* workspace, size_t workspace_bytes, void* flag_dev, void* stream);
+/* A weight of 4 bits with a scale and a zero for every `group` rows of a column (a multiple of 16; the last group may be shorter): w[k][p] = (code - zero) * scale, whole numbers, so
+ * that products equal those with the int32 weight itself.  codes: N rows of (P + 1) / 2 bytes, columns 2 i and 2 i + 1 in byte i, the even one in its low half; scales: int32, ceil(N /
+ * group) rows of P, up to 557047 in magnitude; zeros: bytes of the same shape, 0 .. 15, or null for 8.  All on the device, not read afterwards.  N and P as in zk_i32_rhs_prepare, half
+ * a byte an element is kept.  The handle serves zk_i32_linear and zk_i32_gated, there both weights or none, whose workspace is then zk_i32_rhs_workspace's (for zk_i32_gated both
+ * weights' sizes added up); released with zk_fr_matmul_rhs_free once its last call is through.  No counterpart in the reference. */
+int zk_i32_rhs_prepare_q4(void** prepared, const void* codes, const void* scales_i32, const void* zeros_u8, uint32_t N, uint32_t P, uint32_t group, void* stream);
+size_t zk_i32_rhs_workspace(const void* prepared, uint32_t rows);
+
+/* ---- answering token by token in the prover's integers (an addition) ------------------------------------------------------------ */
+/* As above: int32 tensors in fixed point, whole numbers, flags, workspaces and captured calls.
+ * A cache of keys and values, pages of page_size tokens: token t of a sequence lies in page page_table[sequence][t / page_size] (int32 on the device, rows of table_cols; entries outside
+ * 0 .. pages - 1 raise ZK_VALUES_POSITION) at place t % page_size; without a table sequence s has page s.  Head h of it: dim contiguous int32 at page * page_stride + place * token_stride +
+ * h * head_stride elements, of keys and of values alike.  The struct is read during the call only. */
+typedef struct zk_i32_cache {
+    const void *k, *v;
+    size_t page_stride, token_stride, head_stride;
+    uint32_t page_size, pages;
+    const void* page_table;
+    uint32_t table_cols;
+} zk_i32_cache;
+/* Keys and values of new tokens to their places.  Tokens starts[s] .. starts[s + 1] - 1 are sequence s's (int32, sequences + 1 of them, ascending; null: tokens / sequences each), and
+ * lengths[s] (int32 on the device) is its length with them: the last goes to place lengths[s] - 1.  Strides in elements from token to token and from head to head, heads of dim
+ * contiguous elements.  Tokens before the first start or behind the last are not read; a place or page that there is not raises ZK_VALUES_POSITION, and the token is not written.  Two
+ * sequences that share a page must not write the same place. */
+int zk_i32_cache_append(const zk_i32_cache* cache, const void* k, size_t k_token, size_t k_head, const void* v, size_t v_token, size_t v_head, uint32_t tokens, uint32_t kv_heads, uint32_t dim,
+                        uint32_t sequences, const void* starts_i32, const void* lengths_i32, void* flag_dev, void* stream);
+/* The softmax of zkSoftmax (zksoftmax.cu:34-93) for heads of dim elements: K digits of radices bs, the lowest L not looked at, the highest M zero or the weight is, those between mapped to
+ * thetas' exponentials (K - L - M of them).  Radices up to 2^28 and their product up to 2^63, thetas' product below 1.4e14.  Waits for the stream; any stream may use the handle afterwards. */
+int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs_host, int K, int L, int M, double scaling_factor_in, const double* thetas_host, uint32_t dim, void* stream);
+int zk_i32_softmax_free(void* softmax);          /* once its last call is through */
+size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length);
+/* Attention of queries over the keys and values of a prefix that all sequences share (read once for all of them) and, behind it, of their sequences' own (self-attn.cu:81-98,
+ * zksoftmax.cu:112-173):  x_j = q . k_j,  shift = the nearest integer to scale ln(sum_j exp(x_j / scale)), scale = scaling_factor_in sqrt(dim),  y_j = the product of the tables' values at
+ * the digits of shift - x_j,  out = q_second(q_first(sum_j y_j v_j)).  The sum of exponentials is zk_softmax_shift's, in double precision and in the order of the keys, prefix first: element
+ * for element zkAttn::compute and the two rescalings behind it where they stay within 64 bits.
+ * q, out: tokens x heads of dim elements with strides; out may be q with the same strides and overlaps nothing else.  Head h reads keys and values of head h / (heads / kv_heads).  Tokens belong to sequences
+ * as in zk_i32_cache_append, with their keys already in the cache; tokens of none are left as they are.  lengths[s] is 0 .. max_length, which bounds the work and the workspace.  causal:
+ * token i of a sequence's n sees the prefix and its own keys before place lengths[s] - n + i + 1; else all of them.  A token that sees no key: zeros.
+ * shift (int64, tokens x heads, or null) receives the shifts.  prefix: a cache whose sequence 0 holds
+ * prefix_len tokens, or null and 0.  own: null where there is only a prefix (sequences, starts, lengths are not looked at then, max_length is 0).
+ * dim up to 256, up to 2^24 keys of each kind, 2^20 queries a head of keys.  Elements up to 0x7F7F7F7F, scores and sums within 2^62 (ZK_VALUES_RANGE); a score above the shift or further below it than the
+ * digits reach raises ZK_VALUES_TABLE. */
+int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                     const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts_i32, const void* lengths_i32,
+                     uint32_t max_length, int causal, uint32_t sf_first, uint32_t sf_second, void* shift_i64, void* workspace, size_t workspace_bytes, void* flag_dev, void* stream);
+size_t zk_i32_logits_workspace(uint32_t rows, uint32_t vocab);
+/* Logits before a token is chosen, and the choice.  For a token that stands c > 0 times in its row's history, with the row's penalties (r, f, p), int32:  l -> (l > 0 ? the quotient of
+ * l sf by r : the quotient of l r by sf) - f c - p;  then l -> l + the sum of the token's biases in its row's list;  then the lowest int32, -2^31, where its bit in the row's mask is 0 (bit t % 32 of word
+ * t / 32).  A logit that is -2^31 stays so: such a token cannot be chosen.  token (int32, one a row): the largest, of equals the lowest token, -1 where none is left.
+ * Row r's history is entries starts[r] .. starts[r + 1] - 1 of `history_len` (int32, rows + 1 starts), its biases likewise; each with its starts may be null.  penalties: rows x 3, r > 0.
+ * mask: one row for all (mask_rows 1) or ld_mask words from row to row, or null and 0.  out may be logits with the same leading dimension, or null where only the token is wanted; token may be null.
+ * Entries outside 0 .. vocab - 1 and lists outside their entries raise ZK_VALUES_POSITION and do not count; values that leave int32, or reach -2^31 by themselves, raise ZK_VALUES_RANGE. */
+int zk_i32_logits(void* out, size_t ld_out, void* token_i32, const void* logits, size_t ld, uint32_t rows, uint32_t vocab, const void* history_i32, uint32_t history_len,
+                  const void* history_starts_i32, const void* penalties_i32, const void* bias_tokens_i32, const void* bias_values_i32, uint32_t bias_len, const void* bias_starts_i32,
+                  const void* mask_u32, size_t ld_mask, uint32_t mask_rows, uint32_t sf, void* workspace, size_t workspace_bytes, void* flag_dev, void* stream);
 
 /* ---- measurement helpers (no counterpart in the reference) ---------------------------------------- */
 /* v_mad_u64_u32 issue peak of the device: 16 independent chains per lane, no memory traffic */

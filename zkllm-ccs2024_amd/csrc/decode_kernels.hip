@@ -1,0 +1,873 @@
+// Answering token by token in the prover's integers, for gfx950: the cache of keys and values, attention that reads it, and the logits' way to a token.
+//
+//   append     keys and values of new tokens to their places in the pages of their sequences
+//   attention  x_j = q . k_j;  shift = the nearest integer to scale ln(sum_j exp(x_j / scale));  y_j = prod_i table_i[digit_i(shift - x_j)];
+//              out = Q(Q(sum_j y_j v_j; s1); s2): the softmax of the layer's proof (zksoftmax.cu:4-32, :95-109, :112-173; self-attn.cu:81-98), the sum taken in
+//              double precision and in the order of the keys as zk_softmax_shift takes it, so that results equal the class layer's
+//   logits     penalties for repeated tokens, biases, the mask of a grammar, the best token that is left
+//
+// Positions, pages, lengths and tokens outside their ranges raise bits of a flag on the device; nothing is read or written out of range for them.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+#include "detmath.hpp"
+#include "intvalues.hpp"
+
+using namespace zk;
+
+// ---- the softmax --------------------------------------------------------------------------------------------------------------------------
+static constexpr int DIGITS = 8;
+struct SoftmaxArgs {
+    const int32_t* table[DIGITS];        // of the digits that are kept, lowest first; null: 1 for digit 0 and 0 for others
+    uint32_t radix[DIGITS];
+    int bits[DIGITS];                    // log2 of the radices where all are powers of two
+    int n, drop_bits;
+    uint64_t drop;                       // the product of the radices whose digits are not kept
+    double scale;
+};
+struct SoftmaxPlan { SoftmaxArgs a; int32_t* memory = nullptr; bool pow2 = true; uint32_t dim = 0; };
+
+__global__ void __launch_bounds__(256) k_softmax_table_i32(int32_t* __restrict__ table, double log_theta, double step, uint32_t len) {
+    const uint32_t x = blockIdx.x * 256 + threadIdx.x;
+    if (x < len) table[x] = (int32_t)(uint64_t)(zkd::exp_det(log_theta - step * (double)x) + 0.5);      // zk_softmax_table's values
+}
+// the weight of a key whose score lies d below the shift, below 2^47
+template <bool POW2> __device__ __forceinline__ int64_t softmax_weight(int64_t d, const SoftmaxArgs& s, uint32_t& bad) {
+    if (d < 0) { bad |= ZK_VALUES_TABLE; return 0; }
+    uint64_t t = (uint64_t)d;
+    int64_t y = 1;
+    if constexpr (POW2) {
+        t >>= s.drop_bits;
+        for (int i = 0; i < s.n; ++i) {
+            const uint32_t digit = (uint32_t)t & (s.radix[i] - 1);
+            t >>= s.bits[i];
+            y *= s.table[i] ? s.table[i][digit] : digit == 0 ? 1 : 0;
+        }
+    } else {
+        t /= s.drop;
+        for (int i = 0; i < s.n; ++i) {
+            const uint32_t digit = (uint32_t)(t % s.radix[i]);
+            t /= s.radix[i];
+            y *= s.table[i] ? s.table[i][digit] : digit == 0 ? 1 : 0;
+        }
+    }
+    if (t != 0) { bad |= ZK_VALUES_TABLE; return 0; }
+    return y;
+}
+
+// ---- sequences and their pages ------------------------------------------------------------------------------------------------------------
+struct Sequences {
+    const int32_t *starts, *lengths;     // starts null: the same number of tokens each
+    uint32_t count, tokens, max_length;
+};
+struct Sequence { uint32_t index, first, n, length; };
+__device__ __forceinline__ bool sequence_at(const Sequences& s, uint32_t i, Sequence& q, uint32_t& bad) {
+    q.index = i;
+    if (s.starts) {
+        const int32_t first = s.starts[i], end = s.starts[i + 1];
+        if (first < 0 || end < first || (uint32_t)end > s.tokens) { bad |= ZK_VALUES_POSITION; return false; }
+        q.first = (uint32_t)first; q.n = (uint32_t)(end - first);
+    } else { q.n = s.tokens / s.count; q.first = i * q.n; }
+    const int32_t length = s.lengths[i];
+    if (length < 0 || (uint32_t)length > s.max_length) { bad |= ZK_VALUES_POSITION; return false; }
+    q.length = (uint32_t)length;
+    return true;
+}
+// the sequence that a token belongs to; none: tokens before the first and behind the last
+__device__ __forceinline__ bool sequence_of(const Sequences& s, uint32_t token, Sequence& q, uint32_t& bad) {
+    uint32_t i = 0;
+    if (s.starts) {
+        uint32_t lo = 0, hi = s.count;   // starts[lo] <= token or lo = 0
+        while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (s.starts[mid] <= (int32_t)token) lo = mid;
+            else hi = mid;
+        }
+        i = lo;
+    } else i = token / (s.tokens / s.count);
+    return sequence_at(s, i, q, bad) && token >= q.first && token - q.first < q.n;
+}
+// where a token's heads lie in a cache
+__device__ __forceinline__ size_t cache_at(const zk_i32_cache& c, uint32_t sequence, uint32_t t, uint32_t& bad) {
+    if (!c.page_table) return sequence * c.page_stride + t * c.token_stride;
+    const uint32_t in = t / c.page_size, page = (uint32_t)((const int32_t*)c.page_table)[(size_t)sequence * c.table_cols + in];
+    const bool has = page < c.pages;
+    bad |= has ? 0u : (uint32_t)ZK_VALUES_POSITION;
+    return (has ? page : 0u) * c.page_stride + (t - in * c.page_size) * c.token_stride;
+}
+
+// ---- append -------------------------------------------------------------------------------------------------------------------------------
+struct AppendArgs {
+    zk_i32_cache cache;
+    const int32_t *k, *v;
+    size_t k_token, k_head, v_token, v_head;
+    uint32_t heads, dim;
+    Sequences seqs;
+    uint32_t* flag;
+};
+// A workgroup a token
+template <int VEC> __global__ void __launch_bounds__(256) k_cache_append(const AppendArgs a) {
+    const uint32_t token = blockIdx.x, units = a.dim / VEC;
+    uint32_t bad = 0;
+    Sequence s;
+    if (sequence_of(a.seqs, token, s, bad)) {
+        const int64_t t = (int64_t)s.length - s.n + (token - s.first);
+        if (t < 0) bad |= ZK_VALUES_POSITION;
+        else {
+            uint32_t off = 0;
+            const size_t to = cache_at(a.cache, s.index, (uint32_t)t, off);
+            bad |= off;
+            for (uint32_t i = threadIdx.x; !off && i < 2 * a.heads * units; i += 256) {
+                const bool value = i >= a.heads * units;
+                const uint32_t j = value ? i - a.heads * units : i, head = j / units, e = (j - head * units) * VEC;
+                const int32_t* from = (value ? a.v + token * a.v_token + head * a.v_head : a.k + token * a.k_token + head * a.k_head) + e;
+                int32_t* at = (int32_t*)(value ? a.cache.v : a.cache.k) + to + head * a.cache.head_stride + e;
+                if constexpr (VEC == 4) *reinterpret_cast<v4i*>(at) = *reinterpret_cast<const v4i*>(from);
+                else *at = *from;
+            }
+        }
+    }
+    if (threadIdx.x == 0) raise(a.flag, bad);
+}
+
+// ---- attention ----------------------------------------------------------------------------------------------------------------------------
+// A row is one query head of a token; the rows of a head of keys are token * group + head in its group.  Tiles are 16 rows: of the prefix's, any; of a sequence's own keys, its own.
+struct AttnArgs {
+    int32_t* out;
+    const int32_t* q;
+    size_t out_token, out_head, q_token, q_head;
+    uint32_t group, dim, kv_heads, kv0;  // kv0: the launch's first head of keys
+    SoftmaxArgs softmax;
+    zk_i32_cache prefix, own;
+    uint32_t prefix_len, prefix_cols;    // prefix_cols: the prefix's length up to a multiple of 16, where a row's own scores begin
+    Sequences seqs;                      // count 0: no own keys
+    int causal;
+    Divisor sf_first, sf_second;
+    int64_t* scores;                     // [head of keys][row][ld]
+    size_t ld;
+    int64_t* shift;                      // [head of keys][row]
+    int64_t* shift_out;                  // [token][head], or null
+    int64_t* parts;                      // [split][head of keys][row][dim][2]
+    uint32_t tokens, heads_here, prefix_tiles, prefix_splits, prefix_step, own_splits, own_step;
+    uint32_t* flag;
+};
+static constexpr int64_t NO_SHIFT = INT64_MIN;   // of a row that belongs to no sequence
+__device__ __forceinline__ uint32_t own_seen(const AttnArgs& a, const Sequence& s, uint32_t token) {      // how many of its sequence's own keys a token sees
+    if (!a.causal) return s.length;
+    const int64_t seen = (int64_t)s.length - s.n + (token - s.first) + 1;
+    return seen < 0 ? 0u : (uint32_t)seen;
+}
+struct Tile16 {
+    uint32_t row0, lo, hi, keys, col0;   // rows lo .. hi - 1 of the 16 from row0 on are its own; keys: the most that one of them sees, behind column col0
+    bool own;
+    Sequence s;
+    __device__ bool has(uint32_t c) const { return row0 + c >= lo && row0 + c < hi; }
+};
+__device__ __forceinline__ bool tile_at(const AttnArgs& a, uint32_t id, Tile16& t, uint32_t& bad) {
+    if (id < a.prefix_tiles) {
+        t.row0 = id * 16; t.lo = 0; t.hi = a.tokens * a.group; t.keys = a.prefix_len; t.col0 = 0; t.own = false;
+        if (a.seqs.starts) {             // tokens before the first sequence and behind the last are nobody's
+            const int32_t first = a.seqs.starts[0], end = a.seqs.starts[a.seqs.count];
+            t.lo = (uint32_t)max(first, 0) * a.group; t.hi = min((uint32_t)max(end, 0), a.tokens) * a.group;
+        }
+        t.lo = max(t.lo, t.row0); t.hi = min(t.hi, t.row0 + 16);
+        return t.lo < t.hi;
+    }
+    id -= a.prefix_tiles;
+    // A sequence's tiles begin at floor(first row / 16) + its index: a place for each of them, since floor(x + y) + 1 >= floor(x) + ceil(y)
+    auto base = [&](uint32_t i) { return (uint32_t)((uint64_t)(a.seqs.starts ? (uint32_t)a.seqs.starts[i] : i * (a.tokens / a.seqs.count)) * a.group / 16) + i; };
+    uint32_t lo = 0, hi = a.seqs.count;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (base(mid) <= id) lo = mid;
+        else hi = mid;
+    }
+    if (!sequence_at(a.seqs, lo, t.s, bad)) return false;
+    const uint32_t b = base(lo), rows = t.s.n * a.group, at = (id - b) * 16;
+    if (id < b || at >= rows) return false;
+    t.row0 = t.lo = t.s.first * a.group + at; t.hi = t.lo + min(16u, rows - at); t.col0 = a.prefix_cols; t.own = true;
+    t.keys = own_seen(a, t.s, (t.hi - 1) / a.group);
+    return true;
+}
+// 16 of a head's values as digit planes: four runs of four, 16 apart, so that four lanes read 64 bytes in one piece.  Which 16 of 64 a lane has is the same for queries and keys.
+template <bool VEC> __device__ __forceinline__ void head_piece(const int32_t* p, uint32_t d0, uint32_t dim, int32_t (&x)[16]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t d = d0 + 16 * w;
+        if constexpr (VEC) {
+            v4i v = {0, 0, 0, 0};
+            if (d < dim) v = *reinterpret_cast<const v4i*>(p + d);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * w + e] = v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * w + e] = d + e < dim ? p[d + e] : 0;
+        }
+    }
+}
+__device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v[2] | v[3]) != 0; }
+
+static constexpr uint32_t SCORE_KEYS = 256;      // a workgroup's keys
+// Scores: a wave takes 16 keys at a time, a lane 16 of 64 dimensions of one of them, straight from memory to the fragments of v_mfma_i32_16x16x64_i8
+template <int U, bool VEC> __global__ void __launch_bounds__(256) k_attn_scores(const AttnArgs a) {
+    uint32_t bad = 0;
+    Tile16 t;
+    if (!tile_at(a, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t key0 = blockIdx.x * SCORE_KEYS;
+    if (key0 >= t.keys) return;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z;
+    v4i b[U][4];
+    bool wide = false;
+    {
+        const uint32_t row = t.has(c) ? t.row0 + c : t.lo, token = row / a.group, head = kv * a.group + (row - token * a.group);
+        const int32_t* p = a.q + token * a.q_token + head * a.q_head;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int32_t x[16];
+            head_piece<VEC>(p, u * 64 + q * 4, a.dim, x);
+            digit_planes(x, b[u], bad);
+            wide |= any_bits(b[u][3]);
+        }
+    }
+    const bool q_wide = __any(wide);
+    const zk_i32_cache& cache = t.own ? a.own : a.prefix;
+    const int32_t* keys = (const int32_t*)cache.k + kv * cache.head_stride;
+    int64_t* out = a.scores + ((size_t)blockIdx.z * a.tokens * a.group + t.row0 + c) * a.ld + t.col0 + 4 * q;
+    for (uint32_t i = wave; i < SCORE_KEYS / 16; i += 4) {
+        const uint32_t key = key0 + i * 16;
+        if (key >= t.keys) break;
+        const int32_t* p = keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + c, t.keys - 1), bad);
+        v4i k[U][4];
+        bool k_wide = false;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            int32_t x[16];
+            head_piece<VEC>(p, u * 64 + q * 4, a.dim, x);
+            digit_planes(x, k[u], bad);
+            k_wide |= any_bits(k[u][3]);
+        }
+        v4i acc[7];
+#pragma unroll
+        for (int s = 0; s < 7; ++s) acc[s] = v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int m = 0; m < 3; ++m)
+#pragma unroll
+                for (int n = 0; n < 3; ++n) acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[u][n], acc[m + n], 0, 0, 0);
+        if (q_wide || __any(k_wide)) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int m = 0; m < 3; ++m) {
+                    acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[u][3], acc[m + 3], 0, 0, 0);
+                    acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[u][m], acc[m + 3], 0, 0, 0);
+                }
+                acc[6] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[u][3], acc[6], 0, 0, 0);
+            }
+        }
+        if (t.has(c)) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                int32_t s[7];
+#pragma unroll
+                for (int m = 0; m < 7; ++m) s[m] = acc[m][e];
+                out[key + e] = joined<7>(s, bad);          // key 4 q + e of the tile, row c
+            }
+        }
+    }
+    raise(a.flag, bad);
+}
+
+// The sum of a row's exponentials in double precision and in the order of the keys, by many lanes.  As long as the sum t stays below a power of two 2^(e + 1), adding a term x
+// to it adds the whole number of units u = 2^(e - 52) that is nearest to x / u, and of two that are equally near the one that leaves t / u even: what a run of terms adds
+// depends on nothing of t but whether t / u is odd.  Such pairs of sums, for even and for odd t / u, are joined in any grouping.  Where the sum would leave 2^(e + 1) -- some fifteen
+// times in a row of thousands -- the lanes before the one where it does are added so and that lane's terms one by one.
+struct Steps { uint64_t even, odd; };
+__device__ __forceinline__ Steps then(const Steps& a, const Steps& b) { return Steps{a.even + (a.even & 1 ? b.odd : b.even), a.odd + (a.odd & 1 ? b.even : b.odd)}; }
+__device__ __forceinline__ void step(Steps& s, double x, int e) {
+    const double w = __builtin_fmin(ldexp(x, 52 - e), 4503599627370496.0);     // 2^52 of them leave 2^(e + 1) already
+    const double near = w + 4503599627370496.0;                                // rounds to whole numbers, ties to even ones
+    const uint64_t units = zkd::double_to_bits(near) - 0x4330000000000000ull;
+    const double rest = w - (near - 4503599627370496.0);
+    const bool tie = rest == 0.5 || rest == -0.5;
+    const uint64_t other = tie ? (rest > 0 ? 1ull : ~0ull) : 0ull;             // to the odd neighbour
+    s.even += units + (s.even & 1 ? other : 0);
+    s.odd += units + (s.odd & 1 ? 0 : other);
+}
+// total with the terms of 64 lanes added, lane by lane, M in a lane
+template <int M> __device__ __forceinline__ double add_in_order(double total, double (&x)[M]) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t from = 0;                         // lanes before this one are in the total
+    while (true) {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < M; ++i) any |= x[i] != 0.0;
+        const unsigned long long left = __ballot(any && lane >= from);
+        if (left == 0 || !(total < __builtin_inf())) return total;
+        uint32_t at = (uint32_t)__builtin_ctzll(left);
+        if (total > 0.0) {
+            const int e = (int)(zkd::double_to_bits(total) >> 52) - 1023;
+            const uint64_t t = (zkd::double_to_bits(total) & 0x000FFFFFFFFFFFFFull) | 0x0010000000000000ull;
+            Steps s{0, 0};
+            if (lane >= from)
+#pragma unroll
+                for (int i = 0; i < M; ++i) step(s, x[i], e);
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {      // sums over the lanes up to this one
+                const Steps before{__shfl_up(s.even, off, 64), __shfl_up(s.odd, off, 64)};
+                const Steps both = then(before, s);
+                if (lane >= (uint32_t)off) s = both;
+            }
+            const uint64_t after = t + (t & 1 ? s.odd : s.even);
+            const unsigned long long out = __ballot(after >= 0x0020000000000000ull);
+            const uint32_t last = out ? (uint32_t)__builtin_ctzll(out) : 64u;      // the lane where the sum leaves 2^(e + 1)
+            if (last > 0) {
+                const uint64_t sum = __shfl(after, last - 1, 64);
+                total = ldexp((double)sum, e - 52);
+            }
+            if (last == 64) return total;
+            at = last;
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i) total = total + __shfl(x[i], at, 64);
+        from = at + 1;
+        if (from == 64) return total;
+    }
+}
+__device__ __forceinline__ uint32_t score_col(const AttnArgs& a, uint32_t j) { return j < a.prefix_len ? j : a.prefix_cols + (j - a.prefix_len); }
+// a wave a row
+__global__ void __launch_bounds__(256) k_attn_shift(const AttnArgs a) {
+    constexpr int M = 8;
+    const uint32_t lane = threadIdx.x & 63u, rows = a.tokens * a.group;
+    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= (size_t)a.heads_here * rows) return;
+    const uint32_t token = (uint32_t)(r % rows) / a.group;
+    uint32_t bad = 0, keys = a.prefix_len;
+    if (a.seqs.count) {
+        Sequence s;
+        if (!sequence_of(a.seqs, token, s, bad)) {
+            if (lane == 0) a.shift[r] = NO_SHIFT;
+            return;
+        }
+        keys += own_seen(a, s, token);
+    }
+    const int64_t* x = a.scores + r * a.ld;
+    double total = 0.0;
+    for (uint32_t j0 = 0; j0 < keys; j0 += 64 * M) {
+        double term[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const uint32_t j = j0 + lane * M + i;
+            term[i] = j < keys ? zkd::exp_det((double)x[score_col(a, j)] / a.softmax.scale) : 0.0;
+        }
+        total = add_in_order<M>(total, term);
+    }
+    const double sv = a.softmax.scale * zkd::log_det(total);
+    if (lane == 0) {
+        const int64_t shift = keys == 0 ? 0 : sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5);
+        a.shift[r] = shift;
+        if (a.shift_out) a.shift_out[((size_t)token * a.kv_heads + a.kv0 + r / rows) * a.group + (r % rows - token * a.group)] = shift;
+    }
+}
+
+// the digits of 16 weights, six planes of them
+__device__ __forceinline__ void weight_planes(const int64_t (&y)[16], v4i (&out)[6]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint64_t d = ((uint64_t)y[4 * w + e] + 0x808080808080ull) ^ 0x808080808080ull;
+            lo[e] = (uint32_t)d;
+            hi[e] = (uint32_t)(d >> 32);
+        }
+        const uint32_t a = __builtin_amdgcn_perm(lo[1], lo[0], 0x05010400u), b = __builtin_amdgcn_perm(lo[1], lo[0], 0x07030602u);
+        const uint32_t c = __builtin_amdgcn_perm(lo[3], lo[2], 0x05010400u), d = __builtin_amdgcn_perm(lo[3], lo[2], 0x07030602u);
+        const uint32_t f = __builtin_amdgcn_perm(hi[1], hi[0], 0x05010400u), g = __builtin_amdgcn_perm(hi[3], hi[2], 0x05010400u);
+        out[0][w] = (int)__builtin_amdgcn_perm(c, a, 0x05040100u);
+        out[1][w] = (int)__builtin_amdgcn_perm(c, a, 0x07060302u);
+        out[2][w] = (int)__builtin_amdgcn_perm(d, b, 0x05040100u);
+        out[3][w] = (int)__builtin_amdgcn_perm(d, b, 0x07060302u);
+        out[4][w] = (int)__builtin_amdgcn_perm(g, f, 0x05040100u);
+        out[5][w] = (int)__builtin_amdgcn_perm(g, f, 0x07060302u);
+    }
+}
+// Sums of weights times values: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each.  A
+// part's sum leaves as its low 64 bits and, in units of 2^32, its size: the parts' sums together say whether the whole fits.
+template <bool VEC, bool POW2> __global__ void __launch_bounds__(256) k_attn_values(const AttnArgs a) {
+    extern __shared__ unsigned long long sums[];           // [16][64 blocks of dimensions][2]
+    uint32_t bad = 0;
+    Tile16 t;
+    if (!tile_at(a, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.x * step;
+    if (first >= t.keys) return;
+    const uint32_t end = min(first + step, t.keys), blocks = (a.dim + 63) / 64, streams = 4 / blocks;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z, block = wave % blocks, stream = wave / blocks;
+    const size_t row = (size_t)blockIdx.z * a.tokens * a.group + t.row0;
+    for (uint32_t i = threadIdx.x; i < 16 * blocks * 64 * 2; i += 256) sums[i] = 0;
+    const zk_i32_cache& cache = t.own ? a.own : a.prefix;
+    const uint32_t d0 = block * 64 + 4 * c;
+    const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride + d0;
+    const uint32_t my_row = t.has(c) ? c : t.lo - t.row0;
+    const int64_t shift = a.shift[row + my_row];
+    const uint32_t seen = !t.has(c) || shift == NO_SHIFT ? 0u : t.own ? own_seen(a, t.s, (t.row0 + my_row) / a.group) : t.keys;
+    const int64_t* scores = a.scores + (row + my_row) * a.ld + t.col0;
+    v4i acc[9][4];
+#pragma unroll
+    for (int s = 0; s < 9; ++s)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[s][n] = v4i{0, 0, 0, 0};
+    if (stream < streams)
+        for (uint32_t k = first + stream * 64; k < end; k += 64 * streams) {
+            const size_t mine = cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad);
+            int32_t x[4][16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int32_t* p = values + __shfl((unsigned long long)mine, (int)(q * 16 + i), 64);
+                if constexpr (VEC) {
+                    v4i v = {0, 0, 0, 0};
+                    if (d0 < a.dim) v = *reinterpret_cast<const v4i*>(p);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) x[n][i] = v[n];
+                } else {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) x[n][i] = d0 + n < a.dim ? p[n] : 0;
+                }
+            }
+            int64_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t key = k + q * 16 + i;
+                y[i] = key < min(seen, end) ? softmax_weight<POW2>(shift - scores[key], a.softmax, bad) : 0;
+            }
+            v4i w[6];
+            weight_planes(y, w);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                v4i v[4];
+                digit_planes(x[n], v, bad);
+#pragma unroll
+                for (int i = 0; i < 6; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[j], acc[i + j][n], 0, 0, 0);
+            }
+        }
+    __syncthreads();
+    if (stream < streams)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {      // row 4 q + e, dimension d0 + n
+                int64_t lo = 0, hi = 0;
+#pragma unroll
+                for (int s = 3; s >= 0; --s) lo = lo * 256 + acc[s][n][e];
+#pragma unroll
+                for (int s = 8; s >= 4; --s) hi = hi * 256 + acc[s][n][e];
+                const uint32_t at = ((4 * q + e) * blocks * 64 + d0 + n) * 2;
+                atomicAdd(&sums[at], (unsigned long long)lo + ((unsigned long long)hi << 32));
+                atomicAdd(&sums[at + 1], (unsigned long long)(hi + (lo >> 32)));
+            }
+    __syncthreads();
+    const size_t all = (size_t)a.heads_here * a.tokens * a.group;
+    unsigned long long* out = (unsigned long long*)a.parts + (((t.own ? a.prefix_splits : 0) + blockIdx.x) * all + row) * a.dim * 2;
+    for (uint32_t i = (t.lo - t.row0) * a.dim * 2 + threadIdx.x; i < (t.hi - t.row0) * a.dim * 2; i += 256) {
+        const uint32_t r = i / (2 * a.dim);
+        out[i] = sums[r * blocks * 128 + (i - r * 2 * a.dim)];
+    }
+    raise(a.flag, bad);
+}
+// The parts' sums added up, and what becomes of them
+__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
+    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)a.tokens * a.group, all = a.heads_here * rows;
+    if (id >= all * a.dim) return;
+    const uint32_t r = (uint32_t)(id / a.dim), d = (uint32_t)(id - (size_t)r * a.dim), kv = (uint32_t)(r / rows), in = (uint32_t)(r - kv * rows), token = in / a.group;
+    uint32_t bad = 0, own = 0;
+    bool has = true;
+    if (a.seqs.count) {
+        Sequence s;
+        has = sequence_of(a.seqs, token, s, bad);
+        if (has) own = (own_seen(a, s, token) + a.own_step - 1) / a.own_step;
+    }
+    if (has) {
+        unsigned long long lo = 0;
+        int64_t size = 0;
+        auto add = [&](uint32_t split) {
+            const unsigned long long* p = (const unsigned long long*)a.parts + ((split * all + r) * a.dim + d) * 2;
+            lo += p[0];
+            size += (int64_t)p[1];
+        };
+        for (uint32_t i = 0; i < a.prefix_splits; ++i) add(i);
+        for (uint32_t i = 0; i < own; ++i) add(a.prefix_splits + i);
+        const int64_t v = (int64_t)lo;
+        if (size > (3ll << 29) || size < -(3ll << 29) || v >= (1ll << 62) || v < -(1ll << 62)) bad |= ZK_VALUES_RANGE;
+        else {
+            auto q = [](int64_t x, const Divisor& s) { return s.shift >= 0 ? quotient<true>(x, s) : quotient<false>(x, s); };
+            a.out[token * a.out_token + ((a.kv0 + kv) * a.group + (in - token * a.group)) * a.out_head + d] = narrow(q(q(v, a.sf_first), a.sf_second), bad);
+        }
+    }
+    raise(a.flag, bad);
+}
+
+// ---- logits -------------------------------------------------------------------------------------------------------------------------------
+static constexpr int32_t NO_TOKEN = INT32_MIN;
+static constexpr uint32_t LOGITS_SPAN = 4096;    // a workgroup's tokens
+struct TokenLists { const int32_t *tokens, *values, *starts; uint32_t total; };      // row r's: starts[r] .. starts[r + 1]
+struct LogitsArgs {
+    int32_t *out, *token;
+    const int32_t* logits;
+    size_t ld_out, ld;
+    uint32_t rows, vocab, spans;
+    TokenLists history, bias;
+    const int32_t* penalties;            // a row's: repeated, by count, once
+    const uint32_t* mask;
+    size_t ld_mask;
+    uint32_t mask_rows;
+    Divisor sf;
+    unsigned long long* best;            // [row][span]
+    uint32_t* flag;
+};
+__device__ __forceinline__ bool list_of(const TokenLists& l, uint32_t row, uint32_t& from, uint32_t& to, uint32_t& bad) {
+    if (!l.starts) return false;
+    const int32_t f = l.starts[row], t = l.starts[row + 1];
+    if (f < 0 || t < f || (uint32_t)t > l.total) { bad |= ZK_VALUES_POSITION; return false; }
+    from = (uint32_t)f; to = (uint32_t)t;
+    return true;
+}
+// larger values first, among equals the lower token; 0: none
+__device__ __forceinline__ unsigned long long choice(int32_t value, uint32_t token) { return value == NO_TOKEN ? 0ull : (unsigned long long)((uint32_t)value ^ 0x80000000u) << 32 | (0xFFFFFFFFu - token); }
+__device__ __forceinline__ int32_t chosen(unsigned long long best) { return best ? (int32_t)(0xFFFFFFFFu - (uint32_t)best) : -1; }
+__device__ __forceinline__ unsigned long long block_best(unsigned long long best, unsigned long long* of_wave) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) best = max(best, (unsigned long long)__shfl_xor(best, off, 64));
+    if ((threadIdx.x & 63u) == 0) of_wave[threadIdx.x >> 6] = best;
+    __syncthreads();
+    best = 0;
+    for (uint32_t i = 0; i < blockDim.x / 64; ++i) best = max(best, of_wave[i]);
+    return best;
+}
+// A workgroup takes a stretch of a row: it reads the row's lists, counts and adds up in LDS what falls into the stretch, then passes over the logits once
+template <bool POW2> __global__ void __launch_bounds__(256) k_logits(const LogitsArgs a) {
+    __shared__ uint32_t count[LOGITS_SPAN];
+    __shared__ unsigned long long add[LOGITS_SPAN];
+    __shared__ unsigned long long of_wave[4];
+    const uint32_t row = blockIdx.y, first = blockIdx.x * LOGITS_SPAN, n = min(LOGITS_SPAN, a.vocab - first);
+    uint32_t bad = 0, from = 0, to = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += 256) { count[i] = 0; add[i] = 0; }
+    __syncthreads();
+    if (list_of(a.history, row, from, to, bad))
+        for (uint32_t i = from + threadIdx.x; i < to; i += 256) {
+            const uint32_t token = (uint32_t)a.history.tokens[i];
+            if (token >= a.vocab) bad |= ZK_VALUES_POSITION;
+            else if (token - first < n) atomicAdd(&count[token - first], 1u);
+        }
+    if (list_of(a.bias, row, from, to, bad))
+        for (uint32_t i = from + threadIdx.x; i < to; i += 256) {
+            const uint32_t token = (uint32_t)a.bias.tokens[i];
+            if (token >= a.vocab) bad |= ZK_VALUES_POSITION;
+            else if (token - first < n) atomicAdd(&add[token - first], (unsigned long long)(int64_t)a.bias.values[i]);
+        }
+    __syncthreads();
+    int32_t repeat = 0, frequency = 0, presence = 0;
+    if (a.penalties) {
+        repeat = a.penalties[3 * (size_t)row]; frequency = a.penalties[3 * (size_t)row + 1]; presence = a.penalties[3 * (size_t)row + 2];
+        if (repeat <= 0) { bad |= ZK_VALUES_RANGE; repeat = 1; }
+    }
+    const uint32_t* mask = a.mask ? a.mask + (a.mask_rows == 1 ? 0 : row) * a.ld_mask : nullptr;
+    const int32_t* in = a.logits + row * a.ld;
+    unsigned long long best = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+        const uint32_t token = first + i, c = count[i];
+        int32_t l = in[token];
+        if (mask && (mask[token >> 5] >> (token & 31u) & 1u) == 0) l = NO_TOKEN;
+        if (l != NO_TOKEN && (c != 0 || add[i] != 0)) {
+            int64_t v = l;
+            if (c != 0 && a.penalties) {
+                if (v > 0) v = (v * a.sf.s + (repeat >> 1)) / repeat;
+                else v = quotient<POW2>(v * repeat, a.sf);
+                v = narrow(v, bad);
+                v -= narrow((int64_t)frequency * c + presence, bad);
+            }
+            v += narrow((int64_t)add[i], bad);
+            l = narrow(v, bad);
+            if (l == NO_TOKEN) bad |= ZK_VALUES_RANGE;
+        }
+        if (a.out) a.out[row * a.ld_out + token] = l;
+        best = max(best, choice(l, token));
+    }
+    if (a.token) {
+        best = block_best(best, of_wave);
+        if (threadIdx.x == 0) {
+            if (a.spans == 1) a.token[row] = chosen(best);
+            else a.best[(size_t)row * a.spans + blockIdx.x] = best;
+        }
+    }
+    raise(a.flag, bad);
+}
+__global__ void __launch_bounds__(64) k_logits_best(int32_t* __restrict__ token, const unsigned long long* __restrict__ best, uint32_t spans) {
+    __shared__ unsigned long long of_wave[1];
+    unsigned long long b = 0;
+    for (uint32_t i = threadIdx.x; i < spans; i += 64) b = max(b, best[(size_t)blockIdx.x * spans + i]);
+    b = block_best(b, of_wave);
+    if (threadIdx.x == 0) token[blockIdx.x] = chosen(b);
+}
+
+// ---- entry points -----------------------------------------------------------------------------------------------------------------------------------
+static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequences, uint32_t most, uint32_t heads, uint32_t dim) {
+    ZK_ARG(c->k != nullptr && c->v != nullptr, std::string(name) + ": a cache without keys or values");
+    ZK_ARG(c->page_size > 0 && c->pages > 0, std::string(name) + ": a cache without pages");
+    ZK_ARG(c->page_table != nullptr ? (uint64_t)c->table_cols * c->page_size >= most : c->page_size >= most && c->pages >= sequences,
+           std::string(name) + ": a cache with fewer places than sequences or tokens");
+    ZK_ARG((c->page_size == 1 || c->token_stride >= dim) && (heads == 1 || c->head_stride >= dim), std::string(name) + ": a cache whose heads overlap (a stride below the head's width)");
+    const unsigned __int128 of_heads = (unsigned __int128)(heads - 1) * c->head_stride + dim, of_tokens = (unsigned __int128)(c->page_size - 1) * c->token_stride + dim;
+    ZK_ARG(heads == 1 || c->page_size == 1 || c->token_stride >= of_heads || c->head_stride >= of_tokens, std::string(name) + ": a cache whose heads overlap");
+    const unsigned __int128 page = std::max((unsigned __int128)(heads - 1) * c->head_stride + (unsigned __int128)(c->page_size - 1) * c->token_stride + dim, (unsigned __int128)0);
+    ZK_ARG(c->pages == 1 || c->page_stride >= page || (heads > 1 && c->head_stride >= (unsigned __int128)(c->pages - 1) * c->page_stride + of_tokens && c->page_stride >= of_tokens),
+           std::string(name) + ": a cache whose pages overlap");
+    return 0;
+}
+static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
+
+// How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
+struct AttnPlan { uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t cols, scores, shift, parts; };
+static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
+    AttnPlan p{};
+    const uint32_t group = heads / kv_heads;
+    const size_t rows = (size_t)tokens * group;
+    p.prefix_tiles = prefix_len ? cdiv(rows, 16) : 0;
+    p.own_tiles = sequences ? (uint32_t)(rows / 16) + sequences : 0;
+    p.cols = ((size_t)prefix_len + 15) / 16 * 16 + ((size_t)max_length + 15) / 16 * 16;
+    auto cut = [&](uint32_t keys, size_t tiles, uint32_t& splits, uint32_t& step) {
+        const size_t want = std::max<size_t>(1, 1024 / std::max<size_t>(1, tiles * kv_heads));
+        splits = (uint32_t)std::min<size_t>(want, cdiv(keys, 256));
+        splits = std::max(splits, cdiv(keys, 8192));
+        step = splits ? (uint32_t)((cdiv(keys, splits) + 63) / 64 * 64) : 64;
+        splits = cdiv(keys, step);
+    };
+    cut(prefix_len, p.prefix_tiles, p.prefix_splits, p.prefix_step);
+    cut(sequences ? max_length : 0, p.own_tiles, p.own_splits, p.own_step);
+    const size_t each = rows * (p.cols * 8 + 8 + (size_t)(p.prefix_splits + p.own_splits) * dim * 16);
+    p.heads = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / std::max<size_t>(each, 1)));
+    auto round = [](size_t b) { return (b + 15) / 16 * 16; };
+    p.scores = round(p.heads * rows * p.cols * 8);
+    p.shift = round(p.heads * rows * 8);
+    p.parts = p.heads * rows * (size_t)(p.prefix_splits + p.own_splits) * dim * 16;
+    return p;
+}
+
+extern "C" {
+
+int zk_i32_cache_append(const zk_i32_cache* cache, const void* k, size_t k_token, size_t k_head, const void* v, size_t v_token, size_t v_head, uint32_t tokens, uint32_t heads, uint32_t dim,
+                        uint32_t sequences, const void* starts, const void* lengths, void* flag_dev, void* stv) {
+    static const char* name = "zk_i32_cache_append";
+    if (tokens == 0 || heads == 0) return 0;
+    ZK_ARG(cache != nullptr && k != nullptr && v != nullptr && lengths != nullptr && sequences > 0 && dim > 0, std::string(name) + ": null argument, no sequences or empty heads");
+    ZK_ARG(starts != nullptr || tokens % sequences == 0, std::string(name) + ": without starts the tokens must divide among the sequences");
+    ZK_ARG((uint64_t)heads * dim <= (1u << 30), std::string(name) + ": more than 2^30 elements a token");
+    if (const int rc = check_cache(cache, name, sequences, 1, heads, dim)) return rc;
+    hipStream_t st = (hipStream_t)stv;
+    CallFlag flag;
+    if (const int rc = flag.begin(flag_dev, st, name)) return rc;
+    const uint64_t most = cache->page_table ? (uint64_t)cache->table_cols * cache->page_size : cache->page_size;
+    const AppendArgs a{*cache, (const int32_t*)k, (const int32_t*)v, k_token, k_head, v_token, v_head, heads, dim,
+                       Sequences{(const int32_t*)starts, (const int32_t*)lengths, sequences, tokens, (uint32_t)std::min<uint64_t>(most, 0x7FFFFFFFu)}, flag.dev};
+    if (dim % 4 == 0 && cache_aligned(cache) && ((k_token | k_head | v_token | v_head) & 3) == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0)
+        hipLaunchKernelGGL(k_cache_append<4>, dim3(tokens), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_cache_append<1>, dim3(tokens), dim3(256), 0, st, a);
+    ZK_LAUNCH_CHECK();
+    return flag.end(name);
+}
+
+int zk_i32_softmax_free(void* softmax) {
+    SoftmaxPlan* s = (SoftmaxPlan*)softmax;
+    if (!s) return 0;
+    int rc = 0;
+    if (s->memory) rc = pool_free(s->memory, nullptr);
+    delete s;
+    return rc;
+}
+int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int M, double scaling_factor_in, const double* thetas, uint32_t dim, void* stv) {
+    static const char* name = "zk_i32_softmax_prepare";
+    hipStream_t st = (hipStream_t)stv;
+    ZK_ARG(softmax != nullptr && bs != nullptr && thetas != nullptr && dim > 0, std::string(name) + ": null argument or empty heads");
+    ZK_ARG(K >= 1 && K <= DIGITS && L >= 0 && M >= 0 && L + M < K, std::string(name) + ": 1 to 8 digits, and at least one of them between the lowest L and the highest M");
+    ZK_ARG(scaling_factor_in >= 1 && scaling_factor_in <= 1e18, std::string(name) + ": the scaling factor must lie within 1 .. 1e18");
+    if (const int rc = CallFlag::not_captured(st, name)) return rc;
+    std::unique_ptr<SoftmaxPlan> s(new SoftmaxPlan);
+    s->dim = dim;
+    SoftmaxArgs& a = s->a;
+    a = SoftmaxArgs{};
+    a.scale = scaling_factor_in * std::sqrt((double)dim);
+    a.drop = 1;
+    a.n = K - L;
+    unsigned __int128 reach = 1;
+    double most = 1;
+    size_t entries = 0;
+    for (int i = 0; i < K; ++i) {
+        ZK_ARG(bs[i] >= 1 && bs[i] <= (1u << 28), std::string(name) + ": a radix must lie within 1 .. 2^28");
+        reach *= bs[i];
+        ZK_ARG(reach <= ((unsigned __int128)1 << 63), std::string(name) + ": the radices' product is above 2^63");
+        const bool p2 = (bs[i] & (bs[i] - 1)) == 0;
+        s->pow2 = s->pow2 && p2;
+        if (i < L) { a.drop *= bs[i]; a.drop_bits += 31 - __builtin_clz(bs[i]); }
+        else {
+            a.radix[i - L] = bs[i];
+            a.bits[i - L] = 31 - __builtin_clz(bs[i]);
+            if (i < K - M) {
+                const double theta = thetas[i - L];
+                ZK_ARG(theta > 0 && theta < 2147483647.0, std::string(name) + ": a factor of the exponentials must lie within 0 .. 2^31 - 1");
+                most *= std::floor(theta + 1.0);
+                entries += bs[i];
+            }
+        }
+    }
+    ZK_ARG(most < 140000000000000.0, std::string(name) + ": weights of 1.4e14 and more (six digits of eight bits)");
+    if (const int rc = pool_alloc((void**)&s->memory, entries * 4, st)) return rc;
+    double weight = 1;
+    size_t at = 0;
+    for (int i = 0; i < K; ++i) {
+        if (i >= L && i < K - M) {
+            a.table[i - L] = s->memory + at;
+            at += bs[i];
+            hipLaunchKernelGGL(k_softmax_table_i32, dim3(cdiv(bs[i], 256)), dim3(256), 0, st, s->memory + at - bs[i], zkd::log_det(thetas[i - L]), weight / a.scale, bs[i]);
+        }
+        weight *= bs[i];
+    }
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = hipStreamSynchronize(st);      // calls on any stream may use the tables
+    if (e != hipSuccess) { (void)pool_free(s->memory, st); return hip_fail(e, "k_softmax_table_i32", __FILE__, __LINE__); }
+    *softmax = s.release();
+    return 0;
+}
+
+size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
+    if (tokens == 0 || kv_heads == 0 || heads < kv_heads) return 0;
+    const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
+    return p.scores + p.shift + p.parts;
+}
+int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
+                     const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts, const void* lengths, uint32_t max_length,
+                     int causal, uint32_t sf_first, uint32_t sf_second, void* shift, void* workspace, size_t workspace_bytes, void* flag_dev, void* stv) {
+    static const char* name = "zk_i32_attention";
+    if (tokens == 0 || heads == 0) return 0;
+    const SoftmaxPlan* s = (const SoftmaxPlan*)softmax;
+    ZK_ARG(out != nullptr && q != nullptr && s != nullptr, std::string(name) + ": null argument");
+    ZK_ARG(dim > 0 && dim <= 256, std::string(name) + ": heads of 1 to 256 elements");
+    ZK_ARG(kv_heads > 0 && heads % kv_heads == 0, std::string(name) + ": the heads must divide among those of keys and values");
+    ZK_ARG((uint64_t)tokens * (heads / kv_heads) <= (1u << 20) && heads <= 65535, std::string(name) + ": more than 2^20 queries for a head of keys in one call, or more than 65535 heads");
+    ZK_ARG(prefix_len <= (1u << 24) && max_length <= (1u << 24), std::string(name) + ": more than 2^24 keys");
+    ZK_ARG((prefix != nullptr && prefix_len > 0) || own != nullptr, std::string(name) + ": neither a prefix nor sequences of their own");
+    ZK_ARG(prefix_len == 0 || prefix != nullptr, std::string(name) + ": no prefix");
+    ZK_ARG(own == nullptr || (sequences > 0 && sequences <= tokens + 65536u && lengths != nullptr), std::string(name) + ": sequences need lengths");
+    ZK_ARG(own != nullptr || max_length == 0, std::string(name) + ": own keys without a cache");
+    ZK_ARG(own == nullptr || starts != nullptr || tokens % sequences == 0, std::string(name) + ": without starts the tokens must divide among the sequences");
+    ZK_ARG(sf_first > 0 && sf_second > 0, std::string(name) + ": a scaling factor of 0");
+    ZK_ARG(out != q || (out_token == q_token && out_head == q_head), std::string(name) + ": in place with other strides");
+    ZK_ARG((tokens == 1 || out_token >= dim) && (heads == 1 || out_head >= dim), std::string(name) + ": heads overlap (a stride below the head's width)");
+    {
+        const unsigned __int128 of_heads = (unsigned __int128)(heads - 1) * out_head + dim, of_tokens = (unsigned __int128)(tokens - 1) * out_token + dim;
+        ZK_ARG(tokens == 1 || heads == 1 || out_token >= of_heads || out_head >= of_tokens, std::string(name) + ": the output's heads overlap");
+    }
+    if (prefix_len) if (const int rc = check_cache(prefix, name, 1, prefix_len, kv_heads, dim)) return rc;
+    if (own) if (const int rc = check_cache(own, name, sequences, max_length, kv_heads, dim)) return rc;
+    if (!own) sequences = 0;
+    const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
+    ZK_ARG(p.prefix_tiles + p.own_tiles <= 65535u, std::string(name) + ": more than 65535 tiles of queries");
+    hipStream_t st = (hipStream_t)stv;
+    const size_t bytes = p.scores + p.shift + p.parts;
+    ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_attention_workspace says");
+    ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
+    ZK_ARG(dim == s->dim, std::string(name) + ": the softmax was prepared for heads of another width");
+    CallFlag flag;
+    if (const int rc = flag.begin(flag_dev, st, name)) return rc;
+    std::unique_ptr<Scratch> scratch;
+    if (!workspace) {
+        if (const int rc = CallFlag::not_captured(st, name)) return rc;
+        scratch.reset(new Scratch(bytes, st));
+        if (scratch->rc) return scratch->rc;
+        workspace = scratch->p;
+    }
+    AttnArgs a{};
+    a.out = (int32_t*)out; a.q = (const int32_t*)q; a.out_token = out_token; a.out_head = out_head; a.q_token = q_token; a.q_head = q_head;
+    a.group = heads / kv_heads; a.dim = dim; a.kv_heads = kv_heads; a.shift_out = (int64_t*)shift; a.softmax = s->a;
+    if (prefix_len) a.prefix = *prefix;
+    if (own) a.own = *own;
+    a.prefix_len = prefix_len; a.prefix_cols = (prefix_len + 15) / 16 * 16;
+    a.seqs = Sequences{own ? (const int32_t*)starts : nullptr, (const int32_t*)lengths, sequences, tokens, max_length};
+    a.causal = causal; a.sf_first = divisor(sf_first); a.sf_second = divisor(sf_second);
+    a.scores = (int64_t*)workspace; a.ld = p.cols; a.shift = (int64_t*)((char*)workspace + p.scores); a.parts = (int64_t*)((char*)workspace + p.scores + p.shift);
+    a.tokens = tokens; a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits; a.prefix_step = p.prefix_step; a.own_splits = p.own_splits; a.own_step = p.own_step;
+    a.flag = flag.dev;
+    const bool vec = dim % 4 == 0 && ((q_token | q_head) & 3) == 0 && ((uintptr_t)q & 15) == 0 && (!prefix_len || cache_aligned(prefix)) && (!own || cache_aligned(own));
+    const unsigned tiles = p.prefix_tiles + p.own_tiles, chunks = std::max(1u, std::max(cdiv(prefix_len, SCORE_KEYS), cdiv(max_length, SCORE_KEYS)));
+    const unsigned splits = std::max(1u, std::max(p.prefix_splits, p.own_splits)), blocks = cdiv(dim, 64);
+    for (a.kv0 = 0; a.kv0 < kv_heads; a.kv0 += p.heads) {
+        a.heads_here = std::min(p.heads, kv_heads - a.kv0);
+        const size_t rows = (size_t)a.heads_here * tokens * a.group;
+        const dim3 grid(chunks, tiles, a.heads_here), vgrid(splits, tiles, a.heads_here);
+        auto scores = [&](auto u) {
+            constexpr int U = decltype(u)::value;
+            if (vec) hipLaunchKernelGGL((k_attn_scores<U, true>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((k_attn_scores<U, false>), grid, dim3(256), 0, st, a);
+        };
+        if (blocks == 1) scores(std::integral_constant<int, 1>());
+        else if (blocks == 2) scores(std::integral_constant<int, 2>());
+        else scores(std::integral_constant<int, 4>());
+        hipLaunchKernelGGL(k_attn_shift, dim3(cdiv(rows, 4)), dim3(256), 0, st, a);
+        const size_t lds = 16 * (size_t)blocks * 64 * 16;
+        if (vec && s->pow2) hipLaunchKernelGGL((k_attn_values<true, true>), vgrid, dim3(256), lds, st, a);
+        else if (vec) hipLaunchKernelGGL((k_attn_values<true, false>), vgrid, dim3(256), lds, st, a);
+        else if (s->pow2) hipLaunchKernelGGL((k_attn_values<false, true>), vgrid, dim3(256), lds, st, a);
+        else hipLaunchKernelGGL((k_attn_values<false, false>), vgrid, dim3(256), lds, st, a);
+        hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 256)), dim3(256), 0, st, a);
+    }
+    ZK_LAUNCH_CHECK();
+    return flag.end(name);
+}
+
+size_t zk_i32_logits_workspace(uint32_t rows, uint32_t vocab) {
+    const size_t spans = cdiv(vocab, LOGITS_SPAN);
+    return spans <= 1 ? 0 : rows * spans * sizeof(unsigned long long);
+}
+int zk_i32_logits(void* out, size_t ld_out, void* token, const void* logits, size_t ld, uint32_t rows, uint32_t vocab, const void* history, uint32_t history_len, const void* history_starts,
+                  const void* penalties, const void* bias_tokens, const void* bias_values, uint32_t bias_len, const void* bias_starts, const void* mask, size_t ld_mask, uint32_t mask_rows, uint32_t sf,
+                  void* workspace, size_t workspace_bytes, void* flag_dev, void* stv) {
+    static const char* name = "zk_i32_logits";
+    if (rows == 0) return 0;
+    ZK_ARG(logits != nullptr && (out != nullptr || token != nullptr) && vocab > 0, std::string(name) + ": null logits, no output or no tokens");
+    ZK_ARG(vocab <= (1u << 30) && rows <= 65535, std::string(name) + ": more than 2^30 tokens or 65535 rows");
+    ZK_ARG(rows == 1 || (ld >= vocab && (out == nullptr || ld_out >= vocab)), std::string(name) + ": rows overlap (a leading dimension below the number of tokens)");
+    ZK_ARG(out != logits || rows == 1 || ld_out == ld, std::string(name) + ": in place with another leading dimension");
+    ZK_ARG(history_starts == nullptr || ((history != nullptr || history_len == 0) && penalties != nullptr), std::string(name) + ": a history needs its tokens and penalties");
+    ZK_ARG(history_starts != nullptr || (history == nullptr && penalties == nullptr), std::string(name) + ": a history or penalties without starts");
+    ZK_ARG(bias_starts == nullptr || (bias_tokens != nullptr && bias_values != nullptr) || bias_len == 0, std::string(name) + ": biases need their tokens and values");
+    ZK_ARG(bias_starts != nullptr || (bias_tokens == nullptr && bias_values == nullptr), std::string(name) + ": biases without starts");
+    ZK_ARG(history_len <= 0x7FFFFFFFu && bias_len <= 0x7FFFFFFFu, std::string(name) + ": a list of more than 2^31 - 1 tokens");
+    ZK_ARG(mask == nullptr ? mask_rows == 0 : (mask_rows == 1 || (mask_rows == rows && ld_mask >= (vocab + 31) / 32)), std::string(name) + ": a mask has one row or a row for each of the logits'");
+    ZK_ARG(sf > 0, std::string(name) + ": a scaling factor of 0");
+    hipStream_t st = (hipStream_t)stv;
+    const size_t bytes = token ? zk_i32_logits_workspace(rows, vocab) : 0;
+    ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_logits_workspace says");
+    ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
+    CallFlag flag;
+    if (const int rc = flag.begin(flag_dev, st, name)) return rc;
+    std::unique_ptr<Scratch> scratch;
+    if (!workspace && bytes) {
+        if (const int rc = CallFlag::not_captured(st, name)) return rc;
+        scratch.reset(new Scratch(bytes, st));
+        if (scratch->rc) return scratch->rc;
+        workspace = scratch->p;
+    }
+    const uint32_t spans = cdiv(vocab, LOGITS_SPAN);
+    const LogitsArgs a{(int32_t*)out, (int32_t*)token, (const int32_t*)logits, ld_out, ld, rows, vocab, spans,
+                       TokenLists{(const int32_t*)history, nullptr, (const int32_t*)history_starts, history_len},
+                       TokenLists{(const int32_t*)bias_tokens, (const int32_t*)bias_values, (const int32_t*)bias_starts, bias_len}, (const int32_t*)penalties, (const uint32_t*)mask, ld_mask, mask_rows,
+                       divisor(sf), (unsigned long long*)workspace, flag.dev};
+    if (a.sf.shift >= 0) hipLaunchKernelGGL(k_logits<true>, dim3(spans, rows), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_logits<false>, dim3(spans, rows), dim3(256), 0, st, a);
+    if (token && spans > 1) hipLaunchKernelGGL(k_logits_best, dim3(rows), dim3(64), 0, st, (int32_t*)token, (const unsigned long long*)workspace, spans);
+    ZK_LAUNCH_CHECK();
+    return flag.end(name);
+}
+
+}  // extern "C"

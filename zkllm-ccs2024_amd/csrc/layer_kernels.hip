@@ -14,41 +14,13 @@
 // or written out of range for them.
 #include <algorithm>
 #include <cmath>
-#include <cstring>
-#include <memory>
 #include <type_traits>
 #include "detmath.hpp"
 #include "field.hpp"
-#include "planes.hpp"
-#include "rt.hpp"
+#include "intvalues.hpp"
 #include "../../include/zkllm_hip.h"
 
 using namespace zk;
-
-// ---- quotients --------------------------------------------------------------------------------------------------------------------------
-// shift >= 0: s is 2^shift, else any.  POW2 is a template argument where a kernel divides often.
-struct Divisor { int64_t s, half; double inv; int shift; };
-static Divisor divisor(uint32_t s) { return Divisor{(int64_t)s, (int64_t)(s >> 1), 1.0 / (double)s, (s & (s - 1)) == 0 ? 31 - __builtin_clz(s) : -1}; }
-// floor((t + s / 2) / s) for |t| <= 2^62, by the divisor's double-precision inverse: the first quotient is off by no more than 3 2^-53 2^62 / s + 1, what
-// it leaves is below s + 2^11 in magnitude and divided exactly up to one unit.  Some 30 instructions against some 100 of a 64-bit division.
-__device__ __forceinline__ int64_t quotient_general(int64_t t, const Divisor& d) {
-    const int64_t n = t + d.half;
-    int64_t q = (int64_t)floor((double)n * d.inv);
-    int64_t r = n - q * d.s;
-    const int64_t more = (int64_t)floor((double)r * d.inv);
-    q += more;
-    r -= more * d.s;
-    return q - (r < 0 ? 1 : 0) + (r >= d.s ? 1 : 0);
-}
-template <bool POW2> __device__ __forceinline__ int64_t quotient(int64_t t, const Divisor& d) {
-    if constexpr (POW2) return (t + d.half) >> d.shift;
-    else return quotient_general(t, d);
-}
-__device__ __forceinline__ int32_t narrow(int64_t v, uint32_t& bad) {
-    bad |= (int32_t)(v >> 32) != ((int32_t)v >> 31) ? (uint32_t)ZK_VALUES_RANGE : 0u;
-    return (int32_t)v;
-}
-__device__ __forceinline__ void raise(uint32_t* flag, uint32_t bad) { if (bad) atomicOr(flag, bad); }
 
 // ---- norms with the residual stream -------------------------------------------------------------------------------------------------------
 struct NormArgs {
@@ -421,44 +393,6 @@ struct ProductArgs {
     Epilogue e;
 };
 static constexpr uint32_t CHUNK = 256;
-// sum_s a[s] 256^s: within -2^62 .. 2^62 - 1, or flagged and 0.  Six planes in all cannot leave that range: p digits hold 128 (256^p - 1) / 255 at most, and
-// 43690 products of three by three digits, or of four by two, stay below 2^61.5.
-template <int NS> __device__ __forceinline__ int64_t joined(const int32_t (&a)[NS], uint32_t& bad) {
-    if constexpr (NS <= 5) {
-        int64_t v = a[0];
-#pragma unroll
-        for (int s = 1; s < NS; ++s) v += (int64_t)a[s] << (8 * s);
-        return v;
-    } else {
-        // |a[s]| < 2^31, so the two low terms are below 2^41 together, and the sum in units of 2^16, which the others' 2^56 leave room for, says whether it fits
-        const int64_t lo = a[0] + (int64_t)a[1] * 256;
-        int64_t hi = 0;
-#pragma unroll
-        for (int s = NS - 1; s >= 2; --s) hi = hi * 256 + a[s];
-        const int64_t units = hi + (lo >> 16);
-        const bool fits = (uint32_t)((int32_t)(units >> 32) + 0x4000) < 0x8000u;      // -2^46 .. 2^46 - 1
-        bad |= fits ? 0u : (uint32_t)ZK_VALUES_RANGE;
-        return fits ? (int64_t)((uint64_t)hi * 65536 + (uint64_t)lo) : 0;
-    }
-}
-// the digits of 16 values, plane by plane: plane j's 16 bytes in out[j]
-__device__ __forceinline__ void digit_planes(const int32_t (&x)[16], v4i (&out)[4], uint32_t& bad) {
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        uint32_t d[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            bad |= x[4 * w + e] > 0x7F7F7F7F ? (uint32_t)ZK_VALUES_RANGE : 0u;      // four digits reach no further
-            d[e] = digit_bytes((uint32_t)x[4 * w + e]);
-        }
-        const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), b = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
-        const uint32_t c = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), e = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
-        out[0][w] = (int)__builtin_amdgcn_perm(c, a, 0x05040100u);
-        out[1][w] = (int)__builtin_amdgcn_perm(c, a, 0x07060302u);
-        out[2][w] = (int)__builtin_amdgcn_perm(e, b, 0x05040100u);
-        out[3][w] = (int)__builtin_amdgcn_perm(e, b, 0x07060302u);
-    }
-}
 // 16 values of a row from column k on; zeros beyond the row's end and for rows that are none
 __device__ __forceinline__ void row_piece(const ProductArgs& g, uint32_t row, uint32_t k, int32_t (&x)[16]) {
 #pragma unroll
@@ -903,56 +837,83 @@ __global__ void __launch_bounds__(256) k_split_cols_i32(int8_t* __restrict__ pla
             *reinterpret_cast<v4i*>(planes + (size_t)j * P * Kp + plane_at(P, p0 + row, k0 + ch * 16)) = *reinterpret_cast<const v4i*>(&tile[j][row][ch * 16]);
 }
 
-// ---- entry points -----------------------------------------------------------------------------------------------------------------------------------
-// The flag of a call: the caller's, or one of the call's own that is looked at before the call returns.
-struct CallFlag {
-    uint32_t* dev = nullptr;
-    std::unique_ptr<Scratch> own;
-    hipStream_t st;
-    int begin(void* flag_dev, hipStream_t stream, const char* name) {
-        st = stream;
-        dev = (uint32_t*)flag_dev;
-        if (dev) return 0;
-        if (const int rc = not_captured(stream, name)) return rc;
-        own.reset(new Scratch(4, stream));
-        if (own->rc) return own->rc;
-        dev = own->as<uint32_t>();
-        return clear_words(dev, 1, stream);
-    }
-    // what a call without a flag of the caller's, or without a workspace, does cannot be captured: it waits, and its memory goes back to the pool
-    static int not_captured(hipStream_t stream, const char* name) {
-        if (!stream) return 0;
-        hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
-        ZK_HIP(hipStreamIsCapturing(stream, &s));
-        if (s != hipStreamCaptureStatusNone) {
-            set_error(ZK_ERR_ARG, std::string(name) + ": a captured call needs a flag and a workspace of the caller's");
-            return ZK_ERR_ARG;
+// ---- weights of 4 bits -------------------------------------------------------------------------------------------------------------------------
+// w = (code - zero) scale, a scale and a zero for every `group` rows of a column.  Codes stand as the fragments of v_mfma_i32_16x16x64_i8 want them: [strip of 16 columns][128
+// rows][lane][16 bytes], a lane's 16 bytes its 16 rows of the first 64 and of the second, so that a wave reads 1 KB in one piece; in a 32-bit word the low halves of the bytes are
+// rows 0 .. 3, the high ones rows 4 .. 7.  A group's scales and zeros: [strip][group][column], scale * 16 + zero.
+struct Q4 { const uint32_t* codes; const int32_t* scales; uint32_t group, groups, units, cols; };
+static size_t q4_code_bytes(uint32_t P, uint32_t Kp) { return (size_t)cdiv(P, 16) * 16 * Kp / 2; }
+static Q4 q4_of(const MatmulRhs* w) { return Q4{(const uint32_t*)w->q4, (const int32_t*)((const char*)w->q4 + q4_code_bytes(w->P, w->Kp)), w->group, w->groups, w->Kp / 64, w->P}; }
+// a lane's 16 rows of unit u in a strip
+__device__ __forceinline__ uint2 q4_codes(const Q4& w, uint32_t strip, uint32_t u, uint32_t lane) {
+    return *reinterpret_cast<const uint2*>(w.codes + (((size_t)strip * (w.units >> 1) + (u >> 1)) * 64 + lane) * 4 + 2 * (u & 1u));
+}
+__device__ __forceinline__ int32_t q4_scale(const Q4& w, uint32_t strip, uint32_t k, uint32_t c) { return w.scales[((size_t)strip * w.groups + min(k / w.group, w.groups - 1)) * 16 + c]; }
+// 16 codes times their scale as digit planes
+template <int PB> __device__ __forceinline__ void q4_planes(uint2 codes, int32_t scale_zero, v4i (&out)[PB]) {
+    const int32_t scale = scale_zero >> 4, off = -(scale_zero & 15) * scale;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const uint32_t half = (w < 2 ? codes.x : codes.y) >> (w & 1 ? 4 : 0);
+        uint32_t d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = digit_bytes((uint32_t)((int32_t)(half >> (8 * e) & 15u) * scale + off));
+        const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), b = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u);
+        out[0][w] = (int)__builtin_amdgcn_perm(b, a, 0x05040100u);
+        out[1][w] = (int)__builtin_amdgcn_perm(b, a, 0x07060302u);
+        if constexpr (PB > 2) {
+            const uint32_t f = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u), g = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+            out[2][w] = (int)__builtin_amdgcn_perm(g, f, 0x05040100u);
         }
-        return 0;
     }
-    int end(const char* name) {
-        if (!own) return 0;
-        void* stage = nullptr;
-        if (const int rc = staging(&stage, 4)) return rc;
-        ZK_HIP(hipMemcpyAsync(stage, dev, 4, hipMemcpyDeviceToHost, st));
-        ZK_HIP(hipStreamSynchronize(st));
-        uint32_t bad = 0;
-        memcpy(&bad, stage, 4);
-        if (!bad) return 0;
-        const char* what = (bad & ZK_VALUES_TABLE) ? ": an activation lies outside the table" : (bad & ZK_VALUES_POSITION) ? ": a position lies outside the table" : ": a value does not fit";
-        set_error(ZK_ERR_ARG, std::string(name) + what);
-        return ZK_ERR_ARG;
+}
+// the planes of a whole weight, for products of many rows
+template <int PB> __global__ void __launch_bounds__(256) k_q4_expand(int8_t* __restrict__ planes, const Q4 w) {
+    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4, strip = blockIdx.x, u = blockIdx.y * 4 + (threadIdx.x >> 6), col = strip * 16 + c;
+    if (u >= w.units || col >= w.cols) return;
+    v4i d[PB];
+    q4_planes<PB>(q4_codes(w, strip, u, lane), q4_scale(w, strip, u * 64 + q * 16, c), d);
+#pragma unroll
+    for (int j = 0; j < PB; ++j) *reinterpret_cast<v4i*>(planes + (size_t)j * w.cols * w.units * 64 + plane_at(w.cols, col, u * 64 + q * 16)) = d[j];
+}
+// Codes and scales to their places, and the largest element's magnitude.  bad[0]: a scale or zero out of range
+__global__ void __launch_bounds__(256) k_q4_scales(int32_t* __restrict__ out, const int32_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint32_t P, uint32_t groups, uint32_t* __restrict__ bad) {
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x, c = at & 15u, g = at / 16 % groups, col = at / 16 / groups * 16 + c;
+    if (at >= (P + 15) / 16 * groups * 16) return;
+    const int32_t s = col < P ? scales[(size_t)g * P + col] : 0;
+    const uint32_t z = col < P && zeros ? zeros[(size_t)g * P + col] : 8u;
+    if (s > 557047 || s < -557047 || z > 15) { atomicOr(bad, 1u); out[at] = 0; return; }
+    out[at] = s * 16 + (int32_t)z;
+}
+__global__ void __launch_bounds__(256) k_q4_codes(uint32_t* __restrict__ out, const uint8_t* __restrict__ codes, const Q4 w, uint32_t N, unsigned long long* __restrict__ most) {
+    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4, strip = blockIdx.x, u = blockIdx.y * 4 + (threadIdx.x >> 6), col = strip * 16 + c, k0 = u * 64 + q * 16;
+    uint32_t m = 0;
+    if (u < w.units) {
+        const int32_t sz = q4_scale(w, strip, k0, c), scale = sz >> 4, zero = sz & 15;
+        uint32_t word[2] = {0, 0};
+        for (uint32_t i = 0; i < 16; ++i) {
+            if (col >= w.cols || k0 + i >= N) continue;
+            const uint32_t code = codes[(size_t)(k0 + i) * ((w.cols + 1) / 2) + col / 2] >> (col & 1u ? 4 : 0) & 15u;
+            word[i >> 3] |= code << (8 * (i & 3u) + (i & 4u));
+            const int32_t v = ((int32_t)code - zero) * scale;
+            m = max(m, (uint32_t)(v < 0 ? -v : v));
+        }
+        *reinterpret_cast<uint2*>(out + (((size_t)strip * (w.units >> 1) + (u >> 1)) * 64 + lane) * 4 + 2 * (u & 1u)) = make_uint2(word[0], word[1]);
     }
-};
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) m = max(m, (uint32_t)__shfl_xor(m, off, 64));
+    if (lane == 0 && m) atomicMax(most, (unsigned long long)m);
+}
 
+// ---- entry points -----------------------------------------------------------------------------------------------------------------------------------
 static constexpr uint32_t MAX_INNER = (1u << 17) / 3;      // three plane pairs of 2^14 a term in an int32 accumulator
 static int check_weight(const MatmulRhs* w, const char* name) {
     ZK_ARG(w != nullptr, std::string(name) + ": null weight");
     ZK_ARG(w->N <= MAX_INNER, std::string(name) + ": an inner dimension above 43690");
-    ZK_ARG(w->planes != nullptr && w->pb >= 1 && w->pb <= 3, std::string(name) + ": the weight has elements beyond 8355711 (three digits of eight bits)");
+    ZK_ARG((w->planes != nullptr || w->q4 != nullptr) && w->pb >= 1 && w->pb <= 3, std::string(name) + ": the weight has elements beyond 8355711 (three digits of eight bits)");
     return 0;
 }
-static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->planes, w->P, w->Kp, w->pb}; }
+static Planes planes_of(const MatmulRhs* w) { return Planes{(const int8_t*)w->planes, w->P, w->Kp, w->q4 ? std::max(w->pb, 2) : w->pb}; }
 
 // Up to here a product is one launch that splits x itself: 16 rows of 4096 x 11008 40 us so and 28 with a launch of k_split_x before, 4 rows 24 and 28.
 static constexpr uint32_t SPLIT_ROWS = 4;
@@ -1009,33 +970,50 @@ template <bool GATED, int PB> static void launch_product(const ProductArgs& g, h
     else if (g.e.pow2) launch_tiles<GATED, PB, true>(g, st);
     else launch_tiles<GATED, PB, false>(g, st);
 }
-template <bool GATED> static int product(const char* name, ProductArgs& g, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
+// the planes that a product of many rows reads, in the workspace where the weight has none of its own
+static size_t expanded(const MatmulRhs* w) { return w->q4 ? (size_t)std::max(w->pb, 2) * w->P * w->Kp : 0; }
+static void expand(const MatmulRhs* w, int8_t* planes, hipStream_t st) {
+    const dim3 grid(cdiv(w->P, 16), cdiv(w->Kp / 64, 4));
+    if (w->pb <= 2) hipLaunchKernelGGL(k_q4_expand<2>, grid, dim3(256), 0, st, planes, q4_of(w));
+    else hipLaunchKernelGGL(k_q4_expand<3>, grid, dim3(256), 0, st, planes, q4_of(w));
+}
+template <bool GATED> static int product(const char* name, ProductArgs& g, const MatmulRhs* w, const MatmulRhs* gate, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
     ZK_ARG(g.x != nullptr && g.e.out != nullptr, std::string(name) + ": null tensor");
     ZK_ARG(g.x != g.e.out, std::string(name) + ": in place");
     ZK_ARG(g.ldx >= g.inner, std::string(name) + ": rows of x overlap (ldx below the inner dimension)");
     ZK_ARG(g.rows <= (1u << 18), std::string(name) + ": more than 262144 rows in one call");
     ZK_ARG(g.cols <= (1u << 22), std::string(name) + ": more than 4194304 columns");
-    ZK_ARG(workspace == nullptr || workspace_bytes >= zk_i32_linear_workspace(g.rows, g.inner), std::string(name) + ": the workspace is smaller than zk_i32_linear_workspace says");
+    const size_t bytes = zk_i32_linear_workspace(g.rows, g.inner), all = bytes + expanded(w) + (GATED ? expanded(gate) : 0);
+    ZK_ARG(workspace == nullptr || workspace_bytes >= all, std::string(name) + ": the workspace is smaller than " + (w->q4 ? "zk_i32_rhs_workspace" : "zk_i32_linear_workspace") + " says");
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
     g.e.flag = flag.dev;
     g.x_aligned = (g.ldx & 3) == 0 && ((uintptr_t)g.x & 15) == 0;
     const int pb = std::max(g.w.n, GATED ? g.gate.n : 0);
+    std::unique_ptr<Scratch> own;
+    if (!workspace && all) {
+        if (const int rc = CallFlag::not_captured(st, name)) return rc;
+        own.reset(new Scratch(all, st));
+        if (own->rc) return own->rc;
+        workspace = own->p;
+    }
+    ZK_ARG(all == 0 || ((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
+    if (w->q4) {
+        int8_t* at = (int8_t*)workspace + bytes;
+        expand(w, at, st);
+        g.w.p = at;
+        if constexpr (GATED) {
+            at += expanded(w);
+            expand(gate, at, st);
+            g.gate.p = at;
+        }
+    }
     if (g.rows <= SPLIT_ROWS) {
         if (pb <= 2) launch_row<GATED, 2>(g, st);
         else launch_row<GATED, 3>(g, st);
         ZK_LAUNCH_CHECK();
         return flag.end(name);
     }
-    const size_t bytes = zk_i32_linear_workspace(g.rows, g.inner);
-    std::unique_ptr<Scratch> own;
-    if (!workspace) {
-        if (const int rc = CallFlag::not_captured(st, name)) return rc;
-        own.reset(new Scratch(bytes, st));
-        if (own->rc) return own->rc;
-        workspace = own->p;
-    }
-    ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
     g.rows_padded = padded_rows(g.rows);
     g.chunks = cdiv(g.w.Kp, CHUNK);
     g.px = (const int8_t*)workspace;
@@ -1207,6 +1185,46 @@ int zk_i32_rhs_prepare(void** prepared, const void* B, uint32_t N, uint32_t P, v
     *prepared = r.release();
     return 0;
 }
+int zk_i32_rhs_prepare_q4(void** prepared, const void* codes, const void* scales, const void* zeros, uint32_t N, uint32_t P, uint32_t group, void* stv) {
+    static const char* name = "zk_i32_rhs_prepare_q4";
+    hipStream_t st = (hipStream_t)stv;
+    ZK_ARG(prepared != nullptr && codes != nullptr && scales != nullptr && N > 0 && P > 0, std::string(name) + ": null argument or empty matrix");
+    ZK_ARG(N <= MAX_INNER && P <= (1u << 22), std::string(name) + ": an inner dimension above 43690, or more than 4194304 columns");
+    ZK_ARG(group >= 16 && group % 16 == 0, std::string(name) + ": groups must be multiples of 16 rows");
+    if (const int rc = CallFlag::not_captured(st, name)) return rc;
+    std::unique_ptr<MatmulRhs> r(new MatmulRhs);
+    r->N = N; r->P = P; r->Kp = (N + GBK - 1) / GBK * GBK; r->group = group; r->groups = cdiv(N, group);
+    const size_t entries = (size_t)cdiv(P, 16) * r->groups * 16, code_bytes = q4_code_bytes(P, r->Kp);
+    ZK_ARG(entries <= 0xFFFFFF00u, std::string(name) + ": too many groups");
+    Scratch found(16, st);       // the largest magnitude, and whether a scale or zero is out of range
+    if (found.rc) return found.rc;
+    if (const int rc = clear_words(found.p, 4, st)) return rc;
+    if (const int rc = pool_alloc(&r->q4, code_bytes + entries * 4, st)) return rc;
+    auto fail = [&](int rc) { (void)pool_free(r->q4, st); return rc; };
+    const Q4 w = q4_of(r.get());
+    hipLaunchKernelGGL(k_q4_scales, dim3(cdiv(entries, 256)), dim3(256), 0, st, (int32_t*)w.scales, (const int32_t*)scales, (const uint8_t*)zeros, P, r->groups, found.as<uint32_t>() + 2);
+    hipLaunchKernelGGL(k_q4_codes, dim3(cdiv(P, 16), cdiv(w.units, 4)), dim3(256), 0, st, (uint32_t*)w.codes, (const uint8_t*)codes, w, N, found.as<unsigned long long>());
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return fail(hip_fail(e, "k_q4_codes", __FILE__, __LINE__));
+    void* stage = nullptr;
+    if (const int rc = staging(&stage, 16)) return fail(rc);
+    hipError_t e = hipMemcpyAsync(stage, found.p, 16, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);        // the codes are the caller's again, and any stream may read the handle's
+    if (e != hipSuccess) return fail(hip_fail(e, "hipStreamSynchronize", __FILE__, __LINE__));
+    uint32_t answer[4];
+    memcpy(answer, stage, 16);
+    if (answer[2]) {
+        set_error(ZK_ERR_ARG, std::string(name) + ": a scale beyond 557047 or a zero above 15");
+        return fail(ZK_ERR_ARG);
+    }
+    r->mb = answer[0];
+    r->pb = digits_for(r->mb);
+    *prepared = r.release();
+    return 0;
+}
+size_t zk_i32_rhs_workspace(const void* prepared, uint32_t rows) {
+    const MatmulRhs* w = (const MatmulRhs*)prepared;
+    return w ? (zk_i32_linear_workspace(rows, w->N) + 15) / 16 * 16 + expanded(w) : 0;
+}
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner) {
     const size_t Kp = ((size_t)inner + GBK - 1) / GBK * GBK;
     if (rows <= SPLIT_ROWS) return 0;
@@ -1220,7 +1238,7 @@ int zk_i32_linear(void* out, const void* x, size_t ldx, const void* prepared, ui
     ProductArgs g{};
     g.x = (const int32_t*)x; g.ldx = ldx; g.rows = rows; g.inner = w->N; g.cols = w->P; g.w = planes_of(w);
     g.e.out = (int32_t*)out; g.e.sf = divisor(sf); g.e.pow2 = g.e.sf.shift >= 0;
-    return product<false>("zk_i32_linear", g, flag_dev, workspace, workspace_bytes, (hipStream_t)stv);
+    return product<false>("zk_i32_linear", g, w, nullptr, flag_dev, workspace, workspace_bytes, (hipStream_t)stv);
 }
 int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared, const void* up_prepared, uint32_t rows, uint32_t sf_gate, uint32_t sf_up, const void* table, int32_t low,
                  uint32_t len, uint32_t sf_hidden, void* workspace, size_t workspace_bytes, void* flag_dev, void* stv) {
@@ -1228,6 +1246,7 @@ int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared
     if (const int rc = check_weight(gate, "zk_i32_gated")) return rc;
     if (const int rc = check_weight(w, "zk_i32_gated")) return rc;
     ZK_ARG(w->N == gate->N && w->P == gate->P, "zk_i32_gated: the two projections have different shapes");
+    ZK_ARG((w->q4 == nullptr) == (gate->q4 == nullptr), "zk_i32_gated: one weight of 4 bits and one that is none");
     ZK_ARG(sf_gate > 0 && sf_up > 0 && sf_hidden > 0, "zk_i32_gated: a scaling factor of 0");
     ZK_ARG(table != nullptr && len > 0, "zk_i32_gated: no table of function values");
     if (rows == 0) return 0;
@@ -1236,7 +1255,7 @@ int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared
     g.e.out = (int32_t*)out; g.e.sf = divisor(sf_up); g.e.sf_gate = divisor(sf_gate); g.e.sf_hidden = divisor(sf_hidden);
     g.e.pow2 = g.e.sf.shift >= 0 && g.e.sf_gate.shift >= 0 && g.e.sf_hidden.shift >= 0;
     g.e.table = (const int32_t*)table; g.e.low = low; g.e.len = len;
-    return product<true>("zk_i32_gated", g, flag_dev, workspace, workspace_bytes, (hipStream_t)stv);
+    return product<true>("zk_i32_gated", g, w, gate, flag_dev, workspace, workspace_bytes, (hipStream_t)stv);
 }
 
 }  // extern "C"

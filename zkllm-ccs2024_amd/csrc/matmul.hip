@@ -1017,6 +1017,7 @@ int zk_fr_matmul_rhs_free(void* prepared) {
     MatmulRhs* r = (MatmulRhs*)prepared;
     if (!r) return 0;
     if (r->planes) (void)pool_free(r->planes, nullptr);
+    if (r->q4) (void)pool_free(r->q4, nullptr);
     delete r;
     return 0;
 }

@@ -29,7 +29,9 @@ static inline int digits_for(unsigned long long absmax) {      // planes needed 
 
 // A right operand kept by the caller for many products (a layer's weight): its largest magnitude and, when it is a matrix of
 // small integers, its digit planes in the GEMM's layout -- neither is computed again per product.  B: the field elements it was made from, null where it was made from int32.
-struct MatmulRhs { const void* B = nullptr; uint32_t N = 0, P = 0, Kp = 0; unsigned long long mb = ~0ull; int pb = 0; void* planes = nullptr; };
+struct MatmulRhs { const void* B = nullptr; uint32_t N = 0, P = 0, Kp = 0; unsigned long long mb = ~0ull; int pb = 0; void* planes = nullptr;
+                   // a weight of 4 bits instead (zk_i32_rhs_prepare_q4): no planes, its codes, then the scales and zeros of `groups` groups of `group` rows
+                   void* q4 = nullptr; uint32_t group = 0, groups = 0; };
 
 // The two 16-byte halves of a row of 32 bytes change places every eight rows in LDS, so that the fragments' reads spread over all banks
 __device__ __forceinline__ uint32_t gemm_half(uint32_t row, uint32_t h) { return h ^ ((row >> 3) & 1u); }
