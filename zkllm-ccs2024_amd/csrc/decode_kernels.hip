@@ -23,9 +23,13 @@ struct SoftmaxArgs {
     int bits[DIGITS];                    // log2 of the radices where all are powers of two
     int n, drop_bits;
     uint64_t drop;                       // the product of the radices whose digits are not kept
-    double scale;
+    double scale, scale_inv;
+    // Two tables whose values need no gathers (a layer's): the first's from four terms of its series, the second's from its first `live` entries, the others being 0
+    double step, theta, guard;
+    uint32_t live;
 };
-struct SoftmaxPlan { SoftmaxArgs a; int32_t* memory = nullptr; bool pow2 = true; uint32_t dim = 0; };
+struct SoftmaxPlan { SoftmaxArgs a; int32_t* memory = nullptr; bool pow2 = true, series = false; uint32_t dim = 0; };
+static constexpr uint32_t MOST_LIVE = 8192;
 
 __global__ void __launch_bounds__(256) k_softmax_table_i32(int32_t* __restrict__ table, double log_theta, double step, uint32_t len) {
     const uint32_t x = blockIdx.x * 256 + threadIdx.x;
@@ -131,7 +135,8 @@ template <int VEC> __global__ void __launch_bounds__(256) k_cache_append(const A
 }
 
 // ---- attention ----------------------------------------------------------------------------------------------------------------------------
-// A row is one query head of a token; the rows of a head of keys are token * group + head in its group.  Tiles are 16 rows: of the prefix's, any; of a sequence's own keys, its own.
+// A row is one query head of a token; the rows of a head of keys are token * group + head in its group.  Four steps, each a launch: scores, a row's softmax to weights, sums of weights times
+// values, and where the keys were cut into parts their sums joined.  Tiles are 16 or 64 rows: of the prefix's, any; of a sequence's own keys, its own.
 struct AttnArgs {
     int32_t* out;
     const int32_t* q;
@@ -139,43 +144,45 @@ struct AttnArgs {
     uint32_t group, dim, kv_heads, kv0;  // kv0: the launch's first head of keys
     SoftmaxArgs softmax;
     zk_i32_cache prefix, own;
-    uint32_t prefix_len, prefix_cols;    // prefix_cols: the prefix's length up to a multiple of 16, where a row's own scores begin
+    uint32_t prefix_len, prefix_cols;    // prefix_cols: the prefix's length up to a multiple of 64, where a row's own keys begin
     Sequences seqs;                      // count 0: no own keys
     int causal;
     Divisor sf_first, sf_second;
     int64_t* scores;                     // [head of keys][row][ld]
-    size_t ld;
-    int64_t* shift;                      // [head of keys][row]
+    int8_t* weights;                     // [head of keys][row][six digits][ld]
+    uint32_t* top;                       // [head of keys][row]: the sixth digit is not all zeros
+    size_t ld;                           // a multiple of 64
     int64_t* shift_out;                  // [token][head], or null
     int64_t* parts;                      // [split][head of keys][row][dim][2]
-    uint32_t tokens, heads_here, prefix_tiles, prefix_splits, prefix_step, own_splits, own_step;
+    int direct;                          // the keys are one part: its sums are the outputs
+    uint32_t tokens, heads_here, prefix_tiles, prefix_splits, prefix_step, own_splits, own_step, score_keys;
     uint32_t* flag;
 };
-static constexpr int64_t NO_SHIFT = INT64_MIN;   // of a row that belongs to no sequence
 __device__ __forceinline__ uint32_t own_seen(const AttnArgs& a, const Sequence& s, uint32_t token) {      // how many of its sequence's own keys a token sees
     if (!a.causal) return s.length;
     const int64_t seen = (int64_t)s.length - s.n + (token - s.first) + 1;
     return seen < 0 ? 0u : (uint32_t)seen;
 }
-struct Tile16 {
-    uint32_t row0, lo, hi, keys, col0;   // rows lo .. hi - 1 of the 16 from row0 on are its own; keys: the most that one of them sees, behind column col0
+struct Tile {
+    uint32_t row0, lo, hi, keys, col0;   // rows lo .. hi - 1 of those from row0 on are its own; keys: the most that one of them sees, behind column col0
     bool own;
     Sequence s;
     __device__ bool has(uint32_t c) const { return row0 + c >= lo && row0 + c < hi; }
 };
-__device__ __forceinline__ bool tile_at(const AttnArgs& a, uint32_t id, Tile16& t, uint32_t& bad) {
-    if (id < a.prefix_tiles) {
-        t.row0 = id * 16; t.lo = 0; t.hi = a.tokens * a.group; t.keys = a.prefix_len; t.col0 = 0; t.own = false;
+// tile `id` of ROWS rows, of the prefix or of the sequences' own keys
+template <uint32_t ROWS> __device__ __forceinline__ bool tile_at(const AttnArgs& a, bool own, uint32_t id, Tile& t, uint32_t& bad) {
+    t.own = own;
+    if (!own) {
+        t.row0 = id * ROWS; t.lo = 0; t.hi = a.tokens * a.group; t.keys = a.prefix_len; t.col0 = 0;
         if (a.seqs.starts) {             // tokens before the first sequence and behind the last are nobody's
             const int32_t first = a.seqs.starts[0], end = a.seqs.starts[a.seqs.count];
             t.lo = (uint32_t)max(first, 0) * a.group; t.hi = min((uint32_t)max(end, 0), a.tokens) * a.group;
         }
-        t.lo = max(t.lo, t.row0); t.hi = min(t.hi, t.row0 + 16);
+        t.lo = max(t.lo, t.row0); t.hi = min(t.hi, t.row0 + ROWS);
         return t.lo < t.hi;
     }
-    id -= a.prefix_tiles;
-    // A sequence's tiles begin at floor(first row / 16) + its index: a place for each of them, since floor(x + y) + 1 >= floor(x) + ceil(y)
-    auto base = [&](uint32_t i) { return (uint32_t)((uint64_t)(a.seqs.starts ? (uint32_t)a.seqs.starts[i] : i * (a.tokens / a.seqs.count)) * a.group / 16) + i; };
+    // A sequence's tiles begin at floor(first row / ROWS) + its index: a place for each of them, since floor(x + y) + 1 >= floor(x) + ceil(y)
+    auto base = [&](uint32_t i) { return (uint32_t)((uint64_t)(a.seqs.starts ? (uint32_t)a.seqs.starts[i] : i * (a.tokens / a.seqs.count)) * a.group / ROWS) + i; };
     uint32_t lo = 0, hi = a.seqs.count;
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) / 2;
@@ -183,9 +190,9 @@ __device__ __forceinline__ bool tile_at(const AttnArgs& a, uint32_t id, Tile16& 
         else hi = mid;
     }
     if (!sequence_at(a.seqs, lo, t.s, bad)) return false;
-    const uint32_t b = base(lo), rows = t.s.n * a.group, at = (id - b) * 16;
+    const uint32_t b = base(lo), rows = t.s.n * a.group, at = (id - b) * ROWS;
     if (id < b || at >= rows) return false;
-    t.row0 = t.lo = t.s.first * a.group + at; t.hi = t.lo + min(16u, rows - at); t.col0 = a.prefix_cols; t.own = true;
+    t.row0 = t.lo = t.s.first * a.group + at; t.hi = t.lo + min(ROWS, rows - at); t.col0 = a.prefix_cols;
     t.keys = own_seen(a, t.s, (t.hi - 1) / a.group);
     return true;
 }
@@ -207,33 +214,33 @@ template <bool VEC> __device__ __forceinline__ void head_piece(const int32_t* p,
 }
 __device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v[2] | v[3]) != 0; }
 
-static constexpr uint32_t SCORE_KEYS = 256;      // a workgroup's keys
-// Scores: a wave takes 16 keys at a time, a lane 16 of 64 dimensions of one of them, straight from memory to the fragments of v_mfma_i32_16x16x64_i8
-template <int U, bool VEC> __global__ void __launch_bounds__(256) k_attn_scores(const AttnArgs a) {
+// Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8
+template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_attn_scores(const AttnArgs a, int own) {
     uint32_t bad = 0;
-    Tile16 t;
-    if (!tile_at(a, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
-    const uint32_t key0 = blockIdx.x * SCORE_KEYS;
+    Tile t;
+    if (!tile_at<16 * RT>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t key0 = blockIdx.x * a.score_keys;
     if (key0 >= t.keys) return;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z;
-    v4i b[U][4];
+    v4i b[RT][U][4];
     bool wide = false;
-    {
-        const uint32_t row = t.has(c) ? t.row0 + c : t.lo, token = row / a.group, head = kv * a.group + (row - token * a.group);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const uint32_t row = t.has(16 * r + c) ? t.row0 + 16 * r + c : t.lo, token = row / a.group, head = kv * a.group + (row - token * a.group);
         const int32_t* p = a.q + token * a.q_token + head * a.q_head;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             int32_t x[16];
             head_piece<VEC>(p, u * 64 + q * 4, a.dim, x);
-            digit_planes(x, b[u], bad);
-            wide |= any_bits(b[u][3]);
+            digit_planes(x, b[r][u], bad);
+            wide |= any_bits(b[r][u][3]);
         }
     }
     const bool q_wide = __any(wide);
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     const int32_t* keys = (const int32_t*)cache.k + kv * cache.head_stride;
     int64_t* out = a.scores + ((size_t)blockIdx.z * a.tokens * a.group + t.row0 + c) * a.ld + t.col0 + 4 * q;
-    for (uint32_t i = wave; i < SCORE_KEYS / 16; i += 4) {
+    for (uint32_t i = wave; i < a.score_keys / 16; i += 4) {
         const uint32_t key = key0 + i * 16;
         if (key >= t.keys) break;
         const int32_t* p = keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + c, t.keys - 1), bad);
@@ -246,34 +253,44 @@ template <int U, bool VEC> __global__ void __launch_bounds__(256) k_attn_scores(
             digit_planes(x, k[u], bad);
             k_wide |= any_bits(k[u][3]);
         }
-        v4i acc[7];
+        const bool four = q_wide || __any(k_wide);
 #pragma unroll
-        for (int s = 0; s < 7; ++s) acc[s] = v4i{0, 0, 0, 0};
+        for (int r = 0; r < RT; ++r) {
+            v4i acc[7];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int s = 0; s < 7; ++s) acc[s] = v4i{0, 0, 0, 0};
 #pragma unroll
-            for (int m = 0; m < 3; ++m)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int n = 0; n < 3; ++n) acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[u][n], acc[m + n], 0, 0, 0);
-        if (q_wide || __any(k_wide)) {
+                for (int m = 0; m < 3; ++m)
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+                    for (int n = 0; n < 3; ++n) acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][n], acc[m + n], 0, 0, 0);
+            if (four) {
 #pragma unroll
-                for (int m = 0; m < 3; ++m) {
-                    acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[u][3], acc[m + 3], 0, 0, 0);
-                    acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[u][m], acc[m + 3], 0, 0, 0);
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int m = 0; m < 3; ++m) {
+                        acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][3], acc[m + 3], 0, 0, 0);
+                        acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][m], acc[m + 3], 0, 0, 0);
+                    }
+                    acc[6] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][3], acc[6], 0, 0, 0);
                 }
-                acc[6] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[u][3], acc[6], 0, 0, 0);
             }
-        }
-        if (t.has(c)) {
+            if (!t.has(16 * r + c)) continue;
+            int64_t v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                int32_t s[7];
+            for (int e = 0; e < 4; ++e) {                  // key 4 q + e of the tile, row c
+                if (four) {
+                    int32_t s[7];
 #pragma unroll
-                for (int m = 0; m < 7; ++m) s[m] = acc[m][e];
-                out[key + e] = joined<7>(s, bad);          // key 4 q + e of the tile, row c
+                    for (int m = 0; m < 7; ++m) s[m] = acc[m][e];
+                    v[e] = joined<7>(s, bad);
+                } else v[e] = (int64_t)acc[0][e] + (int64_t)acc[1][e] * 256 + ((int64_t)(acc[2][e] + acc[3][e] * 256) << 16) + ((int64_t)acc[4][e] << 32);
             }
+            typedef long long v2l __attribute__((ext_vector_type(2)));
+            v2l* to = reinterpret_cast<v2l*>(out + 16 * r * a.ld + key);
+            to[0] = v2l{v[0], v[1]};
+            to[1] = v2l{v[2], v[3]};
         }
     }
     raise(a.flag, bad);
@@ -285,6 +302,9 @@ template <int U, bool VEC> __global__ void __launch_bounds__(256) k_attn_scores(
 // times in a row of thousands -- the lanes before the one where it does are added so and that lane's terms one by one.
 struct Steps { uint64_t even, odd; };
 __device__ __forceinline__ Steps then(const Steps& a, const Steps& b) { return Steps{a.even + (a.even & 1 ? b.odd : b.even), a.odd + (a.odd & 1 ? b.even : b.odd)}; }
+static constexpr uint64_t UNITS = 0x0020000000000000ull;                       // t / u stays below
+__device__ __forceinline__ int exponent(double t) { return (int)(zkd::double_to_bits(t) >> 52) - 1023; }
+__device__ __forceinline__ uint64_t units_of(double t) { return (zkd::double_to_bits(t) & 0x000FFFFFFFFFFFFFull) | 0x0010000000000000ull; }
 __device__ __forceinline__ void step(Steps& s, double x, int e) {
     const double w = __builtin_fmin(ldexp(x, 52 - e), 4503599627370496.0);     // 2^52 of them leave 2^(e + 1) already
     const double near = w + 4503599627370496.0;                                // rounds to whole numbers, ties to even ones
@@ -295,8 +315,19 @@ __device__ __forceinline__ void step(Steps& s, double x, int e) {
     s.even += units + (s.even & 1 ? other : 0);
     s.odd += units + (s.odd & 1 ? 0 : other);
 }
+// steps over the lanes up to this one
+__device__ __forceinline__ Steps steps_up_to(Steps s) {
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const Steps before{__shfl_up(s.even, off, 64), __shfl_up(s.odd, off, 64)};
+        const Steps both = then(before, s);
+        if (lane >= (uint32_t)off) s = both;
+    }
+    return s;
+}
 // total with the terms of 64 lanes added, lane by lane, M in a lane
-template <int M> __device__ __forceinline__ double add_in_order(double total, double (&x)[M]) {
+template <int M> __device__ __forceinline__ double add_in_order(double total, const double (&x)[M]) {
     const uint32_t lane = threadIdx.x & 63u;
     uint32_t from = 0;                         // lanes before this one are in the total
     while (true) {
@@ -307,20 +338,15 @@ template <int M> __device__ __forceinline__ double add_in_order(double total, do
         if (left == 0 || !(total < __builtin_inf())) return total;
         uint32_t at = (uint32_t)__builtin_ctzll(left);
         if (total > 0.0) {
-            const int e = (int)(zkd::double_to_bits(total) >> 52) - 1023;
-            const uint64_t t = (zkd::double_to_bits(total) & 0x000FFFFFFFFFFFFFull) | 0x0010000000000000ull;
+            const int e = exponent(total);
+            const uint64_t t = units_of(total);
             Steps s{0, 0};
             if (lane >= from)
 #pragma unroll
                 for (int i = 0; i < M; ++i) step(s, x[i], e);
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {      // sums over the lanes up to this one
-                const Steps before{__shfl_up(s.even, off, 64), __shfl_up(s.odd, off, 64)};
-                const Steps both = then(before, s);
-                if (lane >= (uint32_t)off) s = both;
-            }
+            s = steps_up_to(s);
             const uint64_t after = t + (t & 1 ? s.odd : s.even);
-            const unsigned long long out = __ballot(after >= 0x0020000000000000ull);
+            const unsigned long long out = __ballot(after >= UNITS);
             const uint32_t last = out ? (uint32_t)__builtin_ctzll(out) : 64u;      // the lane where the sum leaves 2^(e + 1)
             if (last > 0) {
                 const uint64_t sum = __shfl(after, last - 1, 64);
@@ -335,84 +361,232 @@ template <int M> __device__ __forceinline__ double add_in_order(double total, do
         if (from == 64) return total;
     }
 }
-__device__ __forceinline__ uint32_t score_col(const AttnArgs& a, uint32_t j) { return j < a.prefix_len ? j : a.prefix_cols + (j - a.prefix_len); }
-// a wave a row
-__global__ void __launch_bounds__(256) k_attn_shift(const AttnArgs a) {
-    constexpr int M = 8;
-    const uint32_t lane = threadIdx.x & 63u, rows = a.tokens * a.group;
-    const size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= (size_t)a.heads_here * rows) return;
-    const uint32_t token = (uint32_t)(r % rows) / a.group;
-    uint32_t bad = 0, keys = a.prefix_len;
-    if (a.seqs.count) {
-        Sequence s;
-        if (!sequence_of(a.seqs, token, s, bad)) {
-            if (lane == 0) a.shift[r] = NO_SHIFT;
-            return;
-        }
-        keys += own_seen(a, s, token);
-    }
-    const int64_t* x = a.scores + r * a.ld;
-    double total = 0.0;
-    for (uint32_t j0 = 0; j0 < keys; j0 += 64 * M) {
-        double term[M];
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-            const uint32_t j = j0 + lane * M + i;
-            term[i] = j < keys ? zkd::exp_det((double)x[score_col(a, j)] / a.softmax.scale) : 0.0;
-        }
-        total = add_in_order<M>(total, term);
-    }
-    const double sv = a.softmax.scale * zkd::log_det(total);
-    if (lane == 0) {
-        const int64_t shift = keys == 0 ? 0 : sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5);
-        a.shift[r] = shift;
-        if (a.shift_out) a.shift_out[((size_t)token * a.kv_heads + a.kv0 + r / rows) * a.group + (r % rows - token * a.group)] = shift;
-    }
+// (double)x / scale, correctly rounded: two corrections of x / scale's estimate by the scale's correctly rounded inverse, the first of which leaves less than a unit in the last place,
+// from where the second rounds correctly
+__device__ __forceinline__ double divided(int64_t x, const SoftmaxArgs& s) {
+    const double v = (double)x;
+    double q = v * s.scale_inv;
+    q = __builtin_fma(__builtin_fma(-q, s.scale, v), s.scale_inv, q);
+    return __builtin_fma(__builtin_fma(-q, s.scale, v), s.scale_inv, q);
 }
-
-// the digits of 16 weights, six planes of them
-__device__ __forceinline__ void weight_planes(const int64_t (&y)[16], v4i (&out)[6]) {
+// weights as digits: of eight keys, a plane's eight bytes at a time
+struct Digits8 { uint2 p[6]; };
+__device__ __forceinline__ void digits8(const uint64_t (&d)[8], Digits8& out) {      // d: digits in bytes 0 .. 5
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < 2; ++w) {
         uint32_t lo[4], hi[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint64_t d = ((uint64_t)y[4 * w + e] + 0x808080808080ull) ^ 0x808080808080ull;
-            lo[e] = (uint32_t)d;
-            hi[e] = (uint32_t)(d >> 32);
-        }
+        for (int e = 0; e < 4; ++e) { lo[e] = (uint32_t)d[4 * w + e]; hi[e] = (uint32_t)(d[4 * w + e] >> 32); }
         const uint32_t a = __builtin_amdgcn_perm(lo[1], lo[0], 0x05010400u), b = __builtin_amdgcn_perm(lo[1], lo[0], 0x07030602u);
-        const uint32_t c = __builtin_amdgcn_perm(lo[3], lo[2], 0x05010400u), d = __builtin_amdgcn_perm(lo[3], lo[2], 0x07030602u);
-        const uint32_t f = __builtin_amdgcn_perm(hi[1], hi[0], 0x05010400u), g = __builtin_amdgcn_perm(hi[3], hi[2], 0x05010400u);
-        out[0][w] = (int)__builtin_amdgcn_perm(c, a, 0x05040100u);
-        out[1][w] = (int)__builtin_amdgcn_perm(c, a, 0x07060302u);
-        out[2][w] = (int)__builtin_amdgcn_perm(d, b, 0x05040100u);
-        out[3][w] = (int)__builtin_amdgcn_perm(d, b, 0x07060302u);
-        out[4][w] = (int)__builtin_amdgcn_perm(g, f, 0x05040100u);
-        out[5][w] = (int)__builtin_amdgcn_perm(g, f, 0x07060302u);
+        const uint32_t c = __builtin_amdgcn_perm(lo[3], lo[2], 0x05010400u), f = __builtin_amdgcn_perm(lo[3], lo[2], 0x07030602u);
+        const uint32_t g = __builtin_amdgcn_perm(hi[1], hi[0], 0x05010400u), h = __builtin_amdgcn_perm(hi[3], hi[2], 0x05010400u);
+        const uint32_t v[6] = {__builtin_amdgcn_perm(c, a, 0x05040100u), __builtin_amdgcn_perm(c, a, 0x07060302u), __builtin_amdgcn_perm(f, b, 0x05040100u),
+                               __builtin_amdgcn_perm(f, b, 0x07060302u), __builtin_amdgcn_perm(h, g, 0x05040100u), __builtin_amdgcn_perm(h, g, 0x07060302u)};
+#pragma unroll
+        for (int j = 0; j < 6; ++j) (w ? out.p[j].y : out.p[j].x) = v[j];
     }
 }
-// Sums of weights times values: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each.  A
-// part's sum leaves as its low 64 bits and, in units of 2^32, its size: the parts' sums together say whether the whole fits.
-template <bool VEC, bool POW2> __global__ void __launch_bounds__(256) k_attn_values(const AttnArgs a) {
-    extern __shared__ unsigned long long sums[];           // [16][64 blocks of dimensions][2]
+enum class Weights { ANY, POW2, SERIES };
+// A workgroup a row, eight neighbouring keys a lane.  The sum of exponentials is taken in no order first: off from the sum in order by at most (keys + 64) 2^-53 of it, which decides the shift unless it
+// lies that near to a border between two whole numbers (one row in 45 at 2048 keys and a scale of 2^32 sqrt(128)); then the sum in order is taken too, the waves' runs at once where
+// the sum stays within a power of two, and the few others one after the other.
+template <int T, Weights KIND> __global__ void __launch_bounds__(T) k_attn_softmax(const AttnArgs a) {
+    constexpr int M = 8, WAVES = T / 64;
+    extern __shared__ int32_t live[];
+    __shared__ double sums[WAVES];
+    __shared__ Steps steps[WAVES];
+    __shared__ int at_exponent[WAVES];
+    __shared__ double in_order;
+    __shared__ uint32_t any_top;
+    const uint32_t rows = a.tokens * a.group, r = blockIdx.x, in = r % rows, token = in / a.group, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const SoftmaxArgs& s = a.softmax;
+    uint32_t bad = 0, own = 0;
+    Sequence q;
+    if (a.seqs.count) {
+        if (!sequence_of(a.seqs, token, q, bad)) {         // nobody's row: no weights, in case that its tile is somebody's
+            int8_t* w = a.weights + (size_t)r * 6 * a.ld;
+            for (size_t i = threadIdx.x; i < 6 * a.ld / 16; i += T) reinterpret_cast<v4i*>(w)[i] = v4i{0, 0, 0, 0};
+            if (threadIdx.x == 0) a.top[r] = 0;
+            return;
+        }
+        own = own_seen(a, q, token);
+    }
+    if constexpr (KIND == Weights::SERIES)
+        for (uint32_t i = threadIdx.x; i < s.live; i += T) live[i] = s.table[1][i];
+    if (threadIdx.x == 0) any_top = 0;
+    // columns with keys: the prefix's, then the row's own; weights are 0 up to where another row of the tile may see
+    const uint32_t own_end = a.prefix_cols + own, cols = own ? own_end : a.prefix_len, fill = min((uint32_t)a.ld, a.seqs.count ? a.prefix_cols + (own + 127) / 64 * 64 : a.prefix_cols);
+    auto is_key = [&](uint32_t j) { return j < a.prefix_len || (j >= a.prefix_cols && j < own_end); };
+    const int64_t* x = a.scores + (size_t)r * a.ld;
+    const uint32_t chunks = (cols + T * M - 1) / (T * M);
+    int64_t v[M];
+    double term[M];
+    auto load = [&](uint32_t chunk) {
+        const uint32_t j = chunk * T * M + threadIdx.x * M;
+#pragma unroll
+        for (int i = 0; i < M; ++i) v[i] = 0;
+        if (j < cols) {
+            typedef long long v2l __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int i = 0; i < M; i += 2) {
+                const v2l p = *reinterpret_cast<const v2l*>(x + j + i);
+                v[i] = p[0]; v[i + 1] = p[1];
+            }
+        }
+    };
+    auto terms = [&](uint32_t chunk) {
+        const uint32_t j = chunk * T * M + threadIdx.x * M;
+#pragma unroll
+        for (int i = 0; i < M; ++i) term[i] = is_key(j + i) ? zkd::exp_det(divided(v[i], s)) : 0.0;
+    };
+    double total = 0.0;
+    for (uint32_t c = 0; c < chunks; ++c) {
+        load(c);
+        terms(c);
+#pragma unroll
+        for (int i = 0; i < M; ++i) total += term[i];
+    }
+    auto wave_sum = [](double t) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
+        return t;
+    };
+    total = wave_sum(total);
+    if (lane == 0) sums[wave] = total;
+    __syncthreads();
+    total = 0.0;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) total += sums[i];
+    auto shift_of = [&](double t) {
+        const double sv = s.scale * zkd::log_det(t);
+        return sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5);
+    };
+    int64_t shift = 0;
+    if (cols) {
+        const double ln = zkd::log_det(total), sv = s.scale * ln;
+        const double off = s.scale * ((double)(cols + 64) * 1.2e-16 + 3e-15 * (fabs(ln) + 1.0)), from_border = fabs(sv - floor(sv) - 0.5);
+        bool sure = total > 0.0 && total < __builtin_inf() && off < 0.25 && from_border > off;
+        if (sure) shift = shift_of(total);
+        else {
+            double t = 0.0;
+            for (uint32_t c = 0; c < chunks; ++c) {
+                if (chunks > 1) { load(c); terms(c); }
+                double mine = 0.0;
+#pragma unroll
+                for (int i = 0; i < M; ++i) mine += term[i];
+                mine = wave_sum(mine);
+                __syncthreads();                           // the arrays' last use is over
+                if (lane == 0) sums[wave] = mine;
+                __syncthreads();
+                double before = t;
+                for (uint32_t i = 0; i < wave; ++i) before += sums[i];
+                const double behind = before + mine;
+                // a run that stays within a power of two, by a margin that the sums' order cannot reach
+                const int e = before > 0.0 && behind < __builtin_inf() ? exponent(behind * (1.0 + 1e-9)) : 2000;
+                const bool clean = e != 2000 && exponent(before * (1.0 - 1e-9)) == e;
+                if (clean) {
+                    Steps st{0, 0};
+#pragma unroll
+                    for (int i = 0; i < M; ++i) step(st, term[i], e);
+                    st = steps_up_to(st);
+                    if (lane == 63) steps[wave] = st;
+                }
+                if (lane == 0) at_exponent[wave] = clean ? e : 2000;
+                __syncthreads();
+                for (uint32_t i = 0; i < (uint32_t)WAVES; ++i) {
+                    if (at_exponent[i] != 2000 && t > 0.0 && exponent(t) == at_exponent[i]) {
+                        const uint64_t u = units_of(t), after = u + (u & 1 ? steps[i].odd : steps[i].even);
+                        if (after < UNITS) { t = ldexp((double)after, at_exponent[i] - 52); continue; }
+                    }
+                    if (wave == i) {
+                        t = add_in_order<M>(t, term);
+                        if (lane == 0) in_order = t;
+                    }
+                    __syncthreads();
+                    t = in_order;
+                    __syncthreads();
+                }
+            }
+            shift = shift_of(t);
+        }
+    }
+    if (threadIdx.x == 0 && a.shift_out) a.shift_out[((size_t)token * a.kv_heads + a.kv0 + r / rows) * a.group + (in - token * a.group)] = shift;
+    if constexpr (KIND == Weights::SERIES) __syncthreads();
+    bool top = false;
+    for (uint32_t c = 0; c * T * M < fill; ++c) {
+        const uint32_t j = c * T * M + threadIdx.x * M;
+        if (j >= fill) break;
+        if (chunks != 1 || c != 0) load(c);
+        uint64_t d[M];
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            if constexpr (KIND == Weights::SERIES) {
+                // both tables' values and their product are exact in double precision, and so is the number whose low 48 bits are the digits, 128 more each
+                constexpr double BASE = 4503599627370496.0 + 141289400074368.0;
+                double w = BASE;
+                if (is_key(j + i)) {
+                    const int64_t below = shift - v[i];
+                    const uint64_t t = (uint64_t)below >> s.drop_bits, upper = t >> s.bits[0];
+                    bad |= below < 0 || upper >= s.radix[1] ? (uint32_t)ZK_VALUES_TABLE : 0u;
+                    const uint32_t digit = (uint32_t)t & (s.radix[0] - 1);
+                    const double z = s.step * (double)digit;
+                    const double u = __builtin_fma(s.theta, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, 1.0 / 24.0, -1.0 / 6.0), 0.5), -1.0), 1.0), 0.5);
+                    double first = floor(u);
+                    if (fabs(u - first - 0.5) > 0.5 - s.guard) first = (double)s.table[0][digit];      // nearer to a border than the terms left out
+                    w = __builtin_fma(first, below >= 0 && upper < s.live ? (double)live[upper] : 0.0, BASE);
+                }
+                d[i] = zkd::double_to_bits(w) ^ 0x808080808080ull;
+            } else {
+                const int64_t y = is_key(j + i) ? softmax_weight<KIND == Weights::POW2>(shift - v[i], s, bad) : 0;
+                d[i] = ((uint64_t)y + 0x808080808080ull) ^ 0x808080808080ull;
+            }
+            top |= (d[i] >> 40 & 0xFF) != 0;
+        }
+        Digits8 p;
+        digits8(d, p);
+#pragma unroll
+        for (int k = 0; k < 6; ++k) *reinterpret_cast<uint2*>(a.weights + ((size_t)r * 6 + k) * a.ld + j) = p.p[k];
+    }
+    if (__any(top) && lane == 0) any_top = 1;
+    __syncthreads();
+    if (threadIdx.x == 0) a.top[r] = any_top;
+    raise(a.flag, bad);
+}
+
+// What becomes of sums of weights times values: an output element, or a part's sum as its low 64 bits and, in units of 2^32, its size: the parts' sizes together say whether the whole fits
+__device__ __forceinline__ void attn_finish(const AttnArgs& a, unsigned long long lo, int64_t size, uint32_t token, uint32_t head, uint32_t d, uint32_t& bad) {
+    const int64_t v = (int64_t)lo;
+    if (size > (3ll << 29) || size < -(3ll << 29) || v >= (1ll << 62) || v < -(1ll << 62)) { bad |= ZK_VALUES_RANGE; return; }
+    auto q = [](int64_t x, const Divisor& s) { return s.shift >= 0 ? quotient<true>(x, s) : quotient<false>(x, s); };
+    a.out[token * a.out_token + head * a.out_head + d] = narrow(q(q(v, a.sf_first), a.sf_second), bad);
+}
+template <int NS> __device__ __forceinline__ void attn_sum(const int32_t (&s)[NS], unsigned long long& lo, int64_t& size) {
+    int64_t l = 0, h = 0;
+#pragma unroll
+    for (int i = 3; i >= 0; --i) l = l * 256 + s[i];
+#pragma unroll
+    for (int i = NS - 1; i >= 4; --i) h = h * 256 + s[i];
+    lo = (unsigned long long)l + ((unsigned long long)h << 32);
+    size = h + (l >> 32);
+}
+// Few rows: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each
+template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const AttnArgs a, int own) {
+    extern __shared__ unsigned long long sums64[];         // [16][64 blocks of dimensions][2]
     uint32_t bad = 0;
-    Tile16 t;
-    if (!tile_at(a, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    Tile t;
+    if (!tile_at<16>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
     const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.x * step;
-    if (first >= t.keys) return;
+    if (first >= t.keys && !(a.direct && first == 0)) return;
     const uint32_t end = min(first + step, t.keys), blocks = (a.dim + 63) / 64, streams = 4 / blocks;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z, block = wave % blocks, stream = wave / blocks;
     const size_t row = (size_t)blockIdx.z * a.tokens * a.group + t.row0;
-    for (uint32_t i = threadIdx.x; i < 16 * blocks * 64 * 2; i += 256) sums[i] = 0;
+    for (uint32_t i = threadIdx.x; i < 16 * blocks * 64 * 2; i += 256) sums64[i] = 0;
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     const uint32_t d0 = block * 64 + 4 * c;
     const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride + d0;
     const uint32_t my_row = t.has(c) ? c : t.lo - t.row0;
-    const int64_t shift = a.shift[row + my_row];
-    const uint32_t seen = !t.has(c) || shift == NO_SHIFT ? 0u : t.own ? own_seen(a, t.s, (t.row0 + my_row) / a.group) : t.keys;
-    const int64_t* scores = a.scores + (row + my_row) * a.ld + t.col0;
+    const bool top = __any(t.has(c) && a.top[row + my_row] != 0);
+    const int8_t* weights = a.weights + (row + my_row) * 6 * a.ld + t.col0 + q * 16;
     v4i acc[9][4];
 #pragma unroll
     for (int s = 0; s < 9; ++s)
@@ -421,6 +595,9 @@ template <bool VEC, bool POW2> __global__ void __launch_bounds__(256) k_attn_val
     if (stream < streams)
         for (uint32_t k = first + stream * 64; k < end; k += 64 * streams) {
             const size_t mine = cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad);
+            v4i w[6];
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = *reinterpret_cast<const v4i*>(weights + i * a.ld + k);
             int32_t x[4][16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -435,22 +612,21 @@ template <bool VEC, bool POW2> __global__ void __launch_bounds__(256) k_attn_val
                     for (int n = 0; n < 4; ++n) x[n][i] = d0 + n < a.dim ? p[n] : 0;
                 }
             }
-            int64_t y[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t key = k + q * 16 + i;
-                y[i] = key < min(seen, end) ? softmax_weight<POW2>(shift - scores[key], a.softmax, bad) : 0;
-            }
-            v4i w[6];
-            weight_planes(y, w);
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 v4i v[4];
                 digit_planes(x[n], v, bad);
+                const bool four = __any(any_bits(v[3]));
 #pragma unroll
-                for (int i = 0; i < 6; ++i)
+                for (int i = 0; i < 5; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[j], acc[i + j][n], 0, 0, 0);
+                    for (int j = 0; j < 3; ++j) acc[i + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[j], acc[i + j][n], 0, 0, 0);
+                if (top)
+#pragma unroll
+                    for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[5], v[j], acc[5 + j][n], 0, 0, 0);
+                if (four)
+#pragma unroll
+                    for (int i = 0; i < 6; ++i) acc[i + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[3], acc[i + 3][n], 0, 0, 0);
             }
         }
     __syncthreads();
@@ -459,25 +635,159 @@ template <bool VEC, bool POW2> __global__ void __launch_bounds__(256) k_attn_val
         for (int n = 0; n < 4; ++n)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {      // row 4 q + e, dimension d0 + n
-                int64_t lo = 0, hi = 0;
+                int32_t s[9];
 #pragma unroll
-                for (int s = 3; s >= 0; --s) lo = lo * 256 + acc[s][n][e];
-#pragma unroll
-                for (int s = 8; s >= 4; --s) hi = hi * 256 + acc[s][n][e];
+                for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
+                unsigned long long lo;
+                int64_t size;
+                attn_sum<9>(s, lo, size);
                 const uint32_t at = ((4 * q + e) * blocks * 64 + d0 + n) * 2;
-                atomicAdd(&sums[at], (unsigned long long)lo + ((unsigned long long)hi << 32));
-                atomicAdd(&sums[at + 1], (unsigned long long)(hi + (lo >> 32)));
+                atomicAdd(&sums64[at], lo);
+                atomicAdd(&sums64[at + 1], (unsigned long long)size);
             }
     __syncthreads();
-    const size_t all = (size_t)a.heads_here * a.tokens * a.group;
-    unsigned long long* out = (unsigned long long*)a.parts + (((t.own ? a.prefix_splits : 0) + blockIdx.x) * all + row) * a.dim * 2;
-    for (uint32_t i = (t.lo - t.row0) * a.dim * 2 + threadIdx.x; i < (t.hi - t.row0) * a.dim * 2; i += 256) {
-        const uint32_t r = i / (2 * a.dim);
-        out[i] = sums[r * blocks * 128 + (i - r * 2 * a.dim)];
+    if (!a.direct) {
+        const size_t all = (size_t)a.heads_here * a.tokens * a.group;
+        unsigned long long* out = (unsigned long long*)a.parts + (((t.own ? a.prefix_splits : 0) + blockIdx.x) * all + row) * a.dim * 2;
+        for (uint32_t i = (t.lo - t.row0) * a.dim * 2 + threadIdx.x; i < (t.hi - t.row0) * a.dim * 2; i += 256) {
+            const uint32_t r = i / (2 * a.dim);
+            out[i] = sums64[r * blocks * 128 + (i - r * 2 * a.dim)];
+        }
+    } else
+        for (uint32_t i = (t.lo - t.row0) * a.dim + threadIdx.x; i < (t.hi - t.row0) * a.dim; i += 256) {
+            const uint32_t r = i / a.dim, d = i - r * a.dim, token = (t.row0 + r) / a.group, at = (r * blocks * 64 + d) * 2;
+            attn_finish(a, sums64[at], (int64_t)sums64[at + 1], token, kv * a.group + (t.row0 + r - token * a.group), d, bad);
+        }
+    raise(a.flag, bad);
+}
+// Many rows: 64 rows by 128 dimensions, a wave 16 by 64.  The workgroup splits 64 keys' values into digits together, the next ones while this step's are multiplied: a lane four keys of four
+// dimensions, in LDS as fragments.
+template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile(const AttnArgs a, int own) {
+    __shared__ __attribute__((aligned(16))) int8_t planes[2][4][8][64][16];
+    __shared__ uint32_t wide[3];                           // of the step, the next and the one after that
+    uint32_t bad = 0;
+    Tile t;
+    const uint32_t dim_blocks = (a.dim + 127) / 128, z = blockIdx.z / dim_blocks, dim0 = (blockIdx.z - z * dim_blocks) * 128;
+    if (!tile_at<64>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.x * step;
+    if (first >= t.keys && !(a.direct && first == 0)) return;
+    const uint32_t end = min(first + step, t.keys), steps = (end - first + 63) / 64;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + z, row_in = (wave >> 1) * 16, block = wave & 1u;
+    const size_t row = (size_t)z * a.tokens * a.group + t.row0;
+    const zk_i32_cache& cache = t.own ? a.own : a.prefix;
+    // a lane's share of the values: dimensions 4 dq .. 4 dq + 3 of keys 4 kq .. 4 kq + 3
+    const uint32_t dq = threadIdx.x & 31u, kq = threadIdx.x >> 5, d0 = dim0 + 4 * dq;
+    const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride + d0;
+    const uint32_t mine = t.has(row_in + c) ? row_in + c : t.lo - t.row0;
+    const bool top = __any(a.top[row + mine] != 0);
+    const int8_t* weights = a.weights + (row + mine) * 6 * a.ld + t.col0 + q * 16 + first;
+    int32_t x[4][4];
+    v4i w[6];
+    auto fetch = [&](uint32_t i) {
+        const size_t at = cache_at(cache, t.own ? t.s.index : 0u, min(first + i * 64 + wave * 8 + (lane & 7u), t.keys - 1), bad);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int32_t* p = values + __shfl((unsigned long long)at, (int)((kq & 1u) * 4 + e), 64);
+            if constexpr (VEC) {
+                v4i v = {0, 0, 0, 0};
+                if (d0 < a.dim) v = *reinterpret_cast<const v4i*>(p);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[e][n] = v[n];
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) x[e][n] = d0 + n < a.dim ? p[n] : 0;
+            }
+        }
+    };
+    auto fetch_weights = [&](uint32_t i) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = *reinterpret_cast<const v4i*>(weights + k * a.ld + i * 64);
+    };
+    auto split = [&](uint32_t i) {
+        uint32_t over = 0, upper = 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            uint32_t d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                over |= x[e][n] > 0x7F7F7F7F ? 1u : 0u;
+                d[e] = digit_bytes((uint32_t)x[e][n]);
+                upper |= d[e];
+            }
+            const uint32_t f = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), g = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
+            const uint32_t h = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), j = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+            const uint32_t p[4] = {__builtin_amdgcn_perm(h, f, 0x05040100u), __builtin_amdgcn_perm(h, f, 0x07060302u), __builtin_amdgcn_perm(j, g, 0x05040100u), __builtin_amdgcn_perm(j, g, 0x07060302u)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) *reinterpret_cast<uint32_t*>(&planes[i & 1u][k][(dq >> 4) * 4 + n][(kq >> 2) * 16 + (dq & 15u)][(kq & 3u) * 4]) = p[k];
+        }
+        bad |= over ? (uint32_t)ZK_VALUES_RANGE : 0u;
+        if (upper >> 24) wide[i % 3] = 1;
+    };
+    v4i acc[9][4];
+#pragma unroll
+    for (int s = 0; s < 9; ++s)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[s][n] = v4i{0, 0, 0, 0};
+    if (threadIdx.x < 3) wide[threadIdx.x] = 0;
+    __syncthreads();
+    if (steps) {
+        fetch(0);
+        fetch_weights(0);
+        split(0);
+    }
+    __syncthreads();
+    for (uint32_t i = 0; i < steps; ++i) {
+        if (i + 1 < steps) fetch(i + 1);
+        if (threadIdx.x == 0) wide[(i + 2) % 3] = 0;       // read last in the step before, written next in the step behind
+        const bool four = wide[i % 3] != 0;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            v4i v[3];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) v[j] = *reinterpret_cast<const v4i*>(&planes[i & 1u][j][block * 4 + n][lane][0]);
+#pragma unroll
+            for (int k = 0; k < 5; ++k)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) acc[k + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[k], v[j], acc[k + j][n], 0, 0, 0);
+            if (top)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[5], v[j], acc[5 + j][n], 0, 0, 0);
+            if (four) {
+                const v4i u = *reinterpret_cast<const v4i*>(&planes[i & 1u][3][block * 4 + n][lane][0]);
+#pragma unroll
+                for (int k = 0; k < 6; ++k) acc[k + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[k], u, acc[k + 3][n], 0, 0, 0);
+            }
+        }
+        if (i + 1 < steps) {
+            fetch_weights(i + 1);
+            split(i + 1);
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t at = row_in + 4 * q + e, in = t.row0 + at, token = in / a.group;
+        if (!t.has(at)) continue;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t d = dim0 + block * 64 + 4 * c + n;
+            if (d >= a.dim) continue;
+            int32_t s[9];
+#pragma unroll
+            for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
+            unsigned long long lo;
+            int64_t size;
+            attn_sum<9>(s, lo, size);
+            if (!a.direct) {
+                unsigned long long* out = (unsigned long long*)a.parts + ((((t.own ? a.prefix_splits : 0) + blockIdx.x) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d) * 2;
+                out[0] = lo;
+                out[1] = (unsigned long long)size;
+            } else attn_finish(a, lo, size, token, kv * a.group + (in - token * a.group), d, bad);
+        }
     }
     raise(a.flag, bad);
 }
-// The parts' sums added up, and what becomes of them
+// The parts' sums added up; rows that see no key
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)a.tokens * a.group, all = a.heads_here * rows;
     if (id >= all * a.dim) return;
@@ -499,12 +809,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
         };
         for (uint32_t i = 0; i < a.prefix_splits; ++i) add(i);
         for (uint32_t i = 0; i < own; ++i) add(a.prefix_splits + i);
-        const int64_t v = (int64_t)lo;
-        if (size > (3ll << 29) || size < -(3ll << 29) || v >= (1ll << 62) || v < -(1ll << 62)) bad |= ZK_VALUES_RANGE;
-        else {
-            auto q = [](int64_t x, const Divisor& s) { return s.shift >= 0 ? quotient<true>(x, s) : quotient<false>(x, s); };
-            a.out[token * a.out_token + ((a.kv0 + kv) * a.group + (in - token * a.group)) * a.out_head + d] = narrow(q(q(v, a.sf_first), a.sf_second), bad);
-        }
+        attn_finish(a, lo, size, token, (a.kv0 + kv) * a.group + (in - token * a.group), d, bad);
     }
     raise(a.flag, bad);
 }
@@ -629,29 +934,35 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
 static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
 
 // How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
-struct AttnPlan { uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t cols, scores, shift, parts; };
+struct AttnPlan { bool prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, parts; };
 static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     AttnPlan p{};
     const uint32_t group = heads / kv_heads;
     const size_t rows = (size_t)tokens * group;
-    p.prefix_tiles = prefix_len ? cdiv(rows, 16) : 0;
-    p.own_tiles = sequences ? (uint32_t)(rows / 16) + sequences : 0;
-    p.cols = ((size_t)prefix_len + 15) / 16 * 16 + ((size_t)max_length + 15) / 16 * 16;
-    auto cut = [&](uint32_t keys, size_t tiles, uint32_t& splits, uint32_t& step) {
-        const size_t want = std::max<size_t>(1, 1024 / std::max<size_t>(1, tiles * kv_heads));
+    p.prefix64 = rows > 16;
+    p.own64 = sequences && rows / sequences > 32;
+    p.prefix_tiles = prefix_len ? cdiv(rows, p.prefix64 ? 64 : 16) : 0;
+    p.own_tiles = sequences ? (uint32_t)(rows / (p.own64 ? 64 : 16)) + sequences : 0;
+    p.prefix_cols = ((size_t)prefix_len + 63) / 64 * 64;
+    p.cols = p.prefix_cols + ((size_t)max_length + 63) / 64 * 64;
+    auto cut = [&](uint32_t keys, size_t tiles, bool many, uint32_t& splits, uint32_t& step) {
+        const size_t want = std::max<size_t>(1, (many ? 512 : 1024) / std::max<size_t>(1, tiles * kv_heads));
         splits = (uint32_t)std::min<size_t>(want, cdiv(keys, 256));
         splits = std::max(splits, cdiv(keys, 8192));
         step = splits ? (uint32_t)((cdiv(keys, splits) + 63) / 64 * 64) : 64;
         splits = cdiv(keys, step);
     };
-    cut(prefix_len, p.prefix_tiles, p.prefix_splits, p.prefix_step);
-    cut(sequences ? max_length : 0, p.own_tiles, p.own_splits, p.own_step);
-    const size_t each = rows * (p.cols * 8 + 8 + (size_t)(p.prefix_splits + p.own_splits) * dim * 16);
+    cut(prefix_len, p.prefix_tiles, p.prefix64, p.prefix_splits, p.prefix_step);
+    cut(sequences ? max_length : 0, p.own_tiles, p.own64, p.own_splits, p.own_step);
+    const uint32_t splits = p.prefix_splits + p.own_splits;
+    p.direct = splits == 1;
+    const size_t each = rows * (p.cols * 14 + 4 + (size_t)(p.direct ? 0 : splits) * dim * 16);
     p.heads = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / std::max<size_t>(each, 1)));
     auto round = [](size_t b) { return (b + 15) / 16 * 16; };
-    p.scores = round(p.heads * rows * p.cols * 8);
-    p.shift = round(p.heads * rows * 8);
-    p.parts = p.heads * rows * (size_t)(p.prefix_splits + p.own_splits) * dim * 16;
+    p.scores = p.heads * rows * p.cols * 8;
+    p.weights = p.heads * rows * p.cols * 6;
+    p.top = round(p.heads * rows * 4);
+    p.parts = p.heads * rows * (size_t)(p.direct ? 0 : splits) * dim * 16;
     return p;
 }
 
@@ -698,6 +1009,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
     SoftmaxArgs& a = s->a;
     a = SoftmaxArgs{};
     a.scale = scaling_factor_in * std::sqrt((double)dim);
+    a.scale_inv = 1.0 / a.scale;
     a.drop = 1;
     a.n = K - L;
     unsigned __int128 reach = 1;
@@ -733,6 +1045,14 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
         }
         weight *= bs[i];
     }
+    if (s->pow2 && M == 0 && a.n == 2) {
+        const double w0 = (double)a.drop, w1 = w0 * bs[L], z = w0 / a.scale * bs[L], reach = std::log(thetas[1]) + 0.75;      // beyond exp(-reach) theta is below 0.5
+        a.step = w0 / a.scale; a.theta = thetas[0];
+        a.guard = thetas[0] * (z * z * z * z * z / 60.0 + 0x1p-46);
+        const double live = reach / (w1 / a.scale) + 2.0;
+        a.live = (uint32_t)std::min<double>(live, bs[L + 1]);
+        s->series = z <= 0x1p-7 && a.guard < 0.01 && a.live <= MOST_LIVE;
+    }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) e = hipStreamSynchronize(st);      // calls on any stream may use the tables
     if (e != hipSuccess) { (void)pool_free(s->memory, st); return hip_fail(e, "k_softmax_table_i32", __FILE__, __LINE__); }
@@ -743,7 +1063,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
 size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     if (tokens == 0 || kv_heads == 0 || heads < kv_heads) return 0;
     const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
-    return p.scores + p.shift + p.parts;
+    return p.scores + p.weights + p.top + p.parts;
 }
 int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                      const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts, const void* lengths, uint32_t max_length,
@@ -772,9 +1092,9 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     if (own) if (const int rc = check_cache(own, name, sequences, max_length, kv_heads, dim)) return rc;
     if (!own) sequences = 0;
     const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
-    ZK_ARG(p.prefix_tiles + p.own_tiles <= 65535u, std::string(name) + ": more than 65535 tiles of queries");
+    ZK_ARG(p.prefix_tiles <= 65535u && p.own_tiles <= 65535u && (uint64_t)p.heads * cdiv(dim, 128) <= 65535u, std::string(name) + ": more than 65535 tiles of queries");
     hipStream_t st = (hipStream_t)stv;
-    const size_t bytes = p.scores + p.shift + p.parts;
+    const size_t bytes = p.scores + p.weights + p.top + p.parts;
     ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_attention_workspace says");
     ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
     ZK_ARG(dim == s->dim, std::string(name) + ": the softmax was prepared for heads of another width");
@@ -792,34 +1112,61 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     a.group = heads / kv_heads; a.dim = dim; a.kv_heads = kv_heads; a.shift_out = (int64_t*)shift; a.softmax = s->a;
     if (prefix_len) a.prefix = *prefix;
     if (own) a.own = *own;
-    a.prefix_len = prefix_len; a.prefix_cols = (prefix_len + 15) / 16 * 16;
+    a.prefix_len = prefix_len; a.prefix_cols = (uint32_t)p.prefix_cols;
     a.seqs = Sequences{own ? (const int32_t*)starts : nullptr, (const int32_t*)lengths, sequences, tokens, max_length};
     a.causal = causal; a.sf_first = divisor(sf_first); a.sf_second = divisor(sf_second);
-    a.scores = (int64_t*)workspace; a.ld = p.cols; a.shift = (int64_t*)((char*)workspace + p.scores); a.parts = (int64_t*)((char*)workspace + p.scores + p.shift);
+    a.scores = (int64_t*)workspace; a.ld = p.cols; a.weights = (int8_t*)workspace + p.scores; a.top = (uint32_t*)(a.weights + p.weights);
+    a.parts = (int64_t*)((char*)a.top + p.top); a.direct = p.direct;
     a.tokens = tokens; a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits; a.prefix_step = p.prefix_step; a.own_splits = p.own_splits; a.own_step = p.own_step;
     a.flag = flag.dev;
     const bool vec = dim % 4 == 0 && ((q_token | q_head) & 3) == 0 && ((uintptr_t)q & 15) == 0 && (!prefix_len || cache_aligned(prefix)) && (!own || cache_aligned(own));
-    const unsigned tiles = p.prefix_tiles + p.own_tiles, chunks = std::max(1u, std::max(cdiv(prefix_len, SCORE_KEYS), cdiv(max_length, SCORE_KEYS)));
-    const unsigned splits = std::max(1u, std::max(p.prefix_splits, p.own_splits)), blocks = cdiv(dim, 64);
+    const unsigned blocks = cdiv(dim, 64);
     for (a.kv0 = 0; a.kv0 < kv_heads; a.kv0 += p.heads) {
         a.heads_here = std::min(p.heads, kv_heads - a.kv0);
         const size_t rows = (size_t)a.heads_here * tokens * a.group;
-        const dim3 grid(chunks, tiles, a.heads_here), vgrid(splits, tiles, a.heads_here);
-        auto scores = [&](auto u) {
-            constexpr int U = decltype(u)::value;
-            if (vec) hipLaunchKernelGGL((k_attn_scores<U, true>), grid, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((k_attn_scores<U, false>), grid, dim3(256), 0, st, a);
+        // the prefix's keys, then the sequences' own
+        auto both = [&](auto f) {
+            if (p.prefix_tiles) f(0, p.prefix64, p.prefix_tiles, prefix_len, p.prefix_splits);
+            if (p.own_tiles && max_length) f(1, p.own64, p.own_tiles, max_length, p.own_splits);
         };
-        if (blocks == 1) scores(std::integral_constant<int, 1>());
-        else if (blocks == 2) scores(std::integral_constant<int, 2>());
-        else scores(std::integral_constant<int, 4>());
-        hipLaunchKernelGGL(k_attn_shift, dim3(cdiv(rows, 4)), dim3(256), 0, st, a);
-        const size_t lds = 16 * (size_t)blocks * 64 * 16;
-        if (vec && s->pow2) hipLaunchKernelGGL((k_attn_values<true, true>), vgrid, dim3(256), lds, st, a);
-        else if (vec) hipLaunchKernelGGL((k_attn_values<true, false>), vgrid, dim3(256), lds, st, a);
-        else if (s->pow2) hipLaunchKernelGGL((k_attn_values<false, true>), vgrid, dim3(256), lds, st, a);
-        else hipLaunchKernelGGL((k_attn_values<false, false>), vgrid, dim3(256), lds, st, a);
-        hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 256)), dim3(256), 0, st, a);
+        both([&](int of_own, bool many, unsigned tiles, uint32_t keys, unsigned) {
+            a.score_keys = (size_t)cdiv(keys, 256) * tiles * a.heads_here >= 512 ? 256 : 64;
+            const dim3 grid(cdiv(keys, a.score_keys), tiles, a.heads_here);
+            auto scores = [&](auto u, auto rt) {
+                constexpr int U = decltype(u)::value, RT = decltype(rt)::value;
+                if (vec) hipLaunchKernelGGL((k_attn_scores<U, RT, true>), grid, dim3(256), 0, st, a, of_own);
+                else hipLaunchKernelGGL((k_attn_scores<U, RT, false>), grid, dim3(256), 0, st, a, of_own);
+            };
+            auto wide = [&](auto u) {
+                if (many) scores(u, std::integral_constant<int, 4>());
+                else scores(u, std::integral_constant<int, 1>());
+            };
+            if (blocks == 1) wide(std::integral_constant<int, 1>());
+            else if (blocks == 2) wide(std::integral_constant<int, 2>());
+            else wide(std::integral_constant<int, 4>());
+        });
+        auto softmax_rows = [&](auto kind) {
+            constexpr Weights KIND = decltype(kind)::value;
+            const size_t lds = KIND == Weights::SERIES ? s->a.live * 4 : 0;
+            if (rows >= 512 || p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<256, KIND>), dim3((unsigned)rows), dim3(256), lds, st, a);
+            else hipLaunchKernelGGL((k_attn_softmax<1024, KIND>), dim3((unsigned)rows), dim3(1024), lds, st, a);
+        };
+        if (s->series) softmax_rows(std::integral_constant<Weights, Weights::SERIES>());
+        else if (s->pow2) softmax_rows(std::integral_constant<Weights, Weights::POW2>());
+        else softmax_rows(std::integral_constant<Weights, Weights::ANY>());
+        both([&](int of_own, bool many, unsigned tiles, uint32_t, unsigned splits) {
+            if (many) {
+                const dim3 grid(splits, tiles, a.heads_here * cdiv(dim, 128));
+                if (vec) hipLaunchKernelGGL(k_attn_values_tile<true>, grid, dim3(512), 0, st, a, of_own);
+                else hipLaunchKernelGGL(k_attn_values_tile<false>, grid, dim3(512), 0, st, a, of_own);
+            } else {
+                const dim3 grid(splits, tiles, a.heads_here);
+                const size_t lds = 16 * (size_t)blocks * 64 * 16;
+                if (vec) hipLaunchKernelGGL(k_attn_values<true>, grid, dim3(256), lds, st, a, of_own);
+                else hipLaunchKernelGGL(k_attn_values<false>, grid, dim3(256), lds, st, a, of_own);
+            }
+        });
+        if (!p.direct) hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 256)), dim3(256), 0, st, a);
     }
     ZK_LAUNCH_CHECK();
     return flag.end(name);
