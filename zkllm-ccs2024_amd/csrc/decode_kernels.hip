@@ -23,10 +23,11 @@ struct SoftmaxArgs {
     int bits[DIGITS];                    // log2 of the radices where all are powers of two
     int n, drop_bits;
     uint64_t drop;                       // the product of the radices whose digits are not kept
-    double scale, scale_inv;
-    // Two tables whose values need no gathers (a layer's): the first's from four terms of its series, the second's from its first `live` entries, the others being 0
-    double step, theta, guard;
-    uint32_t live;
+    double scale, scale_inv, scale_64;   // scale_64: 64 / (scale ln 2)
+    // Two tables whose values need no gathers (a layer's): the first's by five terms of its series in the digit, to within `guard`, the second's from its first `live` entries, the others
+    // being 0.  Digits of a distance d: bits from drop_bits on; d's upper half stays below upper_end.
+    double series[5], guard;
+    uint32_t live, upper_end;
 };
 struct SoftmaxPlan { SoftmaxArgs a; int32_t* memory = nullptr; bool pow2 = true, series = false; uint32_t dim = 0; };
 static constexpr uint32_t MOST_LIVE = 8192;
@@ -151,6 +152,7 @@ struct AttnArgs {
     int64_t* scores;                     // [head of keys][row][ld]
     int8_t* weights;                     // [head of keys][row][six digits][ld]
     uint32_t* top;                       // [head of keys][row]: the sixth digit is not all zeros
+    uint32_t* unsure;                    // how many rows need their sum in order, three words, the rows
     size_t ld;                           // a multiple of 64
     int64_t* shift_out;                  // [token][head], or null
     int64_t* parts;                      // [split][head of keys][row][dim][2]
@@ -214,45 +216,57 @@ template <bool VEC> __device__ __forceinline__ void head_piece(const int32_t* p,
 }
 __device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v[2] | v[3]) != 0; }
 
-// Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8
-template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, RT == 1 ? 2 : 1) k_attn_scores(const AttnArgs a, int own) {
+// Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8.  The next keys are
+// on their way while these are multiplied, and the place of those behind them is looked up.
+template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
     uint32_t bad = 0;
     Tile t;
+    if ((blockIdx.x | blockIdx.y | blockIdx.z | threadIdx.x) == 0) *a.unsure = 0;
     if (!tile_at<16 * RT>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
     const uint32_t key0 = blockIdx.x * a.score_keys;
     if (key0 >= t.keys) return;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z;
-    v4i b[RT][U][4];
-    bool wide = false;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z, end = min(key0 + a.score_keys, t.keys);
+    auto query = [&](int r, int u, v4i (&d)[4]) {
         const uint32_t row = t.has(16 * r + c) ? t.row0 + 16 * r + c : t.lo, token = row / a.group, head = kv * a.group + (row - token * a.group);
-        const int32_t* p = a.q + token * a.q_token + head * a.q_head;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            int32_t x[16];
-            head_piece<VEC>(p, u * 64 + q * 4, a.dim, x);
-            digit_planes(x, b[r][u], bad);
-            wide |= any_bits(b[r][u][3]);
-        }
-    }
-    const bool q_wide = __any(wide);
+        int32_t x[16];
+        head_piece<VEC>(a.q + token * a.q_token + head * a.q_head, u * 64 + q * 4, a.dim, x);
+        digit_planes(x, d, bad);
+    };
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     const int32_t* keys = (const int32_t*)cache.k + kv * cache.head_stride;
+    auto place = [&](uint32_t key) { return keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + c, t.keys - 1), bad); };
+    int32_t x[U][16];
+    auto fetch = [&](const int32_t* p) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) head_piece<VEC>(p, u * 64 + q * 4, a.dim, x[u]);
+    };
+    uint32_t key = key0 + wave * 16;
+    if (key < end) fetch(place(key));
+    const int32_t* next = place(key + 64);
+    v4i b[RT][U][3];
+    bool wide = false;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v4i d[4];
+            query(r, u, d);
+#pragma unroll
+            for (int m = 0; m < 3; ++m) b[r][u][m] = d[m];
+            wide |= any_bits(d[3]);
+        }
+    const bool q_wide = __any(wide);
     int64_t* out = a.scores + ((size_t)blockIdx.z * a.tokens * a.group + t.row0 + c) * a.ld + t.col0 + 4 * q;
-    for (uint32_t i = wave; i < a.score_keys / 16; i += 4) {
-        const uint32_t key = key0 + i * 16;
-        if (key >= t.keys) break;
-        const int32_t* p = keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + c, t.keys - 1), bad);
+    for (; key < end; key += 64) {
         v4i k[U][4];
         bool k_wide = false;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            int32_t x[16];
-            head_piece<VEC>(p, u * 64 + q * 4, a.dim, x);
-            digit_planes(x, k[u], bad);
+            digit_planes(x[u], k[u], bad);
             k_wide |= any_bits(k[u][3]);
         }
+        if (key + 64 < end) fetch(next);
+        next = place(key + 128);
         const bool four = q_wide || __any(k_wide);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -268,12 +282,14 @@ template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, RT == 
             if (four) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
+                    v4i d[4];
+                    query(r, u, d);                        // a fourth digit is rare: the queries' is not kept
 #pragma unroll
                     for (int m = 0; m < 3; ++m) {
-                        acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][3], acc[m + 3], 0, 0, 0);
+                        acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], d[3], acc[m + 3], 0, 0, 0);
                         acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][m], acc[m + 3], 0, 0, 0);
                     }
-                    acc[6] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][3], acc[6], 0, 0, 0);
+                    acc[6] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], d[3], acc[6], 0, 0, 0);
                 }
             }
             if (!t.has(16 * r + c)) continue;
@@ -336,7 +352,7 @@ template <int M> __device__ __forceinline__ double add_in_order(double total, co
         for (int i = 0; i < M; ++i) any |= x[i] != 0.0;
         const unsigned long long left = __ballot(any && lane >= from);
         if (left == 0 || !(total < __builtin_inf())) return total;
-        uint32_t at = (uint32_t)__builtin_ctzll(left);
+        uint32_t at = (uint32_t)__builtin_ctzll(left), until = min(at + 128 / M, 64u);      // a row's first terms: every few of them leave a power of two
         if (total > 0.0) {
             const int e = exponent(total);
             const uint64_t t = units_of(total);
@@ -354,20 +370,26 @@ template <int M> __device__ __forceinline__ double add_in_order(double total, co
             }
             if (last == 64) return total;
             at = last;
+            until = at + 1;
         }
+        for (; at < until; ++at)
 #pragma unroll
-        for (int i = 0; i < M; ++i) total = total + __shfl(x[i], at, 64);
-        from = at + 1;
+            for (int i = 0; i < M; ++i) {
+                const uint64_t t = zkd::double_to_bits(x[i]);
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)t, (int)at), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(t >> 32), (int)at);
+                total = total + zkd::bits_to_double((uint64_t)hi << 32 | lo);
+            }
+        from = until;
         if (from == 64) return total;
     }
 }
 // (double)x / scale, correctly rounded: two corrections of x / scale's estimate by the scale's correctly rounded inverse, the first of which leaves less than a unit in the last place,
 // from where the second rounds correctly
-__device__ __forceinline__ double divided(int64_t x, const SoftmaxArgs& s) {
+__device__ __forceinline__ double divided(int64_t x, double scale, double scale_inv) {
     const double v = (double)x;
-    double q = v * s.scale_inv;
-    q = __builtin_fma(__builtin_fma(-q, s.scale, v), s.scale_inv, q);
-    return __builtin_fma(__builtin_fma(-q, s.scale, v), s.scale_inv, q);
+    double q = v * scale_inv;
+    q = __builtin_fma(__builtin_fma(-q, scale, v), scale_inv, q);
+    return __builtin_fma(__builtin_fma(-q, scale, v), scale_inv, q);
 }
 // weights as digits: of eight keys, a plane's eight bytes at a time
 struct Digits8 { uint2 p[6]; };
@@ -387,99 +409,59 @@ __device__ __forceinline__ void digits8(const uint64_t (&d)[8], Digits8& out) { 
     }
 }
 enum class Weights { ANY, POW2, SERIES };
-// A workgroup a row, eight neighbouring keys a lane.  The sum of exponentials is taken in no order first: off from the sum in order by at most (keys + 64) 2^-53 of it, which decides the shift unless it
-// lies that near to a border between two whole numbers (one row in 45 at 2048 keys and a scale of 2^32 sqrt(128)); then the sum in order is taken too, the waves' runs at once where
-// the sum stays within a power of two, and the few others one after the other.
-template <int T, Weights KIND> __global__ void __launch_bounds__(T) k_attn_softmax(const AttnArgs a) {
-    constexpr int M = 8, WAVES = T / 64;
-    extern __shared__ int32_t live[];
-    __shared__ double sums[WAVES];
-    __shared__ Steps steps[WAVES];
-    __shared__ int at_exponent[WAVES];
-    __shared__ double in_order;
-    __shared__ uint32_t any_top;
-    const uint32_t rows = a.tokens * a.group, r = blockIdx.x, in = r % rows, token = in / a.group, lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    const SoftmaxArgs& s = a.softmax;
-    uint32_t bad = 0, own = 0;
-    Sequence q;
-    if (a.seqs.count) {
-        if (!sequence_of(a.seqs, token, q, bad)) {         // nobody's row: no weights, in case that its tile is somebody's
-            int8_t* w = a.weights + (size_t)r * 6 * a.ld;
-            for (size_t i = threadIdx.x; i < 6 * a.ld / 16; i += T) reinterpret_cast<v4i*>(w)[i] = v4i{0, 0, 0, 0};
-            if (threadIdx.x == 0) a.top[r] = 0;
-            return;
-        }
-        own = own_seen(a, q, token);
-    }
-    if constexpr (KIND == Weights::SERIES)
-        for (uint32_t i = threadIdx.x; i < s.live; i += T) live[i] = s.table[1][i];
-    if (threadIdx.x == 0) any_top = 0;
-    // columns with keys: the prefix's, then the row's own; weights are 0 up to where another row of the tile may see
-    const uint32_t own_end = a.prefix_cols + own, cols = own ? own_end : a.prefix_len, fill = min((uint32_t)a.ld, a.seqs.count ? a.prefix_cols + (own + 127) / 64 * 64 : a.prefix_cols);
-    auto is_key = [&](uint32_t j) { return j < a.prefix_len || (j >= a.prefix_cols && j < own_end); };
-    const int64_t* x = a.scores + (size_t)r * a.ld;
-    const uint32_t chunks = (cols + T * M - 1) / (T * M);
-    int64_t v[M];
-    double term[M];
-    auto load = [&](uint32_t chunk) {
-        const uint32_t j = chunk * T * M + threadIdx.x * M;
-#pragma unroll
-        for (int i = 0; i < M; ++i) v[i] = 0;
-        if (j < cols) {
-            typedef long long v2l __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int i = 0; i < M; i += 2) {
-                const v2l p = *reinterpret_cast<const v2l*>(x + j + i);
-                v[i] = p[0]; v[i + 1] = p[1];
-            }
-        }
-    };
-    auto terms = [&](uint32_t chunk) {
-        const uint32_t j = chunk * T * M + threadIdx.x * M;
-#pragma unroll
-        for (int i = 0; i < M; ++i) term[i] = is_key(j + i) ? zkd::exp_det(divided(v[i], s)) : 0.0;
-    };
-    double total = 0.0;
-    for (uint32_t c = 0; c < chunks; ++c) {
-        load(c);
-        terms(c);
-#pragma unroll
-        for (int i = 0; i < M; ++i) total += term[i];
-    }
+enum class Sums { NEAR, IN_ORDER, BOTH };
+static constexpr int64_t NO_KEY = INT64_MIN;      // a score whose exponential is 0: scales are 2^53 at most
+// a b + c with c in scalar registers: the compiler copies a constant to vector registers for every addition otherwise
+__device__ __forceinline__ double fma_s(double a, double b, double c) {
+    double r;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
+    return r;
+}
+// exp(v / scale) to some 2^-50 and what v / scale's rounding adds: 2^(n / 64) out of LDS and five terms behind it
+__device__ __forceinline__ double exp_near(int64_t v, const SoftmaxArgs& s, const double* power) {
+    const double x = __builtin_fmin(__builtin_fmax((double)v * s.scale_64, -1e5), 1e5), n = rint(x), f = x - n;
+    constexpr double L = 0.69314718055994530942 / 64.0;
+    double p = fma_s(f, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
+    p = fma_s(f, p, L * L * L / 6.0);
+    p = fma_s(f, p, L * L / 2.0);
+    p = fma_s(f, p, L);
+    p = __builtin_fma(f, p, 1.0);
+    const int i = (int)n;
+    return ldexp(power[i & 63] * p, i >> 6);
+}
+// the columns of a row's scores: the prefix's, then, from a multiple of 64 on, its own
+struct Columns {
+    uint32_t prefix_len, prefix_cols, own_end, end;
+    __device__ uint32_t keys_at(uint32_t j) const { return j < prefix_cols ? (j < prefix_len ? min(8u, prefix_len - j) : 0u) : j < own_end ? min(8u, own_end - j) : 0u; }      // of eight from j on
+};
+// the sum of a row's exponentials in the order of the keys, by W waves
+template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x, Columns columns, double scale, double scale_inv, double* sums, Steps* steps, int* at_exponent, double* in_order) {
+    constexpr int M = 8, T = 64 * W;
+    const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0 : threadIdx.x >> 6, tid = wave * 64 + lane;
     auto wave_sum = [](double t) {
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
         return t;
     };
-    total = wave_sum(total);
-    if (lane == 0) sums[wave] = total;
-    __syncthreads();
-    total = 0.0;
+    double t = 0.0;
+    constexpr int N = W == 1 ? 2 : M;          // a lane's terms at a time: few, where the registers hold a row's scores
+    for (uint32_t j0 = 0; j0 < columns.end; j0 += T * N) {
+        {
+            const uint32_t j = j0 + tid * N, in8 = j & 7u, keys8 = columns.keys_at(j - in8), keys = keys8 > in8 ? keys8 - in8 : 0u;
+            double term[N], mine = 0.0;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) total += sums[i];
-    auto shift_of = [&](double t) {
-        const double sv = s.scale * zkd::log_det(t);
-        return sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5);
-    };
-    int64_t shift = 0;
-    if (cols) {
-        const double ln = zkd::log_det(total), sv = s.scale * ln;
-        const double off = s.scale * ((double)(cols + 64) * 1.2e-16 + 3e-15 * (fabs(ln) + 1.0)), from_border = fabs(sv - floor(sv) - 0.5);
-        bool sure = total > 0.0 && total < __builtin_inf() && off < 0.25 && from_border > off;
-        if (sure) shift = shift_of(total);
-        else {
-            double t = 0.0;
-            for (uint32_t c = 0; c < chunks; ++c) {
-                if (chunks > 1) { load(c); terms(c); }
-                double mine = 0.0;
-#pragma unroll
-                for (int i = 0; i < M; ++i) mine += term[i];
+            for (int e = 0; e < N; ++e) {
+                term[e] = e < (int)keys ? zkd::exp_det(divided(x[j + e], scale, scale_inv)) : 0.0;
+                mine += term[e];
+            }
+            if constexpr (W == 1) t = add_in_order<N>(t, term);
+            else {
                 mine = wave_sum(mine);
-                __syncthreads();                           // the arrays' last use is over
+                __syncthreads();
                 if (lane == 0) sums[wave] = mine;
                 __syncthreads();
                 double before = t;
-                for (uint32_t i = 0; i < wave; ++i) before += sums[i];
+                for (uint32_t k = 0; k < wave; ++k) before += sums[k];
                 const double behind = before + mine;
                 // a run that stays within a power of two, by a margin that the sums' order cannot reach
                 const int e = before > 0.0 && behind < __builtin_inf() ? exponent(behind * (1.0 + 1e-9)) : 2000;
@@ -487,69 +469,191 @@ template <int T, Weights KIND> __global__ void __launch_bounds__(T) k_attn_softm
                 if (clean) {
                     Steps st{0, 0};
 #pragma unroll
-                    for (int i = 0; i < M; ++i) step(st, term[i], e);
+                    for (int k = 0; k < N; ++k) step(st, term[k], e);
                     st = steps_up_to(st);
                     if (lane == 63) steps[wave] = st;
                 }
                 if (lane == 0) at_exponent[wave] = clean ? e : 2000;
                 __syncthreads();
-                for (uint32_t i = 0; i < (uint32_t)WAVES; ++i) {
-                    if (at_exponent[i] != 2000 && t > 0.0 && exponent(t) == at_exponent[i]) {
-                        const uint64_t u = units_of(t), after = u + (u & 1 ? steps[i].odd : steps[i].even);
-                        if (after < UNITS) { t = ldexp((double)after, at_exponent[i] - 52); continue; }
+                for (uint32_t k = 0; k < (uint32_t)W; ++k) {
+                    if (at_exponent[k] != 2000 && t > 0.0 && exponent(t) == at_exponent[k]) {
+                        const uint64_t u = units_of(t), after = u + (u & 1 ? steps[k].odd : steps[k].even);
+                        if (after < UNITS) { t = ldexp((double)after, at_exponent[k] - 52); continue; }
                     }
-                    if (wave == i) {
-                        t = add_in_order<M>(t, term);
-                        if (lane == 0) in_order = t;
+                    if (wave == k) {
+                        t = add_in_order<N>(t, term);
+                        if (lane == 0) *in_order = t;
                     }
                     __syncthreads();
-                    t = in_order;
+                    t = *in_order;
                     __syncthreads();
                 }
             }
-            shift = shift_of(t);
         }
     }
-    if (threadIdx.x == 0 && a.shift_out) a.shift_out[((size_t)token * a.kv_heads + a.kv0 + r / rows) * a.group + (in - token * a.group)] = shift;
-    if constexpr (KIND == Weights::SERIES) __syncthreads();
-    bool top = false;
-    for (uint32_t c = 0; c * T * M < fill; ++c) {
-        const uint32_t j = c * T * M + threadIdx.x * M;
-        if (j >= fill) break;
-        if (chunks != 1 || c != 0) load(c);
-        uint64_t d[M];
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-            if constexpr (KIND == Weights::SERIES) {
-                // both tables' values and their product are exact in double precision, and so is the number whose low 48 bits are the digits, 128 more each
-                constexpr double BASE = 4503599627370496.0 + 141289400074368.0;
-                double w = BASE;
-                if (is_key(j + i)) {
-                    const int64_t below = shift - v[i];
-                    const uint64_t t = (uint64_t)below >> s.drop_bits, upper = t >> s.bits[0];
-                    bad |= below < 0 || upper >= s.radix[1] ? (uint32_t)ZK_VALUES_TABLE : 0u;
-                    const uint32_t digit = (uint32_t)t & (s.radix[0] - 1);
-                    const double z = s.step * (double)digit;
-                    const double u = __builtin_fma(s.theta, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, 1.0 / 24.0, -1.0 / 6.0), 0.5), -1.0), 1.0), 0.5);
-                    double first = floor(u);
-                    if (fabs(u - first - 0.5) > 0.5 - s.guard) first = (double)s.table[0][digit];      // nearer to a border than the terms left out
-                    w = __builtin_fma(first, below >= 0 && upper < s.live ? (double)live[upper] : 0.0, BASE);
-                }
-                d[i] = zkd::double_to_bits(w) ^ 0x808080808080ull;
-            } else {
-                const int64_t y = is_key(j + i) ? softmax_weight<KIND == Weights::POW2>(shift - v[i], s, bad) : 0;
-                d[i] = ((uint64_t)y + 0x808080808080ull) ^ 0x808080808080ull;
-            }
-            top |= (d[i] >> 40 & 0xFF) != 0;
-        }
-        Digits8 p;
-        digits8(d, p);
-#pragma unroll
-        for (int k = 0; k < 6; ++k) *reinterpret_cast<uint2*>(a.weights + ((size_t)r * 6 + k) * a.ld + j) = p.p[k];
+    return t;
+}
+// W waves a row, eight neighbouring keys a lane at a time, C times in its registers.  The sum of exponentials is taken in no order first, from exponentials that are near: off from the sum in
+// order by at most (keys + 64) 2^-53 of it and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 40 at 2048 keys and
+// a scale of 2^32 sqrt(128)); then the sum in order is taken -- by a launch of its own for such rows, where there are many rows --, the waves' runs at once where the sum stays within a power of
+// two, and the few others one after the other.
+template <int W, int C, Weights KIND, Sums SUMS> __global__ void __launch_bounds__(W > 4 ? 64 * W : 256, SUMS == Sums::NEAR ? 4 : 1) k_attn_softmax(const AttnArgs a) {
+    constexpr int M = 8, T = 64 * W, ROWS = W > 4 ? 1 : 4 / W;      // a workgroup's rows at a time
+    static_assert(W == 1 || ROWS == 1, "waves that share a row meet at the workgroup's barriers");
+    extern __shared__ int32_t live[];
+    __shared__ double sums[W], power[64];
+    __shared__ Steps steps[W];
+    __shared__ int at_exponent[W];
+    __shared__ double in_order;
+    __shared__ uint32_t any_top;
+    const uint32_t rows = a.tokens * a.group, all = a.heads_here * rows, lane = threadIdx.x & 63u, wave = W == 1 ? 0 : threadIdx.x >> 6, tid = wave * 64 + lane;
+    const SoftmaxArgs& s = a.softmax;
+    uint32_t bad = 0;
+    if constexpr (KIND == Weights::SERIES) {
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < s.live; i += T * ROWS) live[i] = s.table[1][i];
     }
-    if (__any(top) && lane == 0) any_top = 1;
+    if (threadIdx.x < 64) power[threadIdx.x] = zkd::exp_det((double)threadIdx.x * (0.69314718055994530942 / 64.0));
     __syncthreads();
-    if (threadIdx.x == 0) a.top[r] = any_top;
+    const uint32_t work = SUMS == Sums::IN_ORDER ? *a.unsure : all;
+    for (uint32_t at = W == 1 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * ROWS + (threadIdx.x >> 6))) : blockIdx.x; at < work; at += gridDim.x * ROWS) {
+        const uint32_t r = SUMS == Sums::IN_ORDER ? a.unsure[4 + at] : at, in = r % rows, token = in / a.group;
+        uint32_t own = 0;
+        Sequence q;
+        if (a.seqs.count) {
+            if (!sequence_of(a.seqs, token, q, bad)) {     // nobody's row: no weights, in case that its tile is somebody's
+                int8_t* w = a.weights + (size_t)r * 6 * a.ld;
+                for (size_t i = tid; i < 6 * a.ld / 16; i += T) reinterpret_cast<v4i*>(w)[i] = v4i{0, 0, 0, 0};
+                if (tid == 0) a.top[r] = 0;
+                continue;
+            }
+            own = own_seen(a, q, token);
+        }
+        // columns with keys: the prefix's, then the row's own; weights are 0 up to where another row of the tile may see
+        const uint32_t own_end = a.prefix_cols + own, cols = own ? own_end : a.prefix_len, fill = min((uint32_t)a.ld, a.seqs.count ? a.prefix_cols + (own + 127) / 64 * 64 : a.prefix_cols);
+        const Columns columns{a.prefix_len, a.prefix_cols, own_end, cols};
+        const int64_t* x = a.scores + (size_t)r * a.ld;
+        const uint32_t stretches = (cols + T * M * C - 1) / (T * M * C);
+        int64_t v[C][M];
+        uint32_t n[C];
+        auto load = [&](uint32_t stretch) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint32_t j = (stretch * C + c) * T * M + tid * M;
+                n[c] = columns.keys_at(j);
+#pragma unroll
+                for (int i = 0; i < M; ++i) v[c][i] = NO_KEY;
+                if (n[c]) {
+                    typedef long long v2l __attribute__((ext_vector_type(2)));
+#pragma unroll
+                    for (int i = 0; i < M; i += 2) {
+                        const v2l p = *reinterpret_cast<const v2l*>(x + j + i);
+                        v[c][i] = p[0]; v[c][i + 1] = p[1];
+                    }
+                    if (n[c] < M)
+#pragma unroll
+                        for (int i = 1; i < M; ++i) v[c][i] = i < (int)n[c] ? v[c][i] : NO_KEY;
+                }
+            }
+        };
+        if (W > 1 && tid == 0) any_top = 0;
+        auto rounded = [](double sv) { return sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5); };
+        int64_t shift = 0;
+        bool sure = cols == 0, loaded = false;
+        if constexpr (SUMS != Sums::IN_ORDER) {
+            double total = 0.0;
+            for (uint32_t i = 0; i < stretches; ++i) {
+                load(i);
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+#pragma unroll
+                    for (int e = 0; e < M; ++e) {
+                        total += exp_near(v[c][e], s, power);
+                        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
+                    }
+                }
+            }
+            loaded = stretches == 1;
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+            if constexpr (W > 1) {
+                __syncthreads();                           // the arrays' last use is over
+                if (lane == 0) sums[wave] = total;
+                __syncthreads();
+                total = 0.0;
+#pragma unroll
+                for (int i = 0; i < W; ++i) total += sums[i];
+            }
+            if (cols) {
+                // An exponential of x is off by 2^-50 and |x| 2^-52; weighted by what it has in the sum t, |x| is |ln t| + ln(keys) at most.  The logarithm: 4e-16 of it, its product with the scale 2^-53.
+                const double ln = zkd::log_det(total), sv = s.scale * ln;
+                const double off = s.scale * ((double)(cols + 64) * 1.2e-16 + 2e-15 * (fabs(ln) + 20.0)), from_border = fabs(sv - floor(sv) - 0.5);
+                sure = total > 1e-280 && total < 1e280 && off < 0.25 && from_border > off;
+                if (sure) shift = rounded(sv);
+            }
+            if constexpr (SUMS == Sums::NEAR)
+                if (!sure) {
+                    if (tid == 0) a.unsure[4 + atomicAdd(a.unsure, 1u)] = r;
+                    continue;
+                }
+        }
+        if constexpr (SUMS != Sums::NEAR)
+            if (!sure) {
+                shift = rounded(s.scale * zkd::log_det(sum_in_order<W>(x, columns, s.scale, s.scale_inv, sums, steps, at_exponent, &in_order)));
+                loaded = false;                            // the registers were needed
+            }
+        if (tid == 0 && a.shift_out) a.shift_out[((size_t)token * a.kv_heads + a.kv0 + r / rows) * a.group + (in - token * a.group)] = shift;
+        // Both tables' values and their product are exact in double precision, and so is the number whose low 48 bits are the digits with 128 added to each
+        constexpr double BASE = 4503599627370496.0 + 141289400074368.0;
+        auto by_series = [&](int64_t score) {
+            const uint64_t below = (uint64_t)(shift - score);
+            const uint32_t lo = (uint32_t)below, hi = (uint32_t)(below >> 32), digit = lo >> s.drop_bits & (s.radix[0] - 1), upper = __builtin_amdgcn_alignbit(hi, lo, s.drop_bits + s.bits[0]);
+            const bool reached = hi < s.upper_end;         // neither negative nor too far
+            bad |= reached ? 0u : (uint32_t)ZK_VALUES_TABLE;
+            const double z = (double)digit;
+            const double u = fma_s(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, s.series[4], s.series[3]), s.series[2]), s.series[1]), s.series[0]);
+            double first = floor(u);
+            if (fabs(u - first - 0.5) > 0.5 - s.guard) first = (double)s.table[0][digit];      // nearer to a border than the terms left out
+            const int32_t second = live[min(upper, s.live - 1)];
+            return __builtin_fma(first, reached && upper < s.live ? (double)second : 0.0, BASE);
+        };
+        bool top = false;
+        const uint32_t fills = (fill + T * M * C - 1) / (T * M * C);
+        for (uint32_t i = 0; i < fills; ++i) {
+            if (!loaded || i != 0) load(i);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                const uint32_t j = (i * C + c) * T * M + tid * M;
+                if (j >= fill) continue;
+                uint64_t d[M];
+                if (n[c] < M)
+#pragma unroll
+                    for (int e = 0; e < M; ++e) v[c][e] = e < (int)n[c] ? v[c][e] : shift;
+#pragma unroll
+                for (int e = 0; e < M; ++e) {
+                    if constexpr (KIND == Weights::SERIES) d[e] = zkd::double_to_bits(by_series(v[c][e])) ^ 0x808080808080ull;
+                    else d[e] = ((uint64_t)softmax_weight<KIND == Weights::POW2>(shift - v[c][e], s, bad) + 0x808080808080ull) ^ 0x808080808080ull;
+                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+                if (n[c] < M)
+#pragma unroll
+                    for (int e = 0; e < M; ++e) d[e] = e < (int)n[c] ? d[e] : 0;
+                Digits8 p;
+                digits8(d, p);
+                top |= (p.p[5].x | p.p[5].y) != 0;
+#pragma unroll
+                for (int k = 0; k < 6; ++k) *reinterpret_cast<uint2*>(a.weights + ((size_t)r * 6 + k) * a.ld + j) = p.p[k];
+            }
+        }
+        const bool wave_top = __any(top);
+        if constexpr (W == 1) {
+            if (lane == 0) a.top[r] = wave_top;
+        } else {
+            if (wave_top && lane == 0) any_top = 1;
+            __syncthreads();
+            if (tid == 0) a.top[r] = any_top;
+        }
+    }
     raise(a.flag, bad);
 }
 
@@ -592,9 +696,12 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const A
     for (int s = 0; s < 9; ++s)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[s][n] = v4i{0, 0, 0, 0};
-    if (stream < streams)
+    auto place = [&](uint32_t k) { return cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad); };
+    if (stream < streams) {
+        size_t next = t.keys ? place(first + stream * 64) : 0;
         for (uint32_t k = first + stream * 64; k < end; k += 64 * streams) {
-            const size_t mine = cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad);
+            const size_t mine = next;
+            next = place(k + 64 * streams);                // looked up a step ahead
             v4i w[6];
 #pragma unroll
             for (int i = 0; i < 6; ++i) w[i] = *reinterpret_cast<const v4i*>(weights + i * a.ld + k);
@@ -629,6 +736,7 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const A
                     for (int i = 0; i < 6; ++i) acc[i + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[3], acc[i + 3][n], 0, 0, 0);
             }
         }
+    }
     __syncthreads();
     if (stream < streams)
 #pragma unroll
@@ -663,7 +771,7 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const A
 // Many rows: 64 rows by 128 dimensions, a wave 16 by 64.  The workgroup splits 64 keys' values into digits together, the next ones while this step's are multiplied: a lane four keys of four
 // dimensions, in LDS as fragments.
 template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile(const AttnArgs a, int own) {
-    __shared__ __attribute__((aligned(16))) int8_t planes[2][4][8][64][16];
+    __shared__ __attribute__((aligned(16))) int8_t planes[2][4][8][64][16], weight[2][4][6][64][16];      // fragments of the values and, [16 rows], of the weights
     __shared__ uint32_t wide[3];                           // of the step, the next and the one after that
     uint32_t bad = 0;
     Tile t;
@@ -682,9 +790,11 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
     const bool top = __any(a.top[row + mine] != 0);
     const int8_t* weights = a.weights + (row + mine) * 6 * a.ld + t.col0 + q * 16 + first;
     int32_t x[4][4];
-    v4i w[6];
+    auto place = [&](uint32_t i) { return cache_at(cache, t.own ? t.s.index : 0u, min(first + i * 64 + wave * 8 + (lane & 7u), t.keys - 1), bad); };
+    size_t next = 0;
     auto fetch = [&](uint32_t i) {
-        const size_t at = cache_at(cache, t.own ? t.s.index : 0u, min(first + i * 64 + wave * 8 + (lane & 7u), t.keys - 1), bad);
+        const size_t at = next;
+        next = place(i + 1);                               // looked up a step ahead
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int32_t* p = values + __shfl((unsigned long long)at, (int)((kq & 1u) * 4 + e), 64);
@@ -699,9 +809,10 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
             }
         }
     };
+    // two waves have the same rows: each brings three digits of them to LDS
     auto fetch_weights = [&](uint32_t i) {
 #pragma unroll
-        for (int k = 0; k < 6; ++k) w[k] = *reinterpret_cast<const v4i*>(weights + k * a.ld + i * 64);
+        for (int k = 0; k < 3; ++k) load_to_lds(weights + (block * 3 + k) * a.ld + i * 64, &weight[i & 1u][wave >> 1][block * 3 + k][0][0]);
     };
     auto split = [&](uint32_t i) {
         uint32_t over = 0, upper = 0;
@@ -731,13 +842,20 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
     if (threadIdx.x < 3) wide[threadIdx.x] = 0;
     __syncthreads();
     if (steps) {
+        next = place(0);
         fetch(0);
         fetch_weights(0);
         split(0);
     }
     __syncthreads();
     for (uint32_t i = 0; i < steps; ++i) {
-        if (i + 1 < steps) fetch(i + 1);
+        v4i w[6];
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = *reinterpret_cast<const v4i*>(&weight[i & 1u][wave >> 1][k][lane][0]);
+        if (i + 1 < steps) {
+            fetch_weights(i + 1);
+            fetch(i + 1);
+        }
         if (threadIdx.x == 0) wide[(i + 2) % 3] = 0;       // read last in the step before, written next in the step behind
         const bool four = wide[i % 3] != 0;
 #pragma unroll
@@ -758,10 +876,7 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
                 for (int k = 0; k < 6; ++k) acc[k + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[k], u, acc[k + 3][n], 0, 0, 0);
             }
         }
-        if (i + 1 < steps) {
-            fetch_weights(i + 1);
-            split(i + 1);
-        }
+        if (i + 1 < steps) split(i + 1);
         __syncthreads();
     }
 #pragma unroll
@@ -787,29 +902,37 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
     }
     raise(a.flag, bad);
 }
-// The parts' sums added up; rows that see no key
+// The parts' sums added up, 64 outputs by four shares of the parts a workgroup; rows that see no key
 __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
-    const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x, rows = (size_t)a.tokens * a.group, all = a.heads_here * rows;
-    if (id >= all * a.dim) return;
-    const uint32_t r = (uint32_t)(id / a.dim), d = (uint32_t)(id - (size_t)r * a.dim), kv = (uint32_t)(r / rows), in = (uint32_t)(r - kv * rows), token = in / a.group;
+    __shared__ unsigned long long sums[4][64][2];
+    const uint32_t share = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+    const size_t id = (size_t)blockIdx.x * 64 + lane, rows = (size_t)a.tokens * a.group, all = a.heads_here * rows;
+    const bool inside = id < all * a.dim;
+    const uint32_t r = inside ? (uint32_t)(id / a.dim) : 0, d = (uint32_t)(id - (size_t)r * a.dim), kv = (uint32_t)(r / rows), in = (uint32_t)(r - kv * rows), token = in / a.group;
     uint32_t bad = 0, own = 0;
-    bool has = true;
-    if (a.seqs.count) {
+    bool has = inside;
+    if (a.seqs.count && inside) {
         Sequence s;
         has = sequence_of(a.seqs, token, s, bad);
         if (has) own = (own_seen(a, s, token) + a.own_step - 1) / a.own_step;
     }
+    unsigned long long lo = 0, size = 0;
     if (has) {
-        unsigned long long lo = 0;
-        int64_t size = 0;
-        auto add = [&](uint32_t split) {
-            const unsigned long long* p = (const unsigned long long*)a.parts + ((split * all + r) * a.dim + d) * 2;
-            lo += p[0];
-            size += (int64_t)p[1];
-        };
-        for (uint32_t i = 0; i < a.prefix_splits; ++i) add(i);
-        for (uint32_t i = 0; i < own; ++i) add(a.prefix_splits + i);
-        attn_finish(a, lo, size, token, (a.kv0 + kv) * a.group + (in - token * a.group), d, bad);
+        const uint32_t parts = a.prefix_splits + own;
+        const unsigned long long* p = (const unsigned long long*)a.parts + ((size_t)r * a.dim + d) * 2;
+#pragma unroll 4
+        for (uint32_t i = share; i < parts; i += 4) {
+            lo += p[i * all * a.dim * 2];
+            size += p[i * all * a.dim * 2 + 1];
+        }
+    }
+    sums[share][lane][0] = lo;
+    sums[share][lane][1] = size;
+    __syncthreads();
+    if (has && share == 0) {
+#pragma unroll
+        for (int i = 1; i < 4; ++i) { lo += sums[i][lane][0]; size += sums[i][lane][1]; }
+        attn_finish(a, lo, (int64_t)size, token, (a.kv0 + kv) * a.group + (in - token * a.group), d, bad);
     }
     raise(a.flag, bad);
 }
@@ -934,7 +1057,7 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
 static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
 
 // How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
-struct AttnPlan { bool prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, parts; };
+struct AttnPlan { bool prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts; };
 static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     AttnPlan p{};
     const uint32_t group = heads / kv_heads;
@@ -956,12 +1079,17 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     cut(sequences ? max_length : 0, p.own_tiles, p.own64, p.own_splits, p.own_step);
     const uint32_t splits = p.prefix_splits + p.own_splits;
     p.direct = splits == 1;
-    const size_t each = rows * (p.cols * 14 + 4 + (size_t)(p.direct ? 0 : splits) * dim * 16);
+    const size_t each = rows * (p.cols * 14 + 8 + (size_t)(p.direct ? 0 : splits) * dim * 16);
     p.heads = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / std::max<size_t>(each, 1)));
+    if (p.heads < kv_heads && p.own64 && p.own_splits == 1) {      // as many as fill the compute units evenly, one workgroup each
+        auto used = [&](uint32_t h) { const size_t w = rows / 64 * h * cdiv(dim, 128); return w ? (double)w / (cdiv(w, 256) * 256.0) : 0.0; };
+        for (uint32_t h = p.heads; h >= std::max(1u, p.heads / 2); --h) if (used(h) > used(p.heads) + 0.02) p.heads = h;
+    }
     auto round = [](size_t b) { return (b + 15) / 16 * 16; };
     p.scores = p.heads * rows * p.cols * 8;
     p.weights = p.heads * rows * p.cols * 6;
     p.top = round(p.heads * rows * 4);
+    p.unsure = 16 + p.top;
     p.parts = p.heads * rows * (size_t)(p.direct ? 0 : splits) * dim * 16;
     return p;
 }
@@ -1002,7 +1130,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
     hipStream_t st = (hipStream_t)stv;
     ZK_ARG(softmax != nullptr && bs != nullptr && thetas != nullptr && dim > 0, std::string(name) + ": null argument or empty heads");
     ZK_ARG(K >= 1 && K <= DIGITS && L >= 0 && M >= 0 && L + M < K, std::string(name) + ": 1 to 8 digits, and at least one of them between the lowest L and the highest M");
-    ZK_ARG(scaling_factor_in >= 1 && scaling_factor_in <= 1e18, std::string(name) + ": the scaling factor must lie within 1 .. 1e18");
+    ZK_ARG(scaling_factor_in >= 1 && scaling_factor_in * std::sqrt((double)dim) <= 9007199254740992.0, std::string(name) + ": the scaling factor must lie within 1 .. 2^53 / sqrt(dim)");
     if (const int rc = CallFlag::not_captured(st, name)) return rc;
     std::unique_ptr<SoftmaxPlan> s(new SoftmaxPlan);
     s->dim = dim;
@@ -1010,6 +1138,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
     a = SoftmaxArgs{};
     a.scale = scaling_factor_in * std::sqrt((double)dim);
     a.scale_inv = 1.0 / a.scale;
+    a.scale_64 = 64.0 / (a.scale * 0.69314718055994530942);
     a.drop = 1;
     a.n = K - L;
     unsigned __int128 reach = 1;
@@ -1045,13 +1174,15 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
         }
         weight *= bs[i];
     }
-    if (s->pow2 && M == 0 && a.n == 2) {
-        const double w0 = (double)a.drop, w1 = w0 * bs[L], z = w0 / a.scale * bs[L], reach = std::log(thetas[1]) + 0.75;      // beyond exp(-reach) theta is below 0.5
-        a.step = w0 / a.scale; a.theta = thetas[0];
+    const int below = a.drop_bits + a.bits[0], all = below + a.bits[1];
+    if (s->pow2 && M == 0 && a.n == 2 && below < 32 && all >= 32 && all < 64) {
+        const double w0 = (double)a.drop / a.scale, w1 = w0 * bs[L], z = w0 * bs[L], reach = std::log(thetas[1]) + 0.75;      // beyond exp(-reach) theta is below 0.5
+        for (int i = 0; i < 5; ++i) a.series[i] = i ? a.series[i - 1] * -w0 / i : thetas[0];      // theta exp(-w0 digit)
+        a.series[0] += 0.5;
         a.guard = thetas[0] * (z * z * z * z * z / 60.0 + 0x1p-46);
-        const double live = reach / (w1 / a.scale) + 2.0;
-        a.live = (uint32_t)std::min<double>(live, bs[L + 1]);
-        s->series = z <= 0x1p-7 && a.guard < 0.01 && a.live <= MOST_LIVE;
+        a.live = (uint32_t)std::min<double>(reach / w1 + 2.0, bs[L + 1]);
+        a.upper_end = 1u << (all - 32);
+        s->series = z <= 0x1p-7 && a.guard < 0.01 && reach / w1 + 2.0 <= MOST_LIVE;
     }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess) e = hipStreamSynchronize(st);      // calls on any stream may use the tables
@@ -1063,7 +1194,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
 size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     if (tokens == 0 || kv_heads == 0 || heads < kv_heads) return 0;
     const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
-    return p.scores + p.weights + p.top + p.parts;
+    return p.scores + p.weights + p.top + p.unsure + p.parts;
 }
 int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                      const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts, const void* lengths, uint32_t max_length,
@@ -1094,7 +1225,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
     ZK_ARG(p.prefix_tiles <= 65535u && p.own_tiles <= 65535u && (uint64_t)p.heads * cdiv(dim, 128) <= 65535u, std::string(name) + ": more than 65535 tiles of queries");
     hipStream_t st = (hipStream_t)stv;
-    const size_t bytes = p.scores + p.weights + p.top + p.parts;
+    const size_t bytes = p.scores + p.weights + p.top + p.unsure + p.parts;
     ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_attention_workspace says");
     ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
     ZK_ARG(dim == s->dim, std::string(name) + ": the softmax was prepared for heads of another width");
@@ -1116,7 +1247,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     a.seqs = Sequences{own ? (const int32_t*)starts : nullptr, (const int32_t*)lengths, sequences, tokens, max_length};
     a.causal = causal; a.sf_first = divisor(sf_first); a.sf_second = divisor(sf_second);
     a.scores = (int64_t*)workspace; a.ld = p.cols; a.weights = (int8_t*)workspace + p.scores; a.top = (uint32_t*)(a.weights + p.weights);
-    a.parts = (int64_t*)((char*)a.top + p.top); a.direct = p.direct;
+    a.unsure = (uint32_t*)((char*)a.top + p.top); a.parts = (int64_t*)((char*)a.unsure + p.unsure); a.direct = p.direct;
     a.tokens = tokens; a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits; a.prefix_step = p.prefix_step; a.own_splits = p.own_splits; a.own_step = p.own_step;
     a.flag = flag.dev;
     const bool vec = dim % 4 == 0 && ((q_token | q_head) & 3) == 0 && ((uintptr_t)q & 15) == 0 && (!prefix_len || cache_aligned(prefix)) && (!own || cache_aligned(own));
@@ -1130,7 +1261,8 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             if (p.own_tiles && max_length) f(1, p.own64, p.own_tiles, max_length, p.own_splits);
         };
         both([&](int of_own, bool many, unsigned tiles, uint32_t keys, unsigned) {
-            a.score_keys = (size_t)cdiv(keys, 256) * tiles * a.heads_here >= 512 ? 256 : 64;
+            a.score_keys = 1024;                   // a workgroup's, where that still makes 512 workgroups
+            while (a.score_keys > 64 && (size_t)cdiv(keys, a.score_keys) * tiles * a.heads_here < 512) a.score_keys /= 2;
             const dim3 grid(cdiv(keys, a.score_keys), tiles, a.heads_here);
             auto scores = [&](auto u, auto rt) {
                 constexpr int U = decltype(u)::value, RT = decltype(rt)::value;
@@ -1148,8 +1280,15 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
         auto softmax_rows = [&](auto kind) {
             constexpr Weights KIND = decltype(kind)::value;
             const size_t lds = KIND == Weights::SERIES ? s->a.live * 4 : 0;
-            if (rows >= 512 || p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<256, KIND>), dim3((unsigned)rows), dim3(256), lds, st, a);
-            else hipLaunchKernelGGL((k_attn_softmax<1024, KIND>), dim3((unsigned)rows), dim3(1024), lds, st, a);
+            if (rows < 256) {
+                if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, 1, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(256), lds, st, a);
+                else hipLaunchKernelGGL((k_attn_softmax<16, 1, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(1024), lds, st, a);
+                return;
+            }
+            if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<1, 1, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(cdiv(rows, 4), 1024)), dim3(256), lds, st, a);
+            else hipLaunchKernelGGL((k_attn_softmax<4, 1, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(rows, 1024)), dim3(256), lds, st, a);
+            if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, 1, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 512)), dim3(256), lds, st, a);
+            else hipLaunchKernelGGL((k_attn_softmax<16, 1, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 256)), dim3(1024), lds, st, a);
         };
         if (s->series) softmax_rows(std::integral_constant<Weights, Weights::SERIES>());
         else if (s->pow2) softmax_rows(std::integral_constant<Weights, Weights::POW2>());
@@ -1166,7 +1305,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
                 else hipLaunchKernelGGL(k_attn_values<false>, grid, dim3(256), lds, st, a, of_own);
             }
         });
-        if (!p.direct) hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 256)), dim3(256), 0, st, a);
+        if (!p.direct) hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 64)), dim3(256), 0, st, a);
     }
     ZK_LAUNCH_CHECK();
     return flag.end(name);
