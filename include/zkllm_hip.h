@@ -527,7 +527,7 @@ int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared
 /* A weight of 4 bits with a scale and a zero for every `group` rows of a column (a multiple of 16; the last group may be shorter): w[k][p] = (code - zero) * scale, whole numbers, so
  * that products equal those with the int32 weight itself.  codes: N rows of (P + 1) / 2 bytes, columns 2 i and 2 i + 1 in byte i, the even one in its low half; scales: int32, ceil(N /
  * group) rows of P, up to 557047 in magnitude; zeros: bytes of the same shape, 0 .. 15, or null for 8.  All on the device, not read afterwards.  N and P as in zk_i32_rhs_prepare, half
- * a byte an element is kept.  The handle serves zk_i32_linear and zk_i32_gated, there both weights or none, whose workspace is then zk_i32_rhs_workspace's (for zk_i32_gated both
+ * a byte an element is kept.  The handle serves zk_i32_linear and zk_i32_gated, there both weights, with groups of one size, or none, whose workspace is then zk_i32_rhs_workspace's (for zk_i32_gated both
  * weights' sizes added up); released with zk_fr_matmul_rhs_free once its last call is through.  No counterpart in the reference. */
 int zk_i32_rhs_prepare_q4(void** prepared, const void* codes, const void* scales_i32, const void* zeros_u8, uint32_t N, uint32_t P, uint32_t group, void* stream);
 size_t zk_i32_rhs_workspace(const void* prepared, uint32_t rows);

@@ -841,14 +841,15 @@ __global__ void __launch_bounds__(256) k_split_cols_i32(int8_t* __restrict__ pla
 // w = (code - zero) scale, a scale and a zero for every `group` rows of a column.  Codes stand as the fragments of v_mfma_i32_16x16x64_i8 want them: [strip of 16 columns][128
 // rows][lane][16 bytes], a lane's 16 bytes its 16 rows of the first 64 and of the second, so that a wave reads 1 KB in one piece; in a 32-bit word the low halves of the bytes are
 // rows 0 .. 3, the high ones rows 4 .. 7.  A group's scales and zeros: [strip][group][column], scale * 16 + zero.
-struct Q4 { const uint32_t* codes; const int32_t* scales; uint32_t group, groups, units, cols; };
+struct Q4 { const uint32_t* codes; const int32_t* scales; uint32_t group, groups, units, cols; int shift; };      // shift: log2 of the group or -1
 static size_t q4_code_bytes(uint32_t P, uint32_t Kp) { return (size_t)cdiv(P, 16) * 16 * Kp / 2; }
-static Q4 q4_of(const MatmulRhs* w) { return Q4{(const uint32_t*)w->q4, (const int32_t*)((const char*)w->q4 + q4_code_bytes(w->P, w->Kp)), w->group, w->groups, w->Kp / 64, w->P}; }
+static Q4 q4_of(const MatmulRhs* w) { return Q4{(const uint32_t*)w->q4, (const int32_t*)((const char*)w->q4 + q4_code_bytes(w->P, w->Kp)), w->group, w->groups, w->Kp / 64, w->P,
+                                                    (w->group & (w->group - 1)) == 0 ? 31 - __builtin_clz(w->group) : -1}; }
 // a lane's 16 rows of unit u in a strip
 __device__ __forceinline__ uint2 q4_codes(const Q4& w, uint32_t strip, uint32_t u, uint32_t lane) {
     return *reinterpret_cast<const uint2*>(w.codes + (((size_t)strip * (w.units >> 1) + (u >> 1)) * 64 + lane) * 4 + 2 * (u & 1u));
 }
-__device__ __forceinline__ int32_t q4_scale(const Q4& w, uint32_t strip, uint32_t k, uint32_t c) { return w.scales[((size_t)strip * w.groups + min(k / w.group, w.groups - 1)) * 16 + c]; }
+__device__ __forceinline__ int32_t q4_scale(const Q4& w, uint32_t strip, uint32_t k, uint32_t c) { return w.scales[((size_t)strip * w.groups + min(w.shift >= 0 ? k >> w.shift : k / w.group, w.groups - 1)) * 16 + c]; }
 // 16 codes times their scale as digit planes
 template <int PB> __device__ __forceinline__ void q4_planes(uint2 codes, int32_t scale_zero, v4i (&out)[PB]) {
     const int32_t scale = scale_zero >> 4, off = -(scale_zero & 15) * scale;
@@ -866,6 +867,233 @@ template <int PB> __device__ __forceinline__ void q4_planes(uint2 codes, int32_t
             out[2][w] = (int)__builtin_amdgcn_perm(g, f, 0x05040100u);
         }
     }
+}
+// Products of few rows with groups of 64 rows and their multiples: codes less their zeros go into the matrix instructions as they are, a quarter of a byte plane's bytes and no digits of
+// the weight; a group's sums, exact in 32 bits, times its scale are added up in 64.
+struct Q4Args {
+    ProductArgs g;
+    Q4 w, gate;                          // gated: w is the up projection
+    uint32_t chunk;                      // of the inner dimension in LDS at a time, a multiple of 128
+};
+// a lane's 16 codes less their zero
+__device__ __forceinline__ v4i q4_codes_less(uint2 codes, int32_t scale_zero) {
+    const uint32_t less = 0x80808080u - (uint32_t)(scale_zero & 15) * 0x01010101u, nibbles = 0x0F0F0F0Fu;      // no borrow passes from byte to byte
+    return v4i{(int)(((codes.x & nibbles) + less) ^ 0x80808080u), (int)(((codes.x >> 4 & nibbles) + less) ^ 0x80808080u), (int)(((codes.y & nibbles) + less) ^ 0x80808080u),
+               (int)(((codes.y >> 4 & nibbles) + less) ^ 0x80808080u)};
+}
+// lo + hi 2^16 of sums below 2^55, within 2^62 or flagged and 0
+__device__ __forceinline__ int64_t q4_joined(int64_t lo, int64_t hi, uint32_t& bad) {
+    const int64_t units = hi + (lo >> 16);
+    const bool fits = (uint32_t)((int32_t)(units >> 32) + 0x4000) < 0x8000u && (units >> 32) == (int64_t)(int32_t)(units >> 32);
+    bad |= fits ? 0u : (uint32_t)ZK_VALUES_RANGE;
+    return fits ? (int64_t)((uint64_t)hi * 65536 + (uint64_t)lo) : 0;
+}
+template <bool GATED> __device__ __forceinline__ void q4_output(const ProductArgs& g, uint32_t row, uint32_t col, const int64_t (&v)[GATED ? 2 : 1], uint32_t& bad) {
+    auto value = [&](auto pow2) {
+        constexpr bool POW2 = decltype(pow2)::value;
+        if constexpr (GATED) {
+            const uint32_t at = activation_at<POW2>(v[0], g.e, bad);
+            return gated_value<POW2>(at == g.e.len ? 0 : g.e.table[at], v[1], g.e, bad);
+        } else return narrow(quotient<POW2>(v[0], g.e.sf), bad);
+    };
+    g.e.out[(size_t)row * g.cols + col] = g.e.pow2 ? value(std::true_type()) : value(std::false_type());
+}
+// Up to four rows, a strip of 16 columns a workgroup: the 16 rows of v_mfma_i32_16x16x64_i8 are the four digits of up to four rows of x, which the workgroup splits into LDS while its first
+// codes are on their way.  A wave takes 128 inner rows at a time, four such loads ahead.
+template <bool GATED, int R, int WAVES> __global__ void __launch_bounds__(64 * WAVES) k_q4_rows(const Q4Args a) {
+    constexpr int MATS = GATED ? 2 : 1, DEPTH = 4;
+    extern __shared__ __attribute__((aligned(16))) int8_t digits[];        // [64 inner rows][a quarter of them][digit][row of x][16]
+    __shared__ unsigned long long sums[MATS][4][R][16];
+    const ProductArgs& g = a.g;
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4, strip = blockIdx.x, Kp = a.w.units * 64;
+    uint32_t bad = 0;
+    for (uint32_t i = threadIdx.x; i < MATS * 4 * R * 16; i += WAVES * 64) (&sums[0][0][0][0])[i] = 0;
+    struct Loaded { uint4 codes; int32_t scale[2]; } w[DEPTH][MATS];
+    auto load = [&](uint32_t k, int d) {                   // the 128 inner rows from k on
+        k = min(k, Kp - 128);                              // behind the last ones those again: never multiplied
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            const Q4& x = GATED && m == 0 ? a.gate : a.w;
+            w[d][m].codes = *reinterpret_cast<const uint4*>(x.codes + (((size_t)strip * (x.units >> 1) + k / 128) * 64 + lane) * 4);
+            w[d][m].scale[0] = q4_scale(x, strip, k, c);
+            w[d][m].scale[1] = q4_scale(x, strip, k + 64, c);
+        }
+    };
+    int64_t acc[MATS][R];
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[m][r] = 0;
+    const uint32_t my_row = min(c & 3u, (uint32_t)R - 1), my_digit = c >> 2;
+    for (uint32_t k0 = 0; k0 < Kp; k0 += a.chunk) {
+        const uint32_t end = min(k0 + a.chunk, Kp);
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) load(k0 + (wave + d * WAVES) * 128, d);
+        if (k0) __syncthreads();                           // the last chunk's digits are read
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            for (uint32_t k = k0 + threadIdx.x * 4; k < end; k += WAVES * 256) {
+                int32_t x[4] = {0, 0, 0, 0};
+                if (r < (int)g.rows) {
+                    const int32_t* p = g.x + r * g.ldx + k;
+                    if (g.x_aligned && k + 4 <= g.inner) {
+                        const v4i v = *reinterpret_cast<const v4i*>(p);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) x[e] = v[e];
+                    } else
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) if (k + e < g.inner) x[e] = p[e];
+                }
+                uint32_t d[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    bad |= x[e] > 0x7F7F7F7F ? (uint32_t)ZK_VALUES_RANGE : 0u;
+                    d[e] = digit_bytes((uint32_t)x[e]);
+                }
+                const uint32_t f = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), h = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
+                const uint32_t i = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), j = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+                const uint32_t plane[4] = {__builtin_amdgcn_perm(i, f, 0x05040100u), __builtin_amdgcn_perm(i, f, 0x07060302u), __builtin_amdgcn_perm(j, h, 0x05040100u), __builtin_amdgcn_perm(j, h, 0x07060302u)};
+                int8_t* to = digits + ((k - k0) >> 4) * (4 * R * 16) + r * 16 + (k & 15u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(to + e * R * 16) = plane[e];
+            }
+        __syncthreads();
+        const int8_t* from = digits + (q * 4 * R + my_digit * R + my_row) * 16;
+        for (uint32_t at = k0 + wave * 128; at < end; at += DEPTH * WAVES * 128)
+#pragma unroll
+            for (int d = 0; d < DEPTH; ++d) {
+                const uint32_t k = at + d * WAVES * 128;
+                if (k < end) {
+                    const int8_t* p = from + ((k - k0) >> 4) * (4 * R * 16);
+                    const v4i x0 = *reinterpret_cast<const v4i*>(p), x1 = *reinterpret_cast<const v4i*>(p + 4 * (4 * R * 16));
+#pragma unroll
+                    for (int m = 0; m < MATS; ++m) {
+                        const v4i w0 = q4_codes_less(make_uint2(w[d][m].codes.x, w[d][m].codes.y), w[d][m].scale[0]), w1 = q4_codes_less(make_uint2(w[d][m].codes.z, w[d][m].codes.w), w[d][m].scale[1]);
+                        const v4i zero = {0, 0, 0, 0};
+                        const v4i s0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x0, w0, zero, 0, 0, 0), s1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(x1, w1, zero, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < R; ++r) acc[m][r] += (int64_t)s0[r] * (w[d][m].scale[0] >> 4) + (int64_t)s1[r] * (w[d][m].scale[1] >> 4);      // digit q of row r
+                    }
+                }
+                load(k + DEPTH * WAVES * 128, d);
+            }
+    }
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int r = 0; r < R; ++r) atomicAdd(&sums[m][q][r][c], (unsigned long long)acc[m][r]);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < R * 16; i += WAVES * 64) {
+        const uint32_t r = i >> 4, col = strip * 16 + (i & 15u);
+        if (r >= g.rows || col >= g.cols) continue;
+        int64_t v[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            int64_t s[4];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) s[d] = (int64_t)sums[m][d][r][i & 15u];
+            v[m] = q4_joined(s[0] + s[1] * 256, s[2] + s[3] * 256, bad);
+        }
+        q4_output<GATED>(g, r, col, v, bad);
+    }
+    raise(g.e.flag, bad);
+}
+// 5 to 32 rows: S strips by 8 / S shares of the inner dimension a workgroup, 128 inner rows at a time; x's planes, which the strips share, go to LDS as fragments a step ahead.
+template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k_q4_strip(const Q4Args a) {
+    constexpr int MATS = GATED ? 2 : 1, SHARES = 8 / S, PIECES = SHARES * 2 * RT * 4, EACH = PIECES / 8;
+    // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
+    __shared__ __attribute__((aligned(16))) int8_t x0[SHARES][2][RT][4][1024], x1[SHARES][2][RT][4][1024];      // [share][64 inner rows][16 rows][digit]
+    __shared__ unsigned long long sums[MATS][2][RT * 16][S * 16];
+    const ProductArgs& g = a.g;
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4, share = wave / S, in = wave % S;
+    const uint32_t strips = (a.w.cols + 15) / 16, strip = min(blockIdx.x * S + in, strips - 1), pairs = a.w.units >> 1, steps = (pairs + SHARES - 1) / SHARES;
+    uint32_t need = 0, bad = 0;
+    for (uint32_t i = lane; i < g.chunks; i += 64) need = max(need, g.need[i]);
+    const bool four = __any(need > 3);
+    const size_t plane = (size_t)g.rows_padded * g.w.Kp;
+    for (uint32_t i = threadIdx.x; i < sizeof(sums) / 8; i += 512) (&sums[0][0][0][0])[i] = 0;
+    auto fetch = [&](uint32_t step, auto& x) {             // this wave's pieces of a step
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const uint32_t piece = wave * EACH + i, d = piece & 3u, r = piece >> 2 & (RT - 1u), u = (piece / (4 * RT)) & 1u, s = piece / (8 * RT), pair = min(step * SHARES + s, pairs - 1);
+            load_to_lds(g.px + d * plane + ((size_t)(pair * 4 + u * 2 + (q >> 1)) * g.rows_padded + r * 16 + c) * 32 + (q & 1u) * 16, &x[s][u][r][d][0]);
+        }
+    };
+    struct Loaded { uint4 codes; int32_t scale[2]; } w[2][MATS];
+    auto load = [&](uint32_t step, int d) {
+        const uint32_t pair = min(step * SHARES + share, pairs - 1);
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            const Q4& x = GATED && m == 0 ? a.gate : a.w;
+            w[d][m].codes = *reinterpret_cast<const uint4*>(x.codes + (((size_t)strip * pairs + pair) * 64 + lane) * 4);
+            w[d][m].scale[0] = q4_scale(x, strip, pair * 128, c);
+            w[d][m].scale[1] = q4_scale(x, strip, pair * 128 + 64, c);
+        }
+    };
+    int64_t acc[MATS][RT][2][4];                           // digits 0 and 1, digits 2 and 3
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[m][r][e >> 2][e & 3] = 0;
+    const bool both = a.w.group % 128 == 0 && (!GATED || a.gate.group % 128 == 0);      // 128 inner rows have one scale
+    auto multiply = [&](uint32_t step, int d, auto& x) {
+        if (step * SHARES + share >= pairs) return;
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) {
+            v4i b[2] = {q4_codes_less(make_uint2(w[d][m].codes.x, w[d][m].codes.y), w[d][m].scale[0]), q4_codes_less(make_uint2(w[d][m].codes.z, w[d][m].codes.w), w[d][m].scale[1])};
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                v4i s[4];
+                auto add = [&](int32_t scale) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc[m][r][0][e] += (int64_t)(s[0][e] + s[1][e] * 256) * scale;
+                        acc[m][r][1][e] += (int64_t)(s[2][e] + (four ? s[3][e] * 256 : 0)) * scale;
+                    }
+                };
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (u == 0 || !both)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[i] = v4i{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) s[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(&x[share][u][r][i][lane * 16]), b[u], s[i], 0, 0, 0);
+                    if (four) s[3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(&x[share][u][r][3][lane * 16]), b[u], s[3], 0, 0, 0);
+                    if (u == 0 && !both) add(w[d][m].scale[0] >> 4);
+                }
+                add(w[d][m].scale[1] >> 4);
+            }
+        }
+    };
+    fetch(0, x0);
+    load(0, 0);
+    for (uint32_t t = 0; t < steps; t += 2) {
+        __syncthreads();                                   // the step's pieces are there, and the other buffer is read
+        if (t + 1 < steps) { fetch(t + 1, x1); load(t + 1, 1); }
+        multiply(t, 0, x0);
+        if (t + 1 >= steps) break;
+        __syncthreads();
+        if (t + 2 < steps) { fetch(t + 2, x0); load(t + 2, 0); }
+        multiply(t + 1, 1, x1);
+    }
+#pragma unroll
+    for (int m = 0; m < MATS; ++m)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) atomicAdd(&sums[m][e >> 2][r * 16 + 4 * q + (e & 3)][in * 16 + c], (unsigned long long)acc[m][r][e >> 2][e & 3]);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < RT * 16 * S * 16; i += 512) {
+        const uint32_t row = i / (S * 16), x = i % (S * 16), col = blockIdx.x * S * 16 + x;
+        if (row >= g.rows || col >= g.cols) continue;
+        int64_t v[MATS];
+#pragma unroll
+        for (int m = 0; m < MATS; ++m) v[m] = q4_joined((int64_t)sums[m][0][row][x], (int64_t)sums[m][1][row][x], bad);
+        q4_output<GATED>(g, row, col, v, bad);
+    }
+    raise(g.e.flag, bad);
 }
 // the planes of a whole weight, for products of many rows
 template <int PB> __global__ void __launch_bounds__(256) k_q4_expand(int8_t* __restrict__ planes, const Q4 w) {
@@ -970,8 +1198,34 @@ template <bool GATED, int PB> static void launch_product(const ProductArgs& g, h
     else if (g.e.pow2) launch_tiles<GATED, PB, true>(g, st);
     else launch_tiles<GATED, PB, false>(g, st);
 }
+// Up to 32 rows with groups that no step of 64 inner rows crosses take the codes as they are
+static bool q4_direct(const MatmulRhs* w, const MatmulRhs* gate, uint32_t rows) { return rows <= 32 && w->group % 64 == 0 && gate->group % 64 == 0; }
+template <bool GATED> static void launch_q4_rows(Q4Args& q, hipStream_t st) {
+    const unsigned strips = cdiv(q.w.cols, 16), Kp = q.w.units * 64;
+    auto rows = [&](auto n) {
+        constexpr int R = decltype(n)::value;
+        q.chunk = std::min(Kp, 14336u / R / 128 * 128);        // 56 KB
+        const size_t lds = (size_t)q.chunk * 4 * R;
+        if (strips > 512) hipLaunchKernelGGL((k_q4_rows<GATED, R, 4>), dim3(strips), dim3(256), lds, st, q);
+        else hipLaunchKernelGGL((k_q4_rows<GATED, R, 8>), dim3(strips), dim3(512), lds, st, q);
+    };
+    if (q.g.rows == 1) rows(std::integral_constant<int, 1>());
+    else if (q.g.rows == 2) rows(std::integral_constant<int, 2>());
+    else rows(std::integral_constant<int, 4>());
+}
+template <bool GATED> static void launch_q4_strips(const Q4Args& q, hipStream_t st) {
+    const unsigned strips = cdiv(q.w.cols, 16);
+    auto by = [&](auto rt) {
+        constexpr int RT = decltype(rt)::value;
+        if (strips >= 640) hipLaunchKernelGGL((k_q4_strip<GATED, RT, 4>), dim3(cdiv(strips, 4)), dim3(512), 0, st, q);
+        else if (RT == 2 || strips >= 320) hipLaunchKernelGGL((k_q4_strip<GATED, RT, 2>), dim3(cdiv(strips, 2)), dim3(512), 0, st, q);
+        else hipLaunchKernelGGL((k_q4_strip<GATED, 1, 1>), dim3(strips), dim3(512), 0, st, q);
+    };
+    if (q.g.rows <= 16) by(std::integral_constant<int, 1>());
+    else by(std::integral_constant<int, 2>());
+}
 // the planes that a product of many rows reads, in the workspace where the weight has none of its own
-static size_t expanded(const MatmulRhs* w) { return w->q4 ? (size_t)std::max(w->pb, 2) * w->P * w->Kp : 0; }
+static size_t expanded(const MatmulRhs* w, uint32_t rows) { return w->q4 && !q4_direct(w, w, rows) ? (size_t)std::max(w->pb, 2) * w->P * w->Kp : 0; }
 static void expand(const MatmulRhs* w, int8_t* planes, hipStream_t st) {
     const dim3 grid(cdiv(w->P, 16), cdiv(w->Kp / 64, 4));
     if (w->pb <= 2) hipLaunchKernelGGL(k_q4_expand<2>, grid, dim3(256), 0, st, planes, q4_of(w));
@@ -983,7 +1237,7 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, const
     ZK_ARG(g.ldx >= g.inner, std::string(name) + ": rows of x overlap (ldx below the inner dimension)");
     ZK_ARG(g.rows <= (1u << 18), std::string(name) + ": more than 262144 rows in one call");
     ZK_ARG(g.cols <= (1u << 22), std::string(name) + ": more than 4194304 columns");
-    const size_t bytes = zk_i32_linear_workspace(g.rows, g.inner), all = bytes + expanded(w) + (GATED ? expanded(gate) : 0);
+    const size_t bytes = zk_i32_linear_workspace(g.rows, g.inner), all = bytes + expanded(w, g.rows) + (GATED ? expanded(gate, g.rows) : 0);
     ZK_ARG(workspace == nullptr || workspace_bytes >= all, std::string(name) + ": the workspace is smaller than " + (w->q4 ? "zk_i32_rhs_workspace" : "zk_i32_linear_workspace") + " says");
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
@@ -998,12 +1252,23 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, const
         workspace = own->p;
     }
     ZK_ARG(all == 0 || ((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
-    if (w->q4) {
+    const bool direct = w->q4 && q4_direct(w, GATED ? gate : w, g.rows);
+    Q4Args q{};
+    if (direct) {
+        q.w = q4_of(w);
+        if constexpr (GATED) q.gate = q4_of(gate);
+        if (g.rows <= SPLIT_ROWS) {
+            q.g = g;
+            launch_q4_rows<GATED>(q, st);
+            ZK_LAUNCH_CHECK();
+            return flag.end(name);
+        }
+    } else if (w->q4) {
         int8_t* at = (int8_t*)workspace + bytes;
         expand(w, at, st);
         g.w.p = at;
         if constexpr (GATED) {
-            at += expanded(w);
+            at += expanded(w, g.rows);
             expand(gate, at, st);
             g.gate.p = at;
         }
@@ -1021,7 +1286,10 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, const
     g.need = (const uint32_t*)(g.zeros + 1024);
     g.parts = may_split(g.rows, g.inner) ? (int64_t*)((char*)workspace + bytes - PARTS_BYTES) : nullptr;
     hipLaunchKernelGGL(k_split_x, dim3(g.chunks, g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
-    if (pb <= 2) launch_product<GATED, 2>(g, st);
+    if (direct) {
+        q.g = g;
+        launch_q4_strips<GATED>(q, st);
+    } else if (pb <= 2) launch_product<GATED, 2>(g, st);
     else launch_product<GATED, 3>(g, st);
     ZK_LAUNCH_CHECK();
     return flag.end(name);
@@ -1223,7 +1491,7 @@ int zk_i32_rhs_prepare_q4(void** prepared, const void* codes, const void* scales
 }
 size_t zk_i32_rhs_workspace(const void* prepared, uint32_t rows) {
     const MatmulRhs* w = (const MatmulRhs*)prepared;
-    return w ? (zk_i32_linear_workspace(rows, w->N) + 15) / 16 * 16 + expanded(w) : 0;
+    return w ? (zk_i32_linear_workspace(rows, w->N) + 15) / 16 * 16 + expanded(w, rows) : 0;
 }
 size_t zk_i32_linear_workspace(uint32_t rows, uint32_t inner) {
     const size_t Kp = ((size_t)inner + GBK - 1) / GBK * GBK;
@@ -1246,7 +1514,7 @@ int zk_i32_gated(void* out, const void* x, size_t ldx, const void* gate_prepared
     if (const int rc = check_weight(gate, "zk_i32_gated")) return rc;
     if (const int rc = check_weight(w, "zk_i32_gated")) return rc;
     ZK_ARG(w->N == gate->N && w->P == gate->P, "zk_i32_gated: the two projections have different shapes");
-    ZK_ARG((w->q4 == nullptr) == (gate->q4 == nullptr), "zk_i32_gated: one weight of 4 bits and one that is none");
+    ZK_ARG((w->q4 == nullptr) == (gate->q4 == nullptr) && w->group == gate->group, "zk_i32_gated: one weight of 4 bits and one that is none, or with other groups");
     ZK_ARG(sf_gate > 0 && sf_up > 0 && sf_hidden > 0, "zk_i32_gated: a scaling factor of 0");
     ZK_ARG(table != nullptr && len > 0, "zk_i32_gated: no table of function values");
     if (rows == 0) return 0;
