@@ -998,12 +998,13 @@ template <bool GATED, int R, int WAVES> __global__ void __launch_bounds__(64 * W
     }
     raise(g.e.flag, bad);
 }
-// 5 to 32 rows: S strips by 8 / S shares of the inner dimension a workgroup, 128 inner rows at a time; x's planes, which the strips share, go to LDS as fragments a step ahead.
+// 5 to 32 rows: S strips by 8 / S shares of the inner dimension a workgroup, 128 inner rows a step; x's planes, which the strips share, go to LDS as fragments and codes to registers up to three
+// steps ahead.
 template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k_q4_strip(const Q4Args a) {
-    constexpr int MATS = GATED ? 2 : 1, SHARES = 8 / S, PIECES = SHARES * 2 * RT * 4, EACH = PIECES / 8;
+    constexpr int MATS = GATED ? 2 : 1, SHARES = 8 / S, PIECES = SHARES * 2 * RT * 4, EACH = PIECES / 8, BUFS = SHARES * RT <= 4 ? 4 : 2, LOADS = EACH + 3 * MATS;
+    typedef int8_t Buffer[SHARES][2][RT][4][1024];         // [share][64 inner rows][16 rows][digit]
     // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
-    __shared__ __attribute__((aligned(16))) int8_t x0[SHARES][2][RT][4][1024], x1[SHARES][2][RT][4][1024];      // [share][64 inner rows][16 rows][digit]
-    __shared__ unsigned long long sums[MATS][2][RT * 16][S * 16];
+    __shared__ __attribute__((aligned(16))) Buffer x0, x1, x2, x3;
     const ProductArgs& g = a.g;
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4, share = wave / S, in = wave % S;
     const uint32_t strips = (a.w.cols + 15) / 16, strip = min(blockIdx.x * S + in, strips - 1), pairs = a.w.units >> 1, steps = (pairs + SHARES - 1) / SHARES;
@@ -1011,24 +1012,41 @@ template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k
     for (uint32_t i = lane; i < g.chunks; i += 64) need = max(need, g.need[i]);
     const bool four = __any(need > 3);
     const size_t plane = (size_t)g.rows_padded * g.w.Kp;
-    for (uint32_t i = threadIdx.x; i < sizeof(sums) / 8; i += 512) (&sums[0][0][0][0])[i] = 0;
-    auto fetch = [&](uint32_t step, auto& x) {             // this wave's pieces of a step
+    struct Loaded { uint4 codes; int32_t scale[2]; } w[BUFS][MATS];
+    // what of a step's places is the same for all steps
+    const uint32_t lane_codes = lane * 16, lane_x = ((q >> 1) * g.rows_padded + c) * 32 + (q & 1u) * 16, pair_x = 4 * g.rows_padded * 32;
+    const char *codes[MATS], *scales[MATS];
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const uint32_t piece = wave * EACH + i, d = piece & 3u, r = piece >> 2 & (RT - 1u), u = (piece / (4 * RT)) & 1u, s = piece / (8 * RT), pair = min(step * SHARES + s, pairs - 1);
-            load_to_lds(g.px + d * plane + ((size_t)(pair * 4 + u * 2 + (q >> 1)) * g.rows_padded + r * 16 + c) * 32 + (q & 1u) * 16, &x[s][u][r][d][0]);
-        }
-    };
-    struct Loaded { uint4 codes; int32_t scale[2]; } w[2][MATS];
-    auto load = [&](uint32_t step, int d) {
-        const uint32_t pair = min(step * SHARES + share, pairs - 1);
+    for (int m = 0; m < MATS; ++m) {
+        const Q4& y = GATED && m == 0 ? a.gate : a.w;
+        codes[m] = (const char*)y.codes + (size_t)strip * pairs * 1024;
+        scales[m] = (const char*)(y.scales + (size_t)strip * y.groups * 16);
+    }
+    // a step's loads, LOADS of them whatever the step: behind the last one that again, never multiplied
+    auto fetch = [&](uint32_t step, int d, Buffer& x) {
+        const uint32_t mine = min(step * SHARES + share, pairs - 1);
+        const uint32_t group0 = min(a.w.shift >= 0 ? mine * 128 >> a.w.shift : mine * 128 / a.w.group, a.w.groups - 1), group1 = min(a.w.shift >= 0 ? (mine * 128 + 64) >> a.w.shift : (mine * 128 + 64) / a.w.group, a.w.groups - 1);
 #pragma unroll
         for (int m = 0; m < MATS; ++m) {
-            const Q4& x = GATED && m == 0 ? a.gate : a.w;
-            w[d][m].codes = *reinterpret_cast<const uint4*>(x.codes + (((size_t)strip * pairs + pair) * 64 + lane) * 4);
-            w[d][m].scale[0] = q4_scale(x, strip, pair * 128, c);
-            w[d][m].scale[1] = q4_scale(x, strip, pair * 128 + 64, c);
+            w[d][m].codes = *reinterpret_cast<const uint4*>(codes[m] + (size_t)mine * 1024 + lane_codes);
+            w[d][m].scale[0] = *reinterpret_cast<const int32_t*>(scales[m] + (size_t)group0 * 64 + c * 4);
+            w[d][m].scale[1] = *reinterpret_cast<const int32_t*>(scales[m] + (size_t)group1 * 64 + c * 4);
         }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const uint32_t piece = wave * EACH + i, p = piece & 3u, r = piece >> 2 & (RT - 1u), u = (piece / (4 * RT)) & 1u, s = piece / (8 * RT), pair = min(step * SHARES + s, pairs - 1);
+            load_to_lds(g.px + p * plane + ((size_t)(u * 2) * g.rows_padded + r * 16) * 32 + (size_t)pair * pair_x + lane_x, &x[s][u][r][p][0]);
+        }
+    };
+    // A step's pieces are in LDS when of every wave's loads only those of younger steps are on their way, and all waves are past the barrier; the buffer read last is free then
+    auto arrived = [&] {
+        constexpr int N = (BUFS - 2) * LOADS;
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 7 << 4);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
     };
     int64_t acc[MATS][RT][2][4];                           // digits 0 and 1, digits 2 and 3
 #pragma unroll
@@ -1037,60 +1055,95 @@ template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k
         for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[m][r][e >> 2][e & 3] = 0;
-    const bool both = a.w.group % 128 == 0 && (!GATED || a.gate.group % 128 == 0);      // 128 inner rows have one scale
-    auto multiply = [&](uint32_t step, int d, auto& x) {
+    const bool both = a.w.group % 128 == 0;                // 128 inner rows have one scale
+    auto multiply = [&](uint32_t step, int d, const Buffer& x) {
         if (step * SHARES + share >= pairs) return;
+        v4i b[MATS][2];
 #pragma unroll
         for (int m = 0; m < MATS; ++m) {
-            v4i b[2] = {q4_codes_less(make_uint2(w[d][m].codes.x, w[d][m].codes.y), w[d][m].scale[0]), q4_codes_less(make_uint2(w[d][m].codes.z, w[d][m].codes.w), w[d][m].scale[1])};
+            b[m][0] = q4_codes_less(make_uint2(w[d][m].codes.x, w[d][m].codes.y), w[d][m].scale[0]);
+            b[m][1] = q4_codes_less(make_uint2(w[d][m].codes.z, w[d][m].codes.w), w[d][m].scale[1]);
+        }
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                v4i s[4];
-                auto add = [&](int32_t scale) {
+        for (int r = 0; r < RT; ++r) {
+            v4i s[MATS][4];
+            auto products = [&](int u, int i, bool first) {
+                const v4i f = *reinterpret_cast<const v4i*>(&x[share][u][r][i][lane * 16]);
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) s[m][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f, b[m][u], first ? v4i{0, 0, 0, 0} : s[m][i], 0, 0, 0);
+            };
+            auto add = [&](int u) {
+#pragma unroll
+                for (int m = 0; m < MATS; ++m) {
+                    const int32_t scale = w[d][m].scale[u] >> 4;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        acc[m][r][0][e] += (int64_t)(s[0][e] + s[1][e] * 256) * scale;
-                        acc[m][r][1][e] += (int64_t)(s[2][e] + (four ? s[3][e] * 256 : 0)) * scale;
+                        acc[m][r][0][e] += (int64_t)(s[m][0][e] + s[m][1][e] * 256) * scale;
+                        acc[m][r][1][e] += (int64_t)s[m][2][e] * scale;
                     }
-                };
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 3; ++i) products(0, i, true);
+            if (both) {
+#pragma unroll
+                for (int i = 0; i < 3; ++i) products(1, i, false);
+            } else {
+                add(0);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) products(1, i, true);
+            }
+            add(1);
+            if (four)                                      // a value of four digits among the rows
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    if (u == 0 || !both)
+                    products(u, 3, true);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[i] = v4i{0, 0, 0, 0};
+                    for (int m = 0; m < MATS; ++m)
 #pragma unroll
-                    for (int i = 0; i < 3; ++i) s[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(&x[share][u][r][i][lane * 16]), b[u], s[i], 0, 0, 0);
-                    if (four) s[3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const v4i*>(&x[share][u][r][3][lane * 16]), b[u], s[3], 0, 0, 0);
-                    if (u == 0 && !both) add(w[d][m].scale[0] >> 4);
+                        for (int e = 0; e < 4; ++e) acc[m][r][1][e] += (int64_t)(s[m][3][e] * 256) * (w[d][m].scale[u] >> 4);
                 }
-                add(w[d][m].scale[1] >> 4);
-            }
         }
     };
-    fetch(0, x0);
-    load(0, 0);
-    for (uint32_t t = 0; t < steps; t += 2) {
-        __syncthreads();                                   // the step's pieces are there, and the other buffer is read
-        if (t + 1 < steps) { fetch(t + 1, x1); load(t + 1, 1); }
-        multiply(t, 0, x0);
-        if (t + 1 >= steps) break;
-        __syncthreads();
-        if (t + 2 < steps) { fetch(t + 2, x0); load(t + 2, 0); }
-        multiply(t + 1, 1, x1);
+    fetch(0, 0, x0);
+    if constexpr (BUFS == 4) { fetch(1, 1, x1); fetch(2, 2, x2); }
+    for (uint32_t t = 0; t < steps; t += BUFS) {
+        if constexpr (BUFS == 4) {
+            arrived(); fetch(t + 3, 3, x3); multiply(t, 0, x0);
+            arrived(); fetch(t + 4, 0, x0); multiply(t + 1, 1, x1);
+            arrived(); fetch(t + 5, 1, x1); multiply(t + 2, 2, x2);
+            arrived(); fetch(t + 6, 2, x2); multiply(t + 3, 3, x3);
+        } else {
+            arrived(); fetch(t + 1, 1, x1); multiply(t, 0, x0);
+            arrived(); fetch(t + 2, 0, x0); multiply(t + 1, 1, x1);
+        }
     }
+    __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);          // vmcnt 0: no load into LDS outlives the workgroup or meets the sums
+    __syncthreads();
+    // the shares' sums, each weight's where a buffer was
+    typedef unsigned long long Sums[2][RT * 16][S * 16];
+    static_assert(sizeof(Sums) <= sizeof(Buffer), "a weight's sums take a buffer's place");
+    Sums& sums0 = *reinterpret_cast<Sums*>(&x0);
+    Sums& sums1 = *reinterpret_cast<Sums*>(&x1);
+    for (uint32_t i = threadIdx.x; i < sizeof(Sums) / 8; i += 512) {
+        (&sums0[0][0][0])[i] = 0;
+        if constexpr (GATED) (&sums1[0][0][0])[i] = 0;
+    }
+    __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MATS; ++m)
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) atomicAdd(&sums[m][e >> 2][r * 16 + 4 * q + (e & 3)][in * 16 + c], (unsigned long long)acc[m][r][e >> 2][e & 3]);
+        for (int e = 0; e < 8; ++e) {
+            atomicAdd(&sums0[e >> 2][r * 16 + 4 * q + (e & 3)][in * 16 + c], (unsigned long long)acc[0][r][e >> 2][e & 3]);
+            if constexpr (GATED) atomicAdd(&sums1[e >> 2][r * 16 + 4 * q + (e & 3)][in * 16 + c], (unsigned long long)acc[1][r][e >> 2][e & 3]);
+        }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < RT * 16 * S * 16; i += 512) {
         const uint32_t row = i / (S * 16), x = i % (S * 16), col = blockIdx.x * S * 16 + x;
         if (row >= g.rows || col >= g.cols) continue;
         int64_t v[MATS];
-#pragma unroll
-        for (int m = 0; m < MATS; ++m) v[m] = q4_joined((int64_t)sums[m][0][row][x], (int64_t)sums[m][1][row][x], bad);
+        v[0] = q4_joined((int64_t)sums0[0][row][x], (int64_t)sums0[1][row][x], bad);
+        if constexpr (GATED) v[1] = q4_joined((int64_t)sums1[0][row][x], (int64_t)sums1[1][row][x], bad);
         q4_output<GATED>(g, row, col, v, bad);
     }
     raise(g.e.flag, bad);
