@@ -573,7 +573,7 @@ size_t zk_i32_logits_workspace(uint32_t rows, uint32_t vocab);
 /* Logits before a token is chosen, and the choice.  For a token that stands c > 0 times in its row's history, with the row's penalties (r, f, p), int32:  l -> (l > 0 ? the quotient of
  * l sf by r : the quotient of l r by sf) - f c - p;  then l -> l + the sum of the token's biases in its row's list;  then the lowest int32, -2^31, where its bit in the row's mask is 0 (bit t % 32 of word
  * t / 32).  A logit that is -2^31 stays so: such a token cannot be chosen.  token (int32, one a row): the largest, of equals the lowest token, -1 where none is left.
- * Row r's history is entries starts[r] .. starts[r + 1] - 1 of `history_len` (int32, rows + 1 starts), its biases likewise; each with its starts may be null.  penalties: rows x 3, r > 0.
+ * Row r's history is entries starts[r] .. starts[r + 1] - 1 of `history_len` (int32, rows + 1 starts), its biases likewise; each with its starts may be null.  penalties: rows x 3, r > 0, sf below 2^31.
  * mask: one row for all (mask_rows 1) or ld_mask words from row to row, or null and 0.  out may be logits with the same leading dimension, or null where only the token is wanted; token may be null.
  * Entries outside 0 .. vocab - 1 and lists outside their entries raise ZK_VALUES_POSITION and do not count; values that leave int32, or reach -2^31 by themselves, raise ZK_VALUES_RANGE. */
 int zk_i32_logits(void* out, size_t ld_out, void* token_i32, const void* logits, size_t ld, uint32_t rows, uint32_t vocab, const void* history_i32, uint32_t history_len,

@@ -847,7 +847,7 @@ def test_q4_refusals():
     ({"logits": None}, "null logits"), ({"out": None, "token": None}, "no output"), ({"vocab": 0}, "no tokens"), ({"ld": 9}, "rows overlap"), ({"ld_out": 9}, "rows overlap"), ({"vocab": (1 << 30) + 1}, "2^30 tokens"),
     ({"rows": 65536}, "65535 rows"), ({"out": "logits", "ld": 12}, "in place"), ({"history_starts": W}, "a history needs"), ({"history_starts": W, "history": W}, "a history needs"),
     ({"history": W}, "without starts"), ({"penalties": W}, "without starts"), ({"bias_starts": W, "bias_len": 3}, "biases need"), ({"bias_tokens": W}, "biases without starts"), ({"mask": W}, "a mask has"),
-    ({"mask": W, "mask_rows": 2}, "a mask has"), ({"mask_rows": 1}, "a mask has"), ({"mask": W, "mask_rows": 3, "ld_mask": 0}, "a mask has"), ({"sf": 0}, "a scaling factor of 0"),
+    ({"mask": W, "mask_rows": 2}, "a mask has"), ({"mask_rows": 1}, "a mask has"), ({"mask": W, "mask_rows": 3, "ld_mask": 0}, "a mask has"), ({"sf": 0}, "a scaling factor of 0"), ({"sf": 1 << 31}, "2^31 and more"),
     ({"bytes": 5, "workspace": 16, "vocab": 5000, "ld": 5000, "ld_out": 5000}, "the workspace is smaller"), ({"bytes": 64, "workspace": 8}, "multiple of 16"),
     ({"history_starts": W, "history": W, "penalties": W, "history_len": 1 << 31}, "2^31 - 1")])
 def test_logits_refusals(change, text):

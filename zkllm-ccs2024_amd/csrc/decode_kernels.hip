@@ -939,7 +939,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
 
 // ---- logits -------------------------------------------------------------------------------------------------------------------------------
 static constexpr int32_t NO_TOKEN = INT32_MIN;
-static constexpr uint32_t LOGITS_SPAN = 4096;    // a workgroup's tokens
+static constexpr uint32_t LOGITS_THREADS = 512, LOGITS_SPAN = 4096;      // a workgroup's lanes and tokens
 struct TokenLists { const int32_t *tokens, *values, *starts; uint32_t total; };      // row r's: starts[r] .. starts[r + 1]
 struct LogitsArgs {
     int32_t *out, *token;
@@ -974,57 +974,85 @@ __device__ __forceinline__ unsigned long long block_best(unsigned long long best
     for (uint32_t i = 0; i < blockDim.x / 64; ++i) best = max(best, of_wave[i]);
     return best;
 }
-// A workgroup takes a stretch of a row: it reads the row's lists, counts and adds up in LDS what falls into the stretch, then passes over the logits once
-template <bool POW2> __global__ void __launch_bounds__(256) k_logits(const LogitsArgs a) {
+// A workgroup takes a stretch of a row, eight tokens a lane.  Its logits and mask are on their way while it reads the row's lists, eight entries a lane at a time, and counts and adds up in LDS what
+// falls into the stretch.  BIAS: there are biases.
+template <bool POW2, bool BIAS> __global__ void __launch_bounds__(LOGITS_THREADS) k_logits(const LogitsArgs a) {
+    constexpr int N = 8, T = LOGITS_THREADS;
+    static_assert(LOGITS_SPAN == N * T, "a stretch is eight tokens a lane");
     __shared__ uint32_t count[LOGITS_SPAN];
-    __shared__ unsigned long long add[LOGITS_SPAN];
-    __shared__ unsigned long long of_wave[4];
+    __shared__ unsigned long long add[BIAS ? LOGITS_SPAN : 1];
+    __shared__ unsigned long long of_wave[LOGITS_THREADS / 64];
     const uint32_t row = blockIdx.y, first = blockIdx.x * LOGITS_SPAN, n = min(LOGITS_SPAN, a.vocab - first);
     uint32_t bad = 0, from = 0, to = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) { count[i] = 0; add[i] = 0; }
+    const uint32_t* mask = a.mask ? a.mask + (a.mask_rows == 1 ? 0 : row) * a.ld_mask : nullptr;
+    const int32_t* in = a.logits + row * a.ld + first;
+    int32_t l[N];
+    uint32_t bits[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {                          // beyond the stretch its last
+        const uint32_t i = min(threadIdx.x + e * T, n - 1);
+        l[e] = in[i];
+        bits[e] = mask ? mask[(first + i) >> 5] : 0xFFFFFFFFu;
+    }
+    for (uint32_t i = threadIdx.x * 4; i < LOGITS_SPAN; i += T * 4) {
+        *reinterpret_cast<v4i*>(&count[i]) = v4i{0, 0, 0, 0};
+        if constexpr (BIAS) {
+            *reinterpret_cast<v4i*>(&add[i]) = v4i{0, 0, 0, 0};
+            *reinterpret_cast<v4i*>(&add[i + 2]) = v4i{0, 0, 0, 0};
+        }
+    }
     __syncthreads();
-    if (list_of(a.history, row, from, to, bad))
-        for (uint32_t i = from + threadIdx.x; i < to; i += 256) {
-            const uint32_t token = (uint32_t)a.history.tokens[i];
-            if (token >= a.vocab) bad |= ZK_VALUES_POSITION;
-            else if (token - first < n) atomicAdd(&count[token - first], 1u);
+    auto list = [&](const TokenLists& lists, auto put) {
+        if (!list_of(lists, row, from, to, bad)) return;
+        for (uint32_t i0 = from + threadIdx.x; i0 < to; i0 += T * N) {
+            uint32_t token[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) token[e] = (uint32_t)lists.tokens[min(i0 + e * T, to - 1)];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const uint32_t i = i0 + e * T;
+                if (i >= to) continue;
+                bad |= token[e] >= a.vocab ? (uint32_t)ZK_VALUES_POSITION : 0u;
+                if (token[e] - first < n) put(token[e] - first, i);
+            }
         }
-    if (list_of(a.bias, row, from, to, bad))
-        for (uint32_t i = from + threadIdx.x; i < to; i += 256) {
-            const uint32_t token = (uint32_t)a.bias.tokens[i];
-            if (token >= a.vocab) bad |= ZK_VALUES_POSITION;
-            else if (token - first < n) atomicAdd(&add[token - first], (unsigned long long)(int64_t)a.bias.values[i]);
-        }
+    };
+    list(a.history, [&](uint32_t at, uint32_t) { atomicAdd(&count[at], 1u); });
+    if constexpr (BIAS) list(a.bias, [&](uint32_t at, uint32_t i) { atomicAdd(&add[at], (unsigned long long)(int64_t)a.bias.values[i]); });
     __syncthreads();
     int32_t repeat = 0, frequency = 0, presence = 0;
     if (a.penalties) {
         repeat = a.penalties[3 * (size_t)row]; frequency = a.penalties[3 * (size_t)row + 1]; presence = a.penalties[3 * (size_t)row + 2];
         if (repeat <= 0) { bad |= ZK_VALUES_RANGE; repeat = 1; }
     }
-    const uint32_t* mask = a.mask ? a.mask + (a.mask_rows == 1 ? 0 : row) * a.ld_mask : nullptr;
-    const int32_t* in = a.logits + row * a.ld;
-    unsigned long long best = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += 256) {
+    const Divisor by_repeat{repeat, repeat >> 1, 1.0 / (double)repeat, -1};
+    int32_t most = NO_TOKEN;
+    uint32_t most_at = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const uint32_t i = threadIdx.x + e * T;
+        if (i >= n) continue;
         const uint32_t token = first + i, c = count[i];
-        int32_t l = in[token];
-        if (mask && (mask[token >> 5] >> (token & 31u) & 1u) == 0) l = NO_TOKEN;
-        if (l != NO_TOKEN && (c != 0 || add[i] != 0)) {
-            int64_t v = l;
+        if ((bits[e] >> (token & 31u) & 1u) == 0) l[e] = NO_TOKEN;
+        bool changed = c != 0;
+        if constexpr (BIAS) changed |= add[i] != 0;
+        if (changed && l[e] != NO_TOKEN) {
+            int64_t v = l[e];
             if (c != 0 && a.penalties) {
-                if (v > 0) v = (v * a.sf.s + (repeat >> 1)) / repeat;
+                if (v > 0) v = quotient_general(v * a.sf.s, by_repeat);
                 else v = quotient<POW2>(v * repeat, a.sf);
                 v = narrow(v, bad);
                 v -= narrow((int64_t)frequency * c + presence, bad);
             }
-            v += narrow((int64_t)add[i], bad);
-            l = narrow(v, bad);
-            if (l == NO_TOKEN) bad |= ZK_VALUES_RANGE;
+            if constexpr (BIAS) v += narrow((int64_t)add[i], bad);
+            l[e] = narrow(v, bad);
+            if (l[e] == NO_TOKEN) bad |= ZK_VALUES_RANGE;
         }
-        if (a.out) a.out[row * a.ld_out + token] = l;
-        best = max(best, choice(l, token));
+        if (a.out) a.out[row * a.ld_out + token] = l[e];
+        if (l[e] > most) { most = l[e]; most_at = token; }             // tokens ascend: the first of equals
     }
     if (a.token) {
-        best = block_best(best, of_wave);
+        const unsigned long long best = block_best(choice(most, most_at), of_wave);
         if (threadIdx.x == 0) {
             if (a.spans == 1) a.token[row] = chosen(best);
             else a.best[(size_t)row * a.spans + blockIdx.x] = best;
@@ -1330,7 +1358,7 @@ int zk_i32_logits(void* out, size_t ld_out, void* token, const void* logits, siz
     ZK_ARG(bias_starts != nullptr || (bias_tokens == nullptr && bias_values == nullptr), std::string(name) + ": biases without starts");
     ZK_ARG(history_len <= 0x7FFFFFFFu && bias_len <= 0x7FFFFFFFu, std::string(name) + ": a list of more than 2^31 - 1 tokens");
     ZK_ARG(mask == nullptr ? mask_rows == 0 : (mask_rows == 1 || (mask_rows == rows && ld_mask >= (vocab + 31) / 32)), std::string(name) + ": a mask has one row or a row for each of the logits'");
-    ZK_ARG(sf > 0, std::string(name) + ": a scaling factor of 0");
+    ZK_ARG(sf > 0 && sf <= 0x7FFFFFFFu, std::string(name) + ": a scaling factor of 0 or of 2^31 and more");
     hipStream_t st = (hipStream_t)stv;
     const size_t bytes = token ? zk_i32_logits_workspace(rows, vocab) : 0;
     ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_logits_workspace says");
@@ -1349,8 +1377,11 @@ int zk_i32_logits(void* out, size_t ld_out, void* token, const void* logits, siz
                        TokenLists{(const int32_t*)history, nullptr, (const int32_t*)history_starts, history_len},
                        TokenLists{(const int32_t*)bias_tokens, (const int32_t*)bias_values, (const int32_t*)bias_starts, bias_len}, (const int32_t*)penalties, (const uint32_t*)mask, ld_mask, mask_rows,
                        divisor(sf), (unsigned long long*)workspace, flag.dev};
-    if (a.sf.shift >= 0) hipLaunchKernelGGL(k_logits<true>, dim3(spans, rows), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(k_logits<false>, dim3(spans, rows), dim3(256), 0, st, a);
+    const bool bias = bias_starts != nullptr && bias_len > 0;
+    if (a.sf.shift >= 0 && bias) hipLaunchKernelGGL((k_logits<true, true>), dim3(spans, rows), dim3(LOGITS_THREADS), 0, st, a);
+    else if (a.sf.shift >= 0) hipLaunchKernelGGL((k_logits<true, false>), dim3(spans, rows), dim3(LOGITS_THREADS), 0, st, a);
+    else if (bias) hipLaunchKernelGGL((k_logits<false, true>), dim3(spans, rows), dim3(LOGITS_THREADS), 0, st, a);
+    else hipLaunchKernelGGL((k_logits<false, false>), dim3(spans, rows), dim3(LOGITS_THREADS), 0, st, a);
     if (token && spans > 1) hipLaunchKernelGGL(k_logits_best, dim3(rows), dim3(64), 0, st, (int32_t*)token, (const unsigned long long*)workspace, spans);
     ZK_LAUNCH_CHECK();
     return flag.end(name);
