@@ -21,9 +21,13 @@ FrTensor IntTensor::to_fr() const {
 }
 
 ValuesFlag::ValuesFlag() : buf(4) { ZKC(zk_i32_fill(buf.p, 0, 1, nullptr)); }
+uint32_t ValuesFlag::bits() const {
+    uint32_t b = 0;
+    ZKC(zk_memcpy_d2h(&b, buf.p, 4, nullptr));
+    return b;
+}
 void ValuesFlag::check(const char* what) const {
-    uint32_t bits = 0;
-    ZKC(zk_memcpy_d2h(&bits, buf.p, 4, nullptr));
+    const uint32_t bits = this->bits();
     if (bits & ZK_VALUES_TABLE) throw std::runtime_error(string(what) + ": an activation lies outside the table of function values");
     if (bits & ZK_VALUES_POSITION) throw std::runtime_error(string(what) + ": a position lies outside the table of angles");
     if (bits) throw std::runtime_error(string(what) + ": a value does not fit");

@@ -24,6 +24,7 @@ class ValuesFlag {
    public:
     ValuesFlag();
     void* dev() const { return buf.p; }
+    uint32_t bits() const;                         // waits
     void check(const char* what) const;            // waits; throws when a bit is raised
 
    private:

@@ -22,6 +22,9 @@ class LayerValues {
     struct Rhs { const void* prepared = nullptr; bool own = false; };
     Rhs q, k, v, o, up, gate, down;
     IntTensor input_norm, post_norm, act;
+    void* softmax = nullptr;       // null where the heads or the softmax are none that zk_i32_attention takes: the proof's own forward pass then
     Rhs rhs(const FrTensor& weight, uint in_dim, uint out_dim);
+    IntTensor run(const IntTensor& X, const ValuesFlag* scores) const;
+    void proof_attention(IntTensor& out, const IntTensor& normed, uint tokens, const ValuesFlag& flag, void* ws, size_t room) const;
     void release();
 };
