@@ -740,8 +740,8 @@ def test_steps_eager_and_captured(hip, S):
 def test_captured_calls_need_their_own_memory(hip):
     import torch
     rng = np.random.default_rng(2)
-    plan, own, w = Plan(hip, dec.Softmax(dim=8)), Pages(rng, 1, 40, 1, 8, 16), Q4(hip, rng, 64, 16, 32)
-    q, lengths, l = dev(normal(rng, (1, 1, 8))), dev([40]), normal(rng, (1, 5000))
+    plan, own, w = Plan(hip, dec.Softmax(dim=8)), Pages(rng, 1, 3000, 1, 8, 16), Q4(hip, rng, 64, 16, 32)
+    q, lengths, l = dev(normal(rng, (1, 1, 8))), dev([3000]), normal(rng, (1, 5000))
     stream, g, flag = torch.cuda.Stream(), torch.cuda.CUDAGraph(), new_flag()
     x, out, dl = dev(normal(rng, (6, 64))), dev(np.zeros((6, 16))), dev(l)
     oc = own.c()
@@ -755,7 +755,7 @@ def test_captured_calls_need_their_own_memory(hip):
 
         for f, ws in ((None, dl), (flag, None)):
             refused("zk_i32_attention", ptr(q), c_size_t(8), c_size_t(8), ptr(q), c_size_t(8), c_size_t(8), c_uint(1), c_uint(1), c_uint(1), c_uint(8), plan.h, None, c_uint(0), ctypes.byref(oc), c_uint(1), None,
-                    ptr(lengths), c_uint(40), c_int(1), c_uint(1), c_uint(1), None, ptr(ws), c_size_t(1 << 20 if ws is not None else 0), ptr(f), st)
+                    ptr(lengths), c_uint(3000), c_int(1), c_uint(1), c_uint(1), None, ptr(ws), c_size_t(1 << 20 if ws is not None else 0), ptr(f), st)
             refused("zk_i32_linear", ptr(out), ptr(x), c_size_t(64), w.h, c_uint(6), c_uint(1), ptr(ws), c_size_t(1 << 20 if ws is not None else 0), ptr(f), st)
             refused("zk_i32_logits", ptr(dl), c_size_t(5000), ptr(out), ptr(dl), c_size_t(5000), c_uint(1), c_uint(5000), None, c_uint(0), None, None, None, None, c_uint(0), None, None, c_size_t(0), c_uint(0),
                     c_uint(1), ptr(ws), c_size_t(1 << 20 if ws is not None else 0), ptr(f), st)

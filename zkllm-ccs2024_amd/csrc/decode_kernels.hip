@@ -198,38 +198,42 @@ template <uint32_t ROWS> __device__ __forceinline__ bool tile_at(const AttnArgs&
     t.keys = own_seen(a, t.s, (t.hi - 1) / a.group);
     return true;
 }
-// 16 of a head's values as digit planes: four runs of four, 16 apart, so that four lanes read 64 bytes in one piece.  Which 16 of 64 a lane has is the same for queries and keys.
-template <bool VEC> __device__ __forceinline__ void head_piece(const int32_t* p, uint32_t d0, uint32_t dim, int32_t (&x)[16]) {
+// How heads are read: an element at a time, four at a time, or four at a time with all 64 dimensions of every block there
+enum class Heads { ANY, FOURS, BLOCKS };
+// 16 of a head's values for its digit planes: four runs of four, 16 apart, so that four lanes read 64 bytes in one piece.  Which 16 of 64 a lane has is the same for queries and keys.  Beyond
+// the head's end queries are zeros (ZEROS), keys anything.
+template <Heads HEADS, bool ZEROS> __device__ __forceinline__ void head_piece(const int32_t* p, uint32_t d0, uint32_t dim, int32_t (&x)[16]) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         const uint32_t d = d0 + 16 * w;
-        if constexpr (VEC) {
-            v4i v = {0, 0, 0, 0};
-            if (d < dim) v = *reinterpret_cast<const v4i*>(p + d);
+        if constexpr (HEADS == Heads::ANY) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * w + e] = v[e];
+            for (int e = 0; e < 4; ++e) {
+                const int32_t v = p[min(d + e, dim - 1)];
+                x[4 * w + e] = ZEROS && d + e >= dim ? 0 : v;
+            }
         } else {
+            const v4i v = *reinterpret_cast<const v4i*>(p + (HEADS == Heads::BLOCKS ? d : min(d, dim - 4)));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * w + e] = d + e < dim ? p[d + e] : 0;
+            for (int e = 0; e < 4; ++e) x[4 * w + e] = ZEROS && HEADS == Heads::FOURS && d >= dim ? 0 : v[e];
         }
     }
+}
+// four neighbouring dimensions from d on, beyond the head's end anything
+template <Heads HEADS> __device__ __forceinline__ v4i four_of(const int32_t* p, uint32_t d, uint32_t dim) {
+    if constexpr (HEADS == Heads::ANY) return v4i{p[min(d, dim - 1)], p[min(d + 1, dim - 1)], p[min(d + 2, dim - 1)], p[min(d + 3, dim - 1)]};
+    else return *reinterpret_cast<const v4i*>(p + (HEADS == Heads::BLOCKS ? d : min(d, dim - 4)));
 }
 __device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v[2] | v[3]) != 0; }
 
 // Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8.  The next keys are
 // on their way while these are multiplied, and the place of those behind them is looked up.
-template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
-    uint32_t bad = 0;
-    Tile t;
-    if ((blockIdx.x | blockIdx.y | blockIdx.z | threadIdx.x) == 0) *a.unsure = 0;
-    if (!tile_at<16 * RT>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
-    const uint32_t key0 = blockIdx.x * a.score_keys;
-    if (key0 >= t.keys) return;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z, end = min(key0 + a.score_keys, t.keys);
+template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, int64_t* out, size_t ld, uint32_t& bad) {
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
     auto query = [&](int r, int u, v4i (&d)[4]) {
         const uint32_t row = t.has(16 * r + c) ? t.row0 + 16 * r + c : t.lo, token = row / a.group, head = kv * a.group + (row - token * a.group);
         int32_t x[16];
-        head_piece<VEC>(a.q + token * a.q_token + head * a.q_head, u * 64 + q * 4, a.dim, x);
+        head_piece<HEADS, true>(a.q + token * a.q_token + head * a.q_head, u * 64 + q * 4, a.dim, x);
         digit_planes(x, d, bad);
     };
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
@@ -238,15 +242,15 @@ template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, 2) k_a
     int32_t x[U][16];
     auto fetch = [&](const int32_t* p) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) head_piece<VEC>(p, u * 64 + q * 4, a.dim, x[u]);
+        for (int u = 0; u < U; ++u) head_piece<HEADS, false>(p, u * 64 + q * 4, a.dim, x[u]);
     };
-    uint32_t key = key0 + wave * 16;
+    uint32_t key = first + wave * 16;
     if (key < end) fetch(place(key));
-    const int32_t* next = place(key + 64);
+    const int32_t* next = place(key + WAVES * 16);
     v4i b[RT][U][3];
     bool wide = false;
 #pragma unroll
-    for (int r = 0; r < RT; ++r)
+    for (int r = 0; r < RT; ++r) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             v4i d[4];
@@ -255,9 +259,11 @@ template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, 2) k_a
             for (int m = 0; m < 3; ++m) b[r][u][m] = d[m];
             wide |= any_bits(d[3]);
         }
+        if (r % 2 == 1) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
+    }
     const bool q_wide = __any(wide);
-    int64_t* out = a.scores + ((size_t)blockIdx.z * a.tokens * a.group + t.row0 + c) * a.ld + t.col0 + 4 * q;
-    for (; key < end; key += 64) {
+    int64_t* const to0 = out + c * ld + 4 * q;
+    for (; key < end; key += WAVES * 16) {
         v4i k[U][4];
         bool k_wide = false;
 #pragma unroll
@@ -265,50 +271,63 @@ template <int U, int RT, bool VEC> __global__ void __launch_bounds__(256, 2) k_a
             digit_planes(x[u], k[u], bad);
             k_wide |= any_bits(k[u][3]);
         }
-        if (key + 64 < end) fetch(next);
-        next = place(key + 128);
+        if (key + WAVES * 16 < end) fetch(next);
+        next = place(key + 2 * WAVES * 16);
         const bool four = q_wide || __any(k_wide);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-            v4i acc[7];
+            v4i acc[5];
 #pragma unroll
-            for (int s = 0; s < 7; ++s) acc[s] = v4i{0, 0, 0, 0};
+            for (int s = 0; s < 5; ++s) acc[s] = v4i{0, 0, 0, 0};
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int m = 0; m < 3; ++m)
 #pragma unroll
                     for (int n = 0; n < 3; ++n) acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][n], acc[m + n], 0, 0, 0);
-            if (four) {
+            int64_t v[4];                                  // key 4 q + e of the tile, row c
+            if (!four) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (U <= 2) v[e] = (int64_t)(acc[0][e] + acc[1][e] * 256) + ((int64_t)(acc[2][e] + acc[3][e] * 256) << 16) + ((int64_t)acc[4][e] << 32);      // two products of 2^14 in 128 dimensions
+                    else v[e] = acc[0][e] + (int64_t)acc[1][e] * 256 + (acc[2][e] + (int64_t)acc[3][e] * 256) * 65536 + ((int64_t)acc[4][e] << 32);
+                }
+            } else {
+                v4i more[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};      // of 256^4 on, but for 256^3
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     v4i d[4];
                     query(r, u, d);                        // a fourth digit is rare: the queries' is not kept
 #pragma unroll
                     for (int m = 0; m < 3; ++m) {
-                        acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], d[3], acc[m + 3], 0, 0, 0);
-                        acc[m + 3] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][m], acc[m + 3], 0, 0, 0);
+                        v4i& to = m == 0 ? acc[3] : m == 1 ? more[0] : more[1];
+                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], d[3], to, 0, 0, 0);
+                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][m], to, 0, 0, 0);
                     }
-                    acc[6] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], d[3], acc[6], 0, 0, 0);
+                    more[2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], d[3], more[2], 0, 0, 0);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int32_t s[7] = {acc[0][e], acc[1][e], acc[2][e], acc[3][e], acc[4][e] + more[0][e], more[1][e], more[2][e]};
+                    v[e] = joined<7>(s, bad);
                 }
             }
             if (!t.has(16 * r + c)) continue;
-            int64_t v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {                  // key 4 q + e of the tile, row c
-                if (four) {
-                    int32_t s[7];
-#pragma unroll
-                    for (int m = 0; m < 7; ++m) s[m] = acc[m][e];
-                    v[e] = joined<7>(s, bad);
-                } else v[e] = (int64_t)acc[0][e] + (int64_t)acc[1][e] * 256 + ((int64_t)(acc[2][e] + acc[3][e] * 256) << 16) + ((int64_t)acc[4][e] << 32);
-            }
             typedef long long v2l __attribute__((ext_vector_type(2)));
-            v2l* to = reinterpret_cast<v2l*>(out + 16 * r * a.ld + key);
+            v2l* to = reinterpret_cast<v2l*>(to0 + 16 * r * ld + key);
             to[0] = v2l{v[0], v[1]};
             to[1] = v2l{v[2], v[3]};
         }
     }
+}
+template <int U, int RT, Heads HEADS> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
+    uint32_t bad = 0;
+    Tile t;
+    if ((blockIdx.x | blockIdx.y | blockIdx.z | threadIdx.x) == 0) *a.unsure = 0;
+    if (!tile_at<16 * RT>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t key0 = blockIdx.x * a.score_keys;
+    if (key0 >= t.keys) return;
+    scores_of<U, RT, HEADS, 4>(a, t, a.kv0 + blockIdx.z, key0, min(key0 + a.score_keys, t.keys), a.scores + ((size_t)blockIdx.z * a.tokens * a.group + t.row0) * a.ld + t.col0, a.ld, bad);
     raise(a.flag, bad);
 }
 
@@ -493,165 +512,169 @@ template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x
     }
     return t;
 }
-// W waves a row, eight neighbouring keys a lane at a time, C times in its registers.  The sum of exponentials is taken in no order first, from exponentials that are near: off from the sum in
+// W waves a row, eight neighbouring keys a lane at a time.  The sum of exponentials is taken in no order first, from exponentials that are near: off from the sum in
 // order by at most (keys + 64) 2^-53 of it and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 40 at 2048 keys and
 // a scale of 2^32 sqrt(128)); then the sum in order is taken -- by a launch of its own for such rows, where there are many rows --, the waves' runs at once where the sum stays within a power of
 // two, and the few others one after the other.
-template <int W, int C, Weights KIND, Sums SUMS> __global__ void __launch_bounds__(W > 4 ? 64 * W : 256, SUMS == Sums::NEAR ? 4 : 1) k_attn_softmax(const AttnArgs a) {
-    constexpr int M = 8, T = 64 * W, ROWS = W > 4 ? 1 : 4 / W;      // a workgroup's rows at a time
-    static_assert(W == 1 || ROWS == 1, "waves that share a row meet at the workgroup's barriers");
-    extern __shared__ int32_t live[];
-    __shared__ double sums[W], power[64];
-    __shared__ Steps steps[W];
-    __shared__ int at_exponent[W];
-    __shared__ double in_order;
-    __shared__ uint32_t any_top;
-    const uint32_t rows = a.tokens * a.group, all = a.heads_here * rows, lane = threadIdx.x & 63u, wave = W == 1 ? 0 : threadIdx.x >> 6, tid = wave * 64 + lane;
-    const SoftmaxArgs& s = a.softmax;
-    uint32_t bad = 0;
+template <int W> struct RowShared { double sums[W], in_order; Steps steps[W]; int at_exponent[W]; uint32_t any_top; };
+// A row's scores x to its weights, zeros up to `fill`; ld from digit to digit.  false: its sum must be taken in order (SUMS NEAR)
+template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softmax_row(const SoftmaxArgs& s, const int64_t* x, int8_t* weights, size_t ld, const Columns& columns, uint32_t fill,
+                                                                                      const int32_t* live, const double* power, RowShared<W>& sh, int64_t& shift, bool& top, uint32_t& bad) {
+    constexpr int M = 8, T = 64 * W;
+    const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0 : threadIdx.x >> 6, tid = wave * 64 + lane;
+    const uint32_t stretches = (columns.end + T * M - 1) / (T * M);
+    int64_t v[M];
+    uint32_t n = 0;
+    auto load = [&](uint32_t stretch) {
+        const uint32_t j = stretch * T * M + tid * M;
+        n = columns.keys_at(j);
+#pragma unroll
+        for (int i = 0; i < M; ++i) v[i] = NO_KEY;
+        if (n) {
+            typedef long long v2l __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int i = 0; i < M; i += 2) {
+                const v2l p = *reinterpret_cast<const v2l*>(x + j + i);
+                v[i] = p[0]; v[i + 1] = p[1];
+            }
+            if (n < M)
+#pragma unroll
+                for (int i = 1; i < M; ++i) v[i] = i < (int)n ? v[i] : NO_KEY;
+        }
+    };
+    auto rounded = [](double sv) { return sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5); };
+    shift = 0;
+    bool sure = columns.end == 0, loaded = false;
+    if constexpr (SUMS != Sums::IN_ORDER) {
+        double total = 0.0;
+        for (uint32_t i = 0; i < stretches; ++i) {
+            load(i);
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                total += exp_near(v[e], s, power);
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
+            }
+        }
+        loaded = stretches == 1;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+        if constexpr (W > 1) {
+            __syncthreads();                           // the arrays' last use is over
+            if (lane == 0) sh.sums[wave] = total;
+            __syncthreads();
+            total = 0.0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) total += sh.sums[i];
+        }
+        if (columns.end) {
+            // Both sums' exponentials of x together are off by 8e-16 and 3.9e-16 |x|; weighted by what they have in the sum t, |x| is |ln t| + 17 at most (17: the logarithm of more keys than
+            // there can be).  Both logarithms are off by 4e-16 of them and their products with the scale by 2^-53.
+            const double ln = zkd::log_det(total), sv = s.scale * ln;
+            const double off = s.scale * ((double)(columns.end + 64) * 1.2e-16 + 1.5e-15 * fabs(ln) + 8e-15), from_border = fabs(sv - floor(sv) - 0.5);
+            sure = total > 1e-280 && total < 1e280 && off < 0.25 && from_border > off;
+            if (sure) shift = rounded(sv);
+        }
+        if constexpr (SUMS == Sums::NEAR)
+            if (!sure) return false;
+    }
+    if constexpr (SUMS != Sums::NEAR)
+        if (!sure) {
+            shift = rounded(s.scale * zkd::log_det(sum_in_order<W>(x, columns, s.scale, s.scale_inv, sh.sums, sh.steps, sh.at_exponent, &sh.in_order)));
+            loaded = false;                            // the registers were needed
+        }
+    // Both tables' values and their product are exact in double precision, and so is the number whose low 48 bits are the digits with 128 added to each
+    constexpr double BASE = 4503599627370496.0 + 141289400074368.0;
+    auto by_series = [&](int64_t score) {
+        const uint64_t below = (uint64_t)(shift - score);
+        const uint32_t lo = (uint32_t)below, hi = (uint32_t)(below >> 32), digit = lo >> s.drop_bits & (s.radix[0] - 1), upper = __builtin_amdgcn_alignbit(hi, lo, s.drop_bits + s.bits[0]);
+        const bool reached = hi < s.upper_end;         // neither negative nor too far
+        bad |= reached ? 0u : (uint32_t)ZK_VALUES_TABLE;
+        const double z = (double)digit;
+        const double u = fma_s(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, s.series[4], s.series[3]), s.series[2]), s.series[1]), s.series[0]);
+        double first = floor(u);
+        if (fabs(u - first - 0.5) > 0.5 - s.guard) first = (double)s.table[0][digit];      // nearer to a border than the terms left out
+        const int32_t second = live[min(upper, s.live - 1)];
+        return __builtin_fma(first, reached && upper < s.live ? (double)second : 0.0, BASE);
+    };
+    top = false;
+    const uint32_t fills = (fill + T * M - 1) / (T * M);
+    for (uint32_t i = 0; i < fills; ++i) {
+        if (!loaded || i != 0) load(i);
+        {
+            const uint32_t j = i * T * M + tid * M;
+            if (j >= fill) continue;
+            uint64_t d[M];
+            if (n < M)
+#pragma unroll
+                for (int e = 0; e < M; ++e) v[e] = e < (int)n ? v[e] : shift;
+#pragma unroll
+            for (int e = 0; e < M; ++e) {
+                if constexpr (KIND == Weights::SERIES) d[e] = zkd::double_to_bits(by_series(v[e])) ^ 0x808080808080ull;
+                else d[e] = ((uint64_t)softmax_weight<KIND == Weights::POW2>(shift - v[e], s, bad) + 0x808080808080ull) ^ 0x808080808080ull;
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+            if (n < M)
+#pragma unroll
+                for (int e = 0; e < M; ++e) d[e] = e < (int)n ? d[e] : 0;
+            Digits8 p;
+            digits8(d, p);
+            top |= (p.p[5].x | p.p[5].y) != 0;
+#pragma unroll
+            for (int k = 0; k < 6; ++k) *reinterpret_cast<uint2*>(weights + k * ld + j) = p.p[k];
+        }
+    }
+    return true;
+}
+// the tables of a workgroup of THREADS lanes
+template <int THREADS, Weights KIND> __device__ __forceinline__ void softmax_tables(const SoftmaxArgs& s, int32_t* live, double* power) {
     if constexpr (KIND == Weights::SERIES) {
 #pragma unroll 4
-        for (uint32_t i = threadIdx.x; i < s.live; i += T * ROWS) live[i] = s.table[1][i];
+        for (uint32_t i = threadIdx.x; i < s.live; i += THREADS) live[i] = s.table[1][i];
     }
     if (threadIdx.x < 64) power[threadIdx.x] = zkd::exp_det((double)threadIdx.x * (0.69314718055994530942 / 64.0));
+}
+template <int W, Weights KIND, Sums SUMS> __global__ void __launch_bounds__(W > 4 ? 64 * W : 256, SUMS == Sums::NEAR ? 4 : 1) k_attn_softmax(const AttnArgs a) {
+    constexpr int T = 64 * W, ROWS = W > 4 ? 1 : 4 / W;    // a workgroup's rows at a time
+    static_assert(W == 1 || ROWS == 1, "waves that share a row meet at the workgroup's barriers");
+    extern __shared__ int32_t live[];
+    __shared__ double power[64];
+    __shared__ RowShared<W> sh;
+    const uint32_t rows = a.tokens * a.group, all = a.heads_here * rows, lane = threadIdx.x & 63u, tid = W == 1 ? lane : threadIdx.x;
+    uint32_t bad = 0;
+    softmax_tables<T * ROWS, KIND>(a.softmax, live, power);
     __syncthreads();
     const uint32_t work = SUMS == Sums::IN_ORDER ? *a.unsure : all;
     for (uint32_t at = W == 1 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)(blockIdx.x * ROWS + (threadIdx.x >> 6))) : blockIdx.x; at < work; at += gridDim.x * ROWS) {
         const uint32_t r = SUMS == Sums::IN_ORDER ? a.unsure[4 + at] : at, in = r % rows, token = in / a.group;
+        int8_t* weights = a.weights + (size_t)r * 6 * a.ld;
         uint32_t own = 0;
         Sequence q;
         if (a.seqs.count) {
             if (!sequence_of(a.seqs, token, q, bad)) {     // nobody's row: no weights, in case that its tile is somebody's
-                int8_t* w = a.weights + (size_t)r * 6 * a.ld;
-                for (size_t i = tid; i < 6 * a.ld / 16; i += T) reinterpret_cast<v4i*>(w)[i] = v4i{0, 0, 0, 0};
+                for (size_t i = tid; i < 6 * a.ld / 16; i += T) reinterpret_cast<v4i*>(weights)[i] = v4i{0, 0, 0, 0};
                 if (tid == 0) a.top[r] = 0;
                 continue;
             }
             own = own_seen(a, q, token);
         }
-        // columns with keys: the prefix's, then the row's own; weights are 0 up to where another row of the tile may see
-        const uint32_t own_end = a.prefix_cols + own, cols = own ? own_end : a.prefix_len, fill = min((uint32_t)a.ld, a.seqs.count ? a.prefix_cols + (own + 127) / 64 * 64 : a.prefix_cols);
-        const Columns columns{a.prefix_len, a.prefix_cols, own_end, cols};
-        const int64_t* x = a.scores + (size_t)r * a.ld;
-        const uint32_t stretches = (cols + T * M * C - 1) / (T * M * C);
-        int64_t v[C][M];
-        uint32_t n[C];
-        auto load = [&](uint32_t stretch) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const uint32_t j = (stretch * C + c) * T * M + tid * M;
-                n[c] = columns.keys_at(j);
-#pragma unroll
-                for (int i = 0; i < M; ++i) v[c][i] = NO_KEY;
-                if (n[c]) {
-                    typedef long long v2l __attribute__((ext_vector_type(2)));
-#pragma unroll
-                    for (int i = 0; i < M; i += 2) {
-                        const v2l p = *reinterpret_cast<const v2l*>(x + j + i);
-                        v[c][i] = p[0]; v[c][i + 1] = p[1];
-                    }
-                    if (n[c] < M)
-#pragma unroll
-                        for (int i = 1; i < M; ++i) v[c][i] = i < (int)n[c] ? v[c][i] : NO_KEY;
-                }
-            }
-        };
-        if (W > 1 && tid == 0) any_top = 0;
-        auto rounded = [](double sv) { return sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5); };
-        int64_t shift = 0;
-        bool sure = cols == 0, loaded = false;
-        if constexpr (SUMS != Sums::IN_ORDER) {
-            double total = 0.0;
-            for (uint32_t i = 0; i < stretches; ++i) {
-                load(i);
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-#pragma unroll
-                    for (int e = 0; e < M; ++e) {
-                        total += exp_near(v[c][e], s, power);
-                        if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
-                    }
-                }
-            }
-            loaded = stretches == 1;
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-            if constexpr (W > 1) {
-                __syncthreads();                           // the arrays' last use is over
-                if (lane == 0) sums[wave] = total;
-                __syncthreads();
-                total = 0.0;
-#pragma unroll
-                for (int i = 0; i < W; ++i) total += sums[i];
-            }
-            if (cols) {
-                // An exponential of x is off by 2^-50 and |x| 2^-52; weighted by what it has in the sum t, |x| is |ln t| + ln(keys) at most.  The logarithm: 4e-16 of it, its product with the scale 2^-53.
-                const double ln = zkd::log_det(total), sv = s.scale * ln;
-                const double off = s.scale * ((double)(cols + 64) * 1.2e-16 + 2e-15 * (fabs(ln) + 20.0)), from_border = fabs(sv - floor(sv) - 0.5);
-                sure = total > 1e-280 && total < 1e280 && off < 0.25 && from_border > off;
-                if (sure) shift = rounded(sv);
-            }
-            if constexpr (SUMS == Sums::NEAR)
-                if (!sure) {
-                    if (tid == 0) a.unsure[4 + atomicAdd(a.unsure, 1u)] = r;
-                    continue;
-                }
+        // weights are 0 up to where another row of the tile may see
+        const uint32_t fill = min((uint32_t)a.ld, a.seqs.count ? a.prefix_cols + (own + 127) / 64 * 64 : a.prefix_cols);
+        if (W > 1 && tid == 0) sh.any_top = 0;
+        int64_t shift;
+        bool top;
+        if (!softmax_row<W, KIND, SUMS>(a.softmax, a.scores + (size_t)r * a.ld, weights, a.ld, Columns{a.prefix_len, a.prefix_cols, a.prefix_cols + own, own ? a.prefix_cols + own : a.prefix_len}, fill,
+                                        live, power, sh, shift, top, bad)) {
+            if (tid == 0) a.unsure[4 + atomicAdd(a.unsure, 1u)] = r;
+            continue;
         }
-        if constexpr (SUMS != Sums::NEAR)
-            if (!sure) {
-                shift = rounded(s.scale * zkd::log_det(sum_in_order<W>(x, columns, s.scale, s.scale_inv, sums, steps, at_exponent, &in_order)));
-                loaded = false;                            // the registers were needed
-            }
         if (tid == 0 && a.shift_out) a.shift_out[((size_t)token * a.kv_heads + a.kv0 + r / rows) * a.group + (in - token * a.group)] = shift;
-        // Both tables' values and their product are exact in double precision, and so is the number whose low 48 bits are the digits with 128 added to each
-        constexpr double BASE = 4503599627370496.0 + 141289400074368.0;
-        auto by_series = [&](int64_t score) {
-            const uint64_t below = (uint64_t)(shift - score);
-            const uint32_t lo = (uint32_t)below, hi = (uint32_t)(below >> 32), digit = lo >> s.drop_bits & (s.radix[0] - 1), upper = __builtin_amdgcn_alignbit(hi, lo, s.drop_bits + s.bits[0]);
-            const bool reached = hi < s.upper_end;         // neither negative nor too far
-            bad |= reached ? 0u : (uint32_t)ZK_VALUES_TABLE;
-            const double z = (double)digit;
-            const double u = fma_s(z, __builtin_fma(z, __builtin_fma(z, __builtin_fma(z, s.series[4], s.series[3]), s.series[2]), s.series[1]), s.series[0]);
-            double first = floor(u);
-            if (fabs(u - first - 0.5) > 0.5 - s.guard) first = (double)s.table[0][digit];      // nearer to a border than the terms left out
-            const int32_t second = live[min(upper, s.live - 1)];
-            return __builtin_fma(first, reached && upper < s.live ? (double)second : 0.0, BASE);
-        };
-        bool top = false;
-        const uint32_t fills = (fill + T * M * C - 1) / (T * M * C);
-        for (uint32_t i = 0; i < fills; ++i) {
-            if (!loaded || i != 0) load(i);
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const uint32_t j = (i * C + c) * T * M + tid * M;
-                if (j >= fill) continue;
-                uint64_t d[M];
-                if (n[c] < M)
-#pragma unroll
-                    for (int e = 0; e < M; ++e) v[c][e] = e < (int)n[c] ? v[c][e] : shift;
-#pragma unroll
-                for (int e = 0; e < M; ++e) {
-                    if constexpr (KIND == Weights::SERIES) d[e] = zkd::double_to_bits(by_series(v[c][e])) ^ 0x808080808080ull;
-                    else d[e] = ((uint64_t)softmax_weight<KIND == Weights::POW2>(shift - v[c][e], s, bad) + 0x808080808080ull) ^ 0x808080808080ull;
-                    if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                }
-                if (n[c] < M)
-#pragma unroll
-                    for (int e = 0; e < M; ++e) d[e] = e < (int)n[c] ? d[e] : 0;
-                Digits8 p;
-                digits8(d, p);
-                top |= (p.p[5].x | p.p[5].y) != 0;
-#pragma unroll
-                for (int k = 0; k < 6; ++k) *reinterpret_cast<uint2*>(a.weights + ((size_t)r * 6 + k) * a.ld + j) = p.p[k];
-            }
-        }
         const bool wave_top = __any(top);
         if constexpr (W == 1) {
             if (lane == 0) a.top[r] = wave_top;
         } else {
-            if (wave_top && lane == 0) any_top = 1;
+            if (wave_top && lane == 0) sh.any_top = 1;
             __syncthreads();
-            if (tid == 0) a.top[r] = any_top;
+            if (tid == 0) a.top[r] = sh.any_top;
         }
     }
     raise(a.flag, bad);
@@ -673,8 +696,72 @@ template <int NS> __device__ __forceinline__ void attn_sum(const int32_t (&s)[NS
     lo = (unsigned long long)l + ((unsigned long long)h << 32);
     size = h + (l >> 32);
 }
-// Few rows: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each
-template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const AttnArgs a, int own) {
+// Few rows: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each.  weights: the lane's row and 16 keys of
+// 64; keys from + 64 stream to end, 64 streams apart
+template <Heads HEADS> __device__ __forceinline__ void values_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t block, uint32_t first, uint32_t end, uint32_t stream, uint32_t streams, const int8_t* weights,
+                                                              size_t ld, bool top, v4i (&acc)[9][4], uint32_t& bad) {
+    const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, d0 = block * 64 + 4 * (lane & 15u);
+    if (first + stream * 64 >= end) return;
+    const zk_i32_cache& cache = t.own ? a.own : a.prefix;
+    const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride;
+    auto place = [&](uint32_t k) { return cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad); };
+    size_t next = place(first + stream * 64);
+    for (uint32_t k = first + stream * 64; k < end; k += 64 * streams) {
+        const size_t mine = next;
+        next = place(k + 64 * streams);                // looked up a step ahead
+        v4i w[6];
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = *reinterpret_cast<const v4i*>(weights + i * ld + k);
+        int32_t x[4][16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const v4i v = four_of<HEADS>(values + __shfl((unsigned long long)mine, (int)(q * 16 + i), 64), d0, a.dim);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) x[n][i] = v[n];
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            v4i v[4];
+            digit_planes(x[n], v, bad);
+            const bool four = __any(any_bits(v[3]));
+#pragma unroll
+            for (int i = 0; i < 5; ++i)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) acc[i + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[j], acc[i + j][n], 0, 0, 0);
+            if (top)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[5], v[j], acc[5 + j][n], 0, 0, 0);
+            if (four)
+#pragma unroll
+                for (int i = 0; i < 6; ++i) acc[i + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[3], acc[i + 3][n], 0, 0, 0);
+        }
+    }
+}
+// what 64 lanes have of the sums of 16 rows, added to sums [16][64 blocks of dimensions][2]: row 4 q + e, four dimensions
+__device__ __forceinline__ void add_sums(unsigned long long* sums, uint32_t blocks, uint32_t block, const v4i (&acc)[9][4]) {
+    const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, d0 = block * 64 + 4 * (lane & 15u);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            int32_t s[9];
+#pragma unroll
+            for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
+            unsigned long long lo;
+            int64_t size;
+            attn_sum<9>(s, lo, size);
+            const uint32_t at = ((4 * q + e) * blocks * 64 + d0 + n) * 2;
+            atomicAdd(&sums[at], lo);
+            atomicAdd(&sums[at + 1], (unsigned long long)size);
+        }
+}
+__device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, uint32_t kv, const unsigned long long* sums, uint32_t blocks, uint32_t threads, uint32_t& bad) {
+    for (uint32_t i = (t.lo - t.row0) * a.dim + threadIdx.x; i < (t.hi - t.row0) * a.dim; i += threads) {
+        const uint32_t r = i / a.dim, d = i - r * a.dim, token = (t.row0 + r) / a.group, at = (r * blocks * 64 + d) * 2;
+        attn_finish(a, sums[at], (int64_t)sums[at + 1], token, kv * a.group + (t.row0 + r - token * a.group), d, bad);
+    }
+}
+template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(const AttnArgs a, int own) {
     extern __shared__ unsigned long long sums64[];         // [16][64 blocks of dimensions][2]
     uint32_t bad = 0;
     Tile t;
@@ -685,74 +772,16 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const A
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z, block = wave % blocks, stream = wave / blocks;
     const size_t row = (size_t)blockIdx.z * a.tokens * a.group + t.row0;
     for (uint32_t i = threadIdx.x; i < 16 * blocks * 64 * 2; i += 256) sums64[i] = 0;
-    const zk_i32_cache& cache = t.own ? a.own : a.prefix;
-    const uint32_t d0 = block * 64 + 4 * c;
-    const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride + d0;
     const uint32_t my_row = t.has(c) ? c : t.lo - t.row0;
     const bool top = __any(t.has(c) && a.top[row + my_row] != 0);
-    const int8_t* weights = a.weights + (row + my_row) * 6 * a.ld + t.col0 + q * 16;
     v4i acc[9][4];
 #pragma unroll
     for (int s = 0; s < 9; ++s)
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[s][n] = v4i{0, 0, 0, 0};
-    auto place = [&](uint32_t k) { return cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad); };
-    if (stream < streams) {
-        size_t next = t.keys ? place(first + stream * 64) : 0;
-        for (uint32_t k = first + stream * 64; k < end; k += 64 * streams) {
-            const size_t mine = next;
-            next = place(k + 64 * streams);                // looked up a step ahead
-            v4i w[6];
-#pragma unroll
-            for (int i = 0; i < 6; ++i) w[i] = *reinterpret_cast<const v4i*>(weights + i * a.ld + k);
-            int32_t x[4][16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int32_t* p = values + __shfl((unsigned long long)mine, (int)(q * 16 + i), 64);
-                if constexpr (VEC) {
-                    v4i v = {0, 0, 0, 0};
-                    if (d0 < a.dim) v = *reinterpret_cast<const v4i*>(p);
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) x[n][i] = v[n];
-                } else {
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) x[n][i] = d0 + n < a.dim ? p[n] : 0;
-                }
-            }
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                v4i v[4];
-                digit_planes(x[n], v, bad);
-                const bool four = __any(any_bits(v[3]));
-#pragma unroll
-                for (int i = 0; i < 5; ++i)
-#pragma unroll
-                    for (int j = 0; j < 3; ++j) acc[i + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[j], acc[i + j][n], 0, 0, 0);
-                if (top)
-#pragma unroll
-                    for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[5], v[j], acc[5 + j][n], 0, 0, 0);
-                if (four)
-#pragma unroll
-                    for (int i = 0; i < 6; ++i) acc[i + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[3], acc[i + 3][n], 0, 0, 0);
-            }
-        }
-    }
+    if (stream < streams) values_of<HEADS>(a, t, kv, block, first, end, stream, streams, a.weights + (row + my_row) * 6 * a.ld + t.col0 + q * 16, a.ld, top, acc, bad);
     __syncthreads();
-    if (stream < streams)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {      // row 4 q + e, dimension d0 + n
-                int32_t s[9];
-#pragma unroll
-                for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
-                unsigned long long lo;
-                int64_t size;
-                attn_sum<9>(s, lo, size);
-                const uint32_t at = ((4 * q + e) * blocks * 64 + d0 + n) * 2;
-                atomicAdd(&sums64[at], lo);
-                atomicAdd(&sums64[at + 1], (unsigned long long)size);
-            }
+    if (stream < streams) add_sums(sums64, blocks, block, acc);
     __syncthreads();
     if (!a.direct) {
         const size_t all = (size_t)a.heads_here * a.tokens * a.group;
@@ -761,16 +790,64 @@ template <bool VEC> __global__ void __launch_bounds__(256) k_attn_values(const A
             const uint32_t r = i / (2 * a.dim);
             out[i] = sums64[r * blocks * 128 + (i - r * 2 * a.dim)];
         }
-    } else
-        for (uint32_t i = (t.lo - t.row0) * a.dim + threadIdx.x; i < (t.hi - t.row0) * a.dim; i += 256) {
-            const uint32_t r = i / a.dim, d = i - r * a.dim, token = (t.row0 + r) / a.group, at = (r * blocks * 64 + d) * 2;
-            attn_finish(a, sums64[at], (int64_t)sums64[at + 1], token, kv * a.group + (t.row0 + r - token * a.group), d, bad);
-        }
+    } else finish_tile(a, t, kv, sums64, blocks, 256, bad);
+    raise(a.flag, bad);
+}
+// A tile of 16 rows with few keys, from scores to outputs in one launch: nothing leaves LDS between the steps
+static constexpr uint32_t SMALL_COLS = 640, SMALL_LIVE = 4096;
+template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(512) k_attn_small(const AttnArgs a) {
+    __shared__ __attribute__((aligned(16))) int64_t scores[16 * SMALL_COLS];
+    __shared__ __attribute__((aligned(16))) int8_t weights[16][6 * SMALL_COLS];
+    __shared__ int32_t live[KIND == Weights::SERIES ? SMALL_LIVE : 1];
+    __shared__ double power[64];
+    __shared__ RowShared<1> sh;
+    __shared__ uint32_t tops[16];
+    uint32_t bad = 0;
+    Tile t;
+    if (!tile_at<16>(a, a.seqs.count != 0, blockIdx.x, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = blockIdx.y, blocks = (a.dim + 63) / 64, streams = 8 / blocks, block = wave % blocks, stream = wave / blocks;
+    Tile shared = t;                     // the same rows, the prefix's keys
+    shared.own = false; shared.keys = a.prefix_len; shared.col0 = 0;
+    softmax_tables<512, KIND>(a.softmax, live, power);
+    if (a.prefix_len) scores_of<U, 1, HEADS, 8>(a, shared, kv, 0, a.prefix_len, scores, a.ld, bad);
+    if (t.own && t.keys) scores_of<U, 1, HEADS, 8>(a, t, kv, 0, t.keys, scores + t.col0, a.ld, bad);
+    __syncthreads();
+    for (uint32_t r = wave; r < 16; r += 8) {
+        bool top = false;
+        if (t.has(r)) {
+            const uint32_t token = (t.row0 + r) / a.group, own = t.own ? own_seen(a, t.s, token) : 0;
+            int64_t shift;
+            softmax_row<1, KIND, Sums::BOTH>(a.softmax, scores + r * a.ld, weights[r], a.ld, Columns{a.prefix_len, a.prefix_cols, a.prefix_cols + own, own ? a.prefix_cols + own : a.prefix_len}, (uint32_t)a.ld, live,
+                                             power, sh, shift, top, bad);
+            if (lane == 0 && a.shift_out) a.shift_out[((size_t)token * a.kv_heads + kv) * a.group + (t.row0 + r - token * a.group)] = shift;
+        } else
+            for (uint32_t i = lane; i < 6 * a.ld / 16; i += 64) reinterpret_cast<v4i*>(weights[r])[i] = v4i{0, 0, 0, 0};
+        const bool any = __any(top);
+        if (lane == 0) tops[r] = any;
+    }
+    __syncthreads();
+    unsigned long long* sums = reinterpret_cast<unsigned long long*>(scores);      // the scores are used up
+    for (uint32_t i = threadIdx.x; i < 16 * blocks * 64 * 2; i += 512) sums[i] = 0;
+    const bool top = __any(tops[c] != 0);
+    v4i acc[9][4];
+#pragma unroll
+    for (int s = 0; s < 9; ++s)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[s][n] = v4i{0, 0, 0, 0};
+    if (stream < streams) {
+        const int8_t* mine = weights[c] + q * 16;
+        if (a.prefix_len) values_of<HEADS>(a, shared, kv, block, 0, a.prefix_len, stream, streams, mine, a.ld, top, acc, bad);
+        if (t.own) values_of<HEADS>(a, t, kv, block, 0, t.keys, stream, streams, mine + t.col0, a.ld, top, acc, bad);
+    }
+    __syncthreads();
+    if (stream < streams) add_sums(sums, blocks, block, acc);
+    __syncthreads();
+    finish_tile(a, t, kv, sums, blocks, 512, bad);
     raise(a.flag, bad);
 }
 // Many rows: 64 rows by 128 dimensions, a wave 16 by 64.  The workgroup splits 64 keys' values into digits together, the next ones while this step's are multiplied: a lane four keys of four
 // dimensions, in LDS as fragments.
-template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile(const AttnArgs a, int own) {
+template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_tile(const AttnArgs a, int own) {
     __shared__ __attribute__((aligned(16))) int8_t planes[2][4][8][64][16], weight[2][4][6][64][16];      // fragments of the values and, [16 rows], of the weights
     __shared__ uint32_t wide[3];                           // of the step, the next and the one after that
     uint32_t bad = 0;
@@ -785,7 +862,7 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     // a lane's share of the values: dimensions 4 dq .. 4 dq + 3 of keys 4 kq .. 4 kq + 3
     const uint32_t dq = threadIdx.x & 31u, kq = threadIdx.x >> 5, d0 = dim0 + 4 * dq;
-    const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride + d0;
+    const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride;
     const uint32_t mine = t.has(row_in + c) ? row_in + c : t.lo - t.row0;
     const bool top = __any(a.top[row + mine] != 0);
     const int8_t* weights = a.weights + (row + mine) * 6 * a.ld + t.col0 + q * 16 + first;
@@ -797,16 +874,9 @@ template <bool VEC> __global__ void __launch_bounds__(512, 2) k_attn_values_tile
         next = place(i + 1);                               // looked up a step ahead
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int32_t* p = values + __shfl((unsigned long long)at, (int)((kq & 1u) * 4 + e), 64);
-            if constexpr (VEC) {
-                v4i v = {0, 0, 0, 0};
-                if (d0 < a.dim) v = *reinterpret_cast<const v4i*>(p);
+            const v4i v = four_of<HEADS>(values + __shfl((unsigned long long)at, (int)((kq & 1u) * 4 + e), 64), d0, a.dim);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) x[e][n] = v[n];
-            } else {
-#pragma unroll
-                for (int n = 0; n < 4; ++n) x[e][n] = d0 + n < a.dim ? p[n] : 0;
-            }
+            for (int n = 0; n < 4; ++n) x[e][n] = v[n];
         }
     };
     // two waves have the same rows: each brings three digits of them to LDS
@@ -1085,17 +1155,20 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
 static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
 
 // How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
-struct AttnPlan { bool prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts; };
+struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts; };
 static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     AttnPlan p{};
     const uint32_t group = heads / kv_heads;
     const size_t rows = (size_t)tokens * group;
+    p.prefix_cols = ((size_t)prefix_len + 63) / 64 * 64;
+    p.cols = p.prefix_cols + ((size_t)max_length + 63) / 64 * 64;
+    const size_t small_tiles = sequences ? rows / 16 + sequences : cdiv(rows, 16);
+    p.small = p.cols <= SMALL_COLS && small_tiles * kv_heads <= 512;
+    if (p.small) { p.own_tiles = (uint32_t)small_tiles; p.heads = kv_heads; return p; }
     p.prefix64 = rows > 16;
     p.own64 = sequences && rows / sequences > 32;
     p.prefix_tiles = prefix_len ? cdiv(rows, p.prefix64 ? 64 : 16) : 0;
     p.own_tiles = sequences ? (uint32_t)(rows / (p.own64 ? 64 : 16)) + sequences : 0;
-    p.prefix_cols = ((size_t)prefix_len + 63) / 64 * 64;
-    p.cols = p.prefix_cols + ((size_t)max_length + 63) / 64 * 64;
     auto cut = [&](uint32_t keys, size_t tiles, bool many, uint32_t& splits, uint32_t& step) {
         const size_t want = std::max<size_t>(1, (many ? 512 : 1024) / std::max<size_t>(1, tiles * kv_heads));
         splits = (uint32_t)std::min<size_t>(want, cdiv(keys, 256));
@@ -1260,7 +1333,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     CallFlag flag;
     if (const int rc = flag.begin(flag_dev, st, name)) return rc;
     std::unique_ptr<Scratch> scratch;
-    if (!workspace) {
+    if (!workspace && bytes) {
         if (const int rc = CallFlag::not_captured(st, name)) return rc;
         scratch.reset(new Scratch(bytes, st));
         if (scratch->rc) return scratch->rc;
@@ -1278,8 +1351,30 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     a.unsure = (uint32_t*)((char*)a.top + p.top); a.parts = (int64_t*)((char*)a.unsure + p.unsure); a.direct = p.direct;
     a.tokens = tokens; a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits; a.prefix_step = p.prefix_step; a.own_splits = p.own_splits; a.own_step = p.own_step;
     a.flag = flag.dev;
-    const bool vec = dim % 4 == 0 && ((q_token | q_head) & 3) == 0 && ((uintptr_t)q & 15) == 0 && (!prefix_len || cache_aligned(prefix)) && (!own || cache_aligned(own));
+    const bool fours = dim % 4 == 0 && ((q_token | q_head) & 3) == 0 && ((uintptr_t)q & 15) == 0 && (!prefix_len || cache_aligned(prefix)) && (!own || cache_aligned(own));
     const unsigned blocks = cdiv(dim, 64);
+    auto heads_of = [&](auto launch) {
+        if (fours && (dim == 64 || dim == 128 || dim == 256)) launch(std::integral_constant<Heads, Heads::BLOCKS>());
+        else if (fours) launch(std::integral_constant<Heads, Heads::FOURS>());
+        else launch(std::integral_constant<Heads, Heads::ANY>());
+    };
+    if (p.small) {
+        auto small = [&](auto u, auto kind) {
+            constexpr int U = decltype(u)::value;
+            constexpr Weights KIND = decltype(kind)::value;
+            heads_of([&](auto h) { hipLaunchKernelGGL((k_attn_small<U, decltype(h)::value, KIND>), dim3(p.own_tiles, kv_heads), dim3(512), 0, st, a); });
+        };
+        auto of_kind = [&](auto kind) {
+            if (blocks == 1) small(std::integral_constant<int, 1>(), kind);
+            else if (blocks == 2) small(std::integral_constant<int, 2>(), kind);
+            else small(std::integral_constant<int, 4>(), kind);
+        };
+        if (s->series && a.softmax.live <= SMALL_LIVE) of_kind(std::integral_constant<Weights, Weights::SERIES>());
+        else if (s->pow2) of_kind(std::integral_constant<Weights, Weights::POW2>());
+        else of_kind(std::integral_constant<Weights, Weights::ANY>());
+        ZK_LAUNCH_CHECK();
+        return flag.end(name);
+    }
     for (a.kv0 = 0; a.kv0 < kv_heads; a.kv0 += p.heads) {
         a.heads_here = std::min(p.heads, kv_heads - a.kv0);
         const size_t rows = (size_t)a.heads_here * tokens * a.group;
@@ -1294,8 +1389,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             const dim3 grid(cdiv(keys, a.score_keys), tiles, a.heads_here);
             auto scores = [&](auto u, auto rt) {
                 constexpr int U = decltype(u)::value, RT = decltype(rt)::value;
-                if (vec) hipLaunchKernelGGL((k_attn_scores<U, RT, true>), grid, dim3(256), 0, st, a, of_own);
-                else hipLaunchKernelGGL((k_attn_scores<U, RT, false>), grid, dim3(256), 0, st, a, of_own);
+                heads_of([&](auto h) { hipLaunchKernelGGL((k_attn_scores<U, RT, decltype(h)::value>), grid, dim3(256), 0, st, a, of_own); });
             };
             auto wide = [&](auto u) {
                 if (many) scores(u, std::integral_constant<int, 4>());
@@ -1309,14 +1403,14 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             constexpr Weights KIND = decltype(kind)::value;
             const size_t lds = KIND == Weights::SERIES ? s->a.live * 4 : 0;
             if (rows < 256) {
-                if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, 1, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(256), lds, st, a);
-                else hipLaunchKernelGGL((k_attn_softmax<16, 1, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(1024), lds, st, a);
+                if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(256), lds, st, a);
+                else hipLaunchKernelGGL((k_attn_softmax<16, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(1024), lds, st, a);
                 return;
             }
-            if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<1, 1, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(cdiv(rows, 4), 1024)), dim3(256), lds, st, a);
-            else hipLaunchKernelGGL((k_attn_softmax<4, 1, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(rows, 1024)), dim3(256), lds, st, a);
-            if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, 1, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 512)), dim3(256), lds, st, a);
-            else hipLaunchKernelGGL((k_attn_softmax<16, 1, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 256)), dim3(1024), lds, st, a);
+            if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<1, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(cdiv(rows, 4), 1024)), dim3(256), lds, st, a);
+            else hipLaunchKernelGGL((k_attn_softmax<4, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(rows, 1024)), dim3(256), lds, st, a);
+            if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 512)), dim3(256), lds, st, a);
+            else hipLaunchKernelGGL((k_attn_softmax<16, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 256)), dim3(1024), lds, st, a);
         };
         if (s->series) softmax_rows(std::integral_constant<Weights, Weights::SERIES>());
         else if (s->pow2) softmax_rows(std::integral_constant<Weights, Weights::POW2>());
@@ -1324,13 +1418,11 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
         both([&](int of_own, bool many, unsigned tiles, uint32_t, unsigned splits) {
             if (many) {
                 const dim3 grid(splits, tiles, a.heads_here * cdiv(dim, 128));
-                if (vec) hipLaunchKernelGGL(k_attn_values_tile<true>, grid, dim3(512), 0, st, a, of_own);
-                else hipLaunchKernelGGL(k_attn_values_tile<false>, grid, dim3(512), 0, st, a, of_own);
+                heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values_tile<decltype(h)::value>, grid, dim3(512), 0, st, a, of_own); });
             } else {
                 const dim3 grid(splits, tiles, a.heads_here);
                 const size_t lds = 16 * (size_t)blocks * 64 * 16;
-                if (vec) hipLaunchKernelGGL(k_attn_values<true>, grid, dim3(256), lds, st, a, of_own);
-                else hipLaunchKernelGGL(k_attn_values<false>, grid, dim3(256), lds, st, a, of_own);
+                heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values<decltype(h)::value>, grid, dim3(256), lds, st, a, of_own); });
             }
         });
         if (!p.direct) hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 64)), dim3(256), 0, st, a);
