@@ -228,7 +228,8 @@ __device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v
 
 // Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8.  The next keys are
 // on their way while these are multiplied, and the place of those behind them is looked up.
-template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, int64_t* out, size_t ld, uint32_t& bad) {
+template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, v4i (&fourth)[RT][U][64],
+                                                                                                 int64_t* out, size_t ld, uint32_t& bad) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
     auto query = [&](int r, int u, v4i (&d)[4]) {
         const uint32_t row = t.has(16 * r + c) ? t.row0 + 16 * r + c : t.lo, token = row / a.group, head = kv * a.group + (row - token * a.group);
@@ -238,7 +239,9 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
     };
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     const int32_t* keys = (const int32_t*)cache.k + kv * cache.head_stride;
-    auto place = [&](uint32_t key) { return keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + c, t.keys - 1), bad); };
+    // row 4 q + e of a fragment's product is key 2 q + e, or 8 + 2 q + e - 2: four lanes store 64 bytes in one piece
+    const uint32_t my_key = (c >> 2) * 2 + (c & 1u) + (c & 2u) * 4;
+    auto place = [&](uint32_t key) { return keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + my_key, t.keys - 1), bad); };
     int32_t x[U][16];
     auto fetch = [&](const int32_t* p) {
 #pragma unroll
@@ -257,12 +260,13 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
             query(r, u, d);
 #pragma unroll
             for (int m = 0; m < 3; ++m) b[r][u][m] = d[m];
+            fourth[r][u][lane] = d[3];                     // rarely needed; every wave has the same
             wide |= any_bits(d[3]);
+            if ((r * U + u) % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
         }
-        if (r % 2 == 1) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
     }
     const bool q_wide = __any(wide);
-    int64_t* const to0 = out + c * ld + 4 * q;
+    int64_t* const to0 = out + c * ld + 2 * q;
     for (; key < end; key += WAVES * 16) {
         v4i k[U][4];
         bool k_wide = false;
@@ -278,33 +282,31 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
         for (int r = 0; r < RT; ++r) {
             v4i acc[5];
 #pragma unroll
-            for (int s = 0; s < 5; ++s) acc[s] = v4i{0, 0, 0, 0};
-#pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int m = 0; m < 3; ++m)
 #pragma unroll
-                    for (int n = 0; n < 3; ++n) acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][n], acc[m + n], 0, 0, 0);
-            int64_t v[4];                                  // key 4 q + e of the tile, row c
+                    for (int n = 0; n < 3; ++n)
+                        acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][n], u == 0 && (m == 0 || n == 2) ? v4i{0, 0, 0, 0} : acc[m + n], 0, 0, 0);      // a set's first
+            int64_t v[4];
             if (!four) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    if constexpr (U <= 2) v[e] = (int64_t)(acc[0][e] + acc[1][e] * 256) + ((int64_t)(acc[2][e] + acc[3][e] * 256) << 16) + ((int64_t)acc[4][e] << 32);      // two products of 2^14 in 128 dimensions
+                    if constexpr (U <= 2) v[e] = (int64_t)(acc[2][e] + acc[3][e] * 256) * 65536 + ((int64_t)(acc[0][e] + acc[1][e] * 256) + ((int64_t)acc[4][e] << 32));      // two products of 2^14 in 128 dimensions
                     else v[e] = acc[0][e] + (int64_t)acc[1][e] * 256 + (acc[2][e] + (int64_t)acc[3][e] * 256) * 65536 + ((int64_t)acc[4][e] << 32);
                 }
             } else {
                 v4i more[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};      // of 256^4 on, but for 256^3
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    v4i d[4];
-                    query(r, u, d);                        // a fourth digit is rare: the queries' is not kept
+                    const v4i d3 = fourth[r][u][lane];
 #pragma unroll
                     for (int m = 0; m < 3; ++m) {
                         v4i& to = m == 0 ? acc[3] : m == 1 ? more[0] : more[1];
-                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], d[3], to, 0, 0, 0);
+                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], d3, to, 0, 0, 0);
                         to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][m], to, 0, 0, 0);
                     }
-                    more[2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], d[3], more[2], 0, 0, 0);
+                    more[2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], d3, more[2], 0, 0, 0);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -316,18 +318,20 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
             typedef long long v2l __attribute__((ext_vector_type(2)));
             v2l* to = reinterpret_cast<v2l*>(to0 + 16 * r * ld + key);
             to[0] = v2l{v[0], v[1]};
-            to[1] = v2l{v[2], v[3]};
+            to[4] = v2l{v[2], v[3]};
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
 template <int U, int RT, Heads HEADS> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
+    __shared__ v4i fourth[RT][U][64];
     uint32_t bad = 0;
     Tile t;
-    if ((blockIdx.x | blockIdx.y | blockIdx.z | threadIdx.x) == 0) *a.unsure = 0;
-    if (!tile_at<16 * RT>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
-    const uint32_t key0 = blockIdx.x * a.score_keys;
+    if ((blockIdx.y | blockIdx.z | blockIdx.x | threadIdx.x) == 0) *a.unsure = 0;
+    if (!tile_at<16 * RT>(a, own, blockIdx.z, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t key0 = blockIdx.y * a.score_keys;
     if (key0 >= t.keys) return;
-    scores_of<U, RT, HEADS, 4>(a, t, a.kv0 + blockIdx.z, key0, min(key0 + a.score_keys, t.keys), a.scores + ((size_t)blockIdx.z * a.tokens * a.group + t.row0) * a.ld + t.col0, a.ld, bad);
+    scores_of<U, RT, HEADS, 4>(a, t, a.kv0 + blockIdx.x, key0, min(key0 + a.score_keys, t.keys), fourth, a.scores + ((size_t)blockIdx.x * a.tokens * a.group + t.row0) * a.ld + t.col0, a.ld, bad);
     raise(a.flag, bad);
 }
 
@@ -438,14 +442,15 @@ __device__ __forceinline__ double fma_s(double a, double b, double c) {
 }
 // exp(v / scale) to some 2^-50 and what v / scale's rounding adds: 2^(n / 64) out of LDS and five terms behind it
 __device__ __forceinline__ double exp_near(int64_t v, const SoftmaxArgs& s, const double* power) {
-    const double x = __builtin_fmin(__builtin_fmax((double)v * s.scale_64, -1e5), 1e5), n = rint(x), f = x - n;
+    const double x = (double)v * s.scale_64, n = rint(x), f = x - n;
     constexpr double L = 0.69314718055994530942 / 64.0;
     double p = fma_s(f, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
     p = fma_s(f, p, L * L * L / 6.0);
     p = fma_s(f, p, L * L / 2.0);
     p = fma_s(f, p, L);
     p = __builtin_fma(f, p, 1.0);
-    const int i = (int)n;
+    int i;                               // far beyond what a double's exponent holds the largest or smallest of its type
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(i) : "v"(n));
     return ldexp(power[i & 63] * p, i >> 6);
 }
 // the columns of a row's scores: the prefix's, then, from a multiple of 64 on, its own
@@ -765,12 +770,12 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(cons
     extern __shared__ unsigned long long sums64[];         // [16][64 blocks of dimensions][2]
     uint32_t bad = 0;
     Tile t;
-    if (!tile_at<16>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
-    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.x * step;
+    if (!tile_at<16>(a, own, blockIdx.z, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.y * step;
     if (first >= t.keys && !(a.direct && first == 0)) return;
     const uint32_t end = min(first + step, t.keys), blocks = (a.dim + 63) / 64, streams = 4 / blocks;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.z, block = wave % blocks, stream = wave / blocks;
-    const size_t row = (size_t)blockIdx.z * a.tokens * a.group + t.row0;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.x, block = wave % blocks, stream = wave / blocks;
+    const size_t row = (size_t)blockIdx.x * a.tokens * a.group + t.row0;
     for (uint32_t i = threadIdx.x; i < 16 * blocks * 64 * 2; i += 256) sums64[i] = 0;
     const uint32_t my_row = t.has(c) ? c : t.lo - t.row0;
     const bool top = __any(t.has(c) && a.top[row + my_row] != 0);
@@ -785,7 +790,7 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(cons
     __syncthreads();
     if (!a.direct) {
         const size_t all = (size_t)a.heads_here * a.tokens * a.group;
-        unsigned long long* out = (unsigned long long*)a.parts + (((t.own ? a.prefix_splits : 0) + blockIdx.x) * all + row) * a.dim * 2;
+        unsigned long long* out = (unsigned long long*)a.parts + (((t.own ? a.prefix_splits : 0) + blockIdx.y) * all + row) * a.dim * 2;
         for (uint32_t i = (t.lo - t.row0) * a.dim * 2 + threadIdx.x; i < (t.hi - t.row0) * a.dim * 2; i += 256) {
             const uint32_t r = i / (2 * a.dim);
             out[i] = sums64[r * blocks * 128 + (i - r * 2 * a.dim)];
@@ -794,7 +799,7 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(cons
     raise(a.flag, bad);
 }
 // A tile of 16 rows with few keys, from scores to outputs in one launch: nothing leaves LDS between the steps
-static constexpr uint32_t SMALL_COLS = 640, SMALL_LIVE = 4096;
+static constexpr uint32_t SMALL_COLS = 576, SMALL_LIVE = 4096;
 template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(512) k_attn_small(const AttnArgs a) {
     __shared__ __attribute__((aligned(16))) int64_t scores[16 * SMALL_COLS];
     __shared__ __attribute__((aligned(16))) int8_t weights[16][6 * SMALL_COLS];
@@ -802,15 +807,16 @@ template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(51
     __shared__ double power[64];
     __shared__ RowShared<1> sh;
     __shared__ uint32_t tops[16];
+    __shared__ v4i fourth[1][U][64];
     uint32_t bad = 0;
     Tile t;
-    if (!tile_at<16>(a, a.seqs.count != 0, blockIdx.x, t, bad)) { raise(a.flag, bad); return; }
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = blockIdx.y, blocks = (a.dim + 63) / 64, streams = 8 / blocks, block = wave % blocks, stream = wave / blocks;
+    if (!tile_at<16>(a, a.seqs.count != 0, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = blockIdx.x, blocks = (a.dim + 63) / 64, streams = 8 / blocks, block = wave % blocks, stream = wave / blocks;
     Tile shared = t;                     // the same rows, the prefix's keys
     shared.own = false; shared.keys = a.prefix_len; shared.col0 = 0;
     softmax_tables<512, KIND>(a.softmax, live, power);
-    if (a.prefix_len) scores_of<U, 1, HEADS, 8>(a, shared, kv, 0, a.prefix_len, scores, a.ld, bad);
-    if (t.own && t.keys) scores_of<U, 1, HEADS, 8>(a, t, kv, 0, t.keys, scores + t.col0, a.ld, bad);
+    if (a.prefix_len) scores_of<U, 1, HEADS, 8>(a, shared, kv, 0, a.prefix_len, fourth, scores, a.ld, bad);
+    if (t.own && t.keys) scores_of<U, 1, HEADS, 8>(a, t, kv, 0, t.keys, fourth, scores + t.col0, a.ld, bad);
     __syncthreads();
     for (uint32_t r = wave; r < 16; r += 8) {
         bool top = false;
@@ -852,9 +858,9 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
     __shared__ uint32_t wide[3];                           // of the step, the next and the one after that
     uint32_t bad = 0;
     Tile t;
-    const uint32_t dim_blocks = (a.dim + 127) / 128, z = blockIdx.z / dim_blocks, dim0 = (blockIdx.z - z * dim_blocks) * 128;
-    if (!tile_at<64>(a, own, blockIdx.y, t, bad)) { raise(a.flag, bad); return; }
-    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.x * step;
+    const uint32_t dim_blocks = (a.dim + 127) / 128, z = blockIdx.x / dim_blocks, dim0 = (blockIdx.x - z * dim_blocks) * 128;
+    if (!tile_at<64>(a, own, blockIdx.z, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.y * step;
     if (first >= t.keys && !(a.direct && first == 0)) return;
     const uint32_t end = min(first + step, t.keys), steps = (end - first + 63) / 64;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + z, row_in = (wave >> 1) * 16, block = wave & 1u;
@@ -885,13 +891,14 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
         for (int k = 0; k < 3; ++k) load_to_lds(weights + (block * 3 + k) * a.ld + i * 64, &weight[i & 1u][wave >> 1][block * 3 + k][0][0]);
     };
     auto split = [&](uint32_t i) {
-        uint32_t over = 0, upper = 0;
+        int32_t most = x[0][0];
+        uint32_t upper = 0;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             uint32_t d[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                over |= x[e][n] > 0x7F7F7F7F ? 1u : 0u;
+                most = max(most, x[e][n]);
                 d[e] = digit_bytes((uint32_t)x[e][n]);
                 upper |= d[e];
             }
@@ -901,7 +908,7 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
 #pragma unroll
             for (int k = 0; k < 4; ++k) *reinterpret_cast<uint32_t*>(&planes[i & 1u][k][(dq >> 4) * 4 + n][(kq >> 2) * 16 + (dq & 15u)][(kq & 3u) * 4]) = p[k];
         }
-        bad |= over ? (uint32_t)ZK_VALUES_RANGE : 0u;
+        bad |= most > 0x7F7F7F7F ? (uint32_t)ZK_VALUES_RANGE : 0u;
         if (upper >> 24) wide[i % 3] = 1;
     };
     v4i acc[9][4];
@@ -964,7 +971,7 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
             int64_t size;
             attn_sum<9>(s, lo, size);
             if (!a.direct) {
-                unsigned long long* out = (unsigned long long*)a.parts + ((((t.own ? a.prefix_splits : 0) + blockIdx.x) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d) * 2;
+                unsigned long long* out = (unsigned long long*)a.parts + ((((t.own ? a.prefix_splits : 0) + blockIdx.y) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d) * 2;
                 out[0] = lo;
                 out[1] = (unsigned long long)size;
             } else attn_finish(a, lo, size, token, kv * a.group + (in - token * a.group), d, bad);
@@ -1362,7 +1369,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
         auto small = [&](auto u, auto kind) {
             constexpr int U = decltype(u)::value;
             constexpr Weights KIND = decltype(kind)::value;
-            heads_of([&](auto h) { hipLaunchKernelGGL((k_attn_small<U, decltype(h)::value, KIND>), dim3(p.own_tiles, kv_heads), dim3(512), 0, st, a); });
+            heads_of([&](auto h) { hipLaunchKernelGGL((k_attn_small<U, decltype(h)::value, KIND>), dim3(kv_heads, p.own_tiles), dim3(512), 0, st, a); });
         };
         auto of_kind = [&](auto kind) {
             if (blocks == 1) small(std::integral_constant<int, 1>(), kind);
@@ -1384,9 +1391,11 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             if (p.own_tiles && max_length) f(1, p.own64, p.own_tiles, max_length, p.own_splits);
         };
         both([&](int of_own, bool many, unsigned tiles, uint32_t keys, unsigned) {
+            const unsigned rt = !many ? 1 : 4;
+            if (many) tiles = of_own ? tokens * a.group / (16 * rt) + sequences : cdiv((size_t)tokens * a.group, 16 * rt);
             a.score_keys = 1024;                   // a workgroup's, where that still makes 512 workgroups
             while (a.score_keys > 64 && (size_t)cdiv(keys, a.score_keys) * tiles * a.heads_here < 512) a.score_keys /= 2;
-            const dim3 grid(cdiv(keys, a.score_keys), tiles, a.heads_here);
+            const dim3 grid(a.heads_here, cdiv(keys, a.score_keys), tiles);      // heads first: workgroups go to the eight dies in turn, and a die's L2 has a head's keys then
             auto scores = [&](auto u, auto rt) {
                 constexpr int U = decltype(u)::value, RT = decltype(rt)::value;
                 heads_of([&](auto h) { hipLaunchKernelGGL((k_attn_scores<U, RT, decltype(h)::value>), grid, dim3(256), 0, st, a, of_own); });
@@ -1417,10 +1426,10 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
         else softmax_rows(std::integral_constant<Weights, Weights::ANY>());
         both([&](int of_own, bool many, unsigned tiles, uint32_t, unsigned splits) {
             if (many) {
-                const dim3 grid(splits, tiles, a.heads_here * cdiv(dim, 128));
+                const dim3 grid(a.heads_here * cdiv(dim, 128), splits, tiles);
                 heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values_tile<decltype(h)::value>, grid, dim3(512), 0, st, a, of_own); });
             } else {
-                const dim3 grid(splits, tiles, a.heads_here);
+                const dim3 grid(a.heads_here, splits, tiles);
                 const size_t lds = 16 * (size_t)blocks * 64 * 16;
                 heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values<decltype(h)::value>, grid, dim3(256), lds, st, a, of_own); });
             }

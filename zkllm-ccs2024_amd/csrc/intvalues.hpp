@@ -57,14 +57,15 @@ template <int NS> __device__ __forceinline__ int64_t joined(const int32_t (&a)[N
 }
 // the digits of 16 values, plane by plane: plane j's 16 bytes in out[j]
 __device__ __forceinline__ void digit_planes(const int32_t (&x)[16], v4i (&out)[4], uint32_t& bad) {
+    int32_t most = x[0];
+#pragma unroll
+    for (int e = 1; e < 16; ++e) most = max(most, x[e]);
+    bad |= most > 0x7F7F7F7F ? (uint32_t)ZK_VALUES_RANGE : 0u;      // four digits reach no further
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
         uint32_t d[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            bad |= x[4 * w + e] > 0x7F7F7F7F ? (uint32_t)ZK_VALUES_RANGE : 0u;      // four digits reach no further
-            d[e] = digit_bytes((uint32_t)x[4 * w + e]);
-        }
+        for (int e = 0; e < 4; ++e) d[e] = digit_bytes((uint32_t)x[4 * w + e]);
         const uint32_t a = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), b = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
         const uint32_t c = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), e = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
         out[0][w] = (int)__builtin_amdgcn_perm(c, a, 0x05040100u);
