@@ -92,13 +92,18 @@ __device__ __forceinline__ bool sequence_of(const Sequences& s, uint32_t token, 
     } else i = token / (s.tokens / s.count);
     return sequence_at(s, i, q, bad) && token >= q.first && token - q.first < q.n;
 }
-// where a token's heads lie in a cache
-__device__ __forceinline__ size_t cache_at(const zk_i32_cache& c, uint32_t sequence, uint32_t t, uint32_t& bad) {
-    if (!c.page_table) return sequence * c.page_stride + t * c.token_stride;
-    const uint32_t in = t / c.page_size, page = (uint32_t)((const int32_t*)c.page_table)[(size_t)sequence * c.table_cols + in];
+// Where a token's heads lie in a cache, in two steps, so that the page is on its way while something else is done: its entry (without a table anything that can be read), then the place
+struct Page { int32_t entry; uint32_t place; };
+__device__ __forceinline__ Page page_of(const zk_i32_cache& c, uint32_t sequence, uint32_t t) {
+    const uint32_t in = c.page_table ? t / c.page_size : 0;
+    const int32_t* entry = c.page_table ? (const int32_t*)c.page_table + (size_t)sequence * c.table_cols + in : (const int32_t*)c.k;
+    return Page{*entry, t - in * c.page_size};
+}
+__device__ __forceinline__ size_t cache_at(const zk_i32_cache& c, uint32_t sequence, const Page& p, uint32_t& bad) {
+    const uint32_t page = c.page_table ? (uint32_t)p.entry : sequence;
     const bool has = page < c.pages;
     bad |= has ? 0u : (uint32_t)ZK_VALUES_POSITION;
-    return (has ? page : 0u) * c.page_stride + (t - in * c.page_size) * c.token_stride;
+    return (has ? page : 0u) * c.page_stride + p.place * c.token_stride;
 }
 
 // ---- append -------------------------------------------------------------------------------------------------------------------------------
@@ -120,7 +125,7 @@ template <int VEC> __global__ void __launch_bounds__(256) k_cache_append(const A
         if (t < 0) bad |= ZK_VALUES_POSITION;
         else {
             uint32_t off = 0;
-            const size_t to = cache_at(a.cache, s.index, (uint32_t)t, off);
+            const size_t to = cache_at(a.cache, s.index, page_of(a.cache, s.index, (uint32_t)t), off);
             bad |= off;
             for (uint32_t i = threadIdx.x; !off && i < 2 * a.heads * units; i += 256) {
                 const bool value = i >= a.heads * units;
@@ -241,15 +246,17 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
     const int32_t* keys = (const int32_t*)cache.k + kv * cache.head_stride;
     // row 4 q + e of a fragment's product is key 2 q + e, or 8 + 2 q + e - 2: four lanes store 64 bytes in one piece
     const uint32_t my_key = (c >> 2) * 2 + (c & 1u) + (c & 2u) * 4;
-    auto place = [&](uint32_t key) { return keys + cache_at(cache, t.own ? t.s.index : 0u, min(key + my_key, t.keys - 1), bad); };
+    const uint32_t sequence = t.own ? t.s.index : 0u;
+    auto page = [&](uint32_t key) { return page_of(cache, sequence, min(key + my_key, t.keys - 1)); };
     int32_t x[U][16];
-    auto fetch = [&](const int32_t* p) {
+    auto fetch = [&](const Page& at) {
+        const int32_t* p = keys + cache_at(cache, sequence, at, bad);
 #pragma unroll
         for (int u = 0; u < U; ++u) head_piece<HEADS, false>(p, u * 64 + q * 4, a.dim, x[u]);
     };
     uint32_t key = first + wave * 16;
-    if (key < end) fetch(place(key));
-    const int32_t* next = place(key + WAVES * 16);
+    Page next = page(key + WAVES * 16);
+    if (key < end) fetch(page(key));
     v4i b[RT][U][3];
     bool wide = false;
 #pragma unroll
@@ -275,8 +282,9 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
             digit_planes(x[u], k[u], bad);
             k_wide |= any_bits(k[u][3]);
         }
+        const Page after = page(key + 2 * WAVES * 16);
         if (key + WAVES * 16 < end) fetch(next);
-        next = place(key + 2 * WAVES * 16);
+        next = after;
         const bool four = q_wide || __any(k_wide);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -284,10 +292,11 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int m = 0; m < 3; ++m)
-#pragma unroll
-                    for (int n = 0; n < 3; ++n)
-                        acc[m + n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], b[r][u][n], u == 0 && (m == 0 || n == 2) ? v4i{0, 0, 0, 0} : acc[m + n], 0, 0, 0);      // a set's first
+                for (int i = 0; i < 9; ++i) {              // in an order that adds to no sum twice in a row
+                    constexpr int M[9] = {0, 0, 0, 1, 2, 1, 1, 2, 2}, N[9] = {0, 1, 2, 2, 2, 0, 1, 1, 0};
+                    const int sum = M[i] + N[i];
+                    acc[sum] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][M[i]], b[r][u][N[i]], u == 0 && i < 5 ? v4i{0, 0, 0, 0} : acc[sum], 0, 0, 0);
+                }
             int64_t v[4];
             if (!four) {
 #pragma unroll
@@ -685,6 +694,8 @@ template <int W, Weights KIND, Sums SUMS> __global__ void __launch_bounds__(W > 
     raise(a.flag, bad);
 }
 
+// the products of five digits by three in an order that adds to no sum twice in a row
+static constexpr int FIRST[15] = {0, 0, 0, 1, 2, 3, 4, 1, 1, 2, 3, 4, 2, 3, 4}, SECOND[15] = {0, 1, 2, 2, 2, 2, 2, 0, 1, 1, 1, 1, 0, 0, 0};
 // What becomes of sums of weights times values: an output element, or a part's sum as its low 64 bits and, in units of 2^32, its size: the parts' sizes together say whether the whole fits
 __device__ __forceinline__ void attn_finish(const AttnArgs& a, unsigned long long lo, int64_t size, uint32_t token, uint32_t head, uint32_t d, uint32_t& bad) {
     const int64_t v = (int64_t)lo;
@@ -709,11 +720,12 @@ template <Heads HEADS> __device__ __forceinline__ void values_of(const AttnArgs&
     if (first + stream * 64 >= end) return;
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride;
-    auto place = [&](uint32_t k) { return cache_at(cache, t.own ? t.s.index : 0u, min(k + lane, t.keys - 1), bad); };
-    size_t next = place(first + stream * 64);
+    const uint32_t sequence = t.own ? t.s.index : 0u;
+    auto page = [&](uint32_t k) { return page_of(cache, sequence, min(k + lane, t.keys - 1)); };
+    Page next = page(first + stream * 64);
     for (uint32_t k = first + stream * 64; k < end; k += 64 * streams) {
-        const size_t mine = next;
-        next = place(k + 64 * streams);                // looked up a step ahead
+        const size_t mine = cache_at(cache, sequence, next, bad);
+        next = page(k + 64 * streams);                     // looked up a step ahead
         v4i w[6];
 #pragma unroll
         for (int i = 0; i < 6; ++i) w[i] = *reinterpret_cast<const v4i*>(weights + i * ld + k);
@@ -730,9 +742,7 @@ template <Heads HEADS> __device__ __forceinline__ void values_of(const AttnArgs&
             digit_planes(x[n], v, bad);
             const bool four = __any(any_bits(v[3]));
 #pragma unroll
-            for (int i = 0; i < 5; ++i)
-#pragma unroll
-                for (int j = 0; j < 3; ++j) acc[i + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], v[j], acc[i + j][n], 0, 0, 0);
+            for (int i = 0; i < 15; ++i) acc[FIRST[i] + SECOND[i]][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[FIRST[i]], v[SECOND[i]], acc[FIRST[i] + SECOND[i]][n], 0, 0, 0);
             if (top)
 #pragma unroll
                 for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[5], v[j], acc[5 + j][n], 0, 0, 0);
@@ -873,11 +883,12 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
     const bool top = __any(a.top[row + mine] != 0);
     const int8_t* weights = a.weights + (row + mine) * 6 * a.ld + t.col0 + q * 16 + first;
     int32_t x[4][4];
-    auto place = [&](uint32_t i) { return cache_at(cache, t.own ? t.s.index : 0u, min(first + i * 64 + wave * 8 + (lane & 7u), t.keys - 1), bad); };
-    size_t next = 0;
+    const uint32_t sequence = t.own ? t.s.index : 0u;
+    auto page = [&](uint32_t i) { return page_of(cache, sequence, min(first + i * 64 + wave * 8 + (lane & 7u), t.keys - 1)); };
+    Page next{0, 0};
     auto fetch = [&](uint32_t i) {
-        const size_t at = next;
-        next = place(i + 1);                               // looked up a step ahead
+        const size_t at = cache_at(cache, sequence, next, bad);
+        next = page(i + 1);                                // looked up a step ahead
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const v4i v = four_of<HEADS>(values + __shfl((unsigned long long)at, (int)((kq & 1u) * 4 + e), 64), d0, a.dim);
@@ -919,7 +930,7 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
     if (threadIdx.x < 3) wide[threadIdx.x] = 0;
     __syncthreads();
     if (steps) {
-        next = place(0);
+        next = page(0);
         fetch(0);
         fetch_weights(0);
         split(0);
@@ -930,8 +941,8 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
 #pragma unroll
         for (int k = 0; k < 6; ++k) w[k] = *reinterpret_cast<const v4i*>(&weight[i & 1u][wave >> 1][k][lane][0]);
         if (i + 1 < steps) {
-            fetch_weights(i + 1);
             fetch(i + 1);
+            fetch_weights(i + 1);
         }
         if (threadIdx.x == 0) wide[(i + 2) % 3] = 0;       // read last in the step before, written next in the step behind
         const bool four = wide[i % 3] != 0;
@@ -941,9 +952,7 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
 #pragma unroll
             for (int j = 0; j < 3; ++j) v[j] = *reinterpret_cast<const v4i*>(&planes[i & 1u][j][block * 4 + n][lane][0]);
 #pragma unroll
-            for (int k = 0; k < 5; ++k)
-#pragma unroll
-                for (int j = 0; j < 3; ++j) acc[k + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[k], v[j], acc[k + j][n], 0, 0, 0);
+            for (int e = 0; e < 15; ++e) acc[FIRST[e] + SECOND[e]][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[FIRST[e]], v[SECOND[e]], acc[FIRST[e] + SECOND[e]][n], 0, 0, 0);
             if (top)
 #pragma unroll
                 for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[5], v[j], acc[5 + j][n], 0, 0, 0);
