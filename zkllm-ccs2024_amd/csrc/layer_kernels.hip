@@ -414,10 +414,9 @@ __device__ __forceinline__ void row_piece(const ProductArgs& g, uint32_t row, ui
 
 // x's planes for the products of many rows.  A workgroup takes 32 rows and CHUNK columns, 32 columns of a wave's 64 at a time: a lane 16 values of a row, so that the
 // wave writes 1 KB of every plane in one piece.  How many planes the stretch needs goes to a place of its own.  2048 x 4096: 14 us, 67 MB.
-__global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __restrict__ planes, uint32_t* __restrict__ need, v4i* __restrict__ zeros) {
-    __shared__ uint32_t most[4];
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) zeros[threadIdx.x] = v4i{0, 0, 0, 0};
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.y * 32 + (lane >> 1), k0 = blockIdx.x * CHUNK + wave * 64 + 16 * (lane & 1u), Kp = g.w.Kp;
+__device__ __forceinline__ void split_x(const ProductArgs& g, uint32_t bx, uint32_t by, int8_t* planes, uint32_t* need, v4i* zeros, uint32_t (&most)[4]) {
+    if (bx == 0 && by == 0 && threadIdx.x < 64) zeros[threadIdx.x] = v4i{0, 0, 0, 0};
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = by * 32 + (lane >> 1), k0 = bx * CHUNK + wave * 64 + 16 * (lane & 1u), Kp = g.w.Kp;
     uint32_t bad = 0, planes_needed = 1;
     int32_t x[2][16];
 #pragma unroll
@@ -438,8 +437,12 @@ __global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __
     for (int off = 32; off > 0; off >>= 1) planes_needed = max(planes_needed, (uint32_t)__shfl_xor(planes_needed, off, 64));
     if (lane == 0) most[wave] = planes_needed;
     __syncthreads();
-    if (threadIdx.x == 0) need[(size_t)blockIdx.y * g.chunks + blockIdx.x] = max(max(most[0], most[1]), max(most[2], most[3]));
+    if (threadIdx.x == 0) need[(size_t)by * g.chunks + bx] = max(max(most[0], most[1]), max(most[2], most[3]));
     raise(g.e.flag, bad);
+}
+__global__ void __launch_bounds__(256) k_split_x(const ProductArgs g, int8_t* __restrict__ planes, uint32_t* __restrict__ need, v4i* __restrict__ zeros) {
+    __shared__ uint32_t most[4];
+    split_x(g, blockIdx.x, blockIdx.y, planes, need, zeros, most);
 }
 
 // What becomes of a tile's sums: outputs, by divisors that are powers of two or any, or parts of sums
@@ -1148,14 +1151,27 @@ template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k
     }
     raise(g.e.flag, bad);
 }
-// the planes of a whole weight, for products of many rows
-template <int PB> __global__ void __launch_bounds__(256) k_q4_expand(int8_t* __restrict__ planes, const Q4 w) {
-    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4, strip = blockIdx.x, u = blockIdx.y * 4 + (threadIdx.x >> 6), col = strip * 16 + c;
+// Before a product of many rows, in one launch: the planes of one whole weight or two, and of x.  Workgroups of four waves: the weights' first, 16 columns by 256 inner rows each
+template <int PB> __device__ __forceinline__ void q4_expand(int8_t* planes, const Q4& w, uint32_t block) {
+    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4, strips = (w.cols + 15) / 16, strip = block % strips, u = block / strips * 4 + (threadIdx.x >> 6), col = strip * 16 + c;
     if (u >= w.units || col >= w.cols) return;
     v4i d[PB];
     q4_planes<PB>(q4_codes(w, strip, u, lane), q4_scale(w, strip, u * 64 + q * 16, c), d);
 #pragma unroll
     for (int j = 0; j < PB; ++j) *reinterpret_cast<v4i*>(planes + (size_t)j * w.cols * w.units * 64 + plane_at(w.cols, col, u * 64 + q * 16)) = d[j];
+}
+struct Q4Expand { Q4 w[2]; int8_t* planes[2]; int three[2]; uint32_t weights, blocks; };      // blocks: a weight's
+__global__ void __launch_bounds__(256) k_q4_expand(const Q4Expand e, const ProductArgs g, int8_t* __restrict__ planes, uint32_t* __restrict__ need, v4i* __restrict__ zeros) {
+    __shared__ uint32_t most[4];
+    const uint32_t of_weights = e.weights * e.blocks;
+    if (blockIdx.x < of_weights) {
+        const uint32_t i = blockIdx.x / e.blocks, block = blockIdx.x - i * e.blocks;
+        if (e.three[i]) q4_expand<3>(e.planes[i], e.w[i], block);
+        else q4_expand<2>(e.planes[i], e.w[i], block);
+    } else {
+        const uint32_t at = blockIdx.x - of_weights;
+        split_x(g, at % g.chunks, at / g.chunks, planes, need, zeros, most);
+    }
 }
 // Codes and scales to their places, and the largest element's magnitude.  bad[0]: a scale or zero out of range
 __global__ void __launch_bounds__(256) k_q4_scales(int32_t* __restrict__ out, const int32_t* __restrict__ scales, const uint8_t* __restrict__ zeros, uint32_t P, uint32_t groups, uint32_t* __restrict__ bad) {
@@ -1279,11 +1295,6 @@ template <bool GATED> static void launch_q4_strips(const Q4Args& q, hipStream_t 
 }
 // the planes that a product of many rows reads, in the workspace where the weight has none of its own
 static size_t expanded(const MatmulRhs* w, uint32_t rows) { return w->q4 && !q4_direct(w, w, rows) ? (size_t)std::max(w->pb, 2) * w->P * w->Kp : 0; }
-static void expand(const MatmulRhs* w, int8_t* planes, hipStream_t st) {
-    const dim3 grid(cdiv(w->P, 16), cdiv(w->Kp / 64, 4));
-    if (w->pb <= 2) hipLaunchKernelGGL(k_q4_expand<2>, grid, dim3(256), 0, st, planes, q4_of(w));
-    else hipLaunchKernelGGL(k_q4_expand<3>, grid, dim3(256), 0, st, planes, q4_of(w));
-}
 template <bool GATED> static int product(const char* name, ProductArgs& g, const MatmulRhs* w, const MatmulRhs* gate, void* flag_dev, void* workspace, size_t workspace_bytes, hipStream_t st) {
     ZK_ARG(g.x != nullptr && g.e.out != nullptr, std::string(name) + ": null tensor");
     ZK_ARG(g.x != g.e.out, std::string(name) + ": in place");
@@ -1316,15 +1327,22 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, const
             ZK_LAUNCH_CHECK();
             return flag.end(name);
         }
-    } else if (w->q4) {
+    }
+    Q4Expand e{};
+    if (w->q4 && !direct) {
+        e.weights = GATED ? 2 : 1;
+        e.blocks = cdiv(w->P, 16) * cdiv(w->Kp / 64, 4);
+        const MatmulRhs* of[2] = {w, gate};
         int8_t* at = (int8_t*)workspace + bytes;
-        expand(w, at, st);
-        g.w.p = at;
-        if constexpr (GATED) {
-            at += expanded(w, g.rows);
-            expand(gate, at, st);
-            g.gate.p = at;
+        for (int i = 0; i < (GATED ? 2 : 1); ++i) {
+            e.w[i] = q4_of(of[i]);
+            e.planes[i] = at;
+            e.three[i] = of[i]->pb > 2;
+            at += expanded(of[i], g.rows);
         }
+        g.w.p = e.planes[0];
+        g.gate.p = e.planes[1];
+        if (g.rows <= SPLIT_ROWS) hipLaunchKernelGGL(k_q4_expand, dim3(e.weights * e.blocks), dim3(256), 0, st, e, g, nullptr, nullptr, nullptr);
     }
     if (g.rows <= SPLIT_ROWS) {
         if (pb <= 2) launch_row<GATED, 2>(g, st);
@@ -1338,7 +1356,8 @@ template <bool GATED> static int product(const char* name, ProductArgs& g, const
     g.zeros = g.px + (size_t)4 * g.rows_padded * g.w.Kp;
     g.need = (const uint32_t*)(g.zeros + 1024);
     g.parts = may_split(g.rows, g.inner) ? (int64_t*)((char*)workspace + bytes - PARTS_BYTES) : nullptr;
-    hipLaunchKernelGGL(k_split_x, dim3(g.chunks, g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
+    if (e.weights) hipLaunchKernelGGL(k_q4_expand, dim3(e.weights * e.blocks + g.chunks * (g.rows_padded / 32)), dim3(256), 0, st, e, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
+    else hipLaunchKernelGGL(k_split_x, dim3(g.chunks, g.rows_padded / 32), dim3(256), 0, st, g, (int8_t*)workspace, (uint32_t*)g.need, (v4i*)g.zeros);
     if (direct) {
         q.g = g;
         launch_q4_strips<GATED>(q, st);
