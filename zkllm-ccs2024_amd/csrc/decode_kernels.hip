@@ -163,7 +163,8 @@ struct AttnArgs {
     uint32_t* unsure;                    // how many rows need their sum in order, three words, the rows
     size_t ld;                           // a multiple of 64
     int64_t* shift_out;                  // [token][head], or null
-    int64_t* parts;                      // [split][head of keys][row][dim][2]
+    int64_t* parts;                      // [split][head of keys][row][dim]: sums' sizes
+    uint32_t* parts_low;                 // as many: their low 32 bits
     int direct;                          // the keys are one part: its sums are the outputs
     SplitPart split[2];                  // of the prefix and of the own keys
     uint32_t split_tiles[2];             // of 16 keys, a multiple of four
@@ -618,10 +619,10 @@ template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x
     return t;
 }
 // W waves a row, eight neighbouring keys a lane at a time.  The sum of exponentials is taken in no order first, from exponentials that are near: off from the sum in
-// order by at most (keys + 64) 2^-53 of it and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 40 at 2048 keys and
+// order by at most 2^-53 of all of that one's partial sums (half of the keys times the whole, where terms are alike) and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 40 at 2048 keys and
 // a scale of 2^32 sqrt(128)); then the sum in order is taken -- by a launch of its own for such rows, where there are many rows --, the waves' runs at once where the sum stays within a power of
 // two, and the few others one after the other.
-template <int W> struct RowShared { double sums[W], in_order; Steps steps[W]; int at_exponent[W]; uint32_t any_top; };
+template <int W> struct RowShared { double sums[W], partial[W], in_order; Steps steps[W]; int at_exponent[W]; uint32_t any_top; };
 // A row's scores x to its weights, zeros up to `fill`; ld from digit to digit.  false: its sum must be taken in order (SUMS NEAR)
 template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softmax_row(const SoftmaxArgs& s, const int64_t* x, int8_t* weights, size_t ld, const Columns& columns, uint32_t fill,
                                                                                       const int32_t* live, const double* power, RowShared<W>& sh, int64_t& shift, bool& top, uint32_t& bad) {
@@ -651,31 +652,33 @@ template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softma
     shift = 0;
     bool sure = columns.end == 0, loaded = false;
     if constexpr (SUMS != Sums::IN_ORDER) {
-        double total = 0.0;
+        double total = 0.0, partial = 0.0;            // partial: of all the sums on the way, each of which is rounded once
         for (uint32_t i = 0; i < stretches; ++i) {
             load(i);
+            const double before = total;
 #pragma unroll
             for (int e = 0; e < M; ++e) {
                 total += exp_near(v[e], s, power);
                 if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);      // more of them at once crowd the registers
             }
+            partial += (total - before) * (double)(columns.end - min(columns.end, i * T * M + tid * M));
         }
         loaded = stretches == 1;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+        for (int off = 32; off > 0; off >>= 1) { total += __shfl_xor(total, off, 64); partial += __shfl_xor(partial, off, 64); }
         if constexpr (W > 1) {
             __syncthreads();                           // the arrays' last use is over
-            if (lane == 0) sh.sums[wave] = total;
+            if (lane == 0) { sh.sums[wave] = total; sh.partial[wave] = partial; }
             __syncthreads();
-            total = 0.0;
+            total = partial = 0.0;
 #pragma unroll
-            for (int i = 0; i < W; ++i) total += sh.sums[i];
+            for (int i = 0; i < W; ++i) { total += sh.sums[i]; partial += sh.partial[i]; }
         }
         if (columns.end) {
-            // Both sums' exponentials of x together are off by 8e-16 and 3.9e-16 |x|; weighted by what they have in the sum t, |x| is |ln t| + 17 at most (17: the logarithm of more keys than
+            // The sum in order is off by 2^-53 of each sum on its way, this one by as much of the whole for each of a lane's terms.  Both sums' exponentials of x together are off by 8e-16 and 3.9e-16 |x|; weighted by what they have in the sum t, |x| is |ln t| + 17 at most (17: the logarithm of more keys than
             // there can be).  Both logarithms are off by 4e-16 of them and their products with the scale by 2^-53.
             const double ln = zkd::log_det(total), sv = s.scale * ln;
-            const double off = s.scale * ((double)(columns.end + 64) * 1.2e-16 + 1.5e-15 * fabs(ln) + 8e-15), from_border = fabs(sv - floor(sv) - 0.5);
+            const double off = s.scale * ((partial / total + (double)(columns.end / 64 + 64)) * 1.2e-16 + 1.5e-15 * fabs(ln) + 8e-15), from_border = fabs(sv - floor(sv) - 0.5);
             sure = total > 1e-280 && total < 1e280 && off < 0.25 && from_border > off;
             if (sure) shift = rounded(sv);
         }
@@ -787,7 +790,8 @@ template <int W, Weights KIND, Sums SUMS> __global__ void __launch_bounds__(W > 
 
 // the products of five digits by three in an order that adds to no sum twice in a row
 static constexpr int FIRST[15] = {0, 0, 0, 1, 2, 3, 4, 1, 1, 2, 3, 4, 2, 3, 4}, SECOND[15] = {0, 1, 2, 2, 2, 2, 2, 0, 1, 1, 1, 1, 0, 0, 0};
-// What becomes of sums of weights times values: an output element, or a part's sum as its low 64 bits and, in units of 2^32, its size: the parts' sizes together say whether the whole fits
+// What becomes of sums of weights times values: an output element, or a part's sum as its low 32 bits and, in units of 2^32, its size: twelve bytes, and the parts' sizes together
+// say whether the whole fits
 __device__ __forceinline__ void attn_finish(const AttnArgs& a, unsigned long long lo, int64_t size, uint32_t token, uint32_t head, uint32_t d, uint32_t& bad) {
     const int64_t v = (int64_t)lo;
     if (size > (3ll << 29) || size < -(3ll << 29) || v >= (1ll << 62) || v < -(1ll << 62)) { bad |= ZK_VALUES_RANGE; return; }
@@ -891,10 +895,11 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(cons
     __syncthreads();
     if (!a.direct) {
         const size_t all = (size_t)a.heads_here * a.tokens * a.group;
-        unsigned long long* out = (unsigned long long*)a.parts + (((t.own ? a.prefix_splits : 0) + blockIdx.y) * all + row) * a.dim * 2;
-        for (uint32_t i = (t.lo - t.row0) * a.dim * 2 + threadIdx.x; i < (t.hi - t.row0) * a.dim * 2; i += 256) {
-            const uint32_t r = i / (2 * a.dim);
-            out[i] = sums64[r * blocks * 128 + (i - r * 2 * a.dim)];
+        const size_t out = (((t.own ? a.prefix_splits : 0) + blockIdx.y) * all + row) * a.dim;
+        for (uint32_t i = (t.lo - t.row0) * a.dim + threadIdx.x; i < (t.hi - t.row0) * a.dim; i += 256) {
+            const uint32_t r = i / a.dim, at = (r * blocks * 64 + (i - r * a.dim)) * 2;
+            a.parts_low[out + i] = (uint32_t)sums64[at];
+            a.parts[out + i] = (int64_t)sums64[at + 1] + (uint32_t)((uint32_t)(sums64[at] >> 32) - (uint32_t)sums64[at + 1]);      // and what the waves' low halves carry
         }
     } else finish_tile(a, t, kv, sums64, blocks, 256, bad);
     raise(a.flag, bad);
@@ -954,26 +959,35 @@ template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(51
 }
 // what a wave has of a tile's sums: 16 rows from row_in on by 64 dimensions from d0 on, of head z of the launch
 __device__ __forceinline__ void tile_out(const AttnArgs& a, const Tile& t, int own, uint32_t kv, uint32_t z, size_t row, uint32_t row_in, uint32_t d0, const v4i (&acc)[9][4], uint32_t& bad) {
-    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4;
+    typedef long long v2l __attribute__((ext_vector_type(2)));
+    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4, d = d0 + 4 * c;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const uint32_t at = row_in + 4 * q + e, in = t.row0 + at, token = in / a.group;
-        if (!t.has(at)) continue;
+        if (!t.has(at) || d >= a.dim) continue;
+        unsigned long long lo[4];
+        int64_t size[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-            const uint32_t d = d0 + 4 * c + n;
-            if (d >= a.dim) continue;
             int32_t s[9];
 #pragma unroll
             for (int i = 0; i < 9; ++i) s[i] = acc[i][n][e];
-            unsigned long long lo;
-            int64_t size;
-            attn_sum<9>(s, lo, size);
+            attn_sum<9>(s, lo[n], size[n]);
+        }
+        const size_t part = (((own ? a.prefix_splits : 0) + blockIdx.y) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d;
+        if (!a.direct && a.dim % 4 == 0) {
+            *reinterpret_cast<v4i*>(a.parts_low + part) = v4i{(int32_t)lo[0], (int32_t)lo[1], (int32_t)lo[2], (int32_t)lo[3]};
+            *reinterpret_cast<v2l*>(a.parts + part) = v2l{size[0], size[1]};
+            *reinterpret_cast<v2l*>(a.parts + part + 2) = v2l{size[2], size[3]};
+            continue;
+        }
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            if (d + n >= a.dim) continue;
             if (!a.direct) {
-                unsigned long long* out = (unsigned long long*)a.parts + ((((own ? a.prefix_splits : 0) + blockIdx.y) * ((size_t)a.heads_here * a.tokens * a.group) + row + at) * a.dim + d) * 2;
-                out[0] = lo;
-                out[1] = (unsigned long long)size;
-            } else attn_finish(a, lo, size, token, kv * a.group + (in - token * a.group), d, bad);
+                a.parts_low[part + n] = (uint32_t)lo[n];
+                a.parts[part + n] = size[n];
+            } else attn_finish(a, lo[n], size[n], token, kv * a.group + (in - token * a.group), d + n, bad);
         }
     }
 }
@@ -1187,12 +1201,13 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     unsigned long long lo = 0, size = 0;
     if (has) {
         const uint32_t parts = a.prefix_splits + own;
-        const unsigned long long* p = (const unsigned long long*)a.parts + ((size_t)r * a.dim + d) * 2;
+        const size_t at = (size_t)r * a.dim + d;
 #pragma unroll 4
         for (uint32_t i = share; i < parts; i += 4) {
-            lo += p[i * all * a.dim * 2];
-            size += p[i * all * a.dim * 2 + 1];
+            lo += a.parts_low[i * all * a.dim + at];
+            size += (unsigned long long)a.parts[i * all * a.dim + at];
         }
+        lo += size << 32;
     }
     sums[share][lane][0] = lo;
     sums[share][lane][1] = size;
@@ -1353,7 +1368,7 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
 static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
 
 // How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
-struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts, split_each; bool split[2]; uint32_t split_tiles[2]; };      // split_each: a head's
+struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts_high, parts, split_each; bool split[2]; uint32_t split_tiles[2]; };      // split_each: a head's
 // From so many rows of a head of keys on its keys and values are split once for all of them. 8 heads of 128: at 128 rows over 8192 keys the split, scores and values take 25 + 35 + 53 us, tiles that each split
 // what they read 46 + 64; at 2048 rows over as many keys 12 + 66 + 73 against 97 + 99
 static constexpr size_t SPLIT_ROWS_FROM = 256;
@@ -1382,7 +1397,7 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     cut(sequences ? max_length : 0, p.own_tiles, p.own64, p.own_splits, p.own_step);
     const uint32_t splits = p.prefix_splits + p.own_splits;
     p.direct = splits == 1;
-    const size_t each = rows * (p.cols * 14 + 8 + (size_t)(p.direct ? 0 : splits) * dim * 16);
+    const size_t each = rows * (p.cols * 14 + 8 + (size_t)(p.direct ? 0 : splits) * dim * 12);
     p.heads = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / std::max<size_t>(each, 1)));
     if (p.heads < kv_heads && p.own64 && p.own_splits == 1) {      // as many as fill the compute units evenly, one workgroup each
         auto used = [&](uint32_t h) { const size_t w = rows / 64 * h * cdiv(dim, 128); return w ? (double)w / (cdiv(w, 256) * 256.0) : 0.0; };
@@ -1400,7 +1415,8 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     p.weights = p.heads * rows * p.cols * 6;
     p.top = round(p.heads * rows * 4);
     p.unsure = 16 + p.top;
-    p.parts = p.heads * rows * (size_t)(p.direct ? 0 : splits) * dim * 16;
+    p.parts_high = round(p.heads * rows * (size_t)(p.direct ? 0 : splits) * dim * 8);
+    p.parts = round(p.parts_high + p.parts_high / 2);
     return p;
 }
 
@@ -1557,7 +1573,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     a.seqs = Sequences{own ? (const int32_t*)starts : nullptr, (const int32_t*)lengths, sequences, tokens, max_length};
     a.causal = causal; a.sf_first = divisor(sf_first); a.sf_second = divisor(sf_second);
     a.scores = (int64_t*)workspace; a.ld = p.cols; a.weights = (int8_t*)workspace + p.scores; a.top = (uint32_t*)(a.weights + p.weights);
-    a.unsure = (uint32_t*)((char*)a.top + p.top); a.parts = (int64_t*)((char*)a.unsure + p.unsure); a.direct = p.direct;
+    a.unsure = (uint32_t*)((char*)a.top + p.top); a.parts = (int64_t*)((char*)a.unsure + p.unsure); a.parts_low = (uint32_t*)((char*)a.parts + p.parts_high); a.direct = p.direct;
     {
         int8_t* at = (int8_t*)a.parts + p.parts;
         for (int i = 0; i < 2; ++i) {
