@@ -466,6 +466,24 @@ __device__ __forceinline__ Steps steps_up_to(Steps s) {
     }
     return s;
 }
+// steps over the lanes from this one on
+__device__ __forceinline__ Steps steps_from(Steps s) {
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const Steps behind{__shfl_down(s.even, off, 64), __shfl_down(s.odd, off, 64)};
+        const Steps both = then(s, behind);
+        if (lane + (uint32_t)off < 64) s = both;
+    }
+    return s;
+}
+__device__ __forceinline__ uint64_t of_lane(uint64_t x, uint32_t lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), (int)lane) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, (int)lane);
+}
+__device__ __forceinline__ double of_lane(double x, uint32_t lane) { return zkd::bits_to_double(of_lane(zkd::double_to_bits(x), lane)); }
+__device__ __forceinline__ uint64_t uniform(uint64_t x) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+}
 // total with the terms of 64 lanes added, lane by lane, M in a lane
 template <int M> __device__ __forceinline__ double add_in_order(double total, const double (&x)[M]) {
     const uint32_t lane = threadIdx.x & 63u;
@@ -476,7 +494,7 @@ template <int M> __device__ __forceinline__ double add_in_order(double total, co
         for (int i = 0; i < M; ++i) any |= x[i] != 0.0;
         const unsigned long long left = __ballot(any && lane >= from);
         if (left == 0 || !(total < __builtin_inf())) return total;
-        uint32_t at = (uint32_t)__builtin_ctzll(left), until = min(at + 128 / M, 64u);      // a row's first terms: every few of them leave a power of two
+        uint32_t at = (uint32_t)__builtin_ctzll(left), until = min(at + 64 / M, 64u);      // a row's first terms: every few of them leave a power of two
         if (total > 0.0) {
             const int e = exponent(total);
             const uint64_t t = units_of(total);
@@ -498,11 +516,7 @@ template <int M> __device__ __forceinline__ double add_in_order(double total, co
         }
         for (; at < until; ++at)
 #pragma unroll
-            for (int i = 0; i < M; ++i) {
-                const uint64_t t = zkd::double_to_bits(x[i]);
-                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)t, (int)at), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(t >> 32), (int)at);
-                total = total + zkd::bits_to_double((uint64_t)hi << 32 | lo);
-            }
+            for (int i = 0; i < M; ++i) total = total + of_lane(x[i], at);
         from = until;
         if (from == 64) return total;
     }
@@ -554,66 +568,148 @@ __device__ __forceinline__ double exp_near(int64_t v, const SoftmaxArgs& s, cons
     asm("v_cvt_i32_f64 %0, %1" : "=v"(i) : "v"(n));
     return ldexp(power[i & 63] * p, i >> 6);
 }
+// zkd::exp_det(x) operation for operation, without branches and with the constants in scalar registers
+__device__ __forceinline__ double exp_exact(double x) {
+    const double at = __builtin_fmin(__builtin_fmax(x, -708.0), 709.0);
+    const double kf = at * 1.44269504088896338700e+00;
+    const int k = (int)(kf + (kf >= 0 ? 0.5 : -0.5));
+    const double kd = (double)k, r = __builtin_fma(-kd, 1.90821492927058770002e-10, __builtin_fma(-kd, 6.93147180369123816490e-01, at));
+    double p = fma_s(r, 1.0 / 87178291200.0, 1.0 / 6227020800.0);
+    p = fma_s(p, r, 1.0 / 479001600.0);
+    p = fma_s(p, r, 1.0 / 39916800.0);
+    p = fma_s(p, r, 1.0 / 3628800.0);
+    p = fma_s(p, r, 1.0 / 362880.0);
+    p = fma_s(p, r, 1.0 / 40320.0);
+    p = fma_s(p, r, 1.0 / 5040.0);
+    p = fma_s(p, r, 1.0 / 720.0);
+    p = fma_s(p, r, 1.0 / 120.0);
+    p = fma_s(p, r, 1.0 / 24.0);
+    p = fma_s(p, r, 1.0 / 6.0);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    const double y = ldexp(p, k);              // exact: a normal number
+    return x > 709.0 ? __builtin_inf() : x < -708.0 ? 0.0 : y;
+}
 // the columns of a row's scores: the prefix's, then, from a multiple of 64 on, its own
 struct Columns {
     uint32_t prefix_len, prefix_cols, own_end, end;
     __device__ uint32_t keys_at(uint32_t j) const { return j < prefix_cols ? (j < prefix_len ? min(8u, prefix_len - j) : 0u) : j < own_end ? min(8u, own_end - j) : 0u; }      // of eight from j on
 };
-// the sum of a row's exponentials in the order of the keys, by W waves
-template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x, Columns columns, double scale, double scale_inv, double* sums, Steps* steps, int* at_exponent, double* in_order) {
-    constexpr int M = 8, T = 64 * W;
-    const uint32_t lane = threadIdx.x & 63u, wave = W == 1 ? 0 : threadIdx.x >> 6, tid = wave * 64 + lane;
-    auto wave_sum = [](double t) {
+// n of eight scores, and in place of the others no keys
+__device__ __forceinline__ void eight_scores(const int64_t* x, uint32_t n, int64_t (&v)[8]) {
+    typedef long long v2l __attribute__((ext_vector_type(2)));
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) t += __shfl_xor(t, off, 64);
-        return t;
-    };
+    for (int i = 0; i < 8; ++i) v[i] = NO_KEY;
+    if (n == 0) return;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const v2l p = *reinterpret_cast<const v2l*>(x + i);
+        v[i] = p[0]; v[i + 1] = p[1];
+    }
+    if (n < 8)
+#pragma unroll
+        for (int i = 1; i < 8; ++i) v[i] = i < (int)n ? v[i] : NO_KEY;
+}
+static constexpr int NO_EXPONENT = 2000;
+template <int W> struct RowShared { double sums[W], partial[W], in_order[2]; Steps steps[W]; int at_exponent[W]; uint32_t any_top; };
+// the sum of a row's exponentials in the order of the keys, by one wave
+__device__ __forceinline__ double sum_in_order(const int64_t* x, const Columns& columns, double scale, double scale_inv) {
+    const uint32_t lane = threadIdx.x & 63u;
     double t = 0.0;
-    constexpr int N = W == 1 ? 2 : M;          // a lane's terms at a time: few, where the registers hold a row's scores
-    for (uint32_t j0 = 0; j0 < columns.end; j0 += T * N) {
-        {
-            const uint32_t j = j0 + tid * N, in8 = j & 7u, keys8 = columns.keys_at(j - in8), keys = keys8 > in8 ? keys8 - in8 : 0u;
-            double term[N], mine = 0.0;
+    for (uint32_t j0 = 0; j0 < columns.end; j0 += 128) {      // few at a time: the registers hold a row's scores
+        const uint32_t j = j0 + lane * 2, in8 = j & 7u, keys8 = columns.keys_at(j - in8), keys = keys8 > in8 ? keys8 - in8 : 0u;
+        double term[2];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                term[e] = e < (int)keys ? zkd::exp_det(divided(x[j + e], scale, scale_inv)) : 0.0;
-                mine += term[e];
-            }
-            if constexpr (W == 1) t = add_in_order<N>(t, term);
-            else {
-                mine = wave_sum(mine);
-                __syncthreads();
-                if (lane == 0) sums[wave] = mine;
-                __syncthreads();
-                double before = t;
-                for (uint32_t k = 0; k < wave; ++k) before += sums[k];
-                const double behind = before + mine;
-                // a run that stays within a power of two, by a margin that the sums' order cannot reach
-                const int e = before > 0.0 && behind < __builtin_inf() ? exponent(behind * (1.0 + 1e-9)) : 2000;
-                const bool clean = e != 2000 && exponent(before * (1.0 - 1e-9)) == e;
-                if (clean) {
-                    Steps st{0, 0};
+        for (int e = 0; e < 2; ++e) term[e] = e < (int)keys ? zkd::exp_det(divided(x[j + e], scale, scale_inv)) : 0.0;
+        t = add_in_order<2>(t, term);
+    }
+    return t;
+}
+// ... by W waves, 512 keys each at a time.  What a wave's terms do to the sum is made ready by all waves at once, for the power of two that the sum will be in, or the two, as sums in no order say; then the
+// sum goes from wave to wave: over one that stays within its power of two in every wave at once, through one that leaves it up to the lane that does, that lane's terms and the lanes behind it, and through
+// one that leaves several, as a row's first, by one
+// power of two after the other (term by term each takes 35 cycles).
+template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x, const Columns& columns, double scale, double scale_inv, RowShared<W>& sh) {
+    constexpr int M = 8, T = 64 * W;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    uint32_t slot = 0;
+    double t = 0.0;
+    for (uint32_t j0 = 0; j0 < columns.end; j0 += T * M) {
+        const uint32_t j = j0 + threadIdx.x * M, keys = columns.keys_at(j);
+        double term[M], mine = 0.0;
+        int64_t v[M];
+        eight_scores(x + j, keys, v);
 #pragma unroll
-                    for (int k = 0; k < N; ++k) step(st, term[k], e);
-                    st = steps_up_to(st);
-                    if (lane == 63) steps[wave] = st;
-                }
-                if (lane == 0) at_exponent[wave] = clean ? e : 2000;
-                __syncthreads();
-                for (uint32_t k = 0; k < (uint32_t)W; ++k) {
-                    if (at_exponent[k] != 2000 && t > 0.0 && exponent(t) == at_exponent[k]) {
-                        const uint64_t u = units_of(t), after = u + (u & 1 ? steps[k].odd : steps[k].even);
-                        if (after < UNITS) { t = ldexp((double)after, at_exponent[k] - 52); continue; }
-                    }
-                    if (wave == k) {
-                        t = add_in_order<N>(t, term);
-                        if (lane == 0) *in_order = t;
-                    }
-                    __syncthreads();
-                    t = *in_order;
-                    __syncthreads();
-                }
+        for (int e = 0; e < M; ++e) {
+            term[e] = exp_exact(divided(v[e], scale, scale_inv));
+            mine += term[e];
+            if (e % 2 == 1) __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) mine += __shfl_xor(mine, off, 64);
+        __syncthreads();
+        if (lane == 0) sh.sums[wave] = mine;
+        __syncthreads();
+        double before = lane < wave ? sh.sums[lane] : 0.0;
+#pragma unroll
+        for (int off = 1; off < W; off <<= 1) before += __shfl_xor(before, off, 64);      // in the first W lanes
+        before = t + of_lane(before, 0);
+        const double behind = before + mine;
+        // the powers of two that the sum can be in, by a margin that the sums' order cannot reach
+        const bool known = before > 0.0 && behind < __builtin_inf();
+        const int low = known ? exponent(before * (1.0 - 1e-9)) : NO_EXPONENT, high = known ? exponent(behind * (1.0 + 1e-9)) : NO_EXPONENT;
+        const bool clean = known && low == high, one = known && low + 1 == high;
+        Steps up{0, 0}, rest{0, 0};
+        if (clean || one) {
+#pragma unroll
+            for (int k = 0; k < M; ++k) step(up, term[k], low);
+            up = steps_up_to(up);
+        }
+        if (one) {
+#pragma unroll
+            for (int k = 0; k < M; ++k) step(rest, term[k], high);
+            rest = steps_from(rest);
+        }
+        if (lane == 63) {
+            sh.steps[wave] = up;
+            sh.at_exponent[wave] = clean ? low : NO_EXPONENT;
+        }
+        __syncthreads();
+        const int es = sh.at_exponent[lane % W];
+        const Steps steps = sh.steps[lane % W];
+#pragma unroll 1                          // code that is run once waits for its instructions
+        for (uint32_t k = 0; k < (uint32_t)W; ++k) {
+            // steps within a power of two are what they add to t's bits
+            const uint64_t bits = uniform(zkd::double_to_bits(t));
+            if (bits != 0 && (int)(bits >> 52) - 1023 == __builtin_amdgcn_readlane(es, (int)k)) {
+                const uint64_t after = bits + (bits & 1 ? of_lane(steps.odd, k) : of_lane(steps.even, k));
+                if (after >> 52 == bits >> 52) { t = zkd::bits_to_double(after); continue; }
             }
+            if (wave == k) {
+                bool added = false;
+                if (one && t > 0.0 && exponent(t) == low) {
+                    const uint64_t u = units_of(t), after = u + (u & 1 ? up.odd : up.even);
+                    const unsigned long long out = __ballot(after >= UNITS);
+                    const uint32_t last = out ? (uint32_t)__builtin_ctzll(out) : 64u;      // the lane where the sum leaves 2^(low + 1)
+                    double r = last ? ldexp((double)__shfl(after, (int)last - 1, 64), low - 52) : t;
+                    if (last < 64)
+#pragma unroll
+                        for (int i = 0; i < M; ++i) r = r + of_lane(term[i], last);
+                    added = last >= 63;
+                    if (!added && exponent(r) == high) {
+                        const uint64_t v = units_of(r), even = __shfl(rest.even, (int)last + 1, 64), odd = __shfl(rest.odd, (int)last + 1, 64), end = v + (v & 1 ? odd : even);
+                        added = end < UNITS;
+                        r = ldexp((double)end, high - 52);
+                    }
+                    if (added) t = r;
+                }
+                if (!added) t = add_in_order<M>(t, term);
+                if (lane == 0) sh.in_order[slot] = t;
+            }
+            __syncthreads();
+            t = sh.in_order[slot];
+            slot ^= 1;                     // the next writer does not wait until every wave has read this one
         }
     }
     return t;
@@ -622,7 +718,6 @@ template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x
 // order by at most 2^-53 of all of that one's partial sums (half of the keys times the whole, where terms are alike) and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 40 at 2048 keys and
 // a scale of 2^32 sqrt(128)); then the sum in order is taken -- by a launch of its own for such rows, where there are many rows --, the waves' runs at once where the sum stays within a power of
 // two, and the few others one after the other.
-template <int W> struct RowShared { double sums[W], partial[W], in_order; Steps steps[W]; int at_exponent[W]; uint32_t any_top; };
 // A row's scores x to its weights, zeros up to `fill`; ld from digit to digit.  false: its sum must be taken in order (SUMS NEAR)
 template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softmax_row(const SoftmaxArgs& s, const int64_t* x, int8_t* weights, size_t ld, const Columns& columns, uint32_t fill,
                                                                                       const int32_t* live, const double* power, RowShared<W>& sh, int64_t& shift, bool& top, uint32_t& bad) {
@@ -634,19 +729,7 @@ template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softma
     auto load = [&](uint32_t stretch) {
         const uint32_t j = stretch * T * M + tid * M;
         n = columns.keys_at(j);
-#pragma unroll
-        for (int i = 0; i < M; ++i) v[i] = NO_KEY;
-        if (n) {
-            typedef long long v2l __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int i = 0; i < M; i += 2) {
-                const v2l p = *reinterpret_cast<const v2l*>(x + j + i);
-                v[i] = p[0]; v[i + 1] = p[1];
-            }
-            if (n < M)
-#pragma unroll
-                for (int i = 1; i < M; ++i) v[i] = i < (int)n ? v[i] : NO_KEY;
-        }
+        eight_scores(x + j, n, v);
     };
     auto rounded = [](double sv) { return sv >= 0 ? (int64_t)(sv + 0.5) : (int64_t)(sv - 0.5); };
     shift = 0;
@@ -687,7 +770,10 @@ template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softma
     }
     if constexpr (SUMS != Sums::NEAR)
         if (!sure) {
-            shift = rounded(s.scale * zkd::log_det(sum_in_order<W>(x, columns, s.scale, s.scale_inv, sh.sums, sh.steps, sh.at_exponent, &sh.in_order)));
+            double sum;
+            if constexpr (W == 1) sum = sum_in_order(x, columns, s.scale, s.scale_inv);
+            else sum = sum_in_order<W>(x, columns, s.scale, s.scale_inv, sh);
+            shift = rounded(s.scale * zkd::log_det(sum));
             loaded = false;                            // the registers were needed
         }
     // Both tables' values and their product are exact in double precision, and so is the number whose low 48 bits are the digits with 128 added to each
@@ -1184,10 +1270,10 @@ __global__ void __launch_bounds__(512, 2) k_attn_values_split(const AttnArgs a, 
     tile_out(a, t, own, kv, z, row, row_in, dim0 + block * 64, acc, bad);
     raise(a.flag, bad);
 }
-// The parts' sums added up, 64 outputs by four shares of the parts a workgroup; rows that see no key
-__global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
-    __shared__ unsigned long long sums[4][64][2];
-    const uint32_t share = threadIdx.x >> 6, lane = threadIdx.x & 63u;
+// The parts' sums added up, 64 outputs a workgroup, by four shares of the parts or, where outputs are few, sixteen; rows that see no key
+__global__ void __launch_bounds__(1024) k_attn_join(const AttnArgs a) {
+    __shared__ unsigned long long sums[16][64][2];
+    const uint32_t share = threadIdx.x >> 6, shares = blockDim.x >> 6, lane = threadIdx.x & 63u;
     const size_t id = (size_t)blockIdx.x * 64 + lane, rows = (size_t)a.tokens * a.group, all = a.heads_here * rows;
     const bool inside = id < all * a.dim;
     const uint32_t r = inside ? (uint32_t)(id / a.dim) : 0, d = (uint32_t)(id - (size_t)r * a.dim), kv = (uint32_t)(r / rows), in = (uint32_t)(r - kv * rows), token = in / a.group;
@@ -1203,7 +1289,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
         const uint32_t parts = a.prefix_splits + own;
         const size_t at = (size_t)r * a.dim + d;
 #pragma unroll 4
-        for (uint32_t i = share; i < parts; i += 4) {
+        for (uint32_t i = share; i < parts; i += shares) {
             lo += a.parts_low[i * all * a.dim + at];
             size += (unsigned long long)a.parts[i * all * a.dim + at];
         }
@@ -1213,8 +1299,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const AttnArgs a) {
     sums[share][lane][1] = size;
     __syncthreads();
     if (has && share == 0) {
-#pragma unroll
-        for (int i = 1; i < 4; ++i) { lo += sums[i][lane][0]; size += sums[i][lane][1]; }
+        for (uint32_t i = 1; i < shares; ++i) { lo += sums[i][lane][0]; size += sums[i][lane][1]; }
         attn_finish(a, lo, (int64_t)size, token, (a.kv0 + kv) * a.group + (in - token * a.group), d, bad);
     }
     raise(a.flag, bad);
@@ -1645,13 +1730,13 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
             const size_t lds = KIND == Weights::SERIES ? s->a.live * 4 : 0;
             if (rows < 256) {
                 if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(256), lds, st, a);
-                else hipLaunchKernelGGL((k_attn_softmax<16, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(1024), lds, st, a);
+                else hipLaunchKernelGGL((k_attn_softmax<8, KIND, Sums::BOTH>), dim3((unsigned)rows), dim3(512), lds, st, a);
                 return;
             }
             if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<1, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(cdiv(rows, 4), 1024)), dim3(256), lds, st, a);
             else hipLaunchKernelGGL((k_attn_softmax<4, KIND, Sums::NEAR>), dim3((unsigned)std::min<size_t>(rows, 1024)), dim3(256), lds, st, a);
             if (p.cols <= 2048) hipLaunchKernelGGL((k_attn_softmax<4, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 512)), dim3(256), lds, st, a);
-            else hipLaunchKernelGGL((k_attn_softmax<16, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 256)), dim3(1024), lds, st, a);
+            else hipLaunchKernelGGL((k_attn_softmax<8, KIND, Sums::IN_ORDER>), dim3((unsigned)std::min<size_t>(rows, 512)), dim3(512), lds, st, a);
         };
         if (s->series) softmax_rows(std::integral_constant<Weights, Weights::SERIES>());
         else if (s->pow2) softmax_rows(std::integral_constant<Weights, Weights::POW2>());
@@ -1667,7 +1752,7 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
                 heads_of([&](auto h) { hipLaunchKernelGGL(k_attn_values<decltype(h)::value>, grid, dim3(256), lds, st, a, of_own); });
             }
         });
-        if (!p.direct) hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 64)), dim3(256), 0, st, a);
+        if (!p.direct) hipLaunchKernelGGL(k_attn_join, dim3(cdiv(rows * dim, 64)), dim3(rows * dim < 65536 ? 1024 : 256), 0, st, a);
     }
     ZK_LAUNCH_CHECK();
     return flag.end(name);
