@@ -444,6 +444,17 @@ def test_attention_in_tiles(hip, counts, lengths, heads, kv_heads, dim, prefix_l
         assert (got[n:] == -77).all()
 
 
+@gpu
+def test_attention_of_many_tokens_without_keys(hip):
+    n, heads, dim = 600, 32, 64
+    own = Pages(np.random.default_rng(3), 1, 1, heads, dim, 16)
+    q = dev(normal(np.random.default_rng(4), (n + 1, heads, dim)))
+    for causal in (True, False):
+        flag = new_flag()
+        out = host(attend(hip, q, Plan(hip, dec.Softmax(dim=dim)), None, 0, own, 1, dev([0, n]), dev([0]), 0, causal, heads, flag=flag))
+        assert host(flag)[0] == 0 and (out[:n] == 0).all() and (out[n] == -77).all()
+
+
 # ---- weights of 4 bits -----------------------------------------------------------------------------------------------------------------------
 class Q4:
     def __init__(self, hip, rng, N, P, group, zeros=True, most=800):
@@ -876,7 +887,7 @@ ATTENTION_REFUSALS = [
     ({"own": None, "most": 0}, "neither a prefix"), ({"own": None, "prefix_len": 4}, "neither a prefix"), ({"prefix_len": 4}, "no prefix"), ({"seqs": 0}, "need lengths"), ({"lengths": None}, "need lengths"),
     ({"own": None, "prefix": {}, "prefix_len": 4}, "own keys without"), ({"tokens": 5}, "divide among"), ({"sf": (0, 1)}, "factor of 0"), ({"sf": (1, 0)}, "factor of 0"), ({"q": "out", "q_token": 12}, "in place"),
     ({"out_token": 3}, "heads overlap"), ({"out_head": 3}, "heads overlap"), ({"out_token": 7}, "output's heads overlap"), ({"prefix": {"page_size": 3}, "prefix_len": 4}, "fewer places"),
-    ({"own": {"page_size": 3}}, "fewer places"), ({"own": {"k": None}}, "without keys"), ({"own": {"page_stride": 63}}, "pages overlap"), ({"bytes": 5, "workspace": 16}, "the workspace is smaller"),
+    ({"own": {"page_size": 3}}, "fewer places"), ({"own": {"k": None}}, "without keys"), ({"own": {"page_stride": 63}}, "pages overlap"), ({"bytes": 5, "workspace": 16, "most": 5000, "own": {"page_size": 5000, "page_stride": 40000}}, "the workspace is smaller"),
     ({"bytes": 1 << 30, "workspace": 8}, "multiple of 16")]
 
 
@@ -892,6 +903,16 @@ def test_attention_refusals(change, text):
     refused("zk_i32_attention", [a["out"], c_size_t(a["out_token"]), c_size_t(a["out_head"]), a["q"], c_size_t(a["q_token"]), c_size_t(a["q_head"]), c_uint(a["tokens"]), c_uint(a["heads"]), c_uint(a["kv_heads"]),
                                  c_uint(a["dim"]), a["plan"], None if pc is None else ctypes.byref(pc), c_uint(a["prefix_len"]), None if oc is None else ctypes.byref(oc), c_uint(a["seqs"]), None, a["lengths"],
                                  c_uint(a["most"]), c_int(1), c_uint(a["sf"][0]), c_uint(a["sf"][1]), None, c_void_p(a["workspace"]), c_size_t(a["bytes"]), W, None], text)
+
+
+def test_attention_workspace_of_the_longest_caches():
+    """Keys and values are split once for many rows as long as a launch can have as many workgroups"""
+    from gpuhelp import pkg
+    workspace_of, most = pkg.load_hip().zk_i32_attention_workspace, 65535 * 64
+    workspace_of.restype = c_size_t
+    size = [workspace_of(c_uint(256), c_uint(1), c_uint(1), c_uint(128), c_uint(keys), c_uint(0), c_uint(0)) for keys in (most, most + 64, 1 << 24)]
+    # a key's row of scores and weights: 256 x 14 bytes, its digits: 128 x 8; parts of 8192 keys, one more for the longest by each as many
+    assert size[0] >= most * (256 * 14 + 128 * 8) > size[1] >= (most + 64) * 256 * 14 and size[2] >= (1 << 24) * 256 * 14
 
 
 def test_q4_refusals():

@@ -1445,7 +1445,7 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
     ZK_ARG((c->page_size == 1 || c->token_stride >= dim) && (heads == 1 || c->head_stride >= dim), std::string(name) + ": a cache whose heads overlap (a stride below the head's width)");
     const unsigned __int128 of_heads = (unsigned __int128)(heads - 1) * c->head_stride + dim, of_tokens = (unsigned __int128)(c->page_size - 1) * c->token_stride + dim;
     ZK_ARG(heads == 1 || c->page_size == 1 || c->token_stride >= of_heads || c->head_stride >= of_tokens, std::string(name) + ": a cache whose heads overlap");
-    const unsigned __int128 page = std::max((unsigned __int128)(heads - 1) * c->head_stride + (unsigned __int128)(c->page_size - 1) * c->token_stride + dim, (unsigned __int128)0);
+    const unsigned __int128 page = (unsigned __int128)(heads - 1) * c->head_stride + (unsigned __int128)(c->page_size - 1) * c->token_stride + dim;
     ZK_ARG(c->pages == 1 || c->page_stride >= page || (heads > 1 && c->head_stride >= (unsigned __int128)(c->pages - 1) * c->page_stride + of_tokens && c->page_stride >= of_tokens),
            std::string(name) + ": a cache whose pages overlap");
     return 0;
@@ -1465,7 +1465,7 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     p.prefix_cols = ((size_t)prefix_len + 63) / 64 * 64;
     p.cols = p.prefix_cols + ((size_t)max_length + 63) / 64 * 64;
     const size_t small_tiles = sequences ? rows / 16 + sequences : cdiv(rows, 16);
-    p.small = p.cols <= SMALL_COLS && small_tiles * kv_heads <= 512;
+    p.small = p.cols == 0 || (p.cols <= SMALL_COLS && small_tiles * kv_heads <= 512);
     if (p.small) { p.own_tiles = (uint32_t)small_tiles; p.heads = kv_heads; return p; }
     p.prefix64 = rows > 16;
     p.own64 = sequences && rows / sequences > 32;
@@ -1490,7 +1490,7 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     }
     auto round = [](size_t b) { return (b + 15) / 16 * 16; };
     auto part = [&](bool many, uint32_t keys, int i) {
-        p.split[i] = many && keys && rows >= SPLIT_ROWS_FROM;
+        p.split[i] = many && keys && rows >= SPLIT_ROWS_FROM && keys <= 65535u * 64;      // a grid's second side
         p.split_tiles[i] = p.split[i] ? cdiv(keys, 64) * 4 : 0;
     };
     part(p.prefix64, prefix_len, 0);
