@@ -551,9 +551,10 @@ typedef struct zk_i32_cache {
 int zk_i32_cache_append(const zk_i32_cache* cache, const void* k, size_t k_token, size_t k_head, const void* v, size_t v_token, size_t v_head, uint32_t tokens, uint32_t kv_heads, uint32_t dim,
                         uint32_t sequences, const void* starts_i32, const void* lengths_i32, void* flag_dev, void* stream);
 /* The softmax of zkSoftmax (zksoftmax.cu:34-93) for heads of dim elements: K digits of radices bs, the lowest L not looked at, the highest M zero or the weight is, those between mapped to
- * thetas' exponentials (K - L - M of them).  Radices up to 2^28 and their product up to 2^63, thetas' product below 1.4e14.  Waits for the stream; any stream may use the handle afterwards. */
+ * thetas' exponentials (K - L - M of them).  Radices up to 2^28 and their product up to 2^63, thetas' product below 1.4e14, scaling_factor_in sqrt(dim) up to 2^53.  Waits for the stream; any stream may use the handle afterwards. */
 int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs_host, int K, int L, int M, double scaling_factor_in, const double* thetas_host, uint32_t dim, void* stream);
 int zk_i32_softmax_free(void* softmax);          /* once its last call is through */
+/* 0 for short calls (a few tokens over up to 576 keys), which need none; otherwise 14 bytes for every row and key of as many heads as fit 512 MB, or of one head */
 size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length);
 /* Attention of queries over the keys and values of a prefix that all sequences share (read once for all of them) and, behind it, of their sequences' own (self-attn.cu:81-98,
  * zksoftmax.cu:112-173):  x_j = q . k_j,  shift = the nearest integer to scale ln(sum_j exp(x_j / scale)), scale = scaling_factor_in sqrt(dim),  y_j = the product of the tables' values at
@@ -562,8 +563,7 @@ size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_h
  * q, out: tokens x heads of dim elements with strides; out may be q with the same strides and overlaps nothing else.  Head h reads keys and values of head h / (heads / kv_heads).  Tokens belong to sequences
  * as in zk_i32_cache_append, with their keys already in the cache; tokens of none are left as they are.  lengths[s] is 0 .. max_length, which bounds the work and the workspace.  causal:
  * token i of a sequence's n sees the prefix and its own keys before place lengths[s] - n + i + 1; else all of them.  A token that sees no key: zeros.
- * shift (int64, tokens x heads, or null) receives the shifts.  prefix: a cache whose sequence 0 holds
- * prefix_len tokens, or null and 0.  own: null where there is only a prefix (sequences, starts, lengths are not looked at then, max_length is 0).
+ * shift (int64, tokens x heads, or null) receives the shifts, 0 for a token that sees no key.  prefix: a cache whose sequence 0 holds prefix_len tokens, or null and 0.  own: null where there is only a prefix (sequences, starts, lengths are not looked at then, max_length is 0).
  * dim up to 256, up to 2^24 keys of each kind, 2^20 queries a head of keys.  Elements up to 0x7F7F7F7F, scores and sums within 2^62 (ZK_VALUES_RANGE); a score above the shift or further below it than the
  * digits reach raises ZK_VALUES_TABLE. */
 int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,

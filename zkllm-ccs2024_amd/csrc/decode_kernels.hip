@@ -115,7 +115,7 @@ struct AppendArgs {
     Sequences seqs;
     uint32_t* flag;
 };
-// A workgroup a token
+// A workgroup a token; HBM bounds many of them: 3200 tokens of 5 x 80, keys and values, 8.4 us, 2.4 TB/s, of which the launch is 2.3 (a single token's)
 template <int VEC> __global__ void __launch_bounds__(256) k_cache_append(const AppendArgs a) {
     const uint32_t token = blockIdx.x, units = a.dim / VEC;
     uint32_t bad = 0;
@@ -143,6 +143,8 @@ template <int VEC> __global__ void __launch_bounds__(256) k_cache_append(const A
 // ---- attention ----------------------------------------------------------------------------------------------------------------------------
 // A row is one query head of a token; the rows of a head of keys are token * group + head in its group.  Four steps, each a launch: scores, a row's softmax to weights, sums of weights times
 // values, and where the keys were cut into parts their sums joined.  Tiles are 16 or 64 rows: of the prefix's, any; of a sequence's own keys, its own.
+// Scores are sums of 3 x 3 digit products (4 x 4 where a fourth digit is there), outputs of 5 x 3 (6 x 4), a digit product 2 * 16 * 16 * 64 operations in 16 cycles.  A prompt of 2048 tokens over as many keys,
+// heads of 128, eight of them (of 32, 1.18 ms): splits 12 us, scores 69, the softmax 118 and 25 (the rows whose sums are taken in order), outputs 72.
 // Keys and values of a part that many rows read, split into digits once for all of them: as the fragments of the matrix instructions, [head of keys][16 keys][64 dimensions][digit][lane][16] of the
 // keys, [head of keys][64 keys][16 dimensions][digit][lane][16] of the values, and whether any of the 16 or 64 keys has a fourth digit
 struct SplitPart { int8_t *k, *v; uint32_t *k_wide, *v_wide; };
@@ -240,7 +242,7 @@ __device__ __forceinline__ bool any_bits(const v4i& v) { return (v[0] | v[1] | v
 
 // A key's place among the 16 of a fragment, and the other way round: row 4 q + e of a product is key 2 q + e, or 8 + 2 q + e - 2, so that four lanes store 64 bytes of scores in one piece
 __device__ __forceinline__ uint32_t key_of_lane(uint32_t c) { return (c >> 2) * 2 + (c & 1u) + (c & 2u) * 4; }
-// A workgroup splits 64 keys of a head: a wave 16 keys, and the values of 64 dimensions
+// A workgroup splits 64 keys of a head: a wave 16 keys, and the values of 64 dimensions.  HBM: 2048 keys of 8 heads of 128 in 11.5 us, 3.3 TB/s read and written
 template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_split(const AttnArgs a, int own) {
     uint32_t bad = 0;
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4, kv = a.kv0 + blockIdx.x, blocks = (a.dim + 63) / 64, units = blocks == 3 ? 4 : blocks, key0 = blockIdx.y * 64;
@@ -301,7 +303,8 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_split(const
     raise(a.flag, bad);
 }
 // Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8.  The next keys are
-// on their way while these are multiplied, and the place of those behind them is looked up.
+// on their way while these are multiplied, and the place of those behind them is looked up.  Few rows wait for memory: 16000 keys of 8 heads of 128, 4 rows each, 17 us, 3.9 TB/s.  Many rows are bound by
+// issue, splitting keys as much as joining sums: 128 rows over 8192 keys 46 us, 0.84 POP/s; with keys split before (SPLIT), 2048 over 2048, 69 us, 1.1 POP/s.  Half as many rows a wave (RT 2) gain nothing.
 template <int U, int RT, Heads HEADS, int WAVES, bool SPLIT> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, v4i (&fourth)[RT][U][64],
                                                                                                  int64_t* out, size_t ld, uint32_t& bad) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
@@ -715,9 +718,12 @@ template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x
     return t;
 }
 // W waves a row, eight neighbouring keys a lane at a time.  The sum of exponentials is taken in no order first, from exponentials that are near: off from the sum in
-// order by at most 2^-53 of all of that one's partial sums (half of the keys times the whole, where terms are alike) and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 40 at 2048 keys and
+// order by at most 2^-53 of all of that one's partial sums (half of the keys times the whole, where terms are alike) and what the exponentials are off.  That decides the shift unless it lies that near to a border between two whole numbers (one row in 65 at 2048 keys and
 // a scale of 2^32 sqrt(128)); then the sum in order is taken -- by a launch of its own for such rows, where there are many rows --, the waves' runs at once where the sum stays within a power of
 // two, and the few others one after the other.
+// Latency bounds it where rows are few: 32 rows of 16000 keys 44 us, of it 9 for the tables and the near sum, 30 for the sum in order (dependent additions, scans and barriers; sixteen waves a row, with half
+// the registers each: 51), 5 for the weights.  Issue where they are many: 16384 rows of 2048 keys 118 us, some 100 instructions a score (four waves a row: 144; all of a row's scores held in registers
+// instead of read a second time: 118), and 25 for the one row in 65 whose sum is taken in order.
 // A row's scores x to its weights, zeros up to `fill`; ld from digit to digit.  false: its sum must be taken in order (SUMS NEAR)
 template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softmax_row(const SoftmaxArgs& s, const int64_t* x, int8_t* weights, size_t ld, const Columns& columns, uint32_t fill,
                                                                                       const int32_t* live, const double* power, RowShared<W>& sh, int64_t& shift, bool& top, uint32_t& bad) {
@@ -894,7 +900,7 @@ template <int NS> __device__ __forceinline__ void attn_sum(const int32_t (&s)[NS
     size = h + (l >> 32);
 }
 // Few rows: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each.  weights: the lane's row and 16 keys of
-// 64; keys from + 64 stream to end, 64 streams apart
+// 64; keys from + 64 stream to end, 64 streams apart.  16000 keys of 8 heads of 128 29 us, 2.3 TB/s: 300 registers leave a wave a unit, so that its loads and its products take turns
 template <Heads HEADS> __device__ __forceinline__ void values_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t block, uint32_t first, uint32_t end, uint32_t stream, uint32_t streams, const int8_t* weights,
                                                               size_t ld, bool top, v4i (&acc)[9][4], uint32_t& bad) {
     const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, d0 = block * 64 + 4 * (lane & 15u);
@@ -990,7 +996,8 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(cons
     } else finish_tile(a, t, kv, sums64, blocks, 256, bad);
     raise(a.flag, bad);
 }
-// A tile of 16 rows with few keys, from scores to outputs in one launch: nothing leaves LDS between the steps
+// A tile of 16 rows with few keys, from scores to outputs in one launch: nothing leaves LDS between the steps.  One token of 32 heads over 200 keys 22 us (four launches: 29), the steps' latencies one after the
+// other.  Up to 576 columns, what LDS holds of 16 rows, and 512 workgroups, two rounds of the units.
 static constexpr uint32_t SMALL_COLS = 576, SMALL_LIVE = 4096;
 template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(512) k_attn_small(const AttnArgs a) {
     __shared__ __attribute__((aligned(16))) int64_t scores[16 * SMALL_COLS];
@@ -1078,7 +1085,7 @@ __device__ __forceinline__ void tile_out(const AttnArgs& a, const Tile& t, int o
     }
 }
 // Many rows: 64 rows by 128 dimensions, a wave 16 by 64.  The workgroup splits 64 keys' values into digits together, the next ones while this step's are multiplied: a lane four keys of four
-// dimensions, in LDS as fragments.
+// dimensions, in LDS as fragments.  128 rows over 8192 keys of 8 heads of 128 46 us, 1.4 POP/s
 template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_tile(const AttnArgs a, int own) {
     __shared__ __attribute__((aligned(16))) int8_t planes[2][4][8][64][16], weight[2][4][6][64][16];      // fragments of the values and, [16 rows], of the weights
     __shared__ uint32_t wide[3];                           // of the step, the next and the one after that
@@ -1184,7 +1191,8 @@ template <Heads HEADS> __global__ void __launch_bounds__(512, 2) k_attn_values_t
     tile_out(a, t, own, kv, z, row, row_in, dim0 + block * 64, acc, bad);
     raise(a.flag, bad);
 }
-// The same where the values have been split already (k_attn_split): their fragments and the weights' go straight to LDS, two steps ahead
+// The same where the values have been split already (k_attn_split): their fragments and the weights' go straight to LDS, two steps ahead.  2048 rows over 2048 keys of 8 heads of
+// 128 72 us, 1.8 POP/s (splitting in every tile: 99); the barrier that every step of 60 matrix instructions a wave ends with bounds it
 __global__ void __launch_bounds__(512, 2) k_attn_values_split(const AttnArgs a, int own) {
     // a variable a buffer: the compiler waits for a direct load before every read of the variable that it writes
     typedef int8_t Values[3][8][1024];                     // [digit][16 dimensions]
@@ -1270,7 +1278,8 @@ __global__ void __launch_bounds__(512, 2) k_attn_values_split(const AttnArgs a, 
     tile_out(a, t, own, kv, z, row, row_in, dim0 + block * 64, acc, bad);
     raise(a.flag, bad);
 }
-// The parts' sums added up, 64 outputs a workgroup, by four shares of the parts or, where outputs are few, sixteen; rows that see no key
+// The parts' sums added up, 64 outputs a workgroup, by four shares of the parts or, where outputs are few, sixteen; rows that see no key.  1024 rows of 128, 33 parts:
+// 15 us, 3.5 TB/s (parts of sixteen bytes: 20)
 __global__ void __launch_bounds__(1024) k_attn_join(const AttnArgs a) {
     __shared__ unsigned long long sums[16][64][2];
     const uint32_t share = threadIdx.x >> 6, shares = blockDim.x >> 6, lane = threadIdx.x & 63u;
@@ -1343,7 +1352,8 @@ __device__ __forceinline__ unsigned long long block_best(unsigned long long best
     return best;
 }
 // A workgroup takes a stretch of a row, eight tokens a lane.  Its logits and mask are on their way while it reads the row's lists, eight entries a lane at a time, and counts and adds up in LDS what
-// falls into the stretch.  BIAS: there are biases.
+// falls into the stretch.  BIAS: there are biases.  Issue bounds it: 64 rows of 128257 with 8000 tokens of history each 29 us, 2.3 TB/s, of which every stretch's way through the row's list
+// is half; one row of 32000 4.9 us, latency.
 template <bool POW2, bool BIAS> __global__ void __launch_bounds__(LOGITS_THREADS) k_logits(const LogitsArgs a) {
     constexpr int N = 8, T = LOGITS_THREADS;
     static_assert(LOGITS_SPAN == N * T, "a stretch is eight tokens a lane");
@@ -1452,7 +1462,7 @@ static int check_cache(const zk_i32_cache* c, const char* name, uint32_t sequenc
 }
 static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->token_stride | c->head_stride) & 3) == 0 && (((uintptr_t)c->k | (uintptr_t)c->v) & 15) == 0; }
 
-// How an attention call is cut: heads of keys at a time, and its keys into parts, so that there are some 1024 workgroups
+// How an attention call is cut: as many heads of keys at a time as keep scores and weights within 512 MB (fewer gain nothing), and its keys into parts, so that there are some 1024 workgroups (512 where rows are many)
 struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts_high, parts, split_each; bool split[2]; uint32_t split_tiles[2]; };      // split_each: a head's
 // From so many rows of a head of keys on its keys and values are split once for all of them. 8 heads of 128: at 128 rows over 8192 keys the split, scores and values take 25 + 35 + 53 us, tiles that each split
 // what they read 46 + 64; at 2048 rows over as many keys 12 + 66 + 73 against 97 + 99

@@ -902,7 +902,8 @@ template <bool GATED> __device__ __forceinline__ void q4_output(const ProductArg
     g.e.out[(size_t)row * g.cols + col] = g.e.pow2 ? value(std::true_type()) : value(std::false_type());
 }
 // Up to four rows, a strip of 16 columns a workgroup: the 16 rows of v_mfma_i32_16x16x64_i8 are the four digits of up to four rows of x, which the workgroup splits into LDS while its first
-// codes are on their way.  A wave takes 128 inner rows at a time, four such loads ahead.
+// codes are on their way.  A wave takes 128 inner rows at a time, four such loads ahead.  Memory: one row of 11008 x 4096 8.2 us, 2.9 TB/s of codes and scales, of which the launch and x's digits are some 3
+// (the same weight as int8 planes: 17.5).
 template <bool GATED, int R, int WAVES> __global__ void __launch_bounds__(64 * WAVES) k_q4_rows(const Q4Args a) {
     constexpr int MATS = GATED ? 2 : 1, DEPTH = 4;
     extern __shared__ __attribute__((aligned(16))) int8_t digits[];        // [64 inner rows][a quarter of them][digit][row of x][16]
@@ -1002,7 +1003,8 @@ template <bool GATED, int R, int WAVES> __global__ void __launch_bounds__(64 * W
     raise(g.e.flag, bad);
 }
 // 5 to 32 rows: S strips by 8 / S shares of the inner dimension a workgroup, 128 inner rows a step; x's planes, which the strips share, go to LDS as fragments and codes to registers up to three
-// steps ahead.
+// steps ahead.  32 rows of both weights of 4096 x 11008 29 us, 1.6 TB/s of codes: a step ends with a barrier, and codes become planes by some 40 instructions a fragment that meets only two tiles of rows (the
+// planes of int8 weights, k_product's strips: 50).
 template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k_q4_strip(const Q4Args a) {
     constexpr int MATS = GATED ? 2 : 1, SHARES = 8 / S, PIECES = SHARES * 2 * RT * 4, EACH = PIECES / 8, BUFS = SHARES * RT <= 4 ? 4 : 2, LOADS = EACH + 3 * MATS;
     typedef int8_t Buffer[SHARES][2][RT][4][1024];         // [share][64 inner rows][16 rows][digit]
@@ -1151,7 +1153,8 @@ template <bool GATED, int RT, int S> __global__ void __launch_bounds__(512, 2) k
     }
     raise(g.e.flag, bad);
 }
-// Before a product of many rows, in one launch: the planes of one whole weight or two, and of x.  Workgroups of four waves: the weights' first, 16 columns by 256 inner rows each
+// Before a product of many rows, in one launch: the planes of one whole weight or two, and of x.  Workgroups of four waves: the weights' first, 16 columns by 256 inner rows each.
+// HBM and the launch: two weights of 1000 x 2750, three planes each, 9 us
 template <int PB> __device__ __forceinline__ void q4_expand(int8_t* planes, const Q4& w, uint32_t block) {
     const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, q = lane >> 4, strips = (w.cols + 15) / 16, strip = block % strips, u = block / strips * 4 + (threadIdx.x >> 6), col = strip * 16 + c;
     if (u >= w.units || col >= w.cols) return;
