@@ -302,6 +302,25 @@ def test_shifts_are_the_sums_of_exponentials_in_order(hip, kind, keys, prefix_le
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["normal", "rising", "falling", "two levels"])
+@pytest.mark.parametrize("keys", [600, 2048, 2500, 9001])
+def test_shifts_of_many_rows(hip, kind, keys):
+    """The same where rows are many: every one of them goes through both launches at this scale"""
+    import torch
+    rng, rows = np.random.default_rng(keys + 1), 300
+    softmax = dec.Softmax((1 << 28, 1 << 28, 1 << 7), 1, 0, float(1 << 49), (1000.0, 1000.0), 1)
+    k = {"normal": rng.normal(0, 1.0, keys), "rising": np.linspace(-20, 3, keys), "falling": np.linspace(3, -20, keys), "two levels": np.where(rng.random(keys) < 0.5, 0.0, -0.6931471805599453)}[kind]
+    k = np.round(k * (1 << 22)).astype(np.int32)
+    q = rng.integers(-(1 << 27), 1 << 27, (rows, 1, 1)).astype(np.int32)
+    own = Pages(rng, 1, keys, 1, 1, keys, False)
+    own.k[:], own.v[:] = k, 1
+    own.dk.copy_(dev(own.k)), own.dv.copy_(dev(own.v))
+    shift = torch.zeros((rows, 1), dtype=torch.int64, device="cuda")
+    attend(hip, dev(q), Plan(hip, softmax), None, 0, own, 1, dev([0, rows]), dev([keys]), keys, False, 1, sf=(1, 1), shift=shift, flag=new_flag())
+    assert (host(shift)[:, 0] == shifts_of(hip, k.astype(np.int64)[None] * q.reshape(rows, 1), softmax.scale)).all()
+
+
+@gpu
 @pytest.mark.parametrize("what,bit", [("query", RANGE), ("key", RANGE), ("value", RANGE), ("score", RANGE), ("output", RANGE), ("far", TABLE), ("page", POSITION), ("length", POSITION), ("negative", POSITION), ("starts", POSITION)])
 def test_attention_raises_flags(hip, what, bit):
     """and leaves the other sequence right"""
