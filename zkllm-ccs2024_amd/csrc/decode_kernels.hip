@@ -722,8 +722,8 @@ template <int W> __device__ __forceinline__ double sum_in_order(const int64_t* x
 // a scale of 2^32 sqrt(128)); then the sum in order is taken -- by a launch of its own for such rows, where there are many rows --, the waves' runs at once where the sum stays within a power of
 // two, and the few others one after the other.
 // Latency bounds it where rows are few: 32 rows of 16000 keys 44 us, of it 9 for the tables and the near sum, 30 for the sum in order (dependent additions, scans and barriers; sixteen waves a row, with half
-// the registers each: 51), 5 for the weights.  Issue where they are many: 16384 rows of 2048 keys 118 us, some 100 instructions a score (four waves a row: 144; all of a row's scores held in registers
-// instead of read a second time: 118), and 25 for the one row in 65 whose sum is taken in order.
+// the registers each: 51), 5 for the weights.  Memory and issue where they are many: 16384 rows of 2048 keys 118 us, scores read twice and weights written 6.2 TB/s, 63 instructions a score 43 % of the
+// slots (four waves a row: 144; all of a row's scores held in registers instead of read a second time: 118; five waves a SIMD instead of four: 138), and 25 for the one row in 65 whose sum is taken in order.
 // A row's scores x to its weights, zeros up to `fill`; ld from digit to digit.  false: its sum must be taken in order (SUMS NEAR)
 template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softmax_row(const SoftmaxArgs& s, const int64_t* x, int8_t* weights, size_t ld, const Columns& columns, uint32_t fill,
                                                                                       const int32_t* live, const double* power, RowShared<W>& sh, int64_t& shift, bool& top, uint32_t& bad) {
