@@ -900,7 +900,8 @@ template <int NS> __device__ __forceinline__ void attn_sum(const int32_t (&s)[NS
     size = h + (l >> 32);
 }
 // Few rows: a wave takes 64 dimensions of 64 keys at a time; a lane reads four neighbouring dimensions of 16 keys, so that it has the 16 keys of a fragment of each.  weights: the lane's row and 16 keys of
-// 64; keys from + 64 stream to end, 64 streams apart.  16000 keys of 8 heads of 128 29 us, 2.3 TB/s: 300 registers leave a wave a unit, so that its loads and its products take turns
+// 64; keys from + 64 stream to end, 64 streams apart.  16000 keys of 8 heads of 128 24 us, 2.7 TB/s, bound by how much is on its way: two waves a SIMD, for
+// which 62 registers are spilled (one wave with all of them: 29)
 template <Heads HEADS> __device__ __forceinline__ void values_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t block, uint32_t first, uint32_t end, uint32_t stream, uint32_t streams, const int8_t* weights,
                                                               size_t ld, bool top, v4i (&acc)[9][4], uint32_t& bad) {
     const uint32_t lane = threadIdx.x & 63u, q = lane >> 4, d0 = block * 64 + 4 * (lane & 15u);
@@ -963,7 +964,7 @@ __device__ __forceinline__ void finish_tile(const AttnArgs& a, const Tile& t, ui
         attn_finish(a, sums[at], (int64_t)sums[at + 1], token, kv * a.group + (t.row0 + r - token * a.group), d, bad);
     }
 }
-template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_values(const AttnArgs a, int own) {
+template <Heads HEADS> __global__ void __launch_bounds__(256, 2) k_attn_values(const AttnArgs a, int own) {
     extern __shared__ unsigned long long sums64[];         // [16][64 blocks of dimensions][2]
     uint32_t bad = 0;
     Tile t;
