@@ -304,7 +304,8 @@ template <Heads HEADS> __global__ void __launch_bounds__(256) k_attn_split(const
 }
 // Scores: a wave takes 16 keys by 16 RT rows at a time, a lane 16 of 64 dimensions of one of the keys, straight from memory to the fragments of v_mfma_i32_16x16x64_i8.  The next keys are
 // on their way while these are multiplied, and the place of those behind them is looked up.  Few rows wait for memory: 16000 keys of 8 heads of 128, 4 rows each, 17 us, 3.9 TB/s.  Many rows are bound by
-// issue, splitting keys as much as joining sums: 128 rows over 8192 keys 46 us, 0.84 POP/s; with keys split before (SPLIT), 2048 over 2048, 69 us, 1.1 POP/s.  Half as many rows a wave (RT 2) gain nothing.
+// issue, splitting keys as much as joining sums: 128 rows over 8192 keys 41 us, 0.94 POP/s (two workgroups a
+// unit, with registers spilled: 46); with keys split before (SPLIT), 2048 over 2048, 69 us, 1.1 POP/s.  Half as many rows a wave (RT 2) gain nothing.
 template <int U, int RT, Heads HEADS, int WAVES, bool SPLIT> __device__ __forceinline__ void scores_of(const AttnArgs& a, const Tile& t, uint32_t kv, uint32_t first, uint32_t end, v4i (&fourth)[RT][U][64],
                                                                                                  int64_t* out, size_t ld, uint32_t& bad) {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, c = lane & 15u, q = lane >> 4;
@@ -427,7 +428,7 @@ template <int U, int RT, Heads HEADS, int WAVES, bool SPLIT> __device__ __forcei
         }
     }
 }
-template <int U, int RT, Heads HEADS, bool SPLIT> __global__ void __launch_bounds__(256, 2) k_attn_scores(const AttnArgs a, int own) {
+template <int U, int RT, Heads HEADS, bool SPLIT> __global__ void __launch_bounds__(256, RT > 1 ? 1 : 2) k_attn_scores(const AttnArgs a, int own) {
     __shared__ v4i fourth[RT][U][64];
     uint32_t bad = 0;
     Tile t;
@@ -1466,7 +1467,7 @@ static bool cache_aligned(const zk_i32_cache* c) { return ((c->page_stride | c->
 // How an attention call is cut: as many heads of keys at a time as keep scores and weights within 512 MB (fewer gain nothing), and its keys into parts, so that there are some 1024 workgroups (512 where rows are many)
 struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, own_tiles, prefix_splits, prefix_step, own_splits, own_step, heads; size_t prefix_cols, cols, scores, weights, top, unsure, parts_high, parts, split_each; bool split[2]; uint32_t split_tiles[2]; };      // split_each: a head's
 // From so many rows of a head of keys on its keys and values are split once for all of them. 8 heads of 128: at 128 rows over 8192 keys the split, scores and values take 25 + 35 + 53 us, tiles that each split
-// what they read 46 + 64; at 2048 rows over as many keys 12 + 66 + 73 against 97 + 99
+// what they read 41 + 46; at 2048 rows over as many keys 12 + 68 + 72 against 97 + 99
 static constexpr size_t SPLIT_ROWS_FROM = 256;
 static uint32_t split_dims(uint32_t dim) { return dim > 128 ? 256 : (dim + 63) / 64 * 64; }
 static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
