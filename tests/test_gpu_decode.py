@@ -240,6 +240,26 @@ def test_attention_softmaxes(hip, softmax, sf):
 
 
 @gpu
+@pytest.mark.parametrize("factor", [0.9, 0.6, 0.45, 0.4, 0.1, 0.001])
+@pytest.mark.parametrize("tokens,keys", [(3, 90), (3, 700), (300, 600)])
+def test_attention_of_small_second_factors(hip, factor, tokens, keys):
+    """Below 0.5 the second table holds zeros alone, from some e^-0.75 = 0.47 down no entry is reached by its bound: every output is 0, in one launch and in several, of few rows and of many"""
+    import torch
+    rng = np.random.default_rng(tokens + keys)
+    dim = 64
+    softmax = dec.Softmax(thetas=(float(1 << 18), factor), dim=dim)
+    own = Pages(rng, 1, keys, 1, dim, 64)
+    q = normal(rng, (tokens, 1, dim))
+    flag, shift = new_flag(), torch.full((tokens, 1), -5, dtype=torch.int64, device="cuda")
+    got = host(attend(hip, dev(q), Plan(hip, softmax), None, 0, own, 1, None, dev([keys]), keys, False, 1, sf=(1 << 10, 1 << 6), shift=shift, flag=flag))
+    assert host(flag)[0] == 0
+    k, v = own.read(0, keys, 0)
+    for i in {0, 1, tokens // 2, tokens - 1}:
+        exp, s = dec.attention(q[i, 0], k, v, softmax, 1 << 10, 1 << 6)
+        assert host(shift)[i, 0] == s and (got[i, 0] == exp).all() and (factor > 0.5 or not exp.any()), i
+
+
+@gpu
 @pytest.mark.parametrize("big_q,big_k,big_v", [(1 << 27, 1 << 27, 1 << 16), (1 << 20, 0x7F7F7F7F, 1 << 20), (0x7F7F7F7F, 1 << 18, 0x7F7F7F7F), (1 << 10, 1 << 10, 0x7F7F7F7F)])
 def test_attention_of_large_values(hip, big_q, big_k, big_v):
     """four digits in some places of the queries, keys and values; the weights are small so that sums fit"""

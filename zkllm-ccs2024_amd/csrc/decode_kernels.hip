@@ -1603,7 +1603,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
         for (int i = 0; i < 5; ++i) a.series[i] = i ? a.series[i - 1] * -w0 / i : thetas[0];      // theta exp(-w0 digit)
         a.series[0] += 0.5;
         a.guard = thetas[0] * (z * z * z * z * z / 60.0 + 0x1p-46);
-        a.live = (uint32_t)std::min<double>(reach / w1 + 2.0, bs[L + 1]);
+        a.live = (uint32_t)std::max(1.0, std::min<double>(reach / w1 + 2.0, bs[L + 1]));      // a factor whose exponentials all lie below 0.5: the first entry, 0 as well
         a.upper_end = 1u << (all - 32);
         s->series = z <= 0x1p-7 && a.guard < 0.01 && reach / w1 + 2.0 <= MOST_LIVE;
     }
