@@ -161,6 +161,85 @@ def test_values_of_a_wider_layer_with_kept_weights(pv):
     pv.layer_free(layer)
 
 
+def by_proof(pv, layer, X):
+    x = pv.from_i32(X)
+    return pv.lib.zkp_layer_values_by_proof(c_void_p(layer), c_void_p(x.h))
+
+
+def equals_the_proof(pv, layer, X, proof_attends, seed=9):
+    got = values(pv, layer, X)
+    assert by_proof(pv, layer, X) == proof_attends
+    pv.seed(seed)
+    out, _ = pv.layer_run(layer, pv.from_i32(X))
+    assert (got == out.host()).all()
+    return got
+
+
+@pytest.mark.parametrize("rope", ROPES)
+def test_values_of_a_layer_take_the_attention_in_integers(pv, rope):
+    cu, cf = layercfg.tiny(open_weights=False)
+    layer = pv.layer_create(cu, cf, layercfg.tiny_weights(7, cu), 1)
+    if rope is not None:
+        set_rope(pv, layer, **rope)
+    equals_the_proof(pv, layer, np.round(np.random.default_rng(17).normal(0, 1, (16, 32)) * 256).astype(np.int32), 0)
+    pv.layer_free(layer)
+
+
+@pytest.mark.parametrize("tokens", [64, 1024])
+def test_values_of_a_layer_whose_weights_are_a_series(pv, tokens):
+    """Two tables of 2^14 entries over heads of 64 at a scale of 2^25: the softmax's weights by the series and the second table's first entries, in one launch and in several"""
+    cu, cf = layercfg.pack(tokens, 256, 4, 352, 1 << 12, 1 << 12, 1 << 8, [1 << 4, 1 << 14, 1 << 14], 1, 0, 1 << 22, [1 << 8, 1 << 8], -(1 << 13), 1 << 14, 256.0, value_scale=256.0, open_weights=False,
+                           head_group=4)
+    layer = pv.layer_create_random(cu, cf, 3, 1)
+    set_rope(pv, layer)
+    equals_the_proof(pv, layer, np.round(np.random.default_rng(tokens).normal(0, 1, (tokens, 256)) * 256).astype(np.int32), 0)
+    pv.layer_free(layer)
+
+
+@pytest.mark.parametrize("head_group", [0, 1])
+def test_values_of_heads_wider_than_the_attention_takes(pv, head_group):
+    """Two heads of 320 elements: the proof's forward pass, in one group and head by head"""
+    cu, cf = layercfg.pack(16, 640, 2, 64, 1 << 8, 1 << 10, 1 << 7, [1 << 8, 1 << 8, 1 << 8], 1, 0, 1 << 16, [1 << 6, 1 << 8], -512, 1024, 64.0, value_scale=256.0, open_weights=False, head_group=head_group)
+    layer = pv.layer_create(cu, cf, layercfg.tiny_weights(5, cu, w_std=0.02), 1)
+    for rope in (None, {}):
+        if rope is not None:
+            set_rope(pv, layer, **rope)
+        equals_the_proof(pv, layer, np.round(np.random.default_rng(2).normal(0, 1, (16, 640)) * 256).astype(np.int32), 1)
+    pv.layer_free(layer)
+
+
+def test_values_of_a_softmax_that_the_attention_does_not_take(pv):
+    """A scale of 2^52 sqrt(16) lies above 2^53: scores are nothing beside it, every weight is a token's share, and the seven digits reach the shift of 2^54 ln 16"""
+    cu, cf = layercfg.pack(16, 32, 2, 64, 1 << 8, 1 << 10, 1 << 7, [1 << 8] * 7, 5, 0, 1 << 52, [1 << 6, 1 << 8], -512, 1024, 64.0, value_scale=256.0, open_weights=False)
+    layer = pv.layer_create(cu, cf, layercfg.tiny_weights(11, cu), 1)
+    equals_the_proof(pv, layer, np.round(np.random.default_rng(3).normal(0, 1, (16, 32)) * 256).astype(np.int32), 1)
+    pv.layer_free(layer)
+
+
+def test_values_where_the_attention_raises_its_flag(pv):
+    """One value between 0x7F7F7F80 and 2^31 - 1, which four digits do not hold and the proof's tensors do: only token 3 has something at place 5, so that its norm's weight reaches nobody else"""
+    cu, cf = layercfg.tiny(open_weights=False)
+    ws = layercfg.tiny_weights(7, cu)
+    X = np.round(np.random.default_rng(17).normal(0, 1, (16, 32)) * 256).astype(np.int32)
+    X[:, 5], X[3] = 0, 0
+    X[3, 5] = 256
+    ws[0][0, 5] = 256 * 48
+    n = ref.norm(X, ws[0][0], 1e-5, 256.0, 256)[0]
+    assert n[3, 5] > 65000 and not n[:3, 5].any() and not n[4:, 5].any()
+    for w in ws[1:4]:                               # what token 3 is to its query, key and value, but for one element
+        w[5] = 0
+    ws[3][5, 20] = round(2143000000 * 256 / n[3, 5])
+    ws[4][20] = 0                                   # and what becomes of that
+    ws[4][20, 9] = 1
+    v = ref.linear(n, ws[3], 256)
+    assert 0x7F7F7F7F < v.max() < 1 << 31 and (np.abs(v) > 0x7F7F7F7F).sum() == 1
+    layer = pv.layer_create(cu, cf, ws, 1)
+    got = equals_the_proof(pv, layer, X, 1)
+    X[3, 5] = 0                                     # the same layer without it
+    assert (equals_the_proof(pv, layer, X, 0) != got).any()
+    pv.layer_free(layer)
+
+
 @pytest.mark.parametrize("base", [-10000.0, 0.5, float("nan")])
 def test_a_base_that_is_none_is_refused(pv, base):
     cu, cf = layercfg.tiny(open_weights=False)

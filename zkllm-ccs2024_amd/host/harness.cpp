@@ -647,6 +647,15 @@ void* zkp_layer_values(void* h, void* X, int repeats, double* ms) {
     return new FrTensor(out.to_fr());
     ZKP_END_PTR
 }
+// which way the layer's output without a proof takes for X: 1 where the proof's forward pass computes the attention, 0 where zk_i32_attention does; negative on error
+int zkp_layer_values_by_proof(void* h, void* X) {
+    try {
+        LayerState& s = *reinterpret_cast<LayerState*>(h);
+        bool by_proof = false;
+        (void)LayerValues(s.cfg, s.w)(IntTensor(FT(X)), &by_proof);
+        return by_proof ? 1 : 0;
+    } catch (const std::exception& e) { g_err = e.what(); return -1; }
+}
 // attention of the layer's heads with its proof (attn_heads_block), as the self-attn executable runs it
 void* zkp_layer_attention(void* h, void* Q, void* K, void* V) {
     ZKP_TRY

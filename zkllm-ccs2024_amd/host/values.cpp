@@ -84,16 +84,7 @@ void LayerValues::proof_attention(IntTensor& out, const IntTensor& n1, uint T, c
     }
 }
 
-IntTensor LayerValues::operator()(const IntTensor& X) const {
-    if (softmax) {
-        ValuesFlag scores;
-        IntTensor out = run(X, &scores);
-        if (scores.bits() == 0) return out;        // else a value that the proof's tensors may hold: its forward pass gives it, or says what is wrong
-    }
-    return run(X, nullptr);
-}
-// scores: the flag of zk_i32_attention, null for the proof's own attention
-IntTensor LayerValues::run(const IntTensor& X, const ValuesFlag* scores) const {
+IntTensor LayerValues::operator()(const IntTensor& X, bool* attention_by_proof) const {
     const uint E = c.embed_dim, Hd = c.hidden_dim, H = c.num_heads, d = E / H, T = X.size / E;
     if (T == 0 || X.size != T * E) throw std::runtime_error("LayerValues: X must be tokens x embed_dim");
     if (T > 0xFFFFu || (unsigned long long)T * std::max(E, Hd) > 0xFFFFFFFFull) throw std::runtime_error("LayerValues: more tokens than a tensor holds scores of");
@@ -108,7 +99,8 @@ IntTensor LayerValues::run(const IntTensor& X, const ValuesFlag* scores) const {
     };
     IntTensor n1(T * E), x2(T * E), proj(T * E);
     norm(nullptr, n1.gpu_data, X.gpu_data, nullptr, input_norm.gpu_data);
-    if (scores) {
+    bool by_proof = softmax == nullptr;
+    if (!by_proof) {
         // every token over all of them, as the proof has it: the sequence is the prefix of all its tokens
         IntTensor Q(T * E), K(T * E), V(T * E);
         linear(Q.gpu_data, n1.gpu_data, E, q);
@@ -123,9 +115,13 @@ IntTensor LayerValues::run(const IntTensor& X, const ValuesFlag* scores) const {
         const zk_i32_cache cache{K.gpu_data, V.gpu_data, (size_t)T * E, E, d, T, 1, nullptr, 0};
         const size_t bytes = zk_i32_attention_workspace(T, H, H, d, T, 0, 0);
         DevBuf attn_ws(bytes);
+        ValuesFlag scores;
         ZKC(zk_i32_attention(proj.gpu_data, E, d, Q.gpu_data, E, d, T, H, H, d, softmax, &cache, T, nullptr, 0, nullptr, nullptr, 0, 0, c.sf_attn, c.sf_attn, nullptr, attn_ws.p, bytes,
-                             scores->dev(), nullptr));
-    } else proof_attention(proj, n1, T, flag, ws.p, room);
+                             scores.dev(), nullptr));
+        by_proof = scores.bits() != 0;             // a value that the proof's tensors may hold: its forward pass gives it, or says what is wrong
+    }
+    if (by_proof) proof_attention(proj, n1, T, flag, ws.p, room);
+    if (attention_by_proof) *attention_by_proof = by_proof;
     linear(n1.gpu_data, proj.gpu_data, E, o);
     norm(x2.gpu_data, n1.gpu_data, X.gpu_data, n1.gpu_data, post_norm.gpu_data);
     {
@@ -134,6 +130,6 @@ IntTensor LayerValues::run(const IntTensor& X, const ValuesFlag* scores) const {
         linear(proj.gpu_data, hidden.gpu_data, Hd, down);
     }
     norm(x2.gpu_data, nullptr, x2.gpu_data, proj.gpu_data, nullptr);
-    if (!scores || scores->bits() == 0) flag.check("LayerValues");
+    flag.check("LayerValues");
     return x2;
 }

@@ -15,7 +15,9 @@ class LayerValues {
     LayerValues& operator=(const LayerValues&) = delete;
     // X: tokens x embed_dim in fixed point, any number of tokens.  Element for element llama_layer's output; throws when a value leaves int32 or the
     // activation table, where the proof's own lookups fail as well or its tensors hold larger numbers.
-    IntTensor operator()(const IntTensor& X) const;
+    // attention_by_proof (may be null) receives whether the proof's forward pass computed the attention: for heads and softmaxes that zk_i32_attention does not take, and
+    // where that raised its flag.
+    IntTensor operator()(const IntTensor& X, bool* attention_by_proof = nullptr) const;
 
    private:
     const LayerConfig& c;
@@ -24,7 +26,6 @@ class LayerValues {
     IntTensor input_norm, post_norm, act;
     void* softmax = nullptr;       // null where the heads or the softmax are none that zk_i32_attention takes: the proof's own forward pass then
     Rhs rhs(const FrTensor& weight, uint in_dim, uint out_dim);
-    IntTensor run(const IntTensor& X, const ValuesFlag* scores) const;
     void proof_attention(IntTensor& out, const IntTensor& normed, uint tokens, const ValuesFlag& flag, void* ws, size_t room) const;
     void release();
 };
