@@ -554,7 +554,10 @@ int zk_i32_cache_append(const zk_i32_cache* cache, const void* k, size_t k_token
  * thetas' exponentials (K - L - M of them).  Radices up to 2^28 and their product up to 2^63, thetas' product below 1.4e14, scaling_factor_in sqrt(dim) up to 2^53.  Waits for the stream; any stream may use the handle afterwards. */
 int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs_host, int K, int L, int M, double scaling_factor_in, const double* thetas_host, uint32_t dim, void* stream);
 int zk_i32_softmax_free(void* softmax);          /* once its last call is through */
-/* 0 for short calls (a few tokens over up to 576 keys), which need none; otherwise 14 bytes for every row and key of as many heads as fit 512 MB, or of one head */
+/* 0 for short calls (a few tokens over up to 576 keys), which need none; otherwise the bytes with which a call is fastest.  That is, for every head of keys that is in work at a time -- as many as fit 512 MB,
+ * one at least --, 14 bytes for each of its queries and keys, 12 dim for each query and part where the keys are cut into parts (1024 workgroups' worth at most, or parts of 8192 keys), and
+ * from 256 queries on 8 bytes an element of the keys that many queries read.  A smaller workspace serves as well, by more passes, down to one head at a time with the first of these and parts of 8192
+ * keys: what zk_i32_attention_workspace says for one call serves every call with the same heads and as many or fewer tokens, sequences and keys of either kind. */
 size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length);
 /* Attention of queries over the keys and values of a prefix that all sequences share (read once for all of them) and, behind it, of their sequences' own (self-attn.cu:81-98,
  * zksoftmax.cu:112-173):  x_j = q . k_j,  shift = the nearest integer to scale ln(sum_j exp(x_j / scale)), scale = scaling_factor_in sqrt(dim),  y_j = the product of the tables' values at

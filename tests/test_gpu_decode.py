@@ -483,6 +483,67 @@ def test_attention_in_tiles(hip, counts, lengths, heads, kv_heads, dim, prefix_l
         assert (got[n:] == -77).all()
 
 
+def smaller_workspaces(hip, lower, upper, call):
+    """the smallest workspace that a call is not refused with, between a size that is too small and one that is enough; call(bytes, plan) with a plan for heads of another width ends at that"""
+    other = Plan(hip, dec.Softmax(dim=1))
+    while lower + 1 < upper:
+        mid = (lower + upper) // 2
+        with pytest.raises(RuntimeError) as e:
+            call(mid, other)
+        small = "the workspace is smaller" in str(e.value)
+        assert small or "another width" in str(e.value)
+        lower, upper = (mid, upper) if small else (lower, mid)
+    return upper
+
+
+# Workspaces below the one that is fastest: five heads of keys in passes of two, two and one or one by one, with parts that are joined, keys and values split before, many sequences of few tokens, a sequence's prompt
+PASSES = [([300], [400], 5, 5, 32, 700, True), ([300], [700], 10, 5, 80, 0, True), ([1] * 70, list(range(560, 630)), 15, 5, 24, 1300, True), ([3, 40, 0, 2], [100, 640, 7, 2], 20, 5, 130, 600, False), ([280], [0], 5, 5, 16, 9000, False),
+          ([9], [20000], 10, 5, 16, 8500, True)]
+
+
+@gpu
+@pytest.mark.parametrize("counts,lengths,heads,kv_heads,dim,prefix_len,causal", PASSES)
+def test_attention_in_smaller_workspaces(hip, counts, lengths, heads, kv_heads, dim, prefix_len, causal):
+    import torch
+    rng = np.random.default_rng(heads * 1000 + dim + sum(lengths))
+    softmax, n, most, group = dec.Softmax(dim=dim), sum(counts), max(lengths), heads // kv_heads
+    prefix = Pages(rng, 1, prefix_len, kv_heads, dim, 48) if prefix_len else None
+    own = Pages(rng, len(counts), most, kv_heads, dim, 64) if most else None
+    q = normal(rng, (n, heads, dim))
+    dq, starts, dl, plan = dev(q), dev(np.cumsum([0] + counts)), dev(lengths), Plan(hip, softmax)
+    full = hip.lib.zk_i32_attention_workspace(c_uint(n), c_uint(heads), c_uint(kv_heads), c_uint(dim), c_uint(prefix_len), c_uint(len(counts) if own else 0), c_uint(most))
+    guard = 4096
+    memory = torch.empty(full + guard, dtype=torch.uint8, device="cuda")
+
+    def call(size, p, out=None, shift=None, flag=None):
+        return attend(hip, dq, p, prefix, prefix_len, own, len(counts), starts, dl, most, causal, kv_heads, out=out, shift=shift, ws=memory[:size], flag=flag)
+
+    cols = -(-prefix_len // 64) * 64 + -(-most // 64) * 64
+    least = smaller_workspaces(hip, n * group * cols * 14 - 1, full, call)
+    results = []
+    for size in (full, full * 2 // 5 + 4096, (full * 2 // 5 + least) // 2, least * 2 + 4096, least):
+        memory.fill_(0x5B)
+        flag, shift = new_flag(), torch.full((n, heads), -5, dtype=torch.int64, device="cuda")
+        out = host(call(size, plan, shift=shift, flag=flag))
+        assert host(flag)[0] == 0 and (host(memory)[size:] == 0x5B).all()
+        results.append((out, host(shift)))
+    for out, shift in results[1:]:
+        assert (out == results[0][0]).all() and (shift == results[0][1]).all()
+    at = 0
+    for s, count in enumerate(counts):
+        for i in range(count):
+            if i in (0, 1, 17, 64, count // 2, count - 1) and (len(counts) < 10 or s in (0, 1, 30, 69)):
+                seen = 0 if not own else max(0, lengths[s] - count + i + 1) if causal else lengths[s]
+                for h in range(heads):
+                    keys = [np.zeros((0, dim), np.int64)] * 2
+                    for c, m, j in ((prefix, prefix_len, 0), (own, seen, s)):
+                        if c:
+                            keys = [np.concatenate(p) for p in zip(keys, c.read(j, m, h // group))]
+                    exp, sh = dec.attention(q[at, h], keys[0], keys[1], softmax, 1 << 20, 1 << 20)
+                    assert (results[0][0][at, h] == exp).all() and results[0][1][at, h] == sh, (s, i, h)
+            at += 1
+
+
 @gpu
 def test_attention_of_many_tokens_without_keys(hip):
     n, heads, dim = 600, 32, 64
@@ -952,6 +1013,70 @@ def test_attention_workspace_of_the_longest_caches():
     size = [workspace_of(c_uint(256), c_uint(1), c_uint(1), c_uint(128), c_uint(keys), c_uint(0), c_uint(0)) for keys in (most, most + 64, 1 << 24)]
     # a key's row of scores and weights: 256 x 14 bytes, its digits: 128 x 8; parts of 8192 keys, one more for the longest by each as many
     assert size[0] >= most * (256 * 14 + 128 * 8) > size[1] >= (most + 64) * 256 * 14 and size[2] >= (1 << 24) * 256 * 14
+
+
+def attention_takes(tokens, heads, kv_heads, dim, prefix_len, sequences, most, size):
+    """whether zk_i32_attention takes a workspace of that size: a handle for heads of no elements is what it is refused for then"""
+    from gpuhelp import pkg
+    lib = pkg.load_hip()
+    plan, other = (ctypes.c_char * 4096)(), (ctypes.c_int32 * 64)()
+    caches = [Cache(ctypes.addressof(W), ctypes.addressof(W), kv_heads * dim << 24, kv_heads * dim, dim, 1 << 24, 1 << 18, None, 0) for _ in range(2)]
+    rc = lib.zk_i32_attention(other, c_size_t(heads * dim), c_size_t(dim), W, c_size_t(heads * dim), c_size_t(dim), c_uint(tokens), c_uint(heads), c_uint(kv_heads), c_uint(dim), plan,
+                              ctypes.byref(caches[0]) if prefix_len else None, c_uint(prefix_len), ctypes.byref(caches[1]) if sequences else None, c_uint(sequences), W, W, c_uint(most), c_int(1), c_uint(1),
+                              c_uint(1), None, c_void_p(1 << 20), c_size_t(size), W, None)
+    text = lib.zk_last_error().decode()
+    assert rc == 10001 and ("another width" in text or "the workspace is smaller" in text), text
+    return "another width" in text
+
+
+def attention_workspace(*sizes):
+    from gpuhelp import pkg
+    f = pkg.load_hip().zk_i32_attention_workspace
+    f.restype = c_size_t
+    return f(*(c_uint(i) for i in sizes))
+
+
+def test_a_workspace_serves_every_smaller_call():
+    """tokens, sequences and both numbers of keys below those that a workspace was asked for, which may take more by itself: more parts, or keys split before"""
+    import random
+    rng = random.Random(1)
+    log = lambda most: int(2 ** rng.uniform(0, np.log2(most + 1)))
+    more = 0
+    for _ in range(1500):
+        kv_heads, dim, group = rng.choice([1, 2, 8, 32]), rng.choice([1, 16, 64, 80, 128, 200, 256]), rng.choice([1, 4, 5])
+        tokens, prefix_len, most = log(5000), rng.choice([0, log(1 << 17), log(3000)]), rng.choice([0, log(1 << 17), log(3000)])
+        sequences = rng.choice([1, min(tokens, log(300)), tokens]) if most or prefix_len == 0 else rng.choice([0, 1, tokens])
+        large = (tokens, group * kv_heads, kv_heads, dim, prefix_len, sequences, most)
+        size = attention_workspace(*large)
+        assert attention_takes(*large, size)
+        cols = (prefix_len + 63) // 64 * 64 + (most + 63) // 64 * 64
+        if size:
+            assert not attention_takes(*large, tokens * group * cols * 14)
+        for _ in range(6):
+            t, p, m = rng.choice([tokens, rng.randint(1, tokens)]), rng.choice([prefix_len, rng.randint(0, prefix_len)]), rng.choice([most, rng.randint(0, most)])
+            s = rng.choice([sequences, rng.randint(0, sequences)])
+            if s == 0:
+                m = 0
+                if p == 0:
+                    continue
+            small = (t, group * kv_heads, kv_heads, dim, p, s, m)
+            assert attention_takes(*small, size), (large, small)
+            more += attention_workspace(*small) > size
+    assert more > 20                                # some of them would be faster with more
+
+
+@pytest.mark.parametrize("large,small", [((33, 32, 8, 128, 8192, 33, 512), (32, 32, 8, 128, 8192, 32, 512)), ((599, 32, 32, 128, 0, 1, 16000), (260, 32, 32, 128, 0, 1, 16000)),
+                                         ((256, 1, 1, 128, 65535 * 64 + 64, 0, 0), (256, 1, 1, 128, 65535 * 64, 0, 0)), ((256, 1, 1, 128, 1 << 24, 1, 1 << 24), (256, 1, 1, 128, 65535 * 64, 1, 65535 * 64))])
+def test_a_workspace_serves_a_smaller_call_that_has_more(large, small):
+    assert attention_workspace(*large) < attention_workspace(*small) or large[4] == 1 << 24
+    assert attention_takes(*small, attention_workspace(*large))
+
+
+@pytest.mark.parametrize("sizes", [(2048, 32, 32, 128, 0, 1, 2048), (260, 32, 32, 128, 0, 1, 16000), (300, 32, 8, 256, 30000, 1, 30000), (64, 32, 8, 128, 8192, 64, 4096)])
+def test_a_workspace_of_more_than_one_head_stays_within_512_mb(sizes):
+    tokens, heads, kv_heads, dim, prefix_len, sequences, most = sizes
+    size, one = attention_workspace(*sizes), attention_workspace(tokens, heads // kv_heads, 1, dim, prefix_len, sequences, most)
+    assert size <= max(512 << 20, one + 64)
 
 
 def test_q4_refusals():

@@ -1470,7 +1470,20 @@ struct AttnPlan { bool small, prefix64, own64, direct; uint32_t prefix_tiles, ow
 // what they read 41 + 46; at 2048 rows over as many keys 12 + 68 + 72 against 97 + 99
 static constexpr size_t SPLIT_ROWS_FROM = 256;
 static uint32_t split_dims(uint32_t dim) { return dim > 128 ? 256 : (dim + 63) / 64 * 64; }
-static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
+static void attn_sizes(AttnPlan& p, uint32_t heads, size_t rows, uint32_t dim) {      // for that many heads of keys at a time
+    auto round = [](size_t b) { return (b + 15) / 16 * 16; };
+    p.heads = heads;
+    p.scores = heads * rows * p.cols * 8;
+    p.weights = heads * rows * p.cols * 6;
+    p.top = round(heads * rows * 4);
+    p.unsure = 16 + p.top;
+    p.parts_high = round(heads * rows * (size_t)(p.direct ? 0 : p.prefix_splits + p.own_splits) * dim * 8);
+    p.parts = round(p.parts_high + p.parts_high / 2);
+}
+static size_t attn_bytes(const AttnPlan& p) { return p.scores + p.weights + p.top + p.unsure + p.parts + p.heads * p.split_each; }
+// room: the workspace.  Where it has none for the plan that is fastest, fewer heads go at a time; where it has none for one head either, nothing is split before and keys are cut as little as sums in 32 bits
+// let them: what one head needs then grows with each of the call's sizes, so that a workspace for a larger call has room for it.
+static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length, size_t room) {
     AttnPlan p{};
     const uint32_t group = heads / kv_heads;
     const size_t rows = (size_t)tokens * group;
@@ -1492,15 +1505,7 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     };
     cut(prefix_len, p.prefix_tiles, p.prefix64, p.prefix_splits, p.prefix_step);
     cut(sequences ? max_length : 0, p.own_tiles, p.own64, p.own_splits, p.own_step);
-    const uint32_t splits = p.prefix_splits + p.own_splits;
-    p.direct = splits == 1;
-    const size_t each = rows * (p.cols * 14 + 8 + (size_t)(p.direct ? 0 : splits) * dim * 12);
-    p.heads = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / std::max<size_t>(each, 1)));
-    if (p.heads < kv_heads && p.own64 && p.own_splits == 1) {      // as many as fill the compute units evenly, one workgroup each
-        auto used = [&](uint32_t h) { const size_t w = rows / 64 * h * cdiv(dim, 128); return w ? (double)w / (cdiv(w, 256) * 256.0) : 0.0; };
-        for (uint32_t h = p.heads; h >= std::max(1u, p.heads / 2); --h) if (used(h) > used(p.heads) + 0.02) p.heads = h;
-    }
-    auto round = [](size_t b) { return (b + 15) / 16 * 16; };
+    p.direct = p.prefix_splits + p.own_splits == 1;
     auto part = [&](bool many, uint32_t keys, int i) {
         p.split[i] = many && keys && rows >= SPLIT_ROWS_FROM && keys <= 65535u * 64;      // a grid's second side
         p.split_tiles[i] = p.split[i] ? cdiv(keys, 64) * 4 : 0;
@@ -1508,12 +1513,31 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     part(p.prefix64, prefix_len, 0);
     part(p.own64 && sequences == 1, max_length, 1);
     p.split_each = (size_t)(p.split_tiles[0] + p.split_tiles[1]) * ((size_t)split_dims(dim) * 128 + 16);
-    p.scores = p.heads * rows * p.cols * 8;
-    p.weights = p.heads * rows * p.cols * 6;
-    p.top = round(p.heads * rows * 4);
-    p.unsure = 16 + p.top;
-    p.parts_high = round(p.heads * rows * (size_t)(p.direct ? 0 : splits) * dim * 8);
-    p.parts = round(p.parts_high + p.parts_high / 2);
+    attn_sizes(p, 1, rows, dim);
+    uint32_t most = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / attn_bytes(p)));
+    if (most < kv_heads && p.own64 && p.own_splits == 1) {      // as many as fill the compute units evenly, one workgroup each
+        auto used = [&](uint32_t h) { const size_t w = rows / 64 * h * cdiv(dim, 128); return w ? (double)w / (cdiv(w, 256) * 256.0) : 0.0; };
+        for (uint32_t h = most; h >= std::max(1u, most / 2); --h) if (used(h) > used(most) + 0.02) most = h;
+    }
+    auto fit = [&] {
+        for (uint32_t h = most; h >= 1; --h) {
+            attn_sizes(p, h, rows, dim);
+            if (attn_bytes(p) <= room) return true;
+        }
+        return false;
+    };
+    if (fit()) return p;
+    auto cut_least = [&](uint32_t keys, uint32_t& splits, uint32_t& step) {
+        step = std::min(MOST_STEP, std::max(64u, cdiv(keys, 64) * 64));
+        splits = cdiv(keys, step);
+    };
+    cut_least(prefix_len, p.prefix_splits, p.prefix_step);
+    cut_least(sequences ? max_length : 0, p.own_splits, p.own_step);
+    p.direct = p.prefix_splits + p.own_splits == 1;
+    p.split[0] = p.split[1] = false;
+    p.split_tiles[0] = p.split_tiles[1] = 0;
+    p.split_each = 0;
+    (void)fit();
     return p;
 }
 
@@ -1616,8 +1640,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
 
 size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim, uint32_t prefix_len, uint32_t sequences, uint32_t max_length) {
     if (tokens == 0 || kv_heads == 0 || heads < kv_heads) return 0;
-    const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
-    return p.scores + p.weights + p.top + p.unsure + p.parts + p.heads * p.split_each;
+    return attn_bytes(attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length, SIZE_MAX));
 }
 int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                      const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts, const void* lengths, uint32_t max_length,
@@ -1645,11 +1668,11 @@ int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q
     if (prefix_len) if (const int rc = check_cache(prefix, name, 1, prefix_len, kv_heads, dim)) return rc;
     if (own) if (const int rc = check_cache(own, name, sequences, max_length, kv_heads, dim)) return rc;
     if (!own) sequences = 0;
-    const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length);
+    const AttnPlan p = attn_plan(tokens, heads, kv_heads, dim, prefix_len, sequences, max_length, workspace ? workspace_bytes : SIZE_MAX);
     ZK_ARG(p.prefix_tiles <= 65535u && p.own_tiles <= 65535u && (uint64_t)p.heads * cdiv(dim, 128) <= 65535u, std::string(name) + ": more than 65535 tiles of queries");
     hipStream_t st = (hipStream_t)stv;
-    const size_t bytes = p.scores + p.weights + p.top + p.unsure + p.parts + p.heads * p.split_each;
-    ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_attention_workspace says");
+    const size_t bytes = attn_bytes(p);
+    ZK_ARG(workspace == nullptr || workspace_bytes >= bytes, std::string(name) + ": the workspace is smaller than zk_i32_attention_workspace says, and than the call needs for one head of keys at a time");
     ZK_ARG(((uintptr_t)workspace & 15) == 0, std::string(name) + ": the workspace must begin at a multiple of 16 bytes");
     ZK_ARG(dim == s->dim, std::string(name) + ": the softmax was prepared for heads of another width");
     CallFlag flag;
