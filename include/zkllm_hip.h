@@ -567,7 +567,8 @@ size_t zk_i32_attention_workspace(uint32_t tokens, uint32_t heads, uint32_t kv_h
  * as in zk_i32_cache_append, with their keys already in the cache; tokens of none are left as they are.  lengths[s] is 0 .. max_length, which bounds the work and the workspace.  causal:
  * token i of a sequence's n sees the prefix and its own keys before place lengths[s] - n + i + 1; else all of them.  A token that sees no key: zeros.
  * shift (int64, tokens x heads, or null) receives the shifts, 0 for a token that sees no key.  prefix: a cache whose sequence 0 holds prefix_len tokens, or null and 0.  own: null where there is only a prefix (sequences, starts, lengths are not looked at then, max_length is 0).
- * dim up to 256, up to 2^24 keys of each kind, 2^20 queries a head of keys.  Elements up to 0x7F7F7F7F, scores and sums within 2^62 (ZK_VALUES_RANGE); a score above the shift or further below it than the
+ * dim up to 256, up to 2^24 keys of each kind, 2^20 queries a head of keys (tokens heads / kv_heads), at most 65535 tiles of them: queries / 64 + sequences where a sequence has more than 32 on average and
+ * there are keys, else queries / 16 + sequences.  Elements up to 0x7F7F7F7F, scores and sums within 2^62 (ZK_VALUES_RANGE); a score above the shift or further below it than the
  * digits reach raises ZK_VALUES_TABLE. */
 int zk_i32_attention(void* out, size_t out_token, size_t out_head, const void* q, size_t q_token, size_t q_head, uint32_t tokens, uint32_t heads, uint32_t kv_heads, uint32_t dim,
                      const void* softmax, const zk_i32_cache* prefix, uint32_t prefix_len, const zk_i32_cache* own, uint32_t sequences, const void* starts_i32, const void* lengths_i32,

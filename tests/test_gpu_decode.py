@@ -555,6 +555,23 @@ def test_attention_of_many_tokens_without_keys(hip):
         assert host(flag)[0] == 0 and (out[:n] == 0).all() and (out[n] == -77).all()
 
 
+@gpu
+@pytest.mark.parametrize("most", [9, 600])
+def test_attention_of_as_many_sequences_as_there_are_tiles(hip, most):
+    """61680 sequences of a token each, from none to `most` keys: 65535 tiles"""
+    rng, n = np.random.default_rng(most), 61680
+    softmax = dec.Softmax(dim=3)
+    own = Pages(rng, n, most, 1, 3, 16 if most < 16 else most, most < 16)
+    lengths, q = rng.integers(0, most + 1, n), normal(rng, (n, 1, 3))
+    lengths[[0, n - 1]] = 0, most
+    flag = new_flag()
+    got = host(attend(hip, dev(q), Plan(hip, softmax), None, 0, own, n, None, dev(lengths), most, True, 1, flag=flag))
+    assert host(flag)[0] == 0 and (got[lengths == 0] == 0).all()
+    for i in [0, 1, 2, 15, 16, 17, n - 2, n - 1] + rng.integers(0, n, 200).tolist():
+        k, v = own.read(i, int(lengths[i]), 0)
+        assert (got[i, 0] == dec.attention(q[i, 0], k, v, softmax, 1 << 20, 1 << 20)[0]).all(), i
+
+
 # ---- weights of 4 bits -----------------------------------------------------------------------------------------------------------------------
 class Q4:
     def __init__(self, hip, rng, N, P, group, zeros=True, most=800):
@@ -1020,12 +1037,12 @@ def attention_takes(tokens, heads, kv_heads, dim, prefix_len, sequences, most, s
     from gpuhelp import pkg
     lib = pkg.load_hip()
     plan, other = (ctypes.c_char * 4096)(), (ctypes.c_int32 * 64)()
-    caches = [Cache(ctypes.addressof(W), ctypes.addressof(W), kv_heads * dim << 24, kv_heads * dim, dim, 1 << 24, 1 << 18, None, 0) for _ in range(2)]
+    caches = [Cache(ctypes.addressof(W), ctypes.addressof(W), kv_heads * dim << 24, kv_heads * dim, dim, 1 << 24, 1 << 21, None, 0) for _ in range(2)]
     rc = lib.zk_i32_attention(other, c_size_t(heads * dim), c_size_t(dim), W, c_size_t(heads * dim), c_size_t(dim), c_uint(tokens), c_uint(heads), c_uint(kv_heads), c_uint(dim), plan,
                               ctypes.byref(caches[0]) if prefix_len else None, c_uint(prefix_len), ctypes.byref(caches[1]) if sequences else None, c_uint(sequences), W, W, c_uint(most), c_int(1), c_uint(1),
                               c_uint(1), None, c_void_p(1 << 20), c_size_t(size), W, None)
     text = lib.zk_last_error().decode()
-    assert rc == 10001 and ("another width" in text or "the workspace is smaller" in text), text
+    assert rc == 10001 and any(i in text for i in ("another width", "the workspace is smaller", "65535 tiles")), text
     return "another width" in text
 
 
@@ -1034,6 +1051,17 @@ def attention_workspace(*sizes):
     f = pkg.load_hip().zk_i32_attention_workspace
     f.restype = c_size_t
     return f(*(c_uint(i) for i in sizes))
+
+
+@pytest.mark.parametrize("tokens,group,sequences,prefix_len,most,takes", [
+    (61680, 1, 61680, 0, 100, True), (61681, 1, 61681, 0, 100, False), (7710 * 4, 32, 3855, 50, 9, True), (1 << 20, 1, 1, 0, 700, True), (1 << 20, 1, 31775, 0, 700, True), (1 << 20, 1, 31776, 0, 700, False),
+    (1 << 20, 1, 31774, 0, 700, True), (65535 * 16 - 1, 1, 1, 0, 0, True), (65535 * 16, 1, 1, 0, 0, False), (65534 * 16 + 15, 1, 1, 0, 0, True), (1 << 20, 1, 0, 700, 0, True), (1 << 18, 4, 1, 0, 0, False), (1 << 18, 4, 1, 0, 9, True)])
+def test_attention_takes_65535_tiles(tokens, group, sequences, prefix_len, most, takes):
+    """of 16 or 64 queries, by the average of a sequence's queries and whether there are keys"""
+    queries = tokens * group
+    tiles = queries // (64 if most and queries // sequences > 32 else 16) + sequences if sequences else 0
+    assert (tiles <= 65535) == takes
+    assert attention_takes(tokens, group, 1, 16, prefix_len, sequences, most, 1 << 50) == takes
 
 
 def test_a_workspace_serves_every_smaller_call():
