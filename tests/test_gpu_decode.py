@@ -545,6 +545,34 @@ def test_attention_in_smaller_workspaces(hip, counts, lengths, heads, kv_heads, 
 
 
 @gpu
+@pytest.mark.parametrize("sequences,tokens,heads,kv_heads,dim,prefix_len,most,rows", [
+    (1, 2048, 20, 20, 16, 0, 2048, (0, 1000, 2047)), (256, 256, 20, 5, 8, 9000, 64, (0, 100, 255)), (1, 6000, 3, 3, 4, 6000, 6000, (0, 63, 64, 5999)), (1, 3000, 5, 5, 70, 3500, 0, (0, 1500, 2999))])
+def test_attention_of_more_heads_than_go_at_a_time(hip, sequences, tokens, heads, kv_heads, dim, prefix_len, most, rows):
+    """Passes of eight heads of keys of twenty, three of five, one of three, three of five: one more would take more than 512 MB, or leave units idle"""
+    import torch
+    rng = np.random.default_rng(tokens)
+    softmax, group = dec.Softmax(dim=dim), heads // kv_heads
+    prefix = Pages(rng, 1, prefix_len, kv_heads, dim, prefix_len, False) if prefix_len else None
+    own = Pages(rng, sequences, most, kv_heads, dim, 64) if most else None
+    lengths = rng.integers(1, most + 1, sequences) if sequences > 1 else [most]
+    q = normal(rng, (tokens, heads, dim))
+    flag, shift = new_flag(), torch.full((tokens, heads), -5, dtype=torch.int64, device="cuda")
+    assert hip.lib.zk_i32_attention_workspace(*(c_uint(i) for i in (tokens, heads, kv_heads, dim, prefix_len, sequences, most))) < kv_heads * tokens * group * (prefix_len + most) * 14
+    got = host(attend(hip, dev(q), Plan(hip, softmax), prefix, prefix_len, own, sequences, None, dev(lengths), most, True, kv_heads, shift=shift, flag=flag))
+    assert host(flag)[0] == 0
+    for i in rows:
+        s, n = (i, 1) if sequences > 1 else (0, tokens)
+        seen = lengths[s] if sequences > 1 else i + 1 if most else 0
+        for h in range(heads):
+            keys = [np.zeros((0, dim), np.int64)] * 2
+            for c, m, j in ((prefix, prefix_len, 0), (own, seen, s)):
+                if c:
+                    keys = [np.concatenate(p) for p in zip(keys, c.read(j, m, h // group))]
+            exp, sh = dec.attention(q[i, h], keys[0], keys[1], softmax, 1 << 20, 1 << 20)
+            assert (got[i, h] == exp).all() and host(shift)[i, h] == sh, (i, h)
+
+
+@gpu
 def test_attention_of_many_tokens_without_keys(hip):
     n, heads, dim = 600, 32, 64
     own = Pages(np.random.default_rng(3), 1, 1, heads, dim, 16)
@@ -647,6 +675,59 @@ def test_gated_of_4_bits(hip, rows, N, P, group, most):
     assert host(flag)[0] == 0
     got = host(out)
     assert (got[:rows] == ref.gated(x, g.w, u.w, 1 << 18, 1 << 18, table, low, 1 << 18)).all() and (got[rows:] == -77).all()
+
+
+def with_four_digits(rng, x):
+    """a few inputs of four digits, in the first and last columns as well"""
+    rows, n = x.shape
+    x[rng.integers(0, rows, 6), rng.integers(0, n, 6)] = rng.integers(-(1 << 29), 1 << 29, 6)
+    x[0, 0], x[-1, -1] = 1 << 29, -(1 << 29)
+    return x
+
+
+# Where a workgroup takes two or four strips of 16 columns (from 5105 and 10225 columns), with fewer and more steps than there are buffers; where it has four waves (from 8193 columns) and where the inner
+# dimension is more than LDS holds of x at a time (14336 of one row, 7168 of two, 3584 of four); groups of 64 and their multiples, powers of two and none
+WIDE_Q4 = [(5, 130, 5201, 64), (16, 1100, 5121, 128), (13, 2300, 5201, 192), (5, 130, 10301, 64), (16, 1100, 10301, 192), (9, 2300, 10240, 128), (17, 130, 10301, 128), (32, 1100, 10301, 64), (32, 2300, 10301, 320),
+           (17, 700, 5201, 64), (1, 1100, 8301, 64), (2, 300, 8301, 192), (3, 1100, 8301, 128), (4, 3700, 8301, 64), (1, 14500, 33, 64), (1, 29000, 17, 192), (2, 7300, 33, 128), (2, 14400, 8, 64), (3, 3700, 33, 192),
+           (4, 11008, 40, 128), (4, 3585, 16, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("rows,N,P,group", WIDE_Q4)
+def test_linear_of_4_bits_in_every_arrangement(hip, rows, N, P, group, four):
+    rng = np.random.default_rng(N * 31 + P + rows)
+    w = Q4(hip, rng, N, P, group, True, 8 if four else 400)
+    x = normal(rng, (rows, N), 20000.0)
+    if four:
+        x = with_four_digits(rng, x)
+    flag = new_flag()
+    got = host(linear(hip, dev(x), w, rows, N, P, flag=flag))
+    assert host(flag)[0] == 0
+    assert (got[:rows] == ref.linear(x, w.w, 65536)).all() and (got[rows:] == -77).all()
+
+
+@gpu
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("rows,N,P,group", WIDE_Q4[:1] + WIDE_Q4[2:9] + [(2, 300, 8301, 192), (4, 1100, 8301, 64), (1, 14500, 33, 64), (2, 7300, 33, 128), (4, 3700, 40, 192)])
+def test_gated_of_4_bits_in_every_arrangement(hip, rows, N, P, group, four):
+    import torch
+    rng = np.random.default_rng(N + rows + P)
+    g, u = Q4(hip, rng, N, P, group, True, 8 if four else 400), Q4(hip, rng, N, P, group, False, 8 if four else 400)
+    low = -(1 << 23 if four else 1 << 18)          # eight inputs of four digits in one row reach 8 * 2^29 * 15 * 8 / 2^16
+    n = -2 * low
+    table = rng.integers(-(1 << 16), 1 << 16, n).astype(np.int32)
+    x = normal(rng, (rows, N), 2000.0 if four else 10000.0)
+    if four:
+        x = with_four_digits(rng, x)
+    sf = (1 << 16, 1 << 16, 1 << 10)
+    assert (np.abs(ref.linear(x, g.w, sf[0])) < -low).all()
+    out, flag, ws, dx, dt = torch.full((rows + 1, P), -77, dtype=torch.int32, device="cuda"), new_flag(), workspace(hip, [g, u], rows), dev(x), dev(table)
+    hip.call("zk_i32_gated", ptr(out), ptr(dx), c_size_t(N), g.h, u.h, c_uint(rows), c_uint(sf[0]), c_uint(sf[1]), ptr(dt), c_int(low), c_uint(n), c_uint(sf[2]), ptr(ws), c_size_t(ws.numel()), ptr(flag), None)
+    exp = ref.gated(x, g.w, u.w, sf[0], sf[1], table, low, sf[2])
+    got = host(out)
+    assert host(flag)[0] == 0 and (np.abs(exp) < 1 << 31).all()
+    assert (got[:rows] == exp).all() and (got[rows:] == -77).all()
 
 
 @gpu
