@@ -765,10 +765,11 @@ template <int W, Weights KIND, Sums SUMS> __device__ __forceinline__ bool softma
             for (int i = 0; i < W; ++i) { total += sh.sums[i]; partial += sh.partial[i]; }
         }
         if (columns.end) {
-            // The sum in order is off by 2^-53 of each sum on its way, this one by as much of the whole for each of a lane's terms.  Both sums' exponentials of x together are off by 8e-16 and 3.9e-16 |x|; weighted by what they have in the sum t, |x| is |ln t| + 17 at most (17: the logarithm of more keys than
-            // there can be).  Both logarithms are off by 4e-16 of them and their products with the scale by 2^-53.
+            // The sum in order is off by 2^-53 of each sum on its way, this one by as much of the whole for each of a lane's terms, of which there are a 64th of the columns and 22 at most.  Both sums'
+            // exponentials of x together are off by 1.2e-15 (4e-16 of exp_det twice, the rest roundings) and, by the roundings of x / scale, 4.8e-16 |x|; weighted by what they have in the sum t,
+            // |x| is |ln t| + 17.4 at most (17.4: the logarithm of 2^25 keys).  Both logarithms are off by 4e-16 of them and their products with the scale by 2^-53.
             const double ln = zkd::log_det(total), sv = s.scale * ln;
-            const double off = s.scale * ((partial / total + (double)(columns.end / 64 + 64)) * 1.2e-16 + 1.5e-15 * fabs(ln) + 8e-15), from_border = fabs(sv - floor(sv) - 0.5);
+            const double off = s.scale * ((partial / total + (double)(columns.end / 64 + 24)) * 1.2e-16 + 1.6e-15 * fabs(ln) + 1e-14), from_border = fabs(sv - floor(sv) - 0.5);
             sure = total > 1e-280 && total < 1e280 && off < 0.25 && from_border > off;
             if (sure) shift = rounded(sv);
         }
@@ -1514,7 +1515,7 @@ static AttnPlan attn_plan(uint32_t tokens, uint32_t heads, uint32_t kv_heads, ui
     part(p.own64 && sequences == 1, max_length, 1);
     p.split_each = (size_t)(p.split_tiles[0] + p.split_tiles[1]) * ((size_t)split_dims(dim) * 128 + 16);
     attn_sizes(p, 1, rows, dim);
-    uint32_t most = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / attn_bytes(p)));
+    uint32_t most = (uint32_t)std::max<size_t>(1, std::min<size_t>(kv_heads, ((size_t)512 << 20) / std::max<size_t>(attn_bytes(p), 1)));
     if (most < kv_heads && p.own64 && p.own_splits == 1) {      // as many as fill the compute units evenly, one workgroup each
         auto used = [&](uint32_t h) { const size_t w = rows / 64 * h * cdiv(dim, 128); return w ? (double)w / (cdiv(w, 256) * 256.0) : 0.0; };
         for (uint32_t h = most; h >= std::max(1u, most / 2); --h) if (used(h) > used(most) + 0.02) most = h;
