@@ -1000,7 +1000,8 @@ template <Heads HEADS> __global__ void __launch_bounds__(256, 2) k_attn_values(c
     raise(a.flag, bad);
 }
 // A tile of 16 rows with few keys, from scores to outputs in one launch: nothing leaves LDS between the steps.  One token of 32 heads over 200 keys 22 us (four launches: 29), the steps' latencies one after the
-// other.  Up to 576 columns, what LDS holds of 16 rows, and 512 workgroups, two rounds of the units.
+// other.  Up to 576 columns, what LDS holds of 16 rows, and 512 workgroups, two rounds of the units.  The sums of nine digits by four dimensions and the keys ahead are more than 256 registers: 55 to 106 are
+// spilled for heads of up to 128 elements, 70 to 240 for longer ones, 448 to 638 where those are read element by element.
 static constexpr uint32_t SMALL_COLS = 576, SMALL_LIVE = 4096;
 template <int U, Heads HEADS, Weights KIND> __global__ void __launch_bounds__(512) k_attn_small(const AttnArgs a) {
     __shared__ __attribute__((aligned(16))) int64_t scores[16 * SMALL_COLS];
@@ -1630,6 +1631,7 @@ int zk_i32_softmax_prepare(void** softmax, const uint32_t* bs, int K, int L, int
         a.guard = thetas[0] * (z * z * z * z * z / 60.0 + 0x1p-46);
         a.live = (uint32_t)std::max(1.0, std::min<double>(reach / w1 + 2.0, bs[L + 1]));      // a factor whose exponentials all lie below 0.5: the first entry, 0 as well
         a.upper_end = 1u << (all - 32);
+        // z: the layer's heads from 64 elements on; `guard` alone would let narrower ones in, which has not been measured
         s->series = z <= 0x1p-7 && a.guard < 0.01 && reach / w1 + 2.0 <= MOST_LIVE;
     }
     hipError_t e = hipGetLastError();
